@@ -14,10 +14,14 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <initializer_list>
 #include <limits>
 #include <map>
 #include <memory>
 #include <mutex>
+#include <optional>
+#include <string>
 #include <tuple>
 #include <utility>
 #include <vector>
@@ -287,12 +291,289 @@ Tensor gather_rows(const Tensor& input, int64_t dim, const Tensor& index) {
   return out;
 }
 
-// The attention operators return nothing and write `out` and `lse`, which torch's own boxed fallbacks
-// overlook: they look after returned tensors only.
+// ------------------------------------------------------------------ 8-bit linear layers
+// The operators' arguments are checked here, on any device, and then refused unless they are on a HIP one.
+int32_t type_of(at::ScalarType t, const char* name) {
+  TORCH_CHECK_VALUE(t == at::kBFloat16 || t == at::kHalf, name, " must be bf16 or fp16");
+  return t == at::kHalf ? HB_DTYPE_F16 : HB_DTYPE_BF16;
+}
+
+void require_hip(const Tensor& t) {
+  TORCH_CHECK_VALUE(t.is_cuda(), "HIP entry points take device tensors on one CUDA (HIP) device");
+}
+
+void one_device(const Tensor& first, std::initializer_list<const Tensor*> others) {
+  for (const Tensor* t : others)
+    TORCH_CHECK_VALUE(!t->defined() || t->device() == first.device(), "all tensors must be on one device");
+}
+
+const Tensor& value_or_none(const std::optional<Tensor>& t) {
+  static const Tensor* none = new Tensor;
+  return t.has_value() ? *t : *none;
+}
+
+void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// Leading dimensions of t, all but the last, as {batch, rows, batch stride, row stride}.
+struct Rows {
+  int64_t batch, rows, batch_stride, row_stride;
+};
+
+Rows rows_of(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.dim() == 2 || t.dim() == 3, name, " must be [rows, columns] or [batch, rows, columns]");
+  TORCH_CHECK_VALUE(t.size(-1) <= 1 || t.stride(-1) == 1, name, " must have a contiguous last dimension");
+  if (t.dim() == 2) return {1, t.size(0), 0, t.stride(0)};
+  return {t.size(0), t.size(1), t.stride(0), t.stride(1)};
+}
+
+// [begin, end) of a view's bytes.
+std::pair<const char*, const char*> bytes_of(const Tensor& t) {
+  int64_t extent = 1;
+  for (int64_t d = 0; d < t.dim(); ++d) extent += (t.size(d) - 1) * t.stride(d);
+  const char* begin = static_cast<const char*>(t.data_ptr());
+  return {begin, begin + (t.numel() ? extent * t.element_size() : 0)};
+}
+
+// What is written has places of its own: no two of its values share one, and no input lies among them.
+void check_written(const Tensor& out, const char* name, std::initializer_list<const Tensor*> inputs) {
+  c10::SmallVector<std::pair<int64_t, int64_t>, 5> dims;
+  for (int64_t d = 0; d < out.dim(); ++d)
+    if (out.size(d) > 1) dims.emplace_back(out.stride(d), out.size(d));
+  std::sort(dims.begin(), dims.end());
+  int64_t extent = 1;
+  for (const auto& [stride, size] : dims) {
+    TORCH_CHECK_VALUE(stride >= extent, name, " must have positive, non-overlapping strides");
+    extent += (size - 1) * stride;
+  }
+  const auto [begin, end] = bytes_of(out);
+  for (const Tensor* t : inputs) {
+    if (!t->defined() || !t->numel()) continue;
+    const auto [first, last] = bytes_of(*t);
+    TORCH_CHECK_VALUE(!(begin < last && first < end), name, " cannot alias the inputs");
+  }
+}
+
+// Checks of 8-bit rows [.., padded] with their scales; returns padded.
+int64_t check_int8(const Tensor& q, const Tensor& scale, const char* name) {
+  TORCH_CHECK_VALUE(q.dim() >= 2 && q.scalar_type() == at::kChar && q.is_contiguous() && q.size(-1) > 0 &&
+                        q.size(-1) % 64 == 0,
+                    name, " must be contiguous int8 rows of a multiple of 64 columns");
+  TORCH_CHECK_VALUE(scale.scalar_type() == at::kFloat && scale.is_contiguous() &&
+                        scale.sizes() == q.sizes().slice(0, q.dim() - 1),
+                    name, " must have one contiguous float32 scale a row");
+  return q.size(-1);
+}
+
+void int8_rows(const Tensor& x, Tensor q, Tensor scale) {
+  const int32_t dtype = type_of(x.scalar_type(), "x");
+  const Rows r = rows_of(x, "x");
+  const int64_t padded = check_int8(q, scale, "q");
+  TORCH_CHECK_VALUE(q.sizes().slice(0, q.dim() - 1) == x.sizes().slice(0, x.dim() - 1) && padded >= x.size(-1),
+                    "q must have x's rows, filled up to a multiple of 64 columns");
+  one_device(x, {&q, &scale});
+  require_hip(x);
+  const at::OptionalDeviceGuard guard(x.device());
+  check(hb_int8_rows(x.data_ptr(), r.batch_stride, r.row_stride, i32(r.batch, "batch"), i32(r.rows, "rows"),
+                     i32(x.size(-1), "features"), i32(padded, "padded"), dtype, static_cast<int8_t*>(q.data_ptr()),
+                     static_cast<float*>(scale.data_ptr()), stream_of(x.device())),
+        "hb_int8_rows");
+}
+
+struct AdaSet {
+  const Tensor &x, &shift, &scale;
+  const std::optional<Tensor>&y, &gate, &x_out;
+  const Tensor &q, &row_scale;
+};
+
+void int8_adaln_sets(std::initializer_list<AdaSet> sets, double eps) {
+  void* pointers[16];
+  int64_t strides[16];
+  int32_t rows[2];
+  const AdaSet& s0 = *sets.begin();
+  const int32_t dtype = type_of(s0.x.scalar_type(), "x");
+  const int64_t batch = s0.x.dim() == 3 ? s0.x.size(0) : 1, padded = check_int8(s0.q, s0.row_scale, "q");
+  const int64_t hidden = s0.x.dim() ? s0.x.size(-1) : 0;
+  int i = 0;
+  for (const AdaSet& s : sets) {
+    const Tensor &y = value_or_none(s.y), &gate = value_or_none(s.gate), &x_out = value_or_none(s.x_out);
+    TORCH_CHECK_VALUE(s.x.dim() == 3 && s.x.size(0) == batch && s.x.size(2) == hidden &&
+                          s.x.scalar_type() == s0.x.scalar_type(),
+                      "x must be [B, rows, hidden], both row sets of one batch, hidden size and dtype");
+    TORCH_CHECK_VALUE(y.defined() == gate.defined(), "y and gate are given together");
+    TORCH_CHECK_VALUE(!x_out.defined() || y.defined(), "x_out is written only with a residual update");
+    for (const Tensor* t : {&y, &x_out})
+      TORCH_CHECK_VALUE(!t->defined() || (t->sizes() == s.x.sizes() && t->scalar_type() == s.x.scalar_type()),
+                        "y and x_out must be like x");
+    for (const Tensor* t : {&s.shift, &s.scale, &gate})
+      TORCH_CHECK_VALUE(!t->defined() || (t->dim() == 2 && t->size(0) == batch && t->size(1) == hidden &&
+                                          (hidden <= 1 || t->stride(1) == 1) && t->scalar_type() == s.x.scalar_type()),
+                        "shift/scale/gate must be [B, hidden] views with a contiguous last dim");
+    TORCH_CHECK_VALUE(batch == 1 || s.shift.stride(0) == s.scale.stride(0), "shift and scale must share one batch stride");
+    TORCH_CHECK_VALUE(check_int8(s.q, s.row_scale, "q") == padded && s.q.dim() == 3 && s.q.size(0) == batch &&
+                          s.q.size(1) == s.x.size(1) && padded >= hidden,
+                      "q must have x's rows, filled up to a multiple of 64 columns");
+    const Rows rx = rows_of(s.x, "x"), ry = y.defined() ? rows_of(y, "y") : Rows{},
+               ro = x_out.defined() ? rows_of(x_out, "x_out") : Rows{};
+    if (x_out.defined()) check_written(x_out, "x_out", {&s.shift, &s.scale, &gate});
+    one_device(s0.x, {&s.x, &s.shift, &s.scale, &y, &gate, &x_out, &s.q, &s.row_scale});
+    void* p[8] = {pointer(s.x), pointer(y), pointer(gate), pointer(x_out), pointer(s.shift), pointer(s.scale),
+                  pointer(s.q), pointer(s.row_scale)};
+    // (a stride of a dimension of one says nothing)
+    const int64_t one = batch == 1 ? 0 : 1;
+    const int64_t st[8] = {one * rx.batch_stride, rx.rows == 1 ? 0 : rx.row_stride, one * ry.batch_stride,
+                           rx.rows == 1 ? 0 : ry.row_stride, gate.defined() ? one * gate.stride(0) : 0,
+                           one * ro.batch_stride, rx.rows == 1 ? 0 : ro.row_stride, one * s.shift.stride(0)};
+    std::copy(p, p + 8, pointers + 8 * i);
+    std::copy(st, st + 8, strides + 8 * i);
+    rows[i++] = i32(rx.rows, "rows");
+  }
+  require_hip(s0.x);
+  const at::OptionalDeviceGuard guard(s0.x.device());
+  check(hb_int8_adaln(i, i32(batch, "batch"), rows, i32(hidden, "hidden"), i32(padded, "padded"), dtype,
+                      static_cast<float>(eps), pointers, strides, stream_of(s0.x.device())),
+        "hb_int8_adaln");
+}
+
+using Maybe = std::optional<Tensor>;
+
+void int8_adaln(const Tensor& x, const Tensor& shift, const Tensor& scale, const Maybe& y, const Maybe& gate,
+                Maybe x_out, Tensor q, Tensor row_scale, double eps) {
+  int8_adaln_sets({{x, shift, scale, y, gate, x_out, q, row_scale}}, eps);
+}
+
+void int8_adaln_pair(const Tensor& x, const Tensor& shift, const Tensor& scale, const Maybe& y, const Maybe& gate,
+                     Maybe x_out, Tensor q, Tensor row_scale, const Tensor& x2, const Tensor& shift2,
+                     const Tensor& scale2, const Maybe& y2, const Maybe& gate2, Maybe x_out2, Tensor q2,
+                     Tensor row_scale2, double eps) {
+  int8_adaln_sets({{x, shift, scale, y, gate, x_out, q, row_scale}, {x2, shift2, scale2, y2, gate2, x_out2, q2, row_scale2}},
+                  eps);
+}
+
+// Checks of a weight [columns, padded] with its scales and bias.
+void check_weight(const Tensor& w, const Tensor& scale, const Tensor& bias, int64_t padded, int64_t columns,
+                  at::ScalarType dtype) {
+  TORCH_CHECK_VALUE(w.dim() == 2 && check_int8(w, scale, "weight") == padded && w.size(0) == columns,
+                    "weight must be [columns, padded features], as the rows are padded");
+  TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == columns && bias.is_contiguous() &&
+                                        bias.scalar_type() == dtype),
+                    "bias must be a contiguous [columns] tensor of the output's dtype");
+}
+
+struct LinearSet {
+  const Tensor &q, &scale, &weight, &weight_scale;
+  const std::optional<Tensor>& bias;
+  const Tensor& out;
+};
+
+void int8_linear_sets(std::initializer_list<LinearSet> sets, bool gelu) {
+  void* pointers[12];
+  int64_t strides[4];
+  int32_t rows[2];
+  const LinearSet& s0 = *sets.begin();
+  const int32_t dtype = type_of(s0.out.scalar_type(), "out");
+  const int64_t padded = check_int8(s0.q, s0.scale, "rows");
+  const int64_t batch = s0.out.dim() == 3 ? s0.out.size(0) : 1;
+  int i = 0;
+  for (const LinearSet& s : sets) {
+    const Tensor& bias = value_or_none(s.bias);
+    const Rows r = rows_of(s.out, "out");
+    TORCH_CHECK_VALUE(check_int8(s.q, s.scale, "rows") == padded && r.batch == batch &&
+                          s.out.scalar_type() == s0.out.scalar_type() && s.out.size(-1) == s0.out.size(-1),
+                      "both row sets must share batch, features, columns and dtype");
+    TORCH_CHECK_VALUE(s.q.sizes().slice(0, s.q.dim() - 1) == s.out.sizes().slice(0, s.out.dim() - 1),
+                      "out must have the rows' leading dimensions");
+    check_weight(s.weight, s.weight_scale, bias, padded, s.out.size(-1), s.out.scalar_type());
+    check_written(s.out, "out", {&s.q, &s.scale, &s.weight, &s.weight_scale, &bias});
+    one_device(s0.q, {&s.q, &s.scale, &s.weight, &s.weight_scale, &bias, &s.out});
+    void* p[6] = {pointer(s.q), pointer(s.scale), pointer(s.weight), pointer(s.weight_scale), pointer(bias), pointer(s.out)};
+    std::copy(p, p + 6, pointers + 6 * i);
+    strides[2 * i] = batch == 1 ? 0 : r.batch_stride;
+    strides[2 * i + 1] = r.rows == 1 ? 0 : r.row_stride;
+    rows[i++] = i32(r.rows, "rows");
+  }
+  require_hip(s0.q);
+  const at::OptionalDeviceGuard guard(s0.q.device());
+  check(hb_int8_linear(i, i32(batch, "batch"), rows, i32(s0.out.size(-1), "columns"), i32(padded, "padded"), dtype, gelu,
+                       pointers, strides, stream_of(s0.q.device())),
+        "hb_int8_linear");
+}
+
+void int8_linear(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
+                 const Maybe& bias, Tensor out, bool gelu) {
+  int8_linear_sets({{q, scale, weight, weight_scale, bias, out}}, gelu);
+}
+
+void int8_linear_pair(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
+                      const Maybe& bias, Tensor out, const Tensor& q2, const Tensor& scale2, const Tensor& weight2,
+                      const Tensor& weight_scale2, const Maybe& bias2, Tensor out2, bool gelu) {
+  int8_linear_sets({{q, scale, weight, weight_scale, bias, out}, {q2, scale2, weight2, weight_scale2, bias2, out2}}, gelu);
+}
+
+// The text set's tensors are given together or not at all (its bias and norms may be missing).
+void int8_qkv(const Maybe& text_q, const Maybe& text_scale, const Maybe& text_weight, const Maybe& text_weight_scale,
+              const Maybe& text_bias, const Maybe& text_norm_q, const Maybe& text_norm_k, const Tensor& q,
+              const Tensor& scale, const Tensor& weight, const Tensor& weight_scale, const Maybe& bias,
+              const Maybe& norm_q, const Maybe& norm_k, const Maybe& cos, const Maybe& sin, Tensor out, double eps) {
+  TORCH_CHECK_VALUE(out.dim() == 5 && out.size(0) == 3 && out.size(3) > 0 && out.size(4) == 128,
+                    "out must be [3, B, N, heads, 128]");
+  const int32_t dtype = type_of(out.scalar_type(), "out");
+  const int64_t batch = out.size(1), tokens = out.size(2), heads = out.size(3), columns = 3 * heads * 128;
+  TORCH_CHECK_VALUE(out.stride(4) == 1 && (heads == 1 || out.stride(3) == 128), "out must have contiguous heads");
+  const Tensor &tq = value_or_none(text_q), &ts = value_or_none(text_scale), &tw = value_or_none(text_weight),
+               &tws = value_or_none(text_weight_scale), &co = value_or_none(cos), &si = value_or_none(sin);
+  TORCH_CHECK_VALUE(tq.defined() == ts.defined() && tq.defined() == tw.defined() && tq.defined() == tws.defined(),
+                    "text rows, their scales and their weight are given together");
+  const int64_t padded = check_int8(q, scale, "image rows");
+  TORCH_CHECK_VALUE(q.dim() == 3 && q.size(0) == batch, "image rows must be [B, n, padded]");
+  int64_t text = 0;
+  void* pointers[14] = {};
+  for (int part = tq.defined() ? 0 : 1; part < 2; ++part) {
+    const Tensor &r = part ? q : tq, &rs = part ? scale : ts, &w = part ? weight : tw, &ws = part ? weight_scale : tws;
+    const Tensor& b = value_or_none(part ? bias : text_bias);
+    TORCH_CHECK_VALUE(check_int8(r, rs, "rows") == padded && r.dim() == 3 && r.size(0) == batch,
+                      "text and image rows must be [B, rows, padded] of one batch and feature count");
+    if (part == 0) text = r.size(1);
+    check_weight(w, ws, b, padded, columns, out.scalar_type());
+    void** p = pointers + 7 * part;
+    void* values[5] = {pointer(r), pointer(rs), pointer(w), pointer(ws), pointer(b)};
+    std::copy(values, values + 5, p);
+    for (int k = 0; k < 2; ++k) {
+      const Tensor& n = value_or_none(part ? (k ? norm_k : norm_q) : (k ? text_norm_k : text_norm_q));
+      TORCH_CHECK_VALUE(!n.defined() || (n.dim() == 1 && n.size(0) == 128 && n.is_contiguous() &&
+                                         n.scalar_type() == out.scalar_type()),
+                        "norm weights are contiguous [128] tensors of out's dtype");
+      p[5 + k] = pointer(n);
+      one_device(q, {&n});
+    }
+    one_device(q, {&r, &rs, &w, &ws, &b});
+    check_written(out, "out", {&r, &rs, &w, &ws, &b});
+  }
+  TORCH_CHECK_VALUE(text + q.size(1) == tokens, "out must hold the text rows and then the image rows");
+  TORCH_CHECK_VALUE(co.defined() == si.defined(), "cos and sin must be given together");
+  for (const Tensor* t : {&co, &si})
+    TORCH_CHECK_VALUE(!t->defined() || (t->dim() == 2 && t->size(0) == tokens && t->size(1) == 128 &&
+                                        t->is_contiguous() && t->scalar_type() == at::kFloat),
+                      "cos/sin must be contiguous float32 [N, 128]");
+  check_written(out, "out", {&co, &si});
+  one_device(q, {&co, &si, &out});
+  require_hip(q);
+  const at::OptionalDeviceGuard guard(q.device());
+  check(hb_int8_qkv(i32(batch, "batch"), i32(text, "text tokens"), i32(tokens, "tokens"), i32(heads, "heads"),
+                    i32(padded, "padded"), dtype, static_cast<float>(eps), pointers, static_cast<float*>(pointer(co)),
+                    static_cast<float*>(pointer(si)), out.data_ptr(), out.stride(0), batch == 1 ? 0 : out.stride(1),
+                    tokens == 1 ? 0 : out.stride(2), stream_of(q.device())),
+        "hb_int8_qkv");
+}
+
+// The attention operators and the 8-bit ones return nothing and write `out` and `lse` (and the like),
+// which torch's own boxed fallbacks overlook: they look after returned tensors only.
+
+constexpr const char* WRITING[] = {"paired_fwd", "sparse_fwd", "int8_rows", "int8_adaln", "int8_adaln_pair",
+                                   "int8_linear", "int8_linear_pair", "int8_qkv"};
 
 // No derivative is recorded (the entry points refuse inputs that need one); a transform that takes one
 // is refused, as torch refuses an autograd.Function in one, for it would get zeros.
-void attention_autograd(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+void no_derivative(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
   const size_t count = op.schema().arguments().size();
   // (included for as long as any torch.func transform is active)
   const bool transformed = at::GradMode::is_enabled() &&
@@ -310,7 +591,7 @@ void attention_autograd(const c10::OperatorHandle& op, c10::DispatchKeySet keys,
 
 // A tensor saved for a backward and then overwritten here has to fail that backward: every written
 // argument's version counts up.
-void attention_writes(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+void counts_writes(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
   const auto& arguments = op.schema().arguments();
   const auto values = torch::jit::last(stack, arguments.size());
   c10::SmallVector<Tensor, 2> written;
@@ -340,6 +621,23 @@ TORCH_LIBRARY(hilberta_hip, m) {
   m.def("pair_rows(Tensor kv_indices, Tensor kv_counts, SymInt total_blocks, SymInt key_block_size, "
         "SymInt paired_width) -> (Tensor, Tensor, Tensor)", tags);
   m.def("gather_rows(Tensor x, SymInt dim, Tensor index) -> Tensor", tags);
+  m.def("int8_rows(Tensor x, Tensor(a1!) q, Tensor(a2!) scale) -> ()", tags);
+  const std::string ada = "Tensor x$, Tensor shift$, Tensor scale$, Tensor? y$, Tensor? gate$, Tensor(x$!)? x_out$, "
+                          "Tensor(q$!) q$, Tensor(s$!) row_scale$, ",
+                    linear = "Tensor q$, Tensor scale$, Tensor weight$, Tensor weight_scale$, Tensor? bias$, "
+                             "Tensor(o$!) out$, ";
+  const auto set = [](std::string text, const std::string& suffix) {
+    for (size_t at; (at = text.find('$')) != std::string::npos;) text.replace(at, 1, suffix);
+    return text;
+  };
+  m.def(("int8_adaln(" + set(ada, "") + "float eps) -> ()").c_str(), tags);
+  m.def(("int8_adaln_pair(" + set(ada, "") + set(ada, "2") + "float eps) -> ()").c_str(), tags);
+  m.def(("int8_linear(" + set(linear, "") + "bool gelu) -> ()").c_str(), tags);
+  m.def(("int8_linear_pair(" + set(linear, "") + set(linear, "2") + "bool gelu) -> ()").c_str(), tags);
+  m.def("int8_qkv(Tensor? text_q, Tensor? text_scale, Tensor? text_weight, Tensor? text_weight_scale, "
+        "Tensor? text_bias, Tensor? text_norm_q, Tensor? text_norm_k, Tensor q, Tensor scale, Tensor weight, "
+        "Tensor weight_scale, Tensor? bias, Tensor? norm_q, Tensor? norm_k, Tensor? cos, Tensor? sin, "
+        "Tensor(a16!) out, float eps) -> ()", tags);
   m.def("_attention_workspace(Device device, int need) -> Tensor");
   m.def("_workspace_keys() -> int[]");
   m.def("_clear_workspaces() -> ()");
@@ -353,6 +651,18 @@ TORCH_LIBRARY_IMPL(hilberta_hip, CUDA, m) {
   m.impl("gather_rows", gather_rows);
 }
 
+// (on CPU tensors the 8-bit operators make their checks and refuse)
+void int8_operators(torch::Library& m) {
+  m.impl("int8_rows", int8_rows);
+  m.impl("int8_adaln", int8_adaln);
+  m.impl("int8_adaln_pair", int8_adaln_pair);
+  m.impl("int8_linear", int8_linear);
+  m.impl("int8_linear_pair", int8_linear_pair);
+  m.impl("int8_qkv", int8_qkv);
+}
+TORCH_LIBRARY_IMPL(hilberta_hip, CUDA, int8_hip) { int8_operators(int8_hip); }
+TORCH_LIBRARY_IMPL(hilberta_hip, CPU, int8_cpu) { int8_operators(int8_cpu); }
+
 TORCH_LIBRARY_IMPL(hilberta_hip, CompositeExplicitAutograd, m) {
   m.impl("_attention_workspace", attention_workspace);
   m.impl("_workspace_keys", workspace_keys);
@@ -364,11 +674,11 @@ TORCH_LIBRARY_IMPL(hilberta_hip, CompositeExplicitAutograd, m) {
 TORCH_LIBRARY_IMPL(hilberta_hip, Autograd, m) {
   for (const char* name : {"pair_rows", "gather_rows"})
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
-  for (const char* name : {"paired_fwd", "sparse_fwd"})
-    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&attention_autograd>());
+  for (const char* name : WRITING)
+    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&no_derivative>());
 }
 
 TORCH_LIBRARY_IMPL(hilberta_hip, ADInplaceOrView, m) {
-  for (const char* name : {"paired_fwd", "sparse_fwd"})
-    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&attention_writes>());
+  for (const char* name : WRITING)
+    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&counts_writes>());
 }

@@ -1,0 +1,187 @@
+"""The denoiser's linear layers in 8-bit integers (csrc/int8_rows.hip, csrc/int8_gemm.hip).
+
+Activations hold one scale a row (token), weights one a row (output channel): value = q * scale.
+
+  quantize_rows     16-bit rows to 8-bit rows:  scale = max|x| / 127,  q = rint(127 x / max|x|)
+  quantize_weight   the same over a [out, in] weight's channels
+  adaln_quantize    flux_norm.adaln_modulate straight into 8-bit rows
+  int8_linear       act(rows @ weight^T + bias),  act = none or GELU(tanh)
+  int8_qkv          the joint Q/K/V projection of [text; image] rows with the heads' RMSNorm of Q and K and
+                    the rotation in the same pass, written as the [B, N, H, 128] storage of each that the
+                    attention kernels read (flux_inputs.qk_prep_pair takes 16-bit projections instead)
+  adaln_quantize_pair, int8_linear_pair
+                    two row sets (a double block's image and text streams) in one launch
+
+The products are summed as whole numbers and what follows is fp32, rounded once to the 16-bit output; a
+row that holds an infinity or a NaN gives NaN.  Inference only: inputs that need a gradient are refused.
+Launches are asynchronous on the current stream, need no workspace and can be captured into a graph.
+The reference runs these layers in 16 bits (in the transformer that hilberta/flux_adapter.py wraps).
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib, ops
+
+HEAD_DIM = 128
+MAX_FEATURES = 1 << 17  # a sum of so many products fits 32 bits
+_DTYPES = (torch.bfloat16, torch.float16)
+
+
+def padded_features(features):
+    """Columns of 8-bit rows of ``features`` values: filled up with zeros to a multiple of 64."""
+    return -(-features // 64) * 64
+
+
+class Int8Rows(NamedTuple):
+    """Activations in 8 bits: q int8 [..., rows, padded_features(features)], zeros past ``features``, scale
+    float32 [..., rows]; ``dtype`` is that of the 16-bit rows they stand for, and of products with them."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+    features: int
+    dtype: torch.dtype
+
+
+class Int8Weight(NamedTuple):
+    """A linear layer's weight in 8 bits: q int8 [out_features, padded_features(features)], zeros past
+    ``features``, scale float32 [out_features]."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+    features: int
+
+
+def _inference(*tensors):
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]):
+        raise ValueError("Inference only; disable autograd")
+
+
+def _new_rows(x):
+    """Unwritten 8-bit rows for x [..., features]."""
+    if x.dtype not in _DTYPES:
+        raise ValueError("rows must be bf16 or fp16")
+    *lead, features = x.shape
+    if x.ndim not in (2, 3) or not 0 < features <= MAX_FEATURES:
+        raise ValueError(f"rows must be [rows, features] or [B, rows, features] of 1 to {MAX_FEATURES} features")
+    return Int8Rows(torch.empty(*lead, padded_features(features), dtype=torch.int8, device=x.device),
+                    torch.empty(lead, dtype=torch.float32, device=x.device), features, x.dtype)
+
+
+def quantize_rows(x):
+    """Int8Rows of 16-bit rows x [rows, features] or [B, rows, features] (contiguous last dimension)."""
+    _inference(x)
+    out = _new_rows(x)
+    if out.scale.numel() or not x.is_cuda:
+        ops.int8_rows(x, out.q, out.scale)
+    return out
+
+
+def quantize_weight(weight):
+    """Int8Weight of a 16-bit weight [out_features, in_features]."""
+    if weight.ndim != 2 or not weight.numel():
+        raise ValueError("weight must be a nonempty [out_features, in_features] matrix")
+    q, scale, features, _ = quantize_rows(weight.detach())
+    return Int8Weight(q, scale, features)
+
+
+def _adaln(x, shift, scale, y=None, gate=None, x_out=None):
+    _inference(x, shift, scale, y, gate, x_out)
+    if x.ndim != 3:
+        raise ValueError("x must be [B, rows, hidden] with a contiguous last dimension")
+    rows = _new_rows(x)
+    return (x, shift, scale, y, gate, x_out, rows.q, rows.scale), rows
+
+
+def adaln_quantize(x, shift, scale, *, y=None, gate=None, x_out=None, eps=1e-6):
+    """Int8Rows of shift + LayerNorm(r) * (1 + scale), r = x + gate * y, in one pass; r is stored in
+    ``x_out`` (which may be x) rounded, and normalised before that rounding.  Arguments as
+    flux_norm.adaln_modulate's; hidden is any multiple of 8 up to 8192."""
+    args, rows = _adaln(x, shift, scale, y, gate, x_out)
+    if rows.scale.numel() or not x.is_cuda:
+        ops.int8_adaln(*args, eps)
+    return rows
+
+
+def adaln_quantize_pair(first, second, *, eps=1e-6):
+    """adaln_quantize of two row sets in one launch: ``first`` and ``second`` are its arguments as dicts, of
+    one batch, hidden size, dtype and device.  Returns both Int8Rows."""
+    a, rows_a = _adaln(**first)
+    b, rows_b = _adaln(**second)
+    ops.int8_adaln_pair(*a, *b, eps)
+    return rows_a, rows_b
+
+
+def _rows(x):
+    return x if isinstance(x, Int8Rows) else quantize_rows(x)
+
+
+def _linear(x, weight, bias=None, out=None):
+    _inference(bias, out)
+    x = _rows(x)
+    q, scale, features, dtype = x
+    if weight.features != features:
+        raise ValueError(f"the weight takes {weight.features} features, the rows have {features}")
+    if out is None:
+        if dtype not in _DTYPES:
+            raise ValueError("rows must be bf16 or fp16")
+        out = torch.empty(*q.shape[:-1], weight.q.shape[0], dtype=dtype, device=q.device)
+    elif out.dtype != dtype:
+        raise ValueError("out must have the rows' dtype")
+    return (q, scale, weight.q, weight.scale, bias, out), out
+
+
+def int8_linear(x, weight, bias=None, *, gelu=False, out=None):
+    """act(x @ weight^T + bias) for x Int8Rows, or 16-bit rows that are quantized first, and an Int8Weight;
+    act is GELU(tanh) with ``gelu``.  bias [out_features] in the rows' dtype.  ``out`` [..., rows,
+    out_features] may be a row range or a column block of a larger buffer."""
+    args, out = _linear(x, weight, bias, out)
+    if out.numel() or not out.is_cuda:
+        ops.int8_linear(*args, gelu)
+    return out
+
+
+def int8_linear_pair(first, second, *, gelu=False):
+    """int8_linear of two row sets in one launch: ``first`` and ``second`` are dicts of x, weight, bias and
+    out, of one batch, layer shape, dtype and device.  Returns both outputs."""
+    a, out_a = _linear(**first)
+    b, out_b = _linear(**second)
+    ops.int8_linear_pair(*a, *b, gelu)
+    return out_a, out_b
+
+
+def int8_qkv(text, image, *, heads, weights, biases=(None, None), norms=((None, None), (None, None)), eps=1e-6,
+             cos=None, sin=None, out=None):
+    """[text; image] tokens -> out [3, B, T + n, heads, 128]: Q and K normalised and rotated, and V.
+
+    ``text`` [B, T, features] (or None: T = 0) and ``image`` [B, n, features] are Int8Rows, or 16-bit rows
+    that are quantized first; ``weights`` and ``biases`` = (text, image) are Int8Weights and biases of the
+    columns [Q | K | V], heads * 128 each; ``norms`` = ((q_text, q_image), (k_text, k_image)) the RMSNorm
+    weights [128] (None: no weight); cos/sin float32 [T + n, 128] in token order (None: no rotation)."""
+    image = _rows(image)
+    if text is not None:
+        text = _rows(text)
+        if text.features != image.features or text.dtype != image.dtype:
+            raise ValueError("text and image rows must share features and dtype")
+        if not text.q.shape[-2]:
+            text = None
+    (wt, wi), (bt, bi), ((qt, qi), (kt, ki)) = weights, biases, norms
+    if any([w.features != image.features for w in (wi,) + ((wt,) if text is not None else ())]):
+        raise ValueError("the weights must take the rows' features")
+    _inference(bt, bi, qt, qi, kt, ki, cos, sin, out)
+    if image.q.ndim != 3 or not image.q.shape[0] or not image.q.shape[1]:
+        raise ValueError("image must be nonempty [B, n, features] rows")
+    B, n = image.q.shape[:2]
+    N = n + (0 if text is None else text.q.shape[-2])
+    if out is None:
+        if image.dtype not in _DTYPES:
+            raise ValueError("rows must be bf16 or fp16")
+        out = torch.empty(3, B, N, heads, HEAD_DIM, dtype=image.dtype, device=image.q.device)
+    elif out.dtype != image.dtype:
+        raise ValueError("out must have the rows' dtype")
+    t = (None,) * 7 if text is None else (text.q, text.scale, wt.q, wt.scale, bt, qt, kt)
+    ops.int8_qkv(*t, image.q, image.scale, wi.q, wi.scale, bi, qi, ki, cos, sin, out, eps)
+    return out

@@ -13,13 +13,21 @@ implementation for tracing and, for pair_rows alone, a CPU one:
   hilberta_hip::gather_rows(x, dim, index) -> Tensor
   hilberta_hip::pair_rows(kv_indices, kv_counts, total_blocks, key_block_size, paired_width)
                            -> (ids, flags, counts)
+  hilberta_hip::int8_rows(x, q!, scale!) -> ()
+  hilberta_hip::int8_adaln(x, shift, scale, y?, gate?, x_out!?, q!, row_scale!, eps) -> ()
+  hilberta_hip::int8_linear(q, scale, weight, weight_scale, bias?, out!, gelu) -> ()
+  hilberta_hip::int8_qkv(text_q?, text_scale?, text_weight?, text_weight_scale?, text_bias?, text_norm_q?,
+                         text_norm_k?, q, scale, weight, weight_scale, bias?, norm_q?, norm_k?, cos?, sin?,
+                         out!, eps) -> ()
+  hilberta_hip::int8_adaln_pair, int8_linear_pair: two row sets' arguments (the second's names end in 2)
 
 The attention ops write into caller-provided outputs (declared mutated), as the reference's
 launches write into ``out``.  Argument checks with the reference's messages stay in the Python
 entry points (paired_attention, sparse_attention) and run before the op; the library repeats the
 cheap ones and reports them as ValueError.  The attention and gather ops have no CPU kernel: on
 CPU tensors they raise.  pair_rows is plan setup and also runs on CPU tensors, through the
-library's host table builder (hb_pair_rows_host, bit-identical to the device kernel).  Without the
+library's host table builder (hb_pair_rows_host, bit-identical to the device kernel).  The 8-bit ops
+(flux_int8.py) check their arguments on any device and refuse CPU tensors.  Without the
 built library the operators do not exist and every use of one raises.
 """
 
@@ -83,17 +91,19 @@ def _load():
                            f"include/hilberta_hip.h declares ABI {declared}: rebuild the libraries "
                            "(python -m hilberta_amd.build)")
     fakes = dict(paired_fwd=_fake_none, sparse_fwd=_fake_none, pair_rows=_fake_pair_rows,
-                 gather_rows=_fake_gather_rows)
+                 gather_rows=_fake_gather_rows, **dict.fromkeys(_INT8_NAMES, _fake_none))
     for name, fake in fakes.items():
         torch.library.register_fake(f"{_NS}::{name}", fake)
     torch.library.impl(f"{_NS}::pair_rows", "cpu", _pair_rows_cpu)
     return [getattr(getattr(torch.ops, _NS), name).default for name in _NAMES]
 
 
+_INT8_NAMES = ("int8_rows", "int8_adaln", "int8_adaln_pair", "int8_linear", "int8_linear_pair", "int8_qkv")
 _NAMES = ("paired_fwd", "sparse_fwd", "pair_rows", "gather_rows", "_attention_workspace",
-          "_workspace_keys", "_clear_workspaces")
+          "_workspace_keys", "_clear_workspaces", *_INT8_NAMES)
 try:
     _bound = _load()
 except (RuntimeError, OSError) as e:  # the package still imports, so that it can be (re)built
     _bound = [_Missing(name, str(e)) for name in _NAMES]
-paired_fwd, sparse_fwd, pair_rows, gather_rows, attention_workspace, workspace_keys, clear_workspaces = _bound
+(paired_fwd, sparse_fwd, pair_rows, gather_rows, attention_workspace, workspace_keys, clear_workspaces,
+ int8_rows, int8_adaln, int8_adaln_pair, int8_linear, int8_linear_pair, int8_qkv) = _bound

@@ -214,6 +214,57 @@ int hb_adaln_modulate_pair(int32_t batch, const int32_t* rows, int32_t hidden, i
                            float eps, void* const* pointers, const int64_t* strides,
                            hb_stream_t stream);
 
+/* ---------------------------------------------------------------- 8-bit linear layers
+ * No counterpart in the reference, which runs the linear layers of the transformer that
+ * hilberta/flux_adapter.py wraps in 16 bits.  Rows and weights are held as int8 [rows, padded], padded the
+ * features filled up with zeros to a multiple of 64, and one fp32 scale a row (a weight's rows are its
+ * output channels): value = q * scale.
+ *
+ * 16-bit rows to 8-bit rows: scale = max|x| / 127, q = rint(127 x / max|x|) (ties to even; a row of zeros
+ * is all zero with scale 0; a row with an infinity or a NaN gets the scale NaN).  x is [batch, rows,
+ * features] by element strides, last dimension contiguous, any alignment; q [batch * rows, padded] and
+ * scale [batch * rows] contiguous, q 16-byte aligned; features up to 2^17. */
+int hb_int8_rows(const void* x, int64_t batch_stride, int64_t row_stride, int32_t batch,
+                 int32_t rows, int32_t features, int32_t padded, int32_t dtype, int8_t* q,
+                 float* scale, hb_stream_t stream);
+
+/* Gated residual update + AdaLN modulation straight into 8-bit rows, for one or two row sets (count) of
+ * one batch, hidden size and type in one launch:
+ *   r = x + gate[b] * y   (skipped when y is NULL: r = x);  x_out = r rounded  (when not NULL; may be x)
+ *   q, row_scale = the 8-bit row of shift[b] + LayerNorm(r) * (1 + scale[b])   (no affine, eps)
+ * all in fp32: unlike hb_adaln_modulate nothing on the way to q is rounded to 16 bits.  Host arrays, set
+ * after set: rows [count]; pointers [count x 8] {x, y, gate, x_out, shift, scale, q, row_scale}; strides
+ * [count x 8] {x batch, x row, y batch, y row, gate batch, x_out batch, x_out row, shift and scale batch}.
+ * hidden a multiple of 8 up to 8192; pointers 16-byte aligned; strides multiples of 8. */
+int hb_int8_adaln(int32_t count, int32_t batch, const int32_t* rows, int32_t hidden,
+                  int32_t padded, int32_t dtype, float eps, void* const* pointers,
+                  const int64_t* strides, hb_stream_t stream);
+
+/* Linear layer of 8-bit rows with an 8-bit weight, for one or two row sets (count) of one batch and layer
+ * shape in one launch:
+ *   out[m, n] = act((sum_k q[m, k] weight[n, k]) * scale[m] * weight_scale[n] + bias[n])
+ * act = GELU(tanh) with gelu = 1, else none; sums in int32, the rest in fp32, one rounding.  Host arrays,
+ * set after set: rows [count]; pointers [count x 6] {q, scale, weight, weight_scale, bias or NULL, out};
+ * strides [count x 2] {out batch, out row}, elements.  q [batch * rows, padded], weight [columns, padded];
+ * q and weight 16-byte aligned.  Rows of out that are 16-byte aligned take 16-byte stores. */
+int hb_int8_linear(int32_t count, int32_t batch, const int32_t* rows, int32_t columns,
+                   int32_t padded, int32_t dtype, int32_t gelu, void* const* pointers,
+                   const int64_t* strides, hb_stream_t stream);
+
+/* Joint Q/K/V projection of 8-bit rows with the heads' RMSNorm and rotation in the same pass:
+ *   p = as hb_int8_linear with columns [Q | K | V] of heads * 128 each
+ *   out[0], out[1] (Q, K): p * rsqrt(mean(p^2) + eps) * norm over each head, pairs (2i, 2i + 1) rotated by
+ *   cos/sin as hb_qk_prep rotates;  out[2] (V): p
+ * all in fp32 with one rounding.  Tokens t < text_tokens of a batch element are the text set's rows, the
+ * others the image set's; out[plane][b, t] holds heads * 128 contiguous values (element strides, multiples
+ * of 8).  pointers: host array [2 x 7], text then image (text unread when text_tokens is 0): {q, scale,
+ * weight, weight_scale, bias or NULL, norm_q or NULL, norm_k or NULL}, norms [128] 16-bit.  cos/sin: fp32
+ * [tokens, 128] or both NULL.  out, cos, sin 16-byte aligned. */
+int hb_int8_qkv(int32_t batch, int32_t text_tokens, int32_t tokens, int32_t heads, int32_t padded,
+                int32_t dtype, float eps, void* const* pointers, const float* cos,
+                const float* sin, void* out, int64_t out_plane_stride, int64_t out_batch_stride,
+                int64_t out_row_stride, hb_stream_t stream);
+
 /* ---------------------------------------------------------------- (b) block tables
  * Hilbert order of a grid_size x grid_size raster (reference hilberta/geometry.py:6-25). */
 int hb_hilbert_order(int32_t grid_size, int64_t* out, hb_stream_t stream);
