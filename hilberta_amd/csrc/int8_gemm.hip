@@ -42,7 +42,8 @@ struct Set {
 struct Args {
   Set set[2];
   int32_t columns, padded;
-  uint32_t tiles0, channel_tiles;  // tiles of set 0; tiles along the channels
+  uint32_t tiles0, tiles, tiles_xcd;  // tiles of set 0, of all, and of an XCD
+  uint32_t channel_tiles;             // tiles along the channels
   int32_t gelu, vectors;           // vectors: every output row takes 16-byte stores
   const float* cos;                // qkv: [rows of both sets, 128] or null
   const float* sin;
@@ -68,20 +69,60 @@ __device__ __forceinline__ u32x4 pack_pair(const float (&even)[4], const float (
   return u32x4{lo[0], hi[0], lo[1], hi[1]};
 }
 
-constexpr int TC = 128, TT = 128;  // channels and tokens of a workgroup's tile
+typedef __attribute__((address_space(3))) void* lds_ptr;
 
-// Four waves, 128 channels x 32 tokens each, operands straight from memory.
-template <bool F16, bool QKV>
-__global__ __launch_bounds__(256) void int8_product_kernel(Args a) {
+// word 3 of a raw buffer resource (32-bit data format, no swizzle)
+constexpr int BUFFER_WORD3 = 0x00020000;
+
+// 16 bytes a lane from base + voffset + soffset into LDS at dst + 16 lane.  (The buffer resource type exists
+// for the device target only; the host pass sees an empty body.)
+__device__ __forceinline__ void load_lds16(const void* base, void* dst, int voffset, int soffset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const __amdgpu_buffer_rsrc_t rsrc =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, BUFFER_WORD3);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)dst, 16, voffset, soffset, 0, 0);
+#endif
+}
+
+// s_waitcnt vmcnt(N) lgkmcnt(0)
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0070);
+}
+
+// A barrier that no access to LDS is moved across.
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+constexpr int TC = 128, TT = 256;              // channels and tokens of a workgroup's tile
+constexpr int STEP = 64;                       // features of a stage: bytes of an LDS row
+constexpr int STAGE = (TC + TT) * STEP;        // 24 KB
+constexpr int LOADS = STAGE / 1024 / 4;        // 1 KB loads of a wave and stage
+constexpr int BAND = 8;                        // token tiles walked together
+
+template <bool F16, bool QKV, bool GELU>
+__global__ __launch_bounds__(256, 2) void int8_product_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds0[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds1[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds2[STAGE];
   __shared__ __attribute__((aligned(16))) float channel[3][TC];  // weight scale, bias, head norm
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
-  uint32_t tile = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+  // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, in bands of BAND token tiles
+  // walked channel tile by channel tile, so that its L2 serves a patch of both operands.
+  uint32_t tile = (blockIdx.x & 7) * a.tiles_xcd + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= a.tiles_xcd || tile >= a.tiles) return;
   const bool second = tile >= a.tiles0;
   const Set& s = a.set[second];
   if (second) tile -= a.tiles0;
-  const uint32_t tt = tile / a.channel_tiles;
-  const int c0 = (tile - tt * a.channel_tiles) * TC;
-  const uint32_t t0 = tt * TT + wave * 32;
+  const uint32_t token_tiles = (s.tokens + TT - 1) / TT;
+  const uint32_t band = tile / (BAND * a.channel_tiles), in_band = tile - band * (BAND * a.channel_tiles);
+  const uint32_t height = min((uint32_t)BAND, token_tiles - band * BAND);
+  const uint32_t ct = in_band / height;
+  const int c0 = ct * TC;
+  const uint32_t t0 = (band * BAND + in_band - ct * height) * TT;
   const int plane = QKV ? c0 / (a.heads * HEAD) : 2;
   for (int i = threadIdx.x; i < TC; i += 256) {
     const int c = min(c0 + i, a.columns - 1);
@@ -89,89 +130,158 @@ __global__ __launch_bounds__(256) void int8_product_kernel(Args a) {
     channel[1][i] = s.bias ? to_f<F16>(s.bias[c]) : 0.f;
     channel[2][i] = QKV && plane < 2 && s.norm[plane] ? to_f<F16>(s.norm[plane][i]) : 1.f;
   }
-  const uint32_t token = min(t0 + col, s.tokens - 1);
-  const int8_t* qp = s.q + (int64_t)token * a.padded + half * 16;
-  const int8_t* wp[4];
+  // Loads: a wave's load j fills LDS rows 16 (4 j + wave) .. + 15, four lanes a row of 64 bytes; rows below
+  // TC are channels, the others tokens.  The lane at slot p of row r loads chunk p ^ (r / 4 % 4), so that
+  // the 16 rows whose chunks a quarter of a wave reads together lie in different banks.
+  const int8_t* wbase = s.w + (int64_t)c0 * a.padded;
+  const int8_t* qbase = s.q + (int64_t)t0 * a.padded;
+  int offset[LOADS];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) wp[i] = s.w + (int64_t)min(c0 + i * 32 + col, a.columns - 1) * a.padded + half * 16;
-  i32x16 acc[4] = {};
-  for (int k = 0; k < a.padded; k += 32) {
-    const i32x4 x = *(const i32x4*)(qp + k);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      acc[i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const i32x4*)(wp[i] + k), x, acc[i], 0, 0, 0);
+  for (int j = 0; j < LOADS; ++j) {
+    const int r = 16 * (4 * j + wave) + (lane >> 2);
+    const int chunk = (lane & 3) ^ (r >> 2 & 3);
+    const int row = 4 * j < TC / 16 ? min(r, a.columns - 1 - c0) : (int)min((uint32_t)(r - TC), s.tokens - 1 - t0);
+    offset[j] = row * a.padded + chunk * 16;
   }
-  __syncthreads();
-  const float scale = s.scale[token];
-  float v[4][16];
-  float squares = 0.f;
+  const int stages = a.padded / STEP;
+  auto load = [&](int8_t* dst, int stage) {
+    const int at = min(stage, stages - 1) * STEP;  // (past the end: the last stage again, never read)
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < LOADS; ++j)
+      load_lds16(4 * j < TC / 16 ? wbase : qbase, dst + 1024 * (4 * j + wave), offset[j], at);
+  };
+  // Operands: lane l holds bytes 16 (l / 32) .. + 15 of a 32-byte step of row l % 32.
+  const int swizzle = (col >> 2 & 3) ^ half;
+  const int read = col * STEP + swizzle * 16;
+  i32x4 w[2][4], x[2][2];
+  auto fetch = [&](const int8_t* src, int u) {
+    const int at = read ^ (u * 32);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int c = i * 32 + (r >> 2) * 8 + half * 4 + (r & 3);
-      v[i][r] = (float)acc[i][r] * scale * channel[0][c] + channel[1][c];
-      if (QKV) squares += v[i][r] * v[i][r];
-      else if (a.gelu) v[i][r] = gelu(v[i][r]);
-    }
-  const bool inside = t0 + col < s.tokens;
-  const uint32_t b = token / s.rows, n = token - b * s.rows;
-  uint16_t* out = s.out + b * s.out_b + (int64_t)n * s.out_n;
-  if (QKV) {
-    out += plane * a.out_p + (c0 - plane * a.heads * HEAD);
-    if (plane < 2) {
-      squares += __shfl_xor(squares, 32, 64);
-      const float rms = __builtin_amdgcn_rsqf(squares * (1.f / HEAD) + a.eps);
+    for (int i = 0; i < 4; ++i) w[u][i] = *(const i32x4*)(src + i * 32 * STEP + at);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) x[u][j] = *(const i32x4*)(src + (TC + wave * 64 + j * 32) * STEP + at);
+  };
+  i32x16 acc[4][2] = {};
+  auto multiply = [&](int u) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[u][i], x[u][j], acc[i][j], 0, 0, 0);
+  };
+  // Stage n is in `cur`, its first operands in w[0], x[0]; stage n + 1 is on its way to `next`.  The barrier
+  // says that everyone's part of it is there, and that nobody still reads `cur`, which stage n + 3 will fill.
+  auto step = [&](int8_t* cur, int8_t* next, int8_t* last, int n) {
+    load(last, n + 2);
+    fetch(cur, 1);
+    multiply(0);
+    wait_loads<LOADS>();
+    barrier();
+    fetch(next, 0);
+    multiply(1);
+  };
+  load(lds0, 0);
+  load(lds1, 1);
+  wait_loads<LOADS>();
+  __syncthreads();
+  fetch(lds0, 0);
+  for (int n = 0;;) {
+    step(lds0, lds1, lds2, n);
+    if (++n == stages) break;
+    step(lds1, lds2, lds0, n);
+    if (++n == stages) break;
+    step(lds2, lds0, lds1, n);
+    if (++n == stages) break;
+  }
+  wait_loads<0>();  // (nothing may still be on its way to LDS when the workgroup ends)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int c = i * 32 + g * 8 + half * 4;
-          float x[4];
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t at = t0 + wave * 64 + j * 32 + col, token = min(at, s.tokens - 1);
+    const float scale = s.scale[token];
+    const uint32_t b = token / s.rows, n = token - b * s.rows;
+    uint16_t* out = s.out + b * s.out_b + (int64_t)n * s.out_n;
+    const float *co = nullptr, *si = nullptr;
+    float v[4][16];
+    float squares = 0.f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = v[i][g * 4 + k] * rms * channel[2][c + k];
-          if (a.cos) {
-            const int64_t at = (int64_t)(s.first + n) * HEAD + c;
-            const f32x4 co = *(const f32x4*)(a.cos + at), si = *(const f32x4*)(a.sin + at);
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; k += 2) {
-              v[i][g * 4 + k] = x[k] * co[k] - x[k + 1] * si[k];
-              v[i][g * 4 + k + 1] = x[k + 1] * co[k + 1] + x[k] * si[k + 1];
+      for (int g = 0; g < 4; ++g) {
+        const int c = i * 32 + g * 8 + half * 4;
+        const f32x4 ws = *(const f32x4*)&channel[0][c], bias = *(const f32x4*)&channel[1][c];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float p = (float)acc[i][j][g * 4 + k] * scale * ws[k] + bias[k];
+          if (QKV) squares += p * p;
+          if (GELU) p = gelu(p);
+          v[i][g * 4 + k] = p;
+        }
+      }
+    if (QKV) {
+      out += plane * a.out_p + (c0 - plane * a.heads * HEAD);
+      if (plane < 2) {
+        squares += __shfl_xor(squares, 32, 64);
+        const float rms = __builtin_amdgcn_rsqf(squares * (1.f / HEAD) + a.eps);
+        co = a.cos ? a.cos + (int64_t)(s.first + n) * HEAD : nullptr;
+        si = a.cos ? a.sin + (int64_t)(s.first + n) * HEAD : nullptr;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int c = i * 32 + g * 8 + half * 4;
+            const f32x4 norm = *(const f32x4*)&channel[2][c];
+            float y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = v[i][g * 4 + k] * rms * norm[k];
+            if (a.cos) {
+              const f32x4 cv = *(const f32x4*)(co + c), sv = *(const f32x4*)(si + c);
+#pragma unroll
+              for (int k = 0; k < 4; k += 2) {
+                v[i][g * 4 + k] = y[k] * cv[k] - y[k + 1] * sv[k];
+                v[i][g * 4 + k + 1] = y[k + 1] * cv[k + 1] + y[k] * sv[k + 1];
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[i][g * 4 + k] = y[k];
             }
+          }
+      }
+    } else {
+      out += c0;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        float even[4], odd[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          even[k] = v[i][8 * p + k];
+          odd[k] = v[i][8 * p + 4 + k];
+        }
+        const u32x4 packed = pack_pair<F16>(even, odd);
+        const int c = i * 32 + p * 16 + half * 8;
+        if (at < s.tokens) {
+          if (QKV || (a.vectors && c0 + c + 8 <= a.columns)) {
+            *(u32x4*)(out + c) = packed;
           } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[i][g * 4 + k] = x[k];
+            for (int k = 0; k < 8; ++k)
+              if (c0 + c + k < a.columns) out[c + k] = (uint16_t)(packed[k >> 1] >> (16 * (k & 1)));
           }
         }
-    }
-  } else {
-    out += c0;
+      }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      float even[4], odd[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        even[k] = v[i][8 * p + k];
-        odd[k] = v[i][8 * p + 4 + k];
-      }
-      const u32x4 packed = pack_pair<F16>(even, odd);
-      const int c = i * 32 + p * 16 + half * 8;
-      if (inside) {
-        if (QKV || (a.vectors && c0 + c + 8 <= a.columns)) {
-          *(u32x4*)(out + c) = packed;
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (c0 + c + k < a.columns) out[c + k] = (uint16_t)(packed[k >> 1] >> (16 * (k & 1)));
-        }
-      }
-    }
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <bool F16, bool QKV>
+void launch_type(const Args& a, hipStream_t st) {
+  const dim3 grid(8 * a.tiles_xcd), block(256);
+  if (a.gelu) hipLaunchKernelGGL((int8_product_kernel<F16, QKV, !QKV>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((int8_product_kernel<F16, QKV, false>), grid, block, 0, st, a);
+}
 
 template <bool QKV>
 int launch(Args& a, int count, int32_t dtype, hipStream_t st) {
@@ -179,12 +289,13 @@ int launch(Args& a, int count, int32_t dtype, hipStream_t st) {
   int64_t tiles = 0;
   for (int i = 0; i < count; ++i) {
     tiles += (int64_t)((a.set[i].tokens + TT - 1) / TT) * a.channel_tiles;
-    HB_REQUIRE(tiles < (1ll << 31), "too many output tiles for one launch");
+    HB_REQUIRE(tiles < (1ll << 30), "too many output tiles for one launch");
     if (i == 0) a.tiles0 = (uint32_t)tiles;
   }
-  const dim3 grid((unsigned)tiles), block(256);
-  if (dtype == HB_DTYPE_F16) hipLaunchKernelGGL((int8_product_kernel<true, QKV>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((int8_product_kernel<false, QKV>), grid, block, 0, st, a);
+  a.tiles = (uint32_t)tiles;
+  a.tiles_xcd = (a.tiles + 7) / 8;
+  if (dtype == HB_DTYPE_F16) launch_type<true, QKV>(a, st);
+  else launch_type<false, QKV>(a, st);
   HB_HIP(hipGetLastError());
   return HB_OK;
 }
