@@ -13,6 +13,10 @@
 // columns: a lane then holds one token's values, 4 consecutive channels an accumulator quarter, so that a
 // token's scale is one register, a rotated pair lies in one lane, and a head's 128 channels in the lanes l
 // and l + 32.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
 #include "common.h"
 #include "../../include/hilberta_hip.h"
 
@@ -84,7 +88,13 @@ __device__ __forceinline__ void load_lds16(const void* base, void* dst, int voff
 #endif
 }
 
-// s_waitcnt vmcnt(N) lgkmcnt(0)
+// s_waitcnt vmcnt(N): all but the last N loads have arrived.
+template <int N>
+__device__ __forceinline__ void wait_arrivals() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);
+}
+
+// The same, and this wave's reads of LDS.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0070);
@@ -97,208 +107,676 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
-constexpr int TC = 128, TT = 256;              // channels and tokens of a workgroup's tile
-constexpr int STEP = 64;                       // features of a stage: bytes of an LDS row
-constexpr int STAGE = (TC + TT) * STEP;        // 24 KB
-constexpr int LOADS = STAGE / 1024 / 4;        // 1 KB loads of a wave and stage
-constexpr int BAND = 8;                        // token tiles walked together
+// ------------------------------------------------------------------ what every kernel does with its sums
+// The epilogue's values of a tile's channels, in LDS: weight scale, bias, head norm.
+template <bool F16, bool QKV, int TC>
+__device__ __forceinline__ void load_channels(const Args& a, const Set& s, int c0, float (&channel)[3][TC]) {
+  const int i = threadIdx.x;
+  if (i >= TC) return;
+  const int c = min(c0 + i, a.columns - 1);
+  const int plane = QKV ? c / (a.heads * HEAD) : 2;
+  channel[0][i] = s.w_scale[c];
+  channel[1][i] = s.bias ? to_f<F16>(s.bias[c]) : 0.f;
+  channel[2][i] = QKV && plane < 2 && s.norm[plane] ? to_f<F16>(s.norm[plane][i & (HEAD - 1)]) : 1.f;
+}
 
-template <bool F16, bool QKV, bool GELU>
-__global__ __launch_bounds__(256, 2) void int8_product_kernel(Args a) {
-  __shared__ __attribute__((aligned(1024))) int8_t lds0[STAGE];
-  __shared__ __attribute__((aligned(1024))) int8_t lds1[STAGE];
-  __shared__ __attribute__((aligned(1024))) int8_t lds2[STAGE];
-  __shared__ __attribute__((aligned(16))) float channel[3][TC];  // weight scale, bias, head norm
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-  // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, in bands of BAND token tiles
-  // walked channel tile by channel tile, so that its L2 serves a patch of both operands.
-  uint32_t tile = (blockIdx.x & 7) * a.tiles_xcd + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= a.tiles_xcd || tile >= a.tiles) return;
-  const bool second = tile >= a.tiles0;
-  const Set& s = a.set[second];
-  if (second) tile -= a.tiles0;
-  const uint32_t token_tiles = (s.tokens + TT - 1) / TT;
+// Where token `at` of a set (clamped to its last) goes, in elements from s.out.
+__device__ __forceinline__ int64_t row_of(const Set& s, uint32_t at) {
+  const uint32_t token = min(at, s.tokens - 1), b = token / s.rows;
+  return b * s.out_b + (int64_t)(token - b * s.rows) * s.out_n;
+}
+
+// Eight values of channels c .. c + 7 to `out`, those of them that there are.
+template <bool QKV>
+__device__ __forceinline__ void store8(const Args& a, uint16_t* out, int c, const u32x4& v) {
+  if (QKV ? c < a.columns : (a.vectors && c + 8 <= a.columns)) {
+    __builtin_nontemporal_store(v, (u32x4*)out);
+  } else if (!QKV) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + k < a.columns) out[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
+  }
+}
+
+// Pairs (2i, 2i + 1) of N values turned by cos and sin.
+template <int N>
+__device__ __forceinline__ void rotate(float (&v)[N], const float* cos, const float* sin) {
+#pragma unroll
+  for (int g = 0; g < N; g += 4) {
+    const f32x4 c = *(const f32x4*)(cos + g), s = *(const f32x4*)(sin + g);
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+      const float even = v[g + k], odd = v[g + k + 1];
+      v[g + k] = even * c[k] - odd * s[k];
+      v[g + k + 1] = odd * c[k + 1] + even * s[k + 1];
+    }
+  }
+}
+
+// The epilogue of a wave's 32 tokens from t0 on and 32 CF channels from c0 on (qkv: one head, CF = 4);
+// `channel` are those channels' values, TC apart.  Lanes l and l + 32 hold token t0 + l % 32.  After
+// pack_pair a 32-channel block of a token is four 16-byte chunks, two in each of those lanes; exchanged with
+// the lane 16 on, four lanes hold a token's four chunks, and a store writes 64 bytes a row (32 without: 16896
+// x 3072 x 12288 586 -> 580 us).  The stores bypass the caches (580 -> 571): the output is larger than they
+// are, and what they hold is wanted by the tiles to come.
+template <bool F16, bool QKV, bool GELU, int CF, int TC>
+__device__ __forceinline__ void finish(const Args& a, const Set& s, const i32x16 (&acc)[CF], float scale,
+                                       const float* channel, int c0, uint32_t t0) {
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int plane = QKV ? c0 / (a.heads * HEAD) : 2;
+  const int chunk = (lane >> 4 & 1) * 2 + half;
+  uint16_t* out[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    out[h] = s.out + row_of(s, t0 + h * 16 + (lane & 15)) + (QKV ? plane * a.out_p - plane * a.heads * HEAD : 0) + c0 + chunk * 8;
+  channel += half * 4;
+  auto value = [&](int i, int r) {
+    const int c = i * 32 + (r >> 2) * 8 + (r & 3);
+    return (float)acc[i][r] * scale * channel[c] + channel[TC + c];
+  };
+  const bool heads = QKV && plane < 2;
+  float rms = 1.f;
+  int64_t table = 0;
+  if (heads) {
+    float squares = 0.f;
+#pragma unroll
+    for (int i = 0; i < CF; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = value(i, r);
+        squares += p * p;
+      }
+    squares += __shfl_xor(squares, 32, 64);
+    rms = __builtin_amdgcn_rsqf(squares * (1.f / HEAD) + a.eps);
+    table = (int64_t)(s.first + min(t0 + col, s.tokens - 1) % s.rows) * HEAD + half * 4;
+  }
+#pragma unroll
+  for (int i = 0; i < CF; ++i) {
+    u32x4 packed[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      float v[2][4];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int c = i * 32 + (2 * p + g) * 8;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float y = value(i, 8 * p + 4 * g + k);
+          if (GELU) y = gelu(y);
+          if (heads) y *= rms * channel[2 * TC + c + k];
+          v[g][k] = y;
+        }
+        if (heads && a.cos) rotate(v[g], a.cos + table + c, a.sin + table + c);
+      }
+      packed[p] = pack_pair<F16>(v[0], v[1]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const auto both = __builtin_amdgcn_permlane16_swap(packed[0][k], packed[1][k], false, false);
+      packed[0][k] = both[0];
+      packed[1][k] = both[1];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (t0 + h * 16 + (lane & 15) < s.tokens) store8<QKV>(a, out[h] + i * 32, c0 + i * 32 + chunk * 8, packed[h]);
+    __builtin_amdgcn_sched_barrier(0);  // (a block at a time: all at once take more registers than there are)
+  }
+}
+
+// Which tile a workgroup takes.
+struct Tile {
+  int set, c0;
+  uint32_t t0;
+};
+
+// Tiles walk bands of `BAND` token tiles, channel tile by channel tile.
+template <int TC, int TT, int BAND>
+__device__ __forceinline__ Tile tile_at(const Args& a, uint32_t tile) {
+  const int set = tile >= a.tiles0;
+  if (set) tile -= a.tiles0;
+  const uint32_t token_tiles = (a.set[set].tokens + TT - 1) / TT;
   const uint32_t band = tile / (BAND * a.channel_tiles), in_band = tile - band * (BAND * a.channel_tiles);
   const uint32_t height = min((uint32_t)BAND, token_tiles - band * BAND);
-  const uint32_t ct = in_band / height;
-  const int c0 = ct * TC;
-  const uint32_t t0 = (band * BAND + in_band - ct * height) * TT;
-  const int plane = QKV ? c0 / (a.heads * HEAD) : 2;
-  for (int i = threadIdx.x; i < TC; i += 256) {
-    const int c = min(c0 + i, a.columns - 1);
-    channel[0][i] = s.w_scale[c];
-    channel[1][i] = s.bias ? to_f<F16>(s.bias[c]) : 0.f;
-    channel[2][i] = QKV && plane < 2 && s.norm[plane] ? to_f<F16>(s.norm[plane][i]) : 1.f;
+  const uint32_t c = in_band / height;
+  return {set, (int)c * TC, (band * BAND + in_band - c * height) * TT};
+}
+
+// Where rows end.  A stage is 128 features, and rows a multiple of 64: what a lane's load asks for past the row
+// (its chunk of a last half stage, or a stage after the last) is moved outside the buffer, from where a load
+// brings zeros and reads nothing.
+struct Ends {
+  int full, beyond;  // whole stages, and what the stage after them adds to this lane's offset
+  __device__ Ends(int padded, int chunk)
+      : full(padded >> 7), beyond((padded & 64) && chunk < 4 ? 0 : (int)0x80000000) {}
+  __device__ int past(int stage) const {
+    return stage < full ? 0 : stage == full ? beyond : (int)0x80000000;
   }
-  // Loads: a wave's load j fills LDS rows 16 (4 j + wave) .. + 15, four lanes a row of 64 bytes; rows below
-  // TC are channels, the others tokens.  The lane at slot p of row r loads chunk p ^ (r / 4 % 4), so that
-  // the 16 rows whose chunks a quarter of a wave reads together lie in different banks.
-  const int8_t* wbase = s.w + (int64_t)c0 * a.padded;
-  const int8_t* qbase = s.q + (int64_t)t0 * a.padded;
-  int offset[LOADS];
+};
+
+// ------------------------------------------------------------------ many rows
+// 256 channels x 256 tokens a workgroup of eight waves, 128 x 64 each; one workgroup a CU, which walks its
+// tiles.  Bound by the loads: the same kernel without them runs at 3.0 PFLOP/s, with them at 2.4.  So the tile
+// is as large as the registers allow (128 x 256 tiles, two workgroups a CU, move half as much again), and a
+// stage is 128 features deep: a row's 128 bytes are one request to the L2 (64-byte rows, twice as many
+// requests, took that kernel from 2.4 to 1.9 PFLOP/s).
+//  * Two stages of 64 KB in LDS, by direct loads: stage n + 2 is asked for as soon as everyone has read stage n
+//    into registers, and has the whole of stage n + 1 (2048 cycles of products) to arrive.
+//  * The operands of a 32-feature step are read while the step before multiplies; the scheduler is held to
+//    that order (left alone it reads them just before their use: 2.25 instead of 2.44 PFLOP/s).
+//  * The last two stages of a tile ask for the first two of the next, which the epilogue then hides.
+//  * An XCD takes a run of the tiles, four token tiles by eight channel tiles at a time (bands of 8 token
+//    tiles: 16896 x 3072 x 12288 630 us, of 4: 586), so that its L2 serves both operands.
+constexpr int WIDE = 256, WIDE_STEP = 128, WIDE_BAND = 4;
+constexpr int WIDE_STAGE = 2 * WIDE * WIDE_STEP;     // 64 KB
+constexpr int WIDE_LOADS = WIDE_STAGE / 1024 / 8;    // 1 KB loads of a wave and stage
+
+__device__ __forceinline__ const int8_t* uniform_pointer(const int8_t* p) {
+  const uint64_t v = (uint64_t)p;
+  return (const int8_t*)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+
+template <bool F16, bool QKV, bool GELU>
+__global__ __launch_bounds__(512, 2) void int8_wide_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds0[WIDE_STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds1[WIDE_STAGE];
+  __shared__ __attribute__((aligned(16))) float channel[2][3][WIDE];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+  const int wc = wave & 1, wt = wave >> 1;
+  const int stages = (a.padded + 2 * WIDE_STEP - 1) / (2 * WIDE_STEP) * 2;  // (an even number)
+  // (workgroups go to the eight XCDs in turn)
+  const uint32_t first = (blockIdx.x & 7) * a.tiles_xcd, stride = gridDim.x >> 3;
+  uint32_t slot = blockIdx.x >> 3;
+  if (slot >= a.tiles_xcd || first + slot >= a.tiles) return;
+  // Loads: a wave's load j fills LDS rows 8 (8 j + wave) .. + 7, eight lanes a row; rows below WIDE are
+  // channels, the others tokens (rows past the operands' ends: the last ones again).  The lane at slot p of
+  // row r loads chunk p ^ (r / 2 % 8), so that the chunks that 16 rows' lanes read together lie in
+  // different banks.
+  const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+  const Ends ends(a.padded, chunk);
+  const int8_t *wbase, *qbase;
+  int offset[WIDE_LOADS];
+  auto aim = [&](const Tile& t) {
+    const Set& s = a.set[t.set];
+    wbase = uniform_pointer(s.w + (int64_t)t.c0 * a.padded);
+    qbase = uniform_pointer(s.q + (int64_t)t.t0 * a.padded);
 #pragma unroll
-  for (int j = 0; j < LOADS; ++j) {
-    const int r = 16 * (4 * j + wave) + (lane >> 2);
-    const int chunk = (lane & 3) ^ (r >> 2 & 3);
-    const int row = 4 * j < TC / 16 ? min(r, a.columns - 1 - c0) : (int)min((uint32_t)(r - TC), s.tokens - 1 - t0);
-    offset[j] = row * a.padded + chunk * 16;
-  }
-  const int stages = a.padded / STEP;
-  auto load = [&](int8_t* dst, int stage) {
-    const int at = min(stage, stages - 1) * STEP;  // (past the end: the last stage again, never read)
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j)
-      load_lds16(4 * j < TC / 16 ? wbase : qbase, dst + 1024 * (4 * j + wave), offset[j], at);
+    for (int j = 0; j < WIDE_LOADS; ++j) {
+      const int r = 8 * (8 * j + wave) + (lane >> 3);
+      const int row = 64 * j < WIDE ? min(r, a.columns - 1 - t.c0) : (int)min((uint32_t)(r - WIDE), s.tokens - 1 - t.t0);
+      offset[j] = row * a.padded + chunk * 16;
+    }
+  };
+  auto load = [&](int8_t* dst, int stage, int j, int past) {
+    load_lds16(64 * j < WIDE ? wbase : qbase, dst + 1024 * (8 * j + wave), offset[j] | past, uniform(stage * WIDE_STEP));
   };
   // Operands: lane l holds bytes 16 (l / 32) .. + 15 of a 32-byte step of row l % 32.
-  const int swizzle = (col >> 2 & 3) ^ half;
-  const int read = col * STEP + swizzle * 16;
+  const int read = col * WIDE_STEP + ((col >> 1 & 7) ^ half) * 16;
   i32x4 w[2][4], x[2][2];
   auto fetch = [&](const int8_t* src, int u) {
     const int at = read ^ (u * 32);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[u][i] = *(const i32x4*)(src + i * 32 * STEP + at);
+    for (int i = 0; i < 4; ++i) w[u & 1][i] = *(const i32x4*)(src + (wc * 128 + i * 32) * WIDE_STEP + at);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) x[u][j] = *(const i32x4*)(src + (TC + wave * 64 + j * 32) * STEP + at);
+    for (int j = 0; j < 2; ++j) x[u & 1][j] = *(const i32x4*)(src + (WIDE + wt * 64 + j * 32) * WIDE_STEP + at);
   };
-  i32x16 acc[4][2] = {};
-  auto multiply = [&](int u) {
+  i32x16 acc[2][4];
+  auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
+  // Eight products, with loads `from` .. `from` + 3 of a stage to `dst` among them.
+  auto multiply = [&](int u, int8_t* dst = nullptr, int stage = 0, int from = 0) {
+    const int past = dst ? ends.past(uniform(stage)) : 0;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[u][i], x[u][j], acc[i][j], 0, 0, 0);
+      for (int i = 0; i < 4; ++i) {
+        acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[u][i], x[u][j], acc[j][i], 0, 0, 0);
+        if (dst && i & 1) {
+          pin();
+          load(dst, stage, from + 2 * j + i / 2, past);
+          pin();
+        }
+      }
+    pin();
   };
-  // Stage n is in `cur`, its first operands in w[0], x[0]; stage n + 1 is on its way to `next`.  The barrier
-  // says that everyone's part of it is there, and that nobody still reads `cur`, which stage n + 3 will fill.
-  auto step = [&](int8_t* cur, int8_t* next, int8_t* last, int n) {
-    load(last, n + 2);
+  // A stage in `cur`, its first operands on their way to w[0], x[0], half of the next in `next` and the other
+  // half asked for here.  Before the barrier everyone's part of `next` is there and nobody reads `cur` any
+  // more, of which `after` then fills half.
+  auto step = [&](int8_t* cur, int8_t* next, int stage, int after, bool last) {
     fetch(cur, 1);
-    multiply(0);
-    wait_loads<LOADS>();
-    barrier();
-    fetch(next, 0);
+    pin();
+    multiply(0, next, stage, 4);
+    fetch(cur, 2);
+    pin();
     multiply(1);
+    fetch(cur, 3);
+    pin();
+    multiply(0);
+    wait_loads<0>();
+    barrier();
+    pin();
+    if (!last) fetch(next, 0);
+    pin();
+    multiply(1, cur, after, 0);
   };
-  load(lds0, 0);
-  load(lds1, 1);
-  wait_loads<LOADS>();
-  __syncthreads();
-  fetch(lds0, 0);
-  for (int n = 0;;) {
-    step(lds0, lds1, lds2, n);
-    if (++n == stages) break;
-    step(lds1, lds2, lds0, n);
-    if (++n == stages) break;
-    step(lds2, lds0, lds1, n);
-    if (++n == stages) break;
+  Tile t = tile_at<WIDE, WIDE, WIDE_BAND>(a, first + slot);
+  aim(t);
+#pragma unroll
+  for (int j = 0; j < WIDE_LOADS; ++j) load(lds0, 0, j, ends.past(0));
+#pragma unroll
+  for (int j = 0; j < WIDE_LOADS / 2; ++j) load(lds1, 1, j, ends.past(1));
+  wait_loads<WIDE_LOADS / 2>();
+  barrier();
+  for (int parity = 0;; parity ^= 1) {
+    const Tile done = t;
+    const Set& s = a.set[done.set];
+    load_channels<F16, QKV>(a, s, done.c0, channel[parity]);  // (read after the next barriers)
+    float scale[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) scale[j] = s.scale[min(done.t0 + wt * 64 + j * 32 + col, s.tokens - 1)];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = i32x16{};
+    fetch(lds0, 0);
+    for (int n = 2; n < stages; n += 2) {
+      step(lds0, lds1, n - 1, n, false);
+      step(lds1, lds0, n, n + 1, false);
+    }
+    slot += stride;
+    const bool more = slot < a.tiles_xcd && first + slot < a.tiles;
+    // (the second half of this tile's last stage goes by its own addresses)
+    fetch(lds0, 1);
+    pin();
+    multiply(0, lds1, stages - 1, 4);
+    if (more) t = tile_at<WIDE, WIDE, WIDE_BAND>(a, first + slot);
+    aim(t);  // (after the last tile: its own first stages once more, never read)
+    fetch(lds0, 2);
+    pin();
+    multiply(1);
+    fetch(lds0, 3);
+    pin();
+    multiply(0);
+    wait_loads<0>();
+    barrier();
+    pin();
+    fetch(lds1, 0);
+    pin();
+    multiply(1, lds0, 0, 0);
+    step(lds1, lds0, 0, 1, true);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      finish<F16, QKV, GELU, 4, WIDE>(a, s, acc[j], scale[j], &channel[parity][0][wc * 128], done.c0 + wc * 128,
+                                      done.t0 + wt * 64 + j * 32);
+    if (!more) break;
   }
   wait_loads<0>();  // (nothing may still be on its way to LDS when the workgroup ends)
+}
+
+// ------------------------------------------------------------------ fewer rows
+// 32 CF channels x 128 tokens a workgroup of eight waves, one workgroup a CU.  With fewer tiles than CUs the
+// instructions of one workgroup bound it, not the chip's rates, so every operand is read from LDS by few
+// waves: four waves share the 128 features of a stage, 32 each, and two the tokens, 64 each.  R stages in LDS;
+// a wave multiplies one stage while it reads the next and asks for the one R - 1 on, its loads spread over its
+// products (all at once they hold up the issue of the products: 512 x 12288 x 3072 46 -> 42 us when four waves
+// shared the tokens alone).  The four sums meet in LDS.
+constexpr int TALL = 128, STEP = 128;
+
+template <bool F16, bool QKV, bool GELU, int CF, int R>
+__global__ __launch_bounds__(512, 2) void int8_tile_kernel(Args a) {
+  constexpr int TC = 32 * CF, STAGE = (TC + TALL) * STEP, LOADS = STAGE / 8192, PRODUCTS = 2 * CF;
+  __shared__ __attribute__((aligned(1024))) int8_t lds0[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds1[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds2[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds3[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds4[R > 4 ? STAGE : 1024];
+  __shared__ __attribute__((aligned(1024))) int8_t lds5[R > 5 ? STAGE : 1024];
+  __shared__ __attribute__((aligned(16))) float channel[3][TC];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+  const int part = wave >> 1, wt = wave & 1;  // of the features, and of the tokens
+  const uint32_t tile = (blockIdx.x & 7) * a.tiles_xcd + (blockIdx.x >> 3);
+  if (tile >= a.tiles) return;
+  const Tile t = tile_at<TC, TALL, 8>(a, tile);
+  const Set& s = a.set[t.set];
+  load_channels<F16, QKV>(a, s, t.c0, channel);
+  // Loads as in the wide kernel.
+  const int8_t *wbase = s.w + (int64_t)t.c0 * a.padded, *qbase = s.q + (int64_t)t.t0 * a.padded;
+  const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+  int offset[LOADS];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const uint32_t at = t0 + wave * 64 + j * 32 + col, token = min(at, s.tokens - 1);
-    const float scale = s.scale[token];
-    const uint32_t b = token / s.rows, n = token - b * s.rows;
-    uint16_t* out = s.out + b * s.out_b + (int64_t)n * s.out_n;
-    const float *co = nullptr, *si = nullptr;
-    float v[4][16];
-    float squares = 0.f;
+  for (int j = 0; j < LOADS; ++j) {
+    const int r = 8 * (8 * j + wave) + (lane >> 3);
+    const int row = 64 * j < TC ? min(r, a.columns - 1 - t.c0) : (int)min((uint32_t)(r - TC), s.tokens - 1 - t.t0);
+    offset[j] = row * a.padded + chunk * 16;
+  }
+  const int stages = (a.padded + STEP - 1) / STEP;
+  const Ends ends(a.padded, chunk);
+  auto load = [&](int8_t* dst, int stage, int j, int past) {
+    load_lds16(64 * j < TC ? wbase : qbase, dst + 1024 * (8 * j + wave), offset[j] | past, uniform(stage * STEP));
+  };
+  const int read = col * STEP + ((col >> 1 & 7) ^ (2 * part + half)) * 16;
+  i32x4 w[2][CF], x[2][2];
+  auto fetch = [&](const int8_t* src, int to) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < CF; ++i) w[to][i] = *(const i32x4*)(src + i * 32 * STEP + read);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) x[to][j] = *(const i32x4*)(src + (TC + (wt * 2 + j) * 32) * STEP + read);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  i32x16 acc[2][CF] = {};
+  // Stage n's operands are in w[from], x[from], or on their way, and stage n + 1 is in `next`.  `free`, whose
+  // reads ended in the last step, takes stage n + R - 1.  Before the barrier stage n + 2 is there.
+  auto step = [&](const int8_t* next, int8_t* free, int n, int from) {
+    const int past = ends.past(uniform(n + R - 1));
+    int done = 0, asked = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < CF; ++i) {
+        acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[from][i], x[from][j], acc[j][i], 0, 0, 0);
+        for (++done; asked * PRODUCTS < done * LOADS; ++asked) {
+          __builtin_amdgcn_sched_barrier(0);
+          load(free, n + R - 1, asked, past);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(next, from ^ 1);
+    wait_arrivals<(R - 3) * LOADS>();
+    barrier();
+  };
+  auto begin = [&](int8_t* dst, int stage) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) load(dst, stage, j, ends.past(stage));
+  };
+  // (Zeros into the last stage, so that the compiler, which tracks what is on its way to which array, has met
+  // them all before the loop: otherwise it waits for everything each time around.)
+  load(R == 6 ? lds5 : lds3, 0, 0, (int)0x80000000);
+  begin(lds0, 0);
+  begin(lds1, 1);
+  begin(lds2, 2);
+  if (R == 6) {
+    begin(lds3, 3);
+    begin(lds4, 4);
+  }
+  wait_arrivals<(R - 3) * LOADS>();
+  barrier();
+  fetch(lds0, 0);
+  for (int n = 0;;) {
+    step(lds1, R == 6 ? lds5 : lds3, n, 0);
+    if (++n == stages) break;
+    step(lds2, lds0, n, 1);
+    if (++n == stages) break;
+    step(lds3, lds1, n, 0);
+    if (++n == stages) break;
+    step(R == 6 ? lds4 : lds0, lds2, n, 1);
+    if (++n == stages) break;
+    if (R == 6) {
+      step(lds5, lds3, n, 0);
+      if (++n == stages) break;
+      step(lds0, lds4, n, 1);
+      if (++n == stages) break;
+    }
+  }
+  wait_loads<0>();  // (nothing is on its way to LDS any more)
+  barrier();
+  // Parts 2 and 3 hand their sums to 0 and 1, which then exchange the second and first 32 tokens and finish
+  // the ones they keep: 16 bytes a lane at a time, as they lie in registers.
+  auto hand = [&](int8_t* to, int j) {
+#pragma unroll
+    for (int i = 0; i < CF; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(i32x4*)(to + ((i * 4 + g) * 64 + lane) * 16) = i32x4{acc[j][i][4 * g], acc[j][i][4 * g + 1], acc[j][i][4 * g + 2], acc[j][i][4 * g + 3]};
+  };
+  auto take = [&](const int8_t* from, int j) {
+#pragma unroll
+    for (int i = 0; i < CF; ++i)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int c = i * 32 + g * 8 + half * 4;
-        const f32x4 ws = *(const f32x4*)&channel[0][c], bias = *(const f32x4*)&channel[1][c];
+        const i32x4 v = *(const i32x4*)(from + ((i * 4 + g) * 64 + lane) * 16);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float p = (float)acc[i][j][g * 4 + k] * scale * ws[k] + bias[k];
-          if (QKV) squares += p * p;
-          if (GELU) p = gelu(p);
-          v[i][g * 4 + k] = p;
-        }
+        for (int k = 0; k < 4; ++k) acc[j][i][4 * g + k] += v[k];
       }
-    if (QKV) {
-      out += plane * a.out_p + (c0 - plane * a.heads * HEAD);
-      if (plane < 2) {
-        squares += __shfl_xor(squares, 32, 64);
-        const float rms = __builtin_amdgcn_rsqf(squares * (1.f / HEAD) + a.eps);
-        co = a.cos ? a.cos + (int64_t)(s.first + n) * HEAD : nullptr;
-        si = a.cos ? a.sin + (int64_t)(s.first + n) * HEAD : nullptr;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int c = i * 32 + g * 8 + half * 4;
-            const f32x4 norm = *(const f32x4*)&channel[2][c];
-            float y[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = v[i][g * 4 + k] * rms * norm[k];
-            if (a.cos) {
-              const f32x4 cv = *(const f32x4*)(co + c), sv = *(const f32x4*)(si + c);
-#pragma unroll
-              for (int k = 0; k < 4; k += 2) {
-                v[i][g * 4 + k] = y[k] * cv[k] - y[k + 1] * sv[k];
-                v[i][g * 4 + k + 1] = y[k + 1] * cv[k + 1] + y[k] * sv[k + 1];
-              }
-            } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) v[i][g * 4 + k] = y[k];
-            }
-          }
-      }
-    } else {
-      out += c0;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        float even[4], odd[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          even[k] = v[i][8 * p + k];
-          odd[k] = v[i][8 * p + 4 + k];
-        }
-        const u32x4 packed = pack_pair<F16>(even, odd);
-        const int c = i * 32 + p * 16 + half * 8;
-        if (at < s.tokens) {
-          if (QKV || (a.vectors && c0 + c + 8 <= a.columns)) {
-            *(u32x4*)(out + c) = packed;
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (c0 + c + k < a.columns) out[c + k] = (uint16_t)(packed[k >> 1] >> (16 * (k & 1)));
-          }
-        }
-      }
+  };
+  constexpr int SUMS = CF * 4096;  // bytes of a wave's sums of 32 tokens
+  static_assert(2 * SUMS <= STAGE, "a stage holds the sums of 64 tokens");
+  int8_t* const box = (part & 1) ? (wt ? lds3 : lds2) : (wt ? lds1 : lds0);
+  if (part >= 2) {
+    hand(box, 0);
+    hand(box + SUMS, 1);
+  }
+  __syncthreads();
+  if (part < 2) {
+    take(box, 0);
+    take(box + SUMS, 1);
+  }
+  __syncthreads();
+  if (part == 0) hand(box, 1);
+  if (part == 1) hand(box, 0);
+  __syncthreads();
+  if (part >= 2) return;
+  int8_t* const other = part ? (wt ? lds1 : lds0) : (wt ? lds3 : lds2);
+  const uint32_t t0 = t.t0 + (wt * 2 + part) * 32;
+  const float scale = s.scale[min(t0 + col, s.tokens - 1)];
+  if (part == 0) {
+    take(other, 0);
+    finish<F16, QKV, GELU, CF, TC>(a, s, acc[0], scale, channel[0], t.c0, t0);
+  } else {
+    take(other, 1);
+    finish<F16, QKV, GELU, CF, TC>(a, s, acc[1], scale, channel[0], t.c0, t0);
   }
 }
 
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// ------------------------------------------------------------------ a few rows
+// Bound by the read of the weights.  Waves read 16 WF channels each straight into the operands of
+// v_mfma_i32_16x16x64_i8 (whose columns are 16 TF tokens), 64 bytes of a row a lane quartet, and split the
+// features between them; the partial sums meet in LDS.  CG channel groups and KS feature splits a workgroup.
+template <bool F16, bool QKV, bool GELU, int TF, int WF, int CG, int KS>
+__global__ __launch_bounds__(64 * CG * KS) void int8_rows_product_kernel(Args a) {
+  constexpr int TC = 16 * WF * CG, TT = 16 * TF, THREADS = 64 * CG * KS;
+  // (a row of sums is four ints longer, so that rows start in different banks)
+  __shared__ __attribute__((aligned(16))) int partial[KS][TT][TC + 4];
+  __shared__ __attribute__((aligned(16))) float channel[3][TC];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, quarter = lane >> 4;
+  const int cg = wave % CG, ks = wave / CG;
+  uint32_t tile = blockIdx.x;
+  const int set = tile >= a.tiles0;
+  if (set) tile -= a.tiles0;
+  const Set& s = a.set[set];
+  const uint32_t tt = tile / a.channel_tiles, t0 = tt * TT;
+  const int c0 = (int)(tile - tt * a.channel_tiles) * TC;
+  const int8_t* wp[WF];
+#pragma unroll
+  for (int i = 0; i < WF; ++i)
+    wp[i] = s.w + (int64_t)min(c0 + (cg * WF + i) * 16 + col, a.columns - 1) * a.padded + quarter * 16;
+  const int8_t* xp[TF];
+#pragma unroll
+  for (int j = 0; j < TF; ++j) xp[j] = s.q + (int64_t)min(t0 + j * 16 + col, s.tokens - 1) * a.padded + quarter * 16;
+  i32x4 acc[TF][WF] = {};
+  // (a split is a whole number of 128-byte lines)
+  const int steps = a.padded / 64, each = ((steps + KS - 1) / KS + 1) & ~1;
+  const int begin = min(ks * each, steps), end = min(begin + each, steps);
+  int n = begin;
+  auto walk = [&](auto steps_at_once) {
+    constexpr int D = decltype(steps_at_once)::value;
+    i32x4 w[D][WF], x[D][TF];
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+#pragma unroll
+      for (int i = 0; i < WF; ++i) w[d][i] = *(const i32x4*)(wp[i] + (n + d) * 64);
+#pragma unroll
+      for (int j = 0; j < TF; ++j) x[d][j] = *(const i32x4*)(xp[j] + (n + d) * 64);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+      for (int j = 0; j < TF; ++j)
+#pragma unroll
+        for (int i = 0; i < WF; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d][i], x[d][j], acc[j][i], 0, 0, 0);
+    n += D;
+  };
+  // (as many steps' loads as possible in flight together)
+  constexpr int MOST = TF * WF >= 4 ? 4 : 8;
+  while (n + MOST <= end) walk(std::integral_constant<int, MOST>());
+  if (MOST > 4 && n + 6 <= end) walk(std::integral_constant<int, 6>());
+  if (MOST > 4 && n + 4 <= end) walk(std::integral_constant<int, 4>());
+  if (n + 2 <= end) walk(std::integral_constant<int, 2>());
+  if (n < end) walk(std::integral_constant<int, 1>());
+  load_channels<F16, QKV>(a, s, c0, channel);
+  // a lane's sums: token col, channels 4 quarter .. + 3 of each 16
+#pragma unroll
+  for (int j = 0; j < TF; ++j)
+#pragma unroll
+    for (int i = 0; i < WF; ++i) *(i32x4*)&partial[ks][j * 16 + col][(cg * WF + i) * 16 + quarter * 4] = acc[j][i];
+  __syncthreads();
+  // eight channels of a token a thread; 16 lanes hold a head
+  const int plane = QKV ? c0 / (a.heads * HEAD) : 2;
+  for (int e = threadIdx.x; e < TT * (TC / 8); e += THREADS) {
+    const int token = e / (TC / 8), c = e % (TC / 8) * 8;
+    i32x4 sum[2] = {};
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) sum[h] += *(const i32x4*)&partial[k][token][c + 4 * h];
+    const uint32_t at = t0 + token;
+    const float scale = s.scale[min(at, s.tokens - 1)];
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = (float)sum[k >> 2][k & 3] * scale * channel[0][c + k] + channel[1][c + k];
+    uint16_t* out = s.out + row_of(s, at) + c0 + c;
+    if (QKV) {
+      out += plane * a.out_p - plane * a.heads * HEAD;
+      if (plane < 2) {
+        float squares = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) squares += v[k] * v[k];
+#pragma unroll
+        for (int m = 8; m >= 1; m >>= 1) squares += __shfl_xor(squares, m, 16);
+        const float rms = __builtin_amdgcn_rsqf(squares * (1.f / HEAD) + a.eps);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= rms * channel[2][c + k];
+        const int64_t table = (int64_t)(s.first + min(at, s.tokens - 1) % s.rows) * HEAD + c;
+        if (a.cos) rotate(v, a.cos + table, a.sin + table);
+      }
+    } else if (GELU) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = gelu(v[k]);
+    }
+    if (at < s.tokens) store8<QKV>(a, out, c0 + c, pack8<F16>(v));
+  }
+}
 
-template <bool F16, bool QKV>
-void launch_type(const Args& a, hipStream_t st) {
-  const dim3 grid(8 * a.tiles_xcd), block(256);
-  if (a.gelu) hipLaunchKernelGGL((int8_product_kernel<F16, QKV, !QKV>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((int8_product_kernel<F16, QKV, false>), grid, block, 0, st, a);
+// ------------------------------------------------------------------ launches
+enum Kernel { ROWS16, ROWS32, TILE64, TILE128, WIDE256, KERNELS };
+
+// What a tile of each kernel covers, and what it takes in us on 256 CUs: a round of tiles, one a CU, is
+// `round` + stages of 128 features x `stage` + `full` (f) f, f the share of the CUs that have one (stages
+// slow each other down where many load).
+struct Shape {
+  int tc, tt;
+  float round, stage, full;
+};
+constexpr Shape SHAPES[KERNELS] = {
+    {16, 16, 0.f, 0.f, 0.f},
+    {32, 32, 0.f, 0.f, 0.f},
+    {64, 128, 2.6f, 0.26f, 0.14f},
+    {128, 128, 5.0f, 0.34f, 0.06f},
+    {256, 256, 6.7f, 1.06f, 0.60f},
+};
+
+// Tiles of TC x TT of both sets.
+int64_t tiles_of(const Args& a, int count, int tc, int tt) {
+  int64_t tiles = 0;
+  for (int i = 0; i < count; ++i)
+    tiles += ((a.set[i].tokens + (int64_t)tt - 1) / tt) * ((a.columns + (int64_t)tc - 1) / tc);
+  return tiles;
+}
+
+// A head's channels stay together.
+int channels_of(Kernel k, bool qkv) { return qkv && SHAPES[k].tc < HEAD ? HEAD : SHAPES[k].tc; }
+
+// The kernel whose estimate is the least.  Up to 16 tokens a set it is the first; measured, rows x features x
+// columns, us: 1 x 3072 x 18432 12.6 (32 x 32 blocks 15.7, 64 x 128 tiles 21.5), 16 x 3072 x 9216 11.2 (11.7,
+// 11.3).  The others, 32 x 32 blocks / 64 x 128 / 128 x 128 / 256 x 256 tiles: 64 x 3072 x 3072 8.5 / 10.6 / 14.7 /
+// 32.4; 200 x 1024 x 1024 4.6 / 6.8 / 9.3 / 15.6; 128 x 3072 x 12288 37 / 13.6 / 17.0 / 32.7; 512 x 12288 x 3072 128 /
+// 33 / 41 / 111; 256 x 3072 x 9216 56 / 24 / 17.4 / 34; 512 x 3072 x 9216 101 / 35 / 34 / 36; 4096 x 3072 x 3072 - / 70 /
+// 57 / 42; 16384 x 256 x 256 - / 10.7 / 8.4 / 10.3.  Blocks are as long as the bytes they read, at 7.5 TB/s.
+Kernel choose(const Args& a, int count, bool qkv) {
+  uint32_t tokens = 0;
+  for (int i = 0; i < count; ++i) tokens = std::max(tokens, a.set[i].tokens);
+  // (a grid holds fewer than 2^32 threads)
+  const auto fits = [&](Kernel k) { return tiles_of(a, count, channels_of(k, qkv), SHAPES[k].tt) < (1 << 21); };
+  if (tokens <= 16 && fits(ROWS16)) return ROWS16;
+  const float stages = (float)((a.padded + 127) / 128), cus = 256.f;
+  Kernel best = WIDE256;
+  float least = 3e38f;
+  for (int i = ROWS32; i < KERNELS; ++i) {
+    const Kernel k = (Kernel)i;
+    const Shape& s = SHAPES[i];
+    const int tc = channels_of(k, qkv);
+    if (k == TILE64 && tc != s.tc) continue;
+    if (k != WIDE256 && !fits(k)) continue;
+    const float tiles = (float)tiles_of(a, count, tc, s.tt);
+    float us;
+    if (k == ROWS32) {
+      us = 3.f + tiles * (float)(tc + s.tt) * (float)a.padded / 7.5e6f;
+    } else {
+      const float rounds = std::floor(tiles / cus), rest = tiles / cus - rounds;
+      us = 2.3f + rounds * (s.round + stages * (s.stage + s.full));
+      if (rest > 0.f) us += s.round + stages * (s.stage + s.full * rest * rest);
+    }
+    if (us < least) {
+      least = us;
+      best = k;
+    }
+  }
+  return best;
+}
+
+template <bool F16, bool QKV, bool GELU>
+int launch_kernel(Args& a, int count, hipStream_t st) {
+  const Kernel kernel = choose(a, count, QKV);
+  const int tc = channels_of(kernel, QKV), tt = SHAPES[kernel].tt;
+  const int64_t tiles = tiles_of(a, count, tc, tt);
+  HB_REQUIRE(tiles < (1ll << 30), "too many output tiles for one launch");
+  a.channel_tiles = (uint32_t)((a.columns + tc - 1) / tc);
+  a.tiles0 = (uint32_t)tiles_of(a, 1, tc, tt);
+  a.tiles = (uint32_t)tiles;
+  a.tiles_xcd = (a.tiles + 7) / 8;
+  const dim3 blocks(a.tiles), each(8 * a.tiles_xcd), eight(512);
+  switch (kernel) {
+    case ROWS16:
+      if constexpr (QKV) hipLaunchKernelGGL((int8_rows_product_kernel<F16, QKV, GELU, 1, 2, 4, 4>), blocks, dim3(1024), 0, st, a);
+      else hipLaunchKernelGGL((int8_rows_product_kernel<F16, QKV, GELU, 1, 1, 1, 8>), blocks, eight, 0, st, a);
+      break;
+    case ROWS32:
+      if constexpr (QKV) hipLaunchKernelGGL((int8_rows_product_kernel<F16, QKV, GELU, 2, 2, 4, 4>), blocks, dim3(1024), 0, st, a);
+      else hipLaunchKernelGGL((int8_rows_product_kernel<F16, QKV, GELU, 2, 2, 1, 8>), blocks, eight, 0, st, a);
+      break;
+    case TILE64:
+      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 2, 6>), each, eight, 0, st, a);
+      break;
+    case TILE128: hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 4, 4>), each, eight, 0, st, a); break;
+    default: {
+      const uint32_t per_xcd = std::max(1, device_cu_count() / 8);
+      hipLaunchKernelGGL((int8_wide_kernel<F16, QKV, GELU>), dim3(8 * std::min(a.tiles_xcd, per_xcd)), eight, 0, st, a);
+    }
+  }
+  HB_HIP(hipGetLastError());
+  return HB_OK;
 }
 
 template <bool QKV>
 int launch(Args& a, int count, int32_t dtype, hipStream_t st) {
-  a.channel_tiles = (uint32_t)((a.columns + TC - 1) / TC);
-  int64_t tiles = 0;
-  for (int i = 0; i < count; ++i) {
-    tiles += (int64_t)((a.set[i].tokens + TT - 1) / TT) * a.channel_tiles;
-    HB_REQUIRE(tiles < (1ll << 30), "too many output tiles for one launch");
-    if (i == 0) a.tiles0 = (uint32_t)tiles;
-  }
-  a.tiles = (uint32_t)tiles;
-  a.tiles_xcd = (a.tiles + 7) / 8;
-  if (dtype == HB_DTYPE_F16) launch_type<true, QKV>(a, st);
-  else launch_type<false, QKV>(a, st);
-  HB_HIP(hipGetLastError());
-  return HB_OK;
+  if constexpr (QKV)
+    return dtype == HB_DTYPE_F16 ? launch_kernel<true, true, false>(a, count, st) : launch_kernel<false, true, false>(a, count, st);
+  else if (dtype == HB_DTYPE_F16)
+    return a.gelu ? launch_kernel<true, false, true>(a, count, st) : launch_kernel<true, false, false>(a, count, st);
+  else
+    return a.gelu ? launch_kernel<false, false, true>(a, count, st) : launch_kernel<false, false, false>(a, count, st);
 }
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // The checks both entry points make of a set's rows and weight.
 int check_set(const Set& s, int32_t batch, int32_t rows, int32_t padded) {
