@@ -41,6 +41,7 @@ struct Set {
   int64_t out_b, out_n;     // output strides of a batch element and a row
   uint32_t rows, tokens;    // rows of a batch element, and of all
   uint32_t first;           // qkv: the first row's place in cos and sin
+  uint32_t start;           // rows of the set before these (which another launch takes)
 };
 
 struct Args {
@@ -120,10 +121,14 @@ __device__ __forceinline__ void load_channels(const Args& a, const Set& s, int c
   channel[2][i] = QKV && plane < 2 && s.norm[plane] ? to_f<F16>(s.norm[plane][i & (HEAD - 1)]) : 1.f;
 }
 
-// Where token `at` of a set (clamped to its last) goes, in elements from s.out.
+// Token `at` of a set (clamped to its last): where it goes, in elements from s.out, and where its row of the
+// rotary tables begins.
 __device__ __forceinline__ int64_t row_of(const Set& s, uint32_t at) {
-  const uint32_t token = min(at, s.tokens - 1), b = token / s.rows;
+  const uint32_t token = s.start + min(at, s.tokens - 1), b = token / s.rows;
   return b * s.out_b + (int64_t)(token - b * s.rows) * s.out_n;
+}
+__device__ __forceinline__ int64_t table_of(const Set& s, uint32_t at) {
+  return (int64_t)(s.first + (s.start + min(at, s.tokens - 1)) % s.rows) * HEAD;
 }
 
 // Eight values of channels c .. c + 7 to `out`, those of them that there are.
@@ -188,7 +193,7 @@ __device__ __forceinline__ void finish(const Args& a, const Set& s, const i32x16
       }
     squares += __shfl_xor(squares, 32, 64);
     rms = __builtin_amdgcn_rsqf(squares * (1.f / HEAD) + a.eps);
-    table = (int64_t)(s.first + min(t0 + col, s.tokens - 1) % s.rows) * HEAD + half * 4;
+    table = table_of(s, t0 + col) + half * 4;
   }
 #pragma unroll
   for (int i = 0; i < CF; ++i) {
@@ -655,7 +660,7 @@ __global__ __launch_bounds__(64 * CG * KS) void int8_rows_product_kernel(Args a)
         const float rms = __builtin_amdgcn_rsqf(squares * (1.f / HEAD) + a.eps);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] *= rms * channel[2][c + k];
-        const int64_t table = (int64_t)(s.first + min(at, s.tokens - 1) % s.rows) * HEAD + c;
+        const int64_t table = table_of(s, at) + c;
         if (a.cos) rotate(v, a.cos + table, a.sin + table);
       }
     } else if (GELU) {
@@ -695,47 +700,64 @@ int64_t tiles_of(const Args& a, int count, int tc, int tt) {
 // A head's channels stay together.
 int channels_of(Kernel k, bool qkv) { return qkv && SHAPES[k].tc < HEAD ? HEAD : SHAPES[k].tc; }
 
+// What a kernel takes for the sets, in us.
+float estimate(const Args& a, int count, Kernel k, bool qkv) {
+  const Shape& s = SHAPES[k];
+  const int tc = channels_of(k, qkv);
+  const float tiles = (float)tiles_of(a, count, tc, s.tt), stages = (float)((a.padded + 127) / 128), cus = 256.f;
+  if (k <= ROWS32) return 3.f + tiles * (float)(tc + s.tt) * (float)a.padded / 7.5e6f;
+  const float rounds = std::floor(tiles / cus), rest = tiles / cus - rounds;
+  return 2.3f + rounds * (s.round + stages * (s.stage + s.full)) +
+         (rest > 0.f ? s.round + stages * (s.stage + s.full * rest * rest) : 0.f);
+}
+
+struct Choice {
+  Kernel kernel;
+  float us;
+};
+
 // The kernel whose estimate is the least.  Up to 16 tokens a set it is the first; measured, rows x features x
 // columns, us: 1 x 3072 x 18432 12.6 (32 x 32 blocks 15.7, 64 x 128 tiles 21.5), 16 x 3072 x 9216 11.2 (11.7,
 // 11.3).  The others, 32 x 32 blocks / 64 x 128 / 128 x 128 / 256 x 256 tiles: 64 x 3072 x 3072 8.5 / 10.6 / 14.7 /
 // 32.4; 200 x 1024 x 1024 4.6 / 6.8 / 9.3 / 15.6; 128 x 3072 x 12288 37 / 13.6 / 17.0 / 32.7; 512 x 12288 x 3072 128 /
 // 33 / 41 / 111; 256 x 3072 x 9216 56 / 24 / 17.4 / 34; 512 x 3072 x 9216 101 / 35 / 34 / 36; 4096 x 3072 x 3072 - / 70 /
 // 57 / 42; 16384 x 256 x 256 - / 10.7 / 8.4 / 10.3.  Blocks are as long as the bytes they read, at 7.5 TB/s.
-Kernel choose(const Args& a, int count, bool qkv) {
+Choice choose(const Args& a, int count, bool qkv) {
   uint32_t tokens = 0;
   for (int i = 0; i < count; ++i) tokens = std::max(tokens, a.set[i].tokens);
   // (a grid holds fewer than 2^32 threads)
   const auto fits = [&](Kernel k) { return tiles_of(a, count, channels_of(k, qkv), SHAPES[k].tt) < (1 << 21); };
-  if (tokens <= 16 && fits(ROWS16)) return ROWS16;
-  const float stages = (float)((a.padded + 127) / 128), cus = 256.f;
-  Kernel best = WIDE256;
-  float least = 3e38f;
-  for (int i = ROWS32; i < KERNELS; ++i) {
+  if (tokens <= 16 && fits(ROWS16)) return {ROWS16, 0.f};
+  Choice best = {WIDE256, estimate(a, count, WIDE256, qkv)};
+  for (int i = ROWS32; i < WIDE256; ++i) {
     const Kernel k = (Kernel)i;
-    const Shape& s = SHAPES[i];
-    const int tc = channels_of(k, qkv);
-    if (k == TILE64 && tc != s.tc) continue;
-    if (k != WIDE256 && !fits(k)) continue;
-    const float tiles = (float)tiles_of(a, count, tc, s.tt);
-    float us;
-    if (k == ROWS32) {
-      us = 3.f + tiles * (float)(tc + s.tt) * (float)a.padded / 7.5e6f;
-    } else {
-      const float rounds = std::floor(tiles / cus), rest = tiles / cus - rounds;
-      us = 2.3f + rounds * (s.round + stages * (s.stage + s.full));
-      if (rest > 0.f) us += s.round + stages * (s.stage + s.full * rest * rest);
-    }
-    if (us < least) {
-      least = us;
-      best = k;
-    }
+    if ((k == TILE64 && qkv) || !fits(k)) continue;
+    const float us = estimate(a, count, k, qkv);
+    if (us < best.us) best = {k, us};
   }
   return best;
 }
 
+// The last rows of the last set that are better off in a launch of their own, because the tiles before them
+// fill whole rounds of the CUs: 16896 x 15360 x 3072, 792 tiles of 256 x 256, 934 us at once, and 728 as
+// 768 of them and 512 rows apart.
+uint32_t apart(const Args& a, int count, const Choice& whole, bool qkv) {
+  const Set& s = a.set[count - 1];
+  const int64_t across = (a.columns + 255) / 256, tiles = tiles_of(a, count, 256, 256);
+  if (whole.kernel != WIDE256 || tiles < 256 || tiles % 256 == 0) return 0;
+  // token tiles to take off, so that what is left is the most that fits the whole rounds
+  const int64_t off = (tiles % 256 + across - 1) / across, token_tiles = (s.tokens + 255) / 256;
+  if (off >= token_tiles) return 0;
+  const uint32_t keep = (uint32_t)(token_tiles - off) * 256;
+  Args main = a, rest = a;
+  main.set[count - 1].tokens = keep;
+  rest.set[0] = s;
+  rest.set[0].tokens = s.tokens - keep;
+  return estimate(main, count, WIDE256, qkv) + choose(rest, 1, qkv).us + 5.f < whole.us ? s.tokens - keep : 0;
+}
+
 template <bool F16, bool QKV, bool GELU>
-int launch_kernel(Args& a, int count, hipStream_t st) {
-  const Kernel kernel = choose(a, count, QKV);
+int launch_kernel(Args& a, int count, Kernel kernel, hipStream_t st) {
   const int tc = channels_of(kernel, QKV), tt = SHAPES[kernel].tt;
   const int64_t tiles = tiles_of(a, count, tc, tt);
   HB_REQUIRE(tiles < (1ll << 30), "too many output tiles for one launch");
@@ -766,14 +788,30 @@ int launch_kernel(Args& a, int count, hipStream_t st) {
   return HB_OK;
 }
 
+template <bool F16, bool QKV, bool GELU>
+int launch_type(Args& a, int count, hipStream_t st) {
+  const Choice whole = choose(a, count, QKV);
+  const uint32_t rest = apart(a, count, whole, QKV);
+  if (!rest) return launch_kernel<F16, QKV, GELU>(a, count, whole.kernel, st);
+  Args b = a;
+  Set& s = b.set[0] = a.set[count - 1];
+  a.set[count - 1].tokens -= rest;
+  s.start = s.tokens - rest;
+  s.q += (int64_t)s.start * a.padded;
+  s.scale += s.start;
+  s.tokens = rest;
+  const int rc = launch_kernel<F16, QKV, GELU>(a, count, WIDE256, st);
+  return rc ? rc : launch_kernel<F16, QKV, GELU>(b, 1, choose(b, 1, QKV).kernel, st);
+}
+
 template <bool QKV>
 int launch(Args& a, int count, int32_t dtype, hipStream_t st) {
   if constexpr (QKV)
-    return dtype == HB_DTYPE_F16 ? launch_kernel<true, true, false>(a, count, st) : launch_kernel<false, true, false>(a, count, st);
+    return dtype == HB_DTYPE_F16 ? launch_type<true, true, false>(a, count, st) : launch_type<false, true, false>(a, count, st);
   else if (dtype == HB_DTYPE_F16)
-    return a.gelu ? launch_kernel<true, false, true>(a, count, st) : launch_kernel<true, false, false>(a, count, st);
+    return a.gelu ? launch_type<true, false, true>(a, count, st) : launch_type<true, false, false>(a, count, st);
   else
-    return a.gelu ? launch_kernel<false, false, true>(a, count, st) : launch_kernel<false, false, false>(a, count, st);
+    return a.gelu ? launch_type<false, false, true>(a, count, st) : launch_type<false, false, false>(a, count, st);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -812,7 +850,7 @@ extern "C" int hb_int8_linear(int32_t count, int32_t batch, const int32_t* rows,
     void* const* p = pointers + 6 * i;
     Set& s = a.set[i];
     s = {(const int8_t*)p[0], (const float*)p[1], (const int8_t*)p[2], (const float*)p[3], (const uint16_t*)p[4],
-         (uint16_t*)p[5], {nullptr, nullptr}, strides[2 * i], strides[2 * i + 1], (uint32_t)rows[i], 0, 0};
+         (uint16_t*)p[5], {nullptr, nullptr}, strides[2 * i], strides[2 * i + 1], (uint32_t)rows[i], 0, 0, 0};
     const int rc = check_set(s, batch, rows[i], padded);
     if (rc) return rc;
     s.tokens = (uint32_t)(batch * rows[i]);
@@ -851,7 +889,7 @@ extern "C" int hb_int8_qkv(int32_t batch, int32_t text_tokens, int32_t tokens, i
     Set& s = a.set[count++];
     s = {(const int8_t*)p[0], (const float*)p[1], (const int8_t*)p[2], (const float*)p[3], (const uint16_t*)p[4],
          (uint16_t*)out + first * out_row_stride, {(const uint16_t*)p[5], (const uint16_t*)p[6]}, out_batch_stride,
-         out_row_stride, (uint32_t)rows, 0, (uint32_t)first};
+         out_row_stride, (uint32_t)rows, 0, (uint32_t)first, 0};
     const int rc = check_set(s, batch, rows, padded);
     if (rc) return rc;
     HB_REQUIRE(((uintptr_t)s.norm[0] & 1) == 0 && ((uintptr_t)s.norm[1] & 1) == 0, "norm weights must be 2-byte aligned");
