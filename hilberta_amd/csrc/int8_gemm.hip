@@ -143,18 +143,13 @@ __device__ __forceinline__ void store8(const Args& a, uint16_t* out, int c, cons
   }
 }
 
-// Pairs (2i, 2i + 1) of N values turned by cos and sin.
-template <int N>
-__device__ __forceinline__ void rotate(float (&v)[N], const float* cos, const float* sin) {
+// Two pairs (2i, 2i + 1) turned by cos and sin.
+__device__ __forceinline__ void rotate(float* v, const f32x4& cos, const f32x4& sin) {
 #pragma unroll
-  for (int g = 0; g < N; g += 4) {
-    const f32x4 c = *(const f32x4*)(cos + g), s = *(const f32x4*)(sin + g);
-#pragma unroll
-    for (int k = 0; k < 4; k += 2) {
-      const float even = v[g + k], odd = v[g + k + 1];
-      v[g + k] = even * c[k] - odd * s[k];
-      v[g + k + 1] = odd * c[k + 1] + even * s[k + 1];
-    }
+  for (int k = 0; k < 4; k += 2) {
+    const float even = v[k], odd = v[k + 1];
+    v[k] = even * cos[k] - odd * sin[k];
+    v[k + 1] = odd * cos[k + 1] + even * sin[k + 1];
   }
 }
 
@@ -181,7 +176,6 @@ __device__ __forceinline__ void finish(const Args& a, const Set& s, const i32x16
   };
   const bool heads = QKV && plane < 2;
   float rms = 1.f;
-  int64_t table = 0;
   if (heads) {
     float squares = 0.f;
 #pragma unroll
@@ -193,13 +187,25 @@ __device__ __forceinline__ void finish(const Args& a, const Set& s, const i32x16
       }
     squares += __shfl_xor(squares, 32, 64);
     rms = __builtin_amdgcn_rsqf(squares * (1.f / HEAD) + a.eps);
-    table = table_of(s, t0 + col) + half * 4;
   }
+  // (a half block's rotary values are asked for half a block ahead)
+  f32x4 cos[2][2], sin[2][2];
+  const int64_t table = heads ? table_of(s, t0 + col) + half * 4 : 0;
+  auto ask = [&](int h) {
+    if (!heads || !a.cos) return;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      cos[h & 1][g] = *(const f32x4*)(a.cos + table + h * 16 + g * 8);
+      sin[h & 1][g] = *(const f32x4*)(a.sin + table + h * 16 + g * 8);
+    }
+  };
+  if (QKV) ask(0);
 #pragma unroll
   for (int i = 0; i < CF; ++i) {
     u32x4 packed[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
+      if (QKV && 2 * i + p + 1 < 2 * CF) ask(2 * i + p + 1);
       float v[2][4];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
@@ -211,7 +217,7 @@ __device__ __forceinline__ void finish(const Args& a, const Set& s, const i32x16
           if (heads) y *= rms * channel[2 * TC + c + k];
           v[g][k] = y;
         }
-        if (heads && a.cos) rotate(v[g], a.cos + table + c, a.sin + table + c);
+        if (heads && a.cos) rotate(v[g], cos[p][g], sin[p][g]);
       }
       packed[p] = pack_pair<F16>(v[0], v[1]);
     }
@@ -661,7 +667,11 @@ __global__ __launch_bounds__(64 * CG * KS) void int8_rows_product_kernel(Args a)
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] *= rms * channel[2][c + k];
         const int64_t table = table_of(s, at) + c;
-        if (a.cos) rotate(v, a.cos + table, a.sin + table);
+        if (a.cos) {
+#pragma unroll
+          for (int g = 0; g < 8; g += 4)
+            rotate(v + g, *(const f32x4*)(a.cos + table + g), *(const f32x4*)(a.sin + table + g));
+        }
       }
     } else if (GELU) {
 #pragma unroll
@@ -684,8 +694,8 @@ struct Shape {
 constexpr Shape SHAPES[KERNELS] = {
     {16, 16, 0.f, 0.f, 0.f},
     {32, 32, 0.f, 0.f, 0.f},
-    {64, 128, 2.6f, 0.26f, 0.14f},
-    {128, 128, 5.0f, 0.34f, 0.06f},
+    {64, 128, 2.6f, 0.26f, 0.10f},
+    {128, 128, 5.0f, 0.34f, 0.20f},
     {256, 256, 6.7f, 1.06f, 0.60f},
 };
 
