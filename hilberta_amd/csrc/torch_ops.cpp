@@ -15,6 +15,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <array>
 #include <initializer_list>
 #include <limits>
 #include <map>
@@ -35,6 +36,8 @@ using at::Tensor;
 // Key blocks per row hb_pair_rows pairs.
 constexpr int64_t PAIR_MAX_BLOCKS = 16384;
 constexpr int64_t MIN_WORKSPACE = 1 << 16;
+// Features of 8-bit rows: a sum of so many products fits 32 bits.
+constexpr int64_t MAX_FEATURES = 1 << 17;
 
 void check(int rc, const char* name) {
   if (rc == 0) return;
@@ -364,35 +367,51 @@ int64_t check_int8(const Tensor& q, const Tensor& scale, const char* name) {
   return q.size(-1);
 }
 
-void int8_rows(const Tensor& x, Tensor q, Tensor scale) {
-  const int32_t dtype = type_of(x.scalar_type(), "x");
-  const Rows r = rows_of(x, "x");
-  const int64_t padded = check_int8(q, scale, "q");
-  TORCH_CHECK_VALUE(q.sizes().slice(0, q.dim() - 1) == x.sizes().slice(0, x.dim() - 1) && padded >= x.size(-1),
-                    "q must have x's rows, filled up to a multiple of 64 columns");
-  one_device(x, {&q, &scale});
+// Columns of 8-bit rows of `features` values.
+int64_t padded_features(int64_t features) { return (features + 63) / 64 * 64; }
+
+// Unwritten 8-bit rows for x [.., features], and their scales.
+std::tuple<Tensor, Tensor> new_int8_rows(const Tensor& x) {
+  auto sizes = x.sizes().vec();
+  sizes.back() = padded_features(sizes.back());
+  Tensor q = at::empty(sizes, x.options().dtype(at::kChar));
+  sizes.pop_back();
+  return {std::move(q), at::empty(sizes, x.options().dtype(at::kFloat))};
+}
+
+// hb_int8_rows: 16-bit rows to 8-bit rows and their scales.
+std::tuple<Tensor, Tensor> int8_rows(const Tensor& x) {
+  const int32_t dtype = type_of(x.scalar_type(), "rows");
+  TORCH_CHECK_VALUE((x.dim() == 2 || x.dim() == 3) && x.size(-1) > 0 && x.size(-1) <= MAX_FEATURES,
+                    "rows must be [rows, features] or [B, rows, features] of 1 to ", MAX_FEATURES, " features");
+  const Rows r = rows_of(x, "rows");
   require_hip(x);
   const at::OptionalDeviceGuard guard(x.device());
-  check(hb_int8_rows(x.data_ptr(), r.batch_stride, r.row_stride, i32(r.batch, "batch"), i32(r.rows, "rows"),
-                     i32(x.size(-1), "features"), i32(padded, "padded"), dtype, static_cast<int8_t*>(q.data_ptr()),
-                     static_cast<float*>(scale.data_ptr()), stream_of(x.device())),
-        "hb_int8_rows");
+  auto [q, scale] = new_int8_rows(x);
+  if (scale.numel())
+    check(hb_int8_rows(x.data_ptr(), r.batch_stride, r.row_stride, i32(r.batch, "batch"), i32(r.rows, "rows"),
+                       i32(x.size(-1), "features"), i32(q.size(-1), "padded"), dtype, static_cast<int8_t*>(q.data_ptr()),
+                       static_cast<float*>(scale.data_ptr()), stream_of(x.device())),
+          "hb_int8_rows");
+  return {std::move(q), std::move(scale)};
 }
 
 struct AdaSet {
   const Tensor &x, &shift, &scale;
   const std::optional<Tensor>&y, &gate, &x_out;
-  const Tensor &q, &row_scale;
 };
 
-void int8_adaln_sets(std::initializer_list<AdaSet> sets, double eps) {
+// hb_int8_adaln of one or two row sets; their 8-bit rows and scales.
+std::array<Tensor, 4> int8_adaln_sets(std::initializer_list<AdaSet> sets, double eps) {
   void* pointers[16];
   int64_t strides[16];
   int32_t rows[2];
   const AdaSet& s0 = *sets.begin();
-  const int32_t dtype = type_of(s0.x.scalar_type(), "x");
-  const int64_t batch = s0.x.dim() == 3 ? s0.x.size(0) : 1, padded = check_int8(s0.q, s0.row_scale, "q");
-  const int64_t hidden = s0.x.dim() ? s0.x.size(-1) : 0;
+  std::array<Tensor, 4> made;
+  const int32_t dtype = type_of(s0.x.scalar_type(), "rows");
+  const int64_t batch = s0.x.dim() == 3 ? s0.x.size(0) : 1, hidden = s0.x.dim() ? s0.x.size(-1) : 0;
+  TORCH_CHECK_VALUE(hidden > 0 && hidden % 8 == 0 && hidden <= 8192, "hidden must be a multiple of 8 up to 8192");
+  const int64_t padded = padded_features(hidden);
   int i = 0;
   for (const AdaSet& s : sets) {
     const Tensor &y = value_or_none(s.y), &gate = value_or_none(s.gate), &x_out = value_or_none(s.x_out);
@@ -409,15 +428,11 @@ void int8_adaln_sets(std::initializer_list<AdaSet> sets, double eps) {
                                           (hidden <= 1 || t->stride(1) == 1) && t->scalar_type() == s.x.scalar_type()),
                         "shift/scale/gate must be [B, hidden] views with a contiguous last dim");
     TORCH_CHECK_VALUE(batch == 1 || s.shift.stride(0) == s.scale.stride(0), "shift and scale must share one batch stride");
-    TORCH_CHECK_VALUE(check_int8(s.q, s.row_scale, "q") == padded && s.q.dim() == 3 && s.q.size(0) == batch &&
-                          s.q.size(1) == s.x.size(1) && padded >= hidden,
-                      "q must have x's rows, filled up to a multiple of 64 columns");
     const Rows rx = rows_of(s.x, "x"), ry = y.defined() ? rows_of(y, "y") : Rows{},
                ro = x_out.defined() ? rows_of(x_out, "x_out") : Rows{};
     if (x_out.defined()) check_written(x_out, "x_out", {&s.shift, &s.scale, &gate});
-    one_device(s0.x, {&s.x, &s.shift, &s.scale, &y, &gate, &x_out, &s.q, &s.row_scale});
-    void* p[8] = {pointer(s.x), pointer(y), pointer(gate), pointer(x_out), pointer(s.shift), pointer(s.scale),
-                  pointer(s.q), pointer(s.row_scale)};
+    one_device(s0.x, {&s.x, &s.shift, &s.scale, &y, &gate, &x_out});
+    void* p[8] = {pointer(s.x), pointer(y), pointer(gate), pointer(x_out), pointer(s.shift), pointer(s.scale), nullptr, nullptr};
     // (a stride of a dimension of one says nothing)
     const int64_t one = batch == 1 ? 0 : 1;
     const int64_t st[8] = {one * rx.batch_stride, rx.rows == 1 ? 0 : rx.row_stride, one * ry.batch_stride,
@@ -429,24 +444,34 @@ void int8_adaln_sets(std::initializer_list<AdaSet> sets, double eps) {
   }
   require_hip(s0.x);
   const at::OptionalDeviceGuard guard(s0.x.device());
+  i = 0;
+  for (const AdaSet& s : sets) {
+    std::tie(made[2 * i], made[2 * i + 1]) = new_int8_rows(s.x);
+    pointers[8 * i + 6] = made[2 * i].data_ptr();
+    pointers[8 * i + 7] = made[2 * i + 1].data_ptr();
+    ++i;
+  }
+  if (i == 1 && !made[1].numel()) return made;
   check(hb_int8_adaln(i, i32(batch, "batch"), rows, i32(hidden, "hidden"), i32(padded, "padded"), dtype,
                       static_cast<float>(eps), pointers, strides, stream_of(s0.x.device())),
         "hb_int8_adaln");
+  return made;
 }
 
 using Maybe = std::optional<Tensor>;
 
-void int8_adaln(const Tensor& x, const Tensor& shift, const Tensor& scale, const Maybe& y, const Maybe& gate,
-                Maybe x_out, Tensor q, Tensor row_scale, double eps) {
-  int8_adaln_sets({{x, shift, scale, y, gate, x_out, q, row_scale}}, eps);
+std::tuple<Tensor, Tensor> int8_adaln(const Tensor& x, const Tensor& shift, const Tensor& scale, const Maybe& y,
+                                      const Maybe& gate, Maybe x_out, double eps) {
+  auto made = int8_adaln_sets({{x, shift, scale, y, gate, x_out}}, eps);
+  return {std::move(made[0]), std::move(made[1])};
 }
 
-void int8_adaln_pair(const Tensor& x, const Tensor& shift, const Tensor& scale, const Maybe& y, const Maybe& gate,
-                     Maybe x_out, Tensor q, Tensor row_scale, const Tensor& x2, const Tensor& shift2,
-                     const Tensor& scale2, const Maybe& y2, const Maybe& gate2, Maybe x_out2, Tensor q2,
-                     Tensor row_scale2, double eps) {
-  int8_adaln_sets({{x, shift, scale, y, gate, x_out, q, row_scale}, {x2, shift2, scale2, y2, gate2, x_out2, q2, row_scale2}},
-                  eps);
+std::tuple<Tensor, Tensor, Tensor, Tensor> int8_adaln_pair(
+    const Tensor& x, const Tensor& shift, const Tensor& scale, const Maybe& y, const Maybe& gate, Maybe x_out,
+    const Tensor& x2, const Tensor& shift2, const Tensor& scale2, const Maybe& y2, const Maybe& gate2, Maybe x_out2,
+    double eps) {
+  auto made = int8_adaln_sets({{x, shift, scale, y, gate, x_out}, {x2, shift2, scale2, y2, gate2, x_out2}}, eps);
+  return {std::move(made[0]), std::move(made[1]), std::move(made[2]), std::move(made[3])};
 }
 
 // Checks of a weight [columns, padded] with its scales and bias.
@@ -498,19 +523,38 @@ void int8_linear_sets(std::initializer_list<LinearSet> sets, bool gelu) {
         "hb_int8_linear");
 }
 
-void int8_linear(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
-                 const Maybe& bias, Tensor out, bool gelu) {
+void int8_linear_out(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
+                     const Maybe& bias, Tensor out, bool gelu) {
+  if (!out.numel() && out.is_cuda()) return;
   int8_linear_sets({{q, scale, weight, weight_scale, bias, out}}, gelu);
 }
 
-void int8_linear_pair(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
+Tensor int8_linear(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
+                   const Maybe& bias, at::ScalarType dtype, bool gelu) {
+  type_of(dtype, "rows");
+  TORCH_CHECK_VALUE((q.dim() == 2 || q.dim() == 3) && weight.dim() == 2,
+                    "rows must be [rows, padded] or [B, rows, padded] and weight [columns, padded]");
+  auto sizes = q.sizes().vec();
+  sizes.back() = weight.size(0);
+  Tensor out = at::empty(sizes, q.options().dtype(dtype));
+  int8_linear_out(q, scale, weight, weight_scale, bias, out, gelu);
+  return out;
+}
+
+// int8_rows and int8_linear in one call: a short layer's time is the host's.
+Tensor int8_linear_rows(const Tensor& x, const Tensor& weight, const Tensor& weight_scale, const Maybe& bias, bool gelu) {
+  const auto [q, scale] = int8_rows(x);
+  return int8_linear(q, scale, weight, weight_scale, bias, x.scalar_type(), gelu);
+}
+
+void int8_linear_pair_out(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
                       const Maybe& bias, Tensor out, const Tensor& q2, const Tensor& scale2, const Tensor& weight2,
                       const Tensor& weight_scale2, const Maybe& bias2, Tensor out2, bool gelu) {
   int8_linear_sets({{q, scale, weight, weight_scale, bias, out}, {q2, scale2, weight2, weight_scale2, bias2, out2}}, gelu);
 }
 
 // The text set's tensors are given together or not at all (its bias and norms may be missing).
-void int8_qkv(const Maybe& text_q, const Maybe& text_scale, const Maybe& text_weight, const Maybe& text_weight_scale,
+void int8_qkv_out(const Maybe& text_q, const Maybe& text_scale, const Maybe& text_weight, const Maybe& text_weight_scale,
               const Maybe& text_bias, const Maybe& text_norm_q, const Maybe& text_norm_k, const Tensor& q,
               const Tensor& scale, const Tensor& weight, const Tensor& weight_scale, const Maybe& bias,
               const Maybe& norm_q, const Maybe& norm_k, const Maybe& cos, const Maybe& sin, Tensor out, double eps) {
@@ -568,8 +612,10 @@ void int8_qkv(const Maybe& text_q, const Maybe& text_scale, const Maybe& text_we
 // The attention operators and the 8-bit ones return nothing and write `out` and `lse` (and the like),
 // which torch's own boxed fallbacks overlook: they look after returned tensors only.
 
-constexpr const char* WRITING[] = {"paired_fwd", "sparse_fwd", "int8_rows", "int8_adaln", "int8_adaln_pair",
-                                   "int8_linear", "int8_linear_pair", "int8_qkv"};
+// (the 8-bit operators that return their results write nothing)
+constexpr const char* WRITING[] = {"paired_fwd", "sparse_fwd", "int8_adaln", "int8_adaln_pair", "int8_linear_out",
+                                   "int8_linear_pair_out", "int8_qkv_out"};
+constexpr const char* RETURNING[] = {"int8_rows", "int8_linear", "int8_linear_rows"};
 
 // No derivative is recorded (the entry points refuse inputs that need one); a transform that takes one
 // is refused, as torch refuses an autograd.Function in one, for it would get zeros.
@@ -621,20 +667,22 @@ TORCH_LIBRARY(hilberta_hip, m) {
   m.def("pair_rows(Tensor kv_indices, Tensor kv_counts, SymInt total_blocks, SymInt key_block_size, "
         "SymInt paired_width) -> (Tensor, Tensor, Tensor)", tags);
   m.def("gather_rows(Tensor x, SymInt dim, Tensor index) -> Tensor", tags);
-  m.def("int8_rows(Tensor x, Tensor(a1!) q, Tensor(a2!) scale) -> ()", tags);
-  const std::string ada = "Tensor x$, Tensor shift$, Tensor scale$, Tensor? y$, Tensor? gate$, Tensor(x$!)? x_out$, "
-                          "Tensor(q$!) q$, Tensor(s$!) row_scale$, ",
+  m.def("int8_rows(Tensor x) -> (Tensor, Tensor)", tags);
+  const std::string ada = "Tensor x$, Tensor shift$, Tensor scale$, Tensor? y$, Tensor? gate$, Tensor(x$!)? x_out$, ",
                     linear = "Tensor q$, Tensor scale$, Tensor weight$, Tensor weight_scale$, Tensor? bias$, "
                              "Tensor(o$!) out$, ";
   const auto set = [](std::string text, const std::string& suffix) {
     for (size_t at; (at = text.find('$')) != std::string::npos;) text.replace(at, 1, suffix);
     return text;
   };
-  m.def(("int8_adaln(" + set(ada, "") + "float eps) -> ()").c_str(), tags);
-  m.def(("int8_adaln_pair(" + set(ada, "") + set(ada, "2") + "float eps) -> ()").c_str(), tags);
-  m.def(("int8_linear(" + set(linear, "") + "bool gelu) -> ()").c_str(), tags);
-  m.def(("int8_linear_pair(" + set(linear, "") + set(linear, "2") + "bool gelu) -> ()").c_str(), tags);
-  m.def("int8_qkv(Tensor? text_q, Tensor? text_scale, Tensor? text_weight, Tensor? text_weight_scale, "
+  m.def(("int8_adaln(" + set(ada, "") + "float eps) -> (Tensor, Tensor)").c_str(), tags);
+  m.def(("int8_adaln_pair(" + set(ada, "") + set(ada, "2") + "float eps) -> (Tensor, Tensor, Tensor, Tensor)").c_str(), tags);
+  m.def("int8_linear(Tensor q, Tensor scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType dtype, "
+        "bool gelu) -> Tensor", tags);
+  m.def("int8_linear_rows(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias, bool gelu) -> Tensor", tags);
+  m.def(("int8_linear_out(" + set(linear, "") + "bool gelu) -> ()").c_str(), tags);
+  m.def(("int8_linear_pair_out(" + set(linear, "") + set(linear, "2") + "bool gelu) -> ()").c_str(), tags);
+  m.def("int8_qkv_out(Tensor? text_q, Tensor? text_scale, Tensor? text_weight, Tensor? text_weight_scale, "
         "Tensor? text_bias, Tensor? text_norm_q, Tensor? text_norm_k, Tensor q, Tensor scale, Tensor weight, "
         "Tensor weight_scale, Tensor? bias, Tensor? norm_q, Tensor? norm_k, Tensor? cos, Tensor? sin, "
         "Tensor(a16!) out, float eps) -> ()", tags);
@@ -657,8 +705,10 @@ void int8_operators(torch::Library& m) {
   m.impl("int8_adaln", int8_adaln);
   m.impl("int8_adaln_pair", int8_adaln_pair);
   m.impl("int8_linear", int8_linear);
-  m.impl("int8_linear_pair", int8_linear_pair);
-  m.impl("int8_qkv", int8_qkv);
+  m.impl("int8_linear_rows", int8_linear_rows);
+  m.impl("int8_linear_out", int8_linear_out);
+  m.impl("int8_linear_pair_out", int8_linear_pair_out);
+  m.impl("int8_qkv_out", int8_qkv_out);
 }
 TORCH_LIBRARY_IMPL(hilberta_hip, CUDA, int8_hip) { int8_operators(int8_hip); }
 TORCH_LIBRARY_IMPL(hilberta_hip, CPU, int8_cpu) { int8_operators(int8_cpu); }
@@ -675,6 +725,8 @@ TORCH_LIBRARY_IMPL(hilberta_hip, Autograd, m) {
   for (const char* name : {"pair_rows", "gather_rows"})
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
   for (const char* name : WRITING)
+    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&no_derivative>());
+  for (const char* name : RETURNING)
     m.impl(name, torch::CppFunction::makeFromBoxedFunction<&no_derivative>());
 }
 

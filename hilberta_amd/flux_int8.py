@@ -24,11 +24,10 @@ from typing import NamedTuple
 
 import torch
 
-from . import _lib, ops
+from . import ops
 
 HEAD_DIM = 128
 MAX_FEATURES = 1 << 17  # a sum of so many products fits 32 bits
-_DTYPES = (torch.bfloat16, torch.float16)
 
 
 def padded_features(features):
@@ -56,92 +55,86 @@ class Int8Weight(NamedTuple):
 
 
 def _inference(*tensors):
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]):
-        raise ValueError("Inference only; disable autograd")
-
-
-def _new_rows(x):
-    """Unwritten 8-bit rows for x [..., features]."""
-    if x.dtype not in _DTYPES:
-        raise ValueError("rows must be bf16 or fp16")
-    *lead, features = x.shape
-    if x.ndim not in (2, 3) or not 0 < features <= MAX_FEATURES:
-        raise ValueError(f"rows must be [rows, features] or [B, rows, features] of 1 to {MAX_FEATURES} features")
-    return Int8Rows(torch.empty(*lead, padded_features(features), dtype=torch.int8, device=x.device),
-                    torch.empty(lead, dtype=torch.float32, device=x.device), features, x.dtype)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("Inference only; disable autograd")
 
 
 def quantize_rows(x):
     """Int8Rows of 16-bit rows x [rows, features] or [B, rows, features] (contiguous last dimension)."""
     _inference(x)
-    out = _new_rows(x)
-    if out.scale.numel() or not x.is_cuda:
-        ops.int8_rows(x, out.q, out.scale)
-    return out
+    q, scale = ops.int8_rows(x)
+    return Int8Rows(q, scale, x.shape[-1], x.dtype)
 
 
 def quantize_weight(weight):
     """Int8Weight of a 16-bit weight [out_features, in_features]."""
     if weight.ndim != 2 or not weight.numel():
         raise ValueError("weight must be a nonempty [out_features, in_features] matrix")
-    q, scale, features, _ = quantize_rows(weight.detach())
-    return Int8Weight(q, scale, features)
-
-
-def _adaln(x, shift, scale, y=None, gate=None, x_out=None):
-    _inference(x, shift, scale, y, gate, x_out)
-    if x.ndim != 3:
-        raise ValueError("x must be [B, rows, hidden] with a contiguous last dimension")
-    rows = _new_rows(x)
-    return (x, shift, scale, y, gate, x_out, rows.q, rows.scale), rows
+    q, scale = ops.int8_rows(weight.detach())
+    return Int8Weight(q, scale, weight.shape[1])
 
 
 def adaln_quantize(x, shift, scale, *, y=None, gate=None, x_out=None, eps=1e-6):
     """Int8Rows of shift + LayerNorm(r) * (1 + scale), r = x + gate * y, in one pass; r is stored in
     ``x_out`` (which may be x) rounded, and normalised before that rounding.  Arguments as
     flux_norm.adaln_modulate's; hidden is any multiple of 8 up to 8192."""
-    args, rows = _adaln(x, shift, scale, y, gate, x_out)
-    if rows.scale.numel() or not x.is_cuda:
-        ops.int8_adaln(*args, eps)
-    return rows
+    _inference(x, shift, scale, y, gate, x_out)
+    q, row_scale = ops.int8_adaln(x, shift, scale, y, gate, x_out, eps)
+    return Int8Rows(q, row_scale, x.shape[-1], x.dtype)
 
 
 def adaln_quantize_pair(first, second, *, eps=1e-6):
     """adaln_quantize of two row sets in one launch: ``first`` and ``second`` are its arguments as dicts, of
     one batch, hidden size, dtype and device.  Returns both Int8Rows."""
-    a, rows_a = _adaln(**first)
-    b, rows_b = _adaln(**second)
-    ops.int8_adaln_pair(*a, *b, eps)
-    return rows_a, rows_b
+    sets = [(s["x"], s["shift"], s["scale"], s.get("y"), s.get("gate"), s.get("x_out")) for s in (first, second)]
+    _inference(*sets[0], *sets[1])
+    q, scale, q2, scale2 = ops.int8_adaln_pair(*sets[0], *sets[1], eps)
+    x, x2 = first["x"], second["x"]
+    return Int8Rows(q, scale, x.shape[-1], x.dtype), Int8Rows(q2, scale2, x2.shape[-1], x2.dtype)
 
 
 def _rows(x):
     return x if isinstance(x, Int8Rows) else quantize_rows(x)
 
 
-def _linear(x, weight, bias=None, out=None):
-    _inference(bias, out)
-    x = _rows(x)
-    q, scale, features, dtype = x
+def _check_features(weight, features):
     if weight.features != features:
         raise ValueError(f"the weight takes {weight.features} features, the rows have {features}")
-    if out is None:
-        if dtype not in _DTYPES:
-            raise ValueError("rows must be bf16 or fp16")
-        out = torch.empty(*q.shape[:-1], weight.q.shape[0], dtype=dtype, device=q.device)
-    elif out.dtype != dtype:
-        raise ValueError("out must have the rows' dtype")
-    return (q, scale, weight.q, weight.scale, bias, out), out
 
 
 def int8_linear(x, weight, bias=None, *, gelu=False, out=None):
     """act(x @ weight^T + bias) for x Int8Rows, or 16-bit rows that are quantized first, and an Int8Weight;
     act is GELU(tanh) with ``gelu``.  bias [out_features] in the rows' dtype.  ``out`` [..., rows,
     out_features] may be a row range or a column block of a larger buffer."""
-    args, out = _linear(x, weight, bias, out)
-    if out.numel() or not out.is_cuda:
-        ops.int8_linear(*args, gelu)
-    return out
+    if out is not None:
+        args, out = _linear(x, weight, bias, out)
+        ops.int8_linear_out(*args, gelu)
+        return out
+    w, w_scale, features = weight
+    if isinstance(x, Int8Rows):
+        _inference(bias)
+        q, scale, n, dtype = x
+        if n != features:
+            _check_features(weight, n)
+        return ops.int8_linear(q, scale, w, w_scale, bias, dtype, gelu)
+    _inference(x, bias)
+    if x.shape[-1] != features:
+        _check_features(weight, x.shape[-1])
+    return ops.int8_linear_rows(x, w, w_scale, bias, gelu)
+
+
+def _linear(x, weight, bias=None, out=None):
+    """Arguments of one row set for the operators that write ``out``, and it."""
+    _inference(bias, out)
+    q, scale, features, dtype = _rows(x)
+    _check_features(weight, features)
+    if out is None:
+        out = torch.empty(*q.shape[:-1], weight.q.shape[0], dtype=dtype, device=q.device)
+    elif out.dtype != dtype:
+        raise ValueError("out must have the rows' dtype")
+    return (q, scale, weight.q, weight.scale, bias, out), out
 
 
 def int8_linear_pair(first, second, *, gelu=False):
@@ -149,7 +142,7 @@ def int8_linear_pair(first, second, *, gelu=False):
     out, of one batch, layer shape, dtype and device.  Returns both outputs."""
     a, out_a = _linear(**first)
     b, out_b = _linear(**second)
-    ops.int8_linear_pair(*a, *b, gelu)
+    ops.int8_linear_pair_out(*a, *b, gelu)
     return out_a, out_b
 
 
@@ -177,11 +170,9 @@ def int8_qkv(text, image, *, heads, weights, biases=(None, None), norms=((None, 
     B, n = image.q.shape[:2]
     N = n + (0 if text is None else text.q.shape[-2])
     if out is None:
-        if image.dtype not in _DTYPES:
-            raise ValueError("rows must be bf16 or fp16")
         out = torch.empty(3, B, N, heads, HEAD_DIM, dtype=image.dtype, device=image.q.device)
     elif out.dtype != image.dtype:
         raise ValueError("out must have the rows' dtype")
     t = (None,) * 7 if text is None else (text.q, text.scale, wt.q, wt.scale, bt, qt, kt)
-    ops.int8_qkv(*t, image.q, image.scale, wi.q, wi.scale, bi, qi, ki, cos, sin, out, eps)
+    ops.int8_qkv_out(*t, image.q, image.scale, wi.q, wi.scale, bi, qi, ki, cos, sin, out, eps)
     return out

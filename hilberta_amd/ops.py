@@ -13,13 +13,15 @@ implementation for tracing and, for pair_rows alone, a CPU one:
   hilberta_hip::gather_rows(x, dim, index) -> Tensor
   hilberta_hip::pair_rows(kv_indices, kv_counts, total_blocks, key_block_size, paired_width)
                            -> (ids, flags, counts)
-  hilberta_hip::int8_rows(x, q!, scale!) -> ()
-  hilberta_hip::int8_adaln(x, shift, scale, y?, gate?, x_out!?, q!, row_scale!, eps) -> ()
-  hilberta_hip::int8_linear(q, scale, weight, weight_scale, bias?, out!, gelu) -> ()
-  hilberta_hip::int8_qkv(text_q?, text_scale?, text_weight?, text_weight_scale?, text_bias?, text_norm_q?,
-                         text_norm_k?, q, scale, weight, weight_scale, bias?, norm_q?, norm_k?, cos?, sin?,
-                         out!, eps) -> ()
-  hilberta_hip::int8_adaln_pair, int8_linear_pair: two row sets' arguments (the second's names end in 2)
+  hilberta_hip::int8_rows(x) -> (q, scale)
+  hilberta_hip::int8_adaln(x, shift, scale, y?, gate?, x_out!?, eps) -> (q, row_scale)
+  hilberta_hip::int8_linear(q, scale, weight, weight_scale, bias?, dtype, gelu) -> Tensor
+  hilberta_hip::int8_linear_rows(x, weight, weight_scale, bias?, gelu) -> Tensor  (int8_rows, then int8_linear)
+  hilberta_hip::int8_linear_out(q, scale, weight, weight_scale, bias?, out!, gelu) -> ()
+  hilberta_hip::int8_qkv_out(text_q?, text_scale?, text_weight?, text_weight_scale?, text_bias?, text_norm_q?,
+                             text_norm_k?, q, scale, weight, weight_scale, bias?, norm_q?, norm_k?, cos?, sin?,
+                             out!, eps) -> ()
+  hilberta_hip::int8_adaln_pair, int8_linear_pair_out: two row sets' arguments (the second's names end in 2)
 
 The attention ops write into caller-provided outputs (declared mutated), as the reference's
 launches write into ``out``.  Argument checks with the reference's messages stay in the Python
@@ -58,6 +60,24 @@ def _fake_gather_rows(x, dim, index):
     return x.new_empty(shape)
 
 
+def _fake_int8_rows(x, *args):
+    *lead, features = x.shape
+    return (x.new_empty((*lead, (features + 63) // 64 * 64), dtype=torch.int8),
+            x.new_empty(lead, dtype=torch.float32))
+
+
+def _fake_int8_adaln_pair(x, shift, scale, y, gate, x_out, x2, *args):
+    return (*_fake_int8_rows(x), *_fake_int8_rows(x2))
+
+
+def _fake_int8_linear(q, scale, weight, weight_scale, bias, dtype, gelu):
+    return q.new_empty((*q.shape[:-1], weight.shape[0]), dtype=dtype)
+
+
+def _fake_int8_linear_rows(x, weight, weight_scale, bias, gelu):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]))
+
+
 def _pair_rows_cpu(kv_indices: Tensor, kv_counts: Tensor, total_blocks: int, key_block_size: int,
                    paired_width: int) -> tuple[Tensor, Tensor, Tensor]:
     """pair_rows of CPU tensors by hb_pair_rows_host."""
@@ -91,19 +111,23 @@ def _load():
                            f"include/hilberta_hip.h declares ABI {declared}: rebuild the libraries "
                            "(python -m hilberta_amd.build)")
     fakes = dict(paired_fwd=_fake_none, sparse_fwd=_fake_none, pair_rows=_fake_pair_rows,
-                 gather_rows=_fake_gather_rows, **dict.fromkeys(_INT8_NAMES, _fake_none))
+                 gather_rows=_fake_gather_rows, int8_rows=_fake_int8_rows, int8_adaln=_fake_int8_rows,
+                 int8_adaln_pair=_fake_int8_adaln_pair, int8_linear=_fake_int8_linear,
+                 int8_linear_rows=_fake_int8_linear_rows, int8_linear_out=_fake_none,
+                 int8_linear_pair_out=_fake_none, int8_qkv_out=_fake_none)
     for name, fake in fakes.items():
         torch.library.register_fake(f"{_NS}::{name}", fake)
     torch.library.impl(f"{_NS}::pair_rows", "cpu", _pair_rows_cpu)
     return [getattr(getattr(torch.ops, _NS), name).default for name in _NAMES]
 
 
-_INT8_NAMES = ("int8_rows", "int8_adaln", "int8_adaln_pair", "int8_linear", "int8_linear_pair", "int8_qkv")
 _NAMES = ("paired_fwd", "sparse_fwd", "pair_rows", "gather_rows", "_attention_workspace",
-          "_workspace_keys", "_clear_workspaces", *_INT8_NAMES)
+          "_workspace_keys", "_clear_workspaces", "int8_rows", "int8_adaln", "int8_adaln_pair", "int8_linear",
+          "int8_linear_rows", "int8_linear_out", "int8_linear_pair_out", "int8_qkv_out")
 try:
     _bound = _load()
 except (RuntimeError, OSError) as e:  # the package still imports, so that it can be (re)built
     _bound = [_Missing(name, str(e)) for name in _NAMES]
 (paired_fwd, sparse_fwd, pair_rows, gather_rows, attention_workspace, workspace_keys, clear_workspaces,
- int8_rows, int8_adaln, int8_adaln_pair, int8_linear, int8_linear_pair, int8_qkv) = _bound
+ int8_rows, int8_adaln, int8_adaln_pair, int8_linear, int8_linear_rows, int8_linear_out, int8_linear_pair_out,
+ int8_qkv_out) = _bound

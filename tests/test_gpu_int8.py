@@ -484,8 +484,14 @@ def test_operators_are_traceable():
     s = _chain_state(35)
     x, w = quantize_rows(s["x"]), s["wo"]
     out = torch.empty(2, 100, 300, dtype=BF16, device="cuda")
-    torch.library.opcheck(torch.ops.hilberta_hip.int8_linear.default, (x.q, x.scale, w.q, w.scale, s["bo"], out, True),
-                          test_utils=("test_schema", "test_faketensor"))
+    hip, checks = torch.ops.hilberta_hip, ("test_schema", "test_faketensor")
+    for op, args in ((hip.int8_rows, (s["x"],)), (hip.int8_linear, (x.q, x.scale, w.q, w.scale, s["bo"], BF16, True)),
+                     (hip.int8_linear_rows, (s["x"], w.q, w.scale, None, False)),
+                     (hip.int8_linear_out, (x.q, x.scale, w.q, w.scale, s["bo"], out, True)),
+                     (hip.int8_adaln, (s["x"], s["sh"], s["sc"], s["y"], s["g"], s["xo"], 1e-6)),
+                     (hip.int8_adaln_pair, (s["x"], s["sh"], s["sc"], s["y"], s["g"], s["xo"],
+                                            s["c"], s["sh"], s["sc"], None, None, None, 1e-6))):
+        torch.library.opcheck(op.default, args, test_utils=checks)
 
 
 def test_writes_count_for_autograd():
