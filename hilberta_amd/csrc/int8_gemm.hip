@@ -715,7 +715,7 @@ float estimate(const Args& a, int count, Kernel k, bool qkv) {
   const Shape& s = SHAPES[k];
   const int tc = channels_of(k, qkv);
   const float tiles = (float)tiles_of(a, count, tc, s.tt), stages = (float)((a.padded + 127) / 128), cus = 256.f;
-  if (k <= ROWS32) return 3.f + tiles * (float)(tc + s.tt) * (float)a.padded / 7.5e6f;
+  if (k <= ROWS32) return 3.f + tiles * (float)(tc + s.tt) * (float)a.padded / 6.5e6f;
   const float rounds = std::floor(tiles / cus), rest = tiles / cus - rounds;
   return 2.3f + rounds * (s.round + stages * (s.stage + s.full)) +
          (rest > 0.f ? s.round + stages * (s.stage + s.full * rest * rest) : 0.f);
@@ -731,7 +731,7 @@ struct Choice {
 // 11.3).  The others, 32 x 32 blocks / 64 x 128 / 128 x 128 / 256 x 256 tiles: 64 x 3072 x 3072 8.5 / 10.6 / 14.7 /
 // 32.4; 200 x 1024 x 1024 4.6 / 6.8 / 9.3 / 15.6; 128 x 3072 x 12288 37 / 13.6 / 17.0 / 32.7; 512 x 12288 x 3072 128 /
 // 33 / 41 / 111; 256 x 3072 x 9216 56 / 24 / 17.4 / 34; 512 x 3072 x 9216 101 / 35 / 34 / 36; 4096 x 3072 x 3072 - / 70 /
-// 57 / 42; 16384 x 256 x 256 - / 10.7 / 8.4 / 10.3.  Blocks are as long as the bytes they read, at 7.5 TB/s.
+// 57 / 42; 16384 x 256 x 256 - / 10.7 / 8.4 / 10.3.  Blocks are as long as the bytes they read, at 6.5 TB/s.
 Choice choose(const Args& a, int count, bool qkv) {
   uint32_t tokens = 0;
   for (int i = 0; i < count; ++i) tokens = std::max(tokens, a.set[i].tokens);
