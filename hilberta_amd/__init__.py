@@ -14,6 +14,8 @@ rebuilt on hand-written HIP kernels behind a C ABI (include/hilberta_hip.h):
   flux_model / sampling_layout
                     a FLUX-shaped denoiser step on these kernels and the sampling-scope layout
   flux_cond         conditioning layers of a few rows (embedders, modulations), streamed by HIP
+  flux_int8         the blocks' linear layers in 8-bit integers: rows, AdaLN rows, products, and the Q/K/V
+                    projection with the heads' RMSNorm and rotation in the same pass
   ops               the entry points as native torch operators (torch.ops.hilberta_hip.*), with
                     fake implementations for tracing
 

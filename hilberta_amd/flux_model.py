@@ -30,7 +30,8 @@ modulation (flux_norm.adaln_modulate).  Two attention modes:
     (sparse_kernel.sparse_attention on unpaired tables) and ``sdpa_reference`` (dense-mask SDPA,
     a correctness reference as at flux_adapter.py:299-306).
 
-Weights and activations are bf16; there is no CPU path.
+Weights and activations are bf16; ``FluxTransformer.quantize`` holds the blocks' linear layers in 8-bit
+integers instead (flux_int8).  There is no CPU path.
 """
 
 from __future__ import annotations
@@ -43,6 +44,14 @@ import torch.nn.functional as F
 
 from .flux_cond import embed, linear_layers, timestep_projection  # noqa: F401
 from .flux_inputs import qk_prep_pair, rotary_tables
+from .flux_int8 import (
+    adaln_quantize,
+    adaln_quantize_pair,
+    int8_linear,
+    int8_linear_pair,
+    int8_qkv,
+    quantize_weight,
+)
 from .flux_norm import adaln_modulate, adaln_modulate_pair
 from .layout import index_select_rows
 
@@ -313,6 +322,7 @@ class FluxTransformer:
             ))
         self.norm_out = init.linear(2 * C, C, mod_std)
         self.proj_out = init.linear(s.in_channels, C)
+        self.int8 = False
 
     def parameters(self):
         def walk(x):
@@ -416,6 +426,133 @@ class FluxTransformer:
             return h, hn
         return None, adaln_modulate(h[:, T:], shift, scale, y=p[:, T:], gate=gate, eps=s.eps)
 
+    def _blocks(self, x, c, cos, sin, attention, double_mods, single_mods, out_mods):
+        """All blocks on embedded image rows x and text rows c; the image rows as the output norm modulates
+        them."""
+        s = self.shape
+        (B, n, _), T = x.shape, c.shape[1]
+        (sx, scx, *_), (sc, scc, *_) = double_mods[0]
+        xn, cn = adaln_modulate_pair(dict(x=x, shift=sx, scale=scx), dict(x=c, shift=sc, scale=scc), eps=s.eps)
+        h = torch.empty(B, T + n, s.hidden, device=x.device, dtype=x.dtype)
+        hn = torch.empty_like(h)
+        for i, w in enumerate(self.double):
+            last = i == len(self.double) - 1
+            if last:
+                nxt = single_mods[0][:2] if self.single else out_mods
+                self._double_block(w, double_mods[i], x, xn, c, cn, cos, sin, attention, i, nxt, (h, hn))
+            else:
+                (nsx, nscx, *_), (nsc, nscc, *_) = double_mods[i + 1]
+                x, xn, c, cn = self._double_block(w, double_mods[i], x, xn, c, cn, cos, sin, attention, i,
+                                                  ((nsx, nscx), (nsc, nscc)), None)
+        del x, xn, c, cn
+        for j, w in enumerate(self.single):
+            nxt = single_mods[j + 1][:2] if j + 1 < len(self.single) else out_mods
+            h, hn = self._single_block(w, single_mods[j], h, hn, T, cos, sin, attention,
+                                       s.num_layers + j, nxt)
+        if hn.shape[1] != n:   # no single blocks: the last double block modulated every row
+            hn = hn[:, T:]
+        return hn
+
+    # ------------------------------------------------------------------ blocks in 8 bits
+    def quantize(self):
+        """Hold the blocks' linear layers in 8-bit integers, one scale an output channel, and run them on
+        8-bit rows, one scale a token (flux_int8); the embedders, the modulations and the output layer stay
+        as they are.  Halves the blocks' weights; the 16-bit ones are dropped.  Returns self."""
+        if self.int8:
+            return self
+        if not self.double:
+            raise ValueError("a transformer without double blocks has no 8-bit form")
+        for w in self.double:
+            for name in ("qkv_x", "qkv_c", "out_x", "out_c"):
+                w[name] = (quantize_weight(w[name][0]), w[name][1])
+            for name in ("ff_x", "ff_c"):
+                w[name] = tuple((quantize_weight(a), b) for a, b in w[name])
+        for w in self.single:
+            for name in ("qkv", "mlp"):
+                w[name] = (quantize_weight(w[name][0]), w[name][1])
+            (wa, ba), (wm, _) = w.pop("out_attn"), w.pop("out_mlp")
+            w["out"] = (quantize_weight(torch.cat([wa, wm], 1)), ba)  # over [attention | mlp] columns
+        self.int8 = True
+        return self
+
+    def _double_block_int8(self, w, mods, x, xn, c, cn, cos, sin, attention, layer, next_mods, joint_out):
+        """_double_block with xn, cn Int8Rows.  With ``joint_out`` = h [B, N, C] the residual streams end
+        there; returns (x, xn, c, cn), the first and third None then.  ``next_mods`` are the (shift, scale)
+        pairs of the image and text rows."""
+        s, H = self.shape, self.shape.heads
+        T = c.shape[1]
+        (_, _, gx, sx2, scx2, gx2), (_, _, gc, sc2, scc2, gc2) = mods
+        q, k, v = int8_qkv(cn, xn, heads=H, weights=(w["qkv_c"][0], w["qkv_x"][0]),
+                           biases=(w["qkv_c"][1], w["qkv_x"][1]), eps=s.eps, cos=cos, sin=sin,
+                           norms=((w["norm_added_q"], w["norm_q"]), (w["norm_added_k"], w["norm_k"])))
+        o = torch.empty_like(q)
+        self._attend(attention, layer, q, k, v, o)
+        del q, k, v
+        o = o.flatten(2)
+        ax, ac = int8_linear_pair(dict(x=o[:, T:], weight=w["out_x"][0], bias=w["out_x"][1]),
+                                  dict(x=o[:, :T], weight=w["out_c"][0], bias=w["out_c"][1]))
+        del o
+        xn, cn = adaln_quantize_pair(dict(x=x, shift=sx2, scale=scx2, y=ax, gate=gx, x_out=x),
+                                     dict(x=c, shift=sc2, scale=scc2, y=ac, gate=gc, x_out=c), eps=s.eps)
+        del ax, ac
+        (w1x, w2x), (w1c, w2c) = w["ff_x"], w["ff_c"]
+        fx, fc = int8_linear_pair(dict(x=xn, weight=w1x[0], bias=w1x[1]), dict(x=cn, weight=w1c[0], bias=w1c[1]),
+                                  gelu=True)
+        fx, fc = int8_linear_pair(dict(x=fx, weight=w2x[0], bias=w2x[1]), dict(x=fc, weight=w2c[0], bias=w2c[1]))
+        (nsx, nscx), (nsc, nscc) = next_mods
+        hx, hc = (x, c) if joint_out is None else (joint_out[:, T:], joint_out[:, :T])
+        xn, cn = adaln_quantize_pair(dict(x=x, shift=nsx, scale=nscx, y=fx, gate=gx2, x_out=hx),
+                                     dict(x=c, shift=nsc, scale=nscc, y=fc, gate=gc2, x_out=hc), eps=s.eps)
+        return (x, xn, c, cn) if joint_out is None else (None, xn, None, cn)
+
+    def _single_block_int8(self, w, mods, h, hn, T, cos, sin, attention, layer, next_mods):
+        """_single_block with hn Int8Rows of the joint rows, or a pair of the text and image rows' (after the
+        last double block)."""
+        s, C, H = self.shape, self.shape.hidden, self.shape.heads
+        B, N, _ = h.shape
+        wq, bq = w["qkv"]
+        wm, bm = w["mlp"]
+        text, image = hn if type(hn) is tuple else (None, hn)
+        norms = ((w["norm_q"], w["norm_q"]), (w["norm_k"], w["norm_k"]))
+        q, k, v = int8_qkv(text, image, heads=H, weights=(wq, wq), biases=(bq, bq), norms=norms, eps=s.eps,
+                           cos=cos, sin=sin)
+        both = h.new_empty(B, N, C + s.mlp_hidden)                          # [attention | GELU(proj_mlp)]
+        if text is None:
+            int8_linear(image, wm, bm, gelu=True, out=both[..., C:])
+        else:
+            int8_linear_pair(dict(x=text, weight=wm, bias=bm, out=both[:, :T, C:]),
+                             dict(x=image, weight=wm, bias=bm, out=both[:, T:, C:]), gelu=True)
+        self._attend(attention, layer, q, k, v, both[..., :C].unflatten(-1, (H, s.head_dim)))
+        del q, k, v
+        p = int8_linear(both, *w["out"])
+        del both
+        shift, scale = next_mods
+        if layer < s.blocks - 1:
+            return h, adaln_quantize(h, shift, scale, y=p, gate=mods[2], x_out=h, eps=s.eps)
+        return None, adaln_modulate(h[:, T:], shift, scale, y=p[:, T:], gate=mods[2], eps=s.eps)
+
+    def _blocks_int8(self, x, c, cos, sin, attention, double_mods, single_mods, out_mods):
+        """All blocks on embedded image rows x and text rows c; the image rows as the output norm modulates
+        them (16 bits)."""
+        s, T = self.shape, c.shape[1]
+        last = len(self.double) - 1
+        # each block's first (shift, scale) for image and text rows; after the double blocks one for both
+        first = [(mx[:2], mc[:2]) for mx, mc in double_mods]
+        first.append((single_mods[0][:2],) * 2 if self.single else (out_mods,) * 2)
+        (sx, scx), (sc, scc) = first[0]
+        xn, cn = adaln_quantize_pair(dict(x=x, shift=sx, scale=scx), dict(x=c, shift=sc, scale=scc), eps=s.eps)
+        h = x.new_empty(x.shape[0], T + x.shape[1], s.hidden)
+        for i, w in enumerate(self.double):
+            x, xn, c, cn = self._double_block_int8(w, double_mods[i], x, xn, c, cn, cos, sin, attention, i,
+                                                   first[i + 1], h if i == last else None)
+        if not self.single:  # (the output layer takes 16-bit rows)
+            return adaln_modulate(h[:, T:], *out_mods, eps=s.eps)
+        hn = (cn, xn)
+        for j, w in enumerate(self.single):
+            nxt = single_mods[j + 1][:2] if j + 1 < len(self.single) else out_mods
+            h, hn = self._single_block_int8(w, single_mods[j], h, hn, T, cos, sin, attention, s.num_layers + j, nxt)
+        return hn
+
     # ------------------------------------------------------------------ forward
     def temb(self, timestep, guidance, pooled, *, silu=False):
         """Summed timestep, guidance and pooled-text embeddings [B, hidden]; with ``silu`` their
@@ -458,26 +595,8 @@ class FluxTransformer:
                                                                          pooled_projections, silu=True))
         x = _linear(hidden_states.to(self.dtype), *self.x_embedder)
         c = _linear(encoder_hidden_states.to(self.dtype), *self.context_embedder)
-        (sx, scx, *_), (sc, scc, *_) = double_mods[0]
-        xn, cn = adaln_modulate_pair(dict(x=x, shift=sx, scale=scx), dict(x=c, shift=sc, scale=scc), eps=s.eps)
-        h = torch.empty(B, N, s.hidden, device=x.device, dtype=x.dtype)
-        hn = torch.empty_like(h)
-        for i, w in enumerate(self.double):
-            last = i == len(self.double) - 1
-            if last:
-                nxt = single_mods[0][:2] if self.single else out_mods
-                self._double_block(w, double_mods[i], x, xn, c, cn, cos, sin, attention, i, nxt, (h, hn))
-            else:
-                (nsx, nscx, *_), (nsc, nscc, *_) = double_mods[i + 1]
-                x, xn, c, cn = self._double_block(w, double_mods[i], x, xn, c, cn, cos, sin, attention, i,
-                                                  ((nsx, nscx), (nsc, nscc)), None)
-        del x, xn, c, cn
-        for j, w in enumerate(self.single):
-            nxt = single_mods[j + 1][:2] if j + 1 < len(self.single) else out_mods
-            h, hn = self._single_block(w, single_mods[j], h, hn, T, cos, sin, attention,
-                                       s.num_layers + j, nxt)
-        if hn.shape[1] != n:   # no single blocks: the last double block modulated every row
-            hn = hn[:, T:]
+        hn = (self._blocks_int8 if self.int8 else self._blocks)(x, c, cos, sin, attention, double_mods, single_mods,
+                                                                out_mods)
         out = _linear(hn, *self.proj_out)
         if layout is not None and layout_scope == "transformer":
             out = index_select_rows(out, 1, layout.inverse)
