@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
+#include <utility>
 
 #include "common.h"
 #include "../../include/hilberta_hip.h"
@@ -134,13 +135,35 @@ __device__ __forceinline__ int64_t table_of(const Set& s, uint32_t at) {
 // Eight values of channels c .. c + 7 to `out`, those of them that there are.
 template <bool QKV>
 __device__ __forceinline__ void store8(const Args& a, uint16_t* out, int c, const u32x4& v) {
-  if (QKV ? c < a.columns : (a.vectors && c + 8 <= a.columns)) {
-    __builtin_nontemporal_store(v, (u32x4*)out);
+  typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint32_t words3 __attribute__((ext_vector_type(3), aligned(4)));
+  if (QKV ? c < a.columns : c + 8 <= a.columns) {
+    if (QKV || a.vectors) {
+      __builtin_nontemporal_store(v, (u32x4*)out);
+    } else if ((uintptr_t)out & 2) {
+      out[0] = (uint16_t)v[0];
+      *(words3*)(out + 1) = words3{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16};
+      out[7] = (uint16_t)(v[3] >> 16);
+    } else {
+      *(words4*)out = v;
+    }
   } else if (!QKV) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (c + k < a.columns) out[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
   }
+}
+
+// The sum over 16 neighbouring lanes, in each of them: of pairs, of quads, of the mirrored half row and row.
+template <int CONTROL>
+__device__ __forceinline__ float moved(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CONTROL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum16(float v) {
+  v += moved<0xb1>(v);
+  v += moved<0x4e>(v);
+  v += moved<0x141>(v);
+  return v + moved<0x140>(v);
 }
 
 // Two pairs (2i, 2i + 1) turned by cos and sin.
@@ -153,71 +176,35 @@ __device__ __forceinline__ void rotate(float* v, const f32x4& cos, const f32x4& 
   }
 }
 
-// The epilogue of a wave's 32 tokens from t0 on and 32 CF channels from c0 on (qkv: one head, CF = 4);
-// `channel` are those channels' values, TC apart.  Lanes l and l + 32 hold token t0 + l % 32.  After
-// pack_pair a 32-channel block of a token is four 16-byte chunks, two in each of those lanes; exchanged with
-// the lane 16 on, four lanes hold a token's four chunks, and a store writes 64 bytes a row (32 without: 16896
-// x 3072 x 12288 586 -> 580 us).  The stores bypass the caches (580 -> 571): the output is larger than they
-// are, and what they hold is wanted by the tiles to come.
-template <bool F16, bool QKV, bool GELU, int CF, int TC>
+// The epilogue of a wave's 32 tokens from t0 on and 32 CF channels from c0 on (linear); `channel` are those
+// channels' values, TC apart.  Lanes l and l + 32 hold token t0 + l % 32.  After pack_pair a 32-channel block of
+// a token is four 16-byte chunks, two in each of those lanes; exchanged with the lane 16 on, four lanes hold a
+// token's four chunks, and a store writes 64 bytes a row (32 without: 16896 x 3072 x 12288 586 -> 580 us).  The
+// stores bypass the caches (580 -> 571): the output is larger than they are, and what they hold is wanted by
+// the tiles to come.
+template <bool F16, bool GELU, int CF, int TC>
 __device__ __forceinline__ void finish(const Args& a, const Set& s, const i32x16 (&acc)[CF], float scale,
                                        const float* channel, int c0, uint32_t t0) {
-  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-  const int plane = QKV ? c0 / (a.heads * HEAD) : 2;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
   const int chunk = (lane >> 4 & 1) * 2 + half;
   uint16_t* out[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    out[h] = s.out + row_of(s, t0 + h * 16 + (lane & 15)) + (QKV ? plane * a.out_p - plane * a.heads * HEAD : 0) + c0 + chunk * 8;
+  for (int h = 0; h < 2; ++h) out[h] = s.out + row_of(s, t0 + h * 16 + (lane & 15)) + c0 + chunk * 8;
   channel += half * 4;
-  auto value = [&](int i, int r) {
-    const int c = i * 32 + (r >> 2) * 8 + (r & 3);
-    return (float)acc[i][r] * scale * channel[c] + channel[TC + c];
-  };
-  const bool heads = QKV && plane < 2;
-  float rms = 1.f;
-  if (heads) {
-    float squares = 0.f;
-#pragma unroll
-    for (int i = 0; i < CF; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = value(i, r);
-        squares += p * p;
-      }
-    squares += __shfl_xor(squares, 32, 64);
-    rms = __builtin_amdgcn_rsqf(squares * (1.f / HEAD) + a.eps);
-  }
-  // (a half block's rotary values are asked for half a block ahead)
-  f32x4 cos[2][2], sin[2][2];
-  const int64_t table = heads ? table_of(s, t0 + col) + half * 4 : 0;
-  auto ask = [&](int h) {
-    if (!heads || !a.cos) return;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      cos[h & 1][g] = *(const f32x4*)(a.cos + table + h * 16 + g * 8);
-      sin[h & 1][g] = *(const f32x4*)(a.sin + table + h * 16 + g * 8);
-    }
-  };
-  if (QKV) ask(0);
 #pragma unroll
   for (int i = 0; i < CF; ++i) {
     u32x4 packed[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      if (QKV && 2 * i + p + 1 < 2 * CF) ask(2 * i + p + 1);
       float v[2][4];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const int c = i * 32 + (2 * p + g) * 8;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          float y = value(i, 8 * p + 4 * g + k);
-          if (GELU) y = gelu(y);
-          if (heads) y *= rms * channel[2 * TC + c + k];
-          v[g][k] = y;
+          const float y = (float)acc[i][8 * p + 4 * g + k] * scale * channel[c + k] + channel[TC + c + k];
+          v[g][k] = GELU ? gelu(y) : y;
         }
-        if (heads && a.cos) rotate(v[g], cos[p][g], sin[p][g]);
       }
       packed[p] = pack_pair<F16>(v[0], v[1]);
     }
@@ -229,8 +216,134 @@ __device__ __forceinline__ void finish(const Args& a, const Set& s, const i32x16
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      if (t0 + h * 16 + (lane & 15) < s.tokens) store8<QKV>(a, out[h] + i * 32, c0 + i * 32 + chunk * 8, packed[h]);
+      if (t0 + h * 16 + (lane & 15) < s.tokens) store8<false>(a, out[h] + i * 32, c0 + i * 32 + chunk * 8, packed[h]);
     __builtin_amdgcn_sched_barrier(0);  // (a block at a time: all at once take more registers than there are)
+  }
+}
+
+// Channels c0 + c .. + 7 of token `at`, of its sums (qkv: 16 neighbouring lanes hold a head).
+template <bool F16, bool QKV, bool GELU, int TC>
+__device__ __forceinline__ void finish8(const Args& a, const Set& s, const i32x4 (&sum)[2], const float (&channel)[3][TC],
+                                        int c0, uint32_t at, int c) {
+  const int plane = QKV ? c0 / (a.heads * HEAD) : 2;
+  const float scale = s.scale[min(at, s.tokens - 1)];
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = (float)sum[k >> 2][k & 3] * scale * channel[0][c + k] + channel[1][c + k];
+  uint16_t* out = s.out + row_of(s, at) + c0 + c;
+  if (QKV) {
+    out += plane * a.out_p - plane * a.heads * HEAD;
+    if (plane < 2) {
+      float squares = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) squares += v[k] * v[k];
+      const float rms = __builtin_amdgcn_rsqf(sum16(squares) * (1.f / HEAD) + a.eps);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= rms * channel[2][c + k];
+      const int64_t table = table_of(s, at) + c;
+      if (a.cos) {
+#pragma unroll
+        for (int g = 0; g < 8; g += 4)
+          rotate(v + g, *(const f32x4*)(a.cos + table + g), *(const f32x4*)(a.sin + table + g));
+      }
+    }
+  } else if (GELU) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = gelu(v[k]);
+  }
+  if (at < s.tokens) store8<QKV>(a, out, c0 + c, pack8<F16>(v));
+}
+
+template <typename Begin, int... I>
+__device__ __forceinline__ void begin_all(Begin& begin, std::integer_sequence<int, I...>) {
+  (begin(std::integral_constant<int, I>()), ...);
+}
+// Whether one of the steps was the last.
+template <typename Step, int... I>
+__device__ __forceinline__ bool step_all(Step& step, std::integer_sequence<int, I...>) {
+  return (step(std::integral_constant<int, I>()) || ...);
+}
+
+// The epilogue of a wave's 32 tokens from t0 on and one head from c0 on (qkv).  Lanes l and l + 32 hold token
+// t0 + l % 32, and would read its rotary rows and write its output 32 bytes at a time.  So 16 tokens at a time go
+// through the wave's own part of a stage, eight pieces of 1 KB, and come back as four tokens of 16 lanes each,
+// whose reads and writes are whole lines (512 + 16384 rows x 3072, 24 heads: 511 -> 484 us).  `channel` are the head's values, TC apart.
+template <bool F16, bool TURN, int TC>
+__device__ __forceinline__ void finish_head(const Args& a, const Set& s, const i32x16 (&acc)[4], float scale,
+                                            const float* channel, int c0, uint32_t t0, int8_t* box) {
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, c = (lane & 15) * 8;
+  const int plane = c0 / (a.heads * HEAD);
+  const bool heads = TURN || plane < 2;
+  uint16_t* const out = s.out + plane * a.out_p + (c0 - plane * a.heads * HEAD) + c;
+  auto place = [&](int token) { return (token >> 1) * 8192 + (token & 1) * 512; };
+  float ws[8], bias[8], norm[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) ws[k] = channel[c + k], bias[k] = channel[TC + c + k], norm[k] = channel[2 * TC + c + k];
+  // Four tokens' places, and their rotary values, asked for four tokens ahead.
+  struct Ahead {
+    uint32_t at;
+    int64_t row;
+    f32x4 cos[2], sin[2];
+  };
+  auto ask = [&](int m) {
+    Ahead to;
+    to.at = t0 + m * 4 + (lane >> 4);
+    const uint32_t token = s.start + min(to.at, s.tokens - 1), b = token / s.rows, n = token - b * s.rows;
+    to.row = b * s.out_b + (int64_t)n * s.out_n;
+    if (TURN) {
+      const int64_t table = (int64_t)(s.first + n) * HEAD + c;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        to.cos[g] = *(const f32x4*)(a.cos + table + g * 4);
+        to.sin[g] = *(const f32x4*)(a.sin + table + g * 4);
+      }
+    }
+    return to;
+  };
+  Ahead next = ask(0);
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    if (col >> 4 == p) {
+      int token = lane & 15;
+      asm volatile("" : "+v"(token));  // (or the addresses stay in registers from here to the next tile)
+      int8_t* const to = box + place(token);
+      // (units of four channels, in an order of the token's, so that tokens' lie in different banks)
+      const int order = token ^ half;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(i32x4*)(to + (((i & 1) * 8 + g * 2) ^ order) * 16 + (i >> 1) * 256) =
+              i32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+      const Ahead now = next;
+      const int token = q * 4 + (lane >> 4);
+      next = ask(p * 4 + q + 1);
+      const float token_scale = __shfl(scale, p * 16 + token, 64);
+      i32x4 sum[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) sum[g] = *(const i32x4*)(box + place(token) + (c / 4 + g ^ token) * 16);
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = (float)sum[k >> 2][k & 3] * token_scale * ws[k] + bias[k];
+      if (heads) {
+        float squares = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) squares += v[k] * v[k];
+        const float rms = __builtin_amdgcn_rsqf(sum16(squares) * (1.f / HEAD) + a.eps);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= rms * norm[k];
+        if (TURN) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) rotate(v + 4 * g, now.cos[g], now.sin[g]);
+        }
+      }
+      if (now.at < s.tokens) __builtin_nontemporal_store(pack8<F16>(v), (u32x4*)(out + now.row));
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -266,17 +379,19 @@ struct Ends {
 
 // ------------------------------------------------------------------ many rows
 // 256 channels x 256 tokens a workgroup of eight waves, 128 x 64 each; one workgroup a CU, which walks its
-// tiles.  Bound by the loads: the same kernel without them runs at 3.0 PFLOP/s, with them at 2.4.  So the tile
-// is as large as the registers allow (128 x 256 tiles, two workgroups a CU, move half as much again), and a
-// stage is 128 features deep: a row's 128 bytes are one request to the L2 (64-byte rows, twice as many
-// requests, took that kernel from 2.4 to 1.9 PFLOP/s).
-//  * Two stages of 64 KB in LDS, by direct loads: stage n + 2 is asked for as soon as everyone has read stage n
-//    into registers, and has the whole of stage n + 1 (2048 cycles of products) to arrive.
+// tiles.  Bound by the loads: the same kernel without them runs at 3.0 POP/s, with them at 2.45 (16384 x 12288 x
+// 3072 in 504 us).  So the tile is as large as the registers allow (128 x 256 tiles, two workgroups a CU, move half
+// as much again: 620 us), and a stage is 128 features deep: a row's 128 bytes are one request to the L2 (64-byte
+// rows, twice as many requests, took the smaller tiles from 2.4 to 1.9 POP/s).
+//  * Two stages of 64 KB in LDS, by direct loads, spread among the products (asked for together they hold up the
+//    products' issue): half of stage n + 2 while the last step of stage n is multiplied, which everyone has read
+//    by then, the other half with the first step of n + 1.
 //  * The operands of a 32-feature step are read while the step before multiplies; the scheduler is held to
-//    that order (left alone it reads them just before their use: 2.25 instead of 2.44 PFLOP/s).
-//  * The last two stages of a tile ask for the first two of the next, which the epilogue then hides.
-//  * An XCD takes a run of the tiles, four token tiles by eight channel tiles at a time (bands of 8 token
-//    tiles: 16896 x 3072 x 12288 630 us, of 4: 586), so that its L2 serves both operands.
+//    that order (left alone it reads them just before their use: 2.25 instead of 2.44 POP/s).
+//  * A tile's last stage asks for the first stages of the next, which the epilogue then hides (qkv: for the
+//    first only, since its epilogue works in the second's place).
+//  * An XCD takes a run of the tiles, four token tiles by all channel tiles at a time (bands of 8 token tiles:
+//    16896 x 3072 x 12288 630 us, of 4: 586), so that its L2 serves both operands.
 constexpr int WIDE = 256, WIDE_STEP = 128, WIDE_BAND = 4;
 constexpr int WIDE_STAGE = 2 * WIDE * WIDE_STEP;     // 64 KB
 constexpr int WIDE_LOADS = WIDE_STAGE / 1024 / 8;    // 1 KB loads of a wave and stage
@@ -333,14 +448,15 @@ __global__ __launch_bounds__(512, 2) void int8_wide_kernel(Args a) {
   i32x16 acc[2][4];
   auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
   // Eight products, with loads `from` .. `from` + 3 of a stage to `dst` among them.
-  auto multiply = [&](int u, int8_t* dst = nullptr, int stage = 0, int from = 0) {
-    const int past = dst ? ends.past(uniform(stage)) : 0;
+  auto products = [&](auto loads, int u, int8_t* dst, int stage, int from) {
+    constexpr bool LOAD = decltype(loads)::value;
+    const int past = LOAD ? ends.past(uniform(stage)) : 0;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[u][i], x[u][j], acc[j][i], 0, 0, 0);
-        if (dst && i & 1) {
+        if (LOAD && i & 1) {
           pin();
           load(dst, stage, from + 2 * j + i / 2, past);
           pin();
@@ -348,13 +464,16 @@ __global__ __launch_bounds__(512, 2) void int8_wide_kernel(Args a) {
       }
     pin();
   };
+  auto multiply = [&](int u) { products(std::false_type(), u, nullptr, 0, 0); };
+  auto multiply_and_load = [&](int u, int8_t* dst, int stage, int from) { products(std::true_type(), u, dst, stage, from); };
   // A stage in `cur`, its first operands on their way to w[0], x[0], half of the next in `next` and the other
   // half asked for here.  Before the barrier everyone's part of `next` is there and nobody reads `cur` any
   // more, of which `after` then fills half.
-  auto step = [&](int8_t* cur, int8_t* next, int stage, int after, bool last) {
+  auto step = [&](auto last, int8_t* cur, int8_t* next, int stage, int after) {
+    constexpr bool LAST = decltype(last)::value;
     fetch(cur, 1);
     pin();
-    multiply(0, next, stage, 4);
+    multiply_and_load(0, next, stage, 4);
     fetch(cur, 2);
     pin();
     multiply(1);
@@ -364,9 +483,10 @@ __global__ __launch_bounds__(512, 2) void int8_wide_kernel(Args a) {
     wait_loads<0>();
     barrier();
     pin();
-    if (!last) fetch(next, 0);
+    if (!LAST) fetch(next, 0);
     pin();
-    multiply(1, cur, after, 0);
+    if (QKV && LAST) multiply(1);  // (the epilogue uses `cur`)
+    else multiply_and_load(1, cur, after, 0);
   };
   Tile t = tile_at<WIDE, WIDE, WIDE_BAND>(a, first + slot);
   aim(t);
@@ -389,15 +509,15 @@ __global__ __launch_bounds__(512, 2) void int8_wide_kernel(Args a) {
       for (int i = 0; i < 4; ++i) acc[j][i] = i32x16{};
     fetch(lds0, 0);
     for (int n = 2; n < stages; n += 2) {
-      step(lds0, lds1, n - 1, n, false);
-      step(lds1, lds0, n, n + 1, false);
+      step(std::false_type(), lds0, lds1, n - 1, n);
+      step(std::false_type(), lds1, lds0, n, n + 1);
     }
     slot += stride;
     const bool more = slot < a.tiles_xcd && first + slot < a.tiles;
     // (the second half of this tile's last stage goes by its own addresses)
     fetch(lds0, 1);
     pin();
-    multiply(0, lds1, stages - 1, 4);
+    multiply_and_load(0, lds1, stages - 1, 4);
     if (more) t = tile_at<WIDE, WIDE, WIDE_BAND>(a, first + slot);
     aim(t);  // (after the last tile: its own first stages once more, never read)
     fetch(lds0, 2);
@@ -411,41 +531,65 @@ __global__ __launch_bounds__(512, 2) void int8_wide_kernel(Args a) {
     pin();
     fetch(lds1, 0);
     pin();
-    multiply(1, lds0, 0, 0);
-    step(lds1, lds0, 0, 1, true);
+    multiply_and_load(1, lds0, 0, 0);
+    step(std::true_type(), lds1, lds0, 0, 1);
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      finish<F16, QKV, GELU, 4, WIDE>(a, s, acc[j], scale[j], &channel[parity][0][wc * 128], done.c0 + wc * 128,
-                                      done.t0 + wt * 64 + j * 32);
+    for (int j = 0; j < 2; ++j) {
+      const float* const values = &channel[parity][0][wc * 128];
+      const int c0 = done.c0 + wc * 128;
+      const uint32_t t0 = done.t0 + wt * 64 + j * 32;
+      if (!QKV) finish<F16, GELU, 4, WIDE>(a, s, acc[j], scale[j], values, c0, t0);
+      else if (c0 < a.columns && a.cos && c0 < 2 * a.heads * HEAD) finish_head<F16, true, WIDE>(a, s, acc[j], scale[j], values, c0, t0, lds1 + 1024 * wave);
+      else if (c0 < a.columns) finish_head<F16, false, WIDE>(a, s, acc[j], scale[j], values, c0, t0, lds1 + 1024 * wave);
+    }
+    if (QKV) {
+#pragma unroll
+      for (int j = 0; j < WIDE_LOADS / 2; ++j) load(lds1, 1, j, ends.past(1));
+    }
     if (!more) break;
   }
   wait_loads<0>();  // (nothing may still be on its way to LDS when the workgroup ends)
 }
 
 // ------------------------------------------------------------------ fewer rows
-// 32 CF channels x 128 tokens a workgroup of eight waves, one workgroup a CU.  With fewer tiles than CUs the
-// instructions of one workgroup bound it, not the chip's rates, so every operand is read from LDS by few
-// waves: four waves share the 128 features of a stage, 32 each, and two the tokens, 64 each.  R stages in LDS;
-// a wave multiplies one stage while it reads the next and asks for the one R - 1 on, its loads spread over its
-// products (all at once they hold up the issue of the products: 512 x 12288 x 3072 46 -> 42 us when four waves
-// shared the tokens alone).  The four sums meet in LDS.
-constexpr int TALL = 128, STEP = 128;
+// TC channels x TT tokens a workgroup of eight waves, in tiles so small that most CUs have one.  What is on its
+// way to a CU bounds it: some 80 bytes a ns and CU with 100 to 140 KB asked for ahead.  So the operands go to LDS by
+// direct loads, into a ring of R stages of 128 features, as many as there is room for (straight into registers,
+// which hold less: 1 x 3072 x 9216 qkv 15.3 us, so 10.9; 77 x 4096 x 3072 12.4 -> 9.5), the loads spread over the
+// products.  Four waves share a stage's features, 32 each, and two of each the tokens (of 32 tokens: the channels),
+// so that LDS is read by few.  The sums meet in LDS, and a thread finishes eight channels of a token: neighbouring
+// lanes read and write whole lines (a wave finishing 32 tokens as they lie in registers: 512 + 1024 x 3072 qkv
+// 88 us of 128 x 128 tiles, so 77).  Rows past the operands' ends are zeros that nothing reads.
+template <int TC, int TT>
+struct Ring {
+  static constexpr int STAGE = (TC + TT) * 128, GROUPS = STAGE / 1024, LOADS = (GROUPS + 7) / 8;
+  static constexpr int CW = TT > 32 ? TC : TC / 2, TW = TT > 32 ? TT / 2 : TT;  // of a wave
+  static constexpr int BOX = TW * CW * 4;                                       // bytes of a wave's sums
+};
 
-template <bool F16, bool QKV, bool GELU, int CF, int R>
+template <bool F16, bool QKV, bool GELU, int TC, int TT, int R>
 __global__ __launch_bounds__(512, 2) void int8_tile_kernel(Args a) {
-  constexpr int TC = 32 * CF, STAGE = (TC + TALL) * STEP, LOADS = STAGE / 8192, PRODUCTS = 2 * CF;
+  typedef Ring<TC, TT> F;
+  constexpr int STAGE = F::STAGE, LOADS = F::LOADS, CW = F::CW, TW = F::TW, CF = CW / 32, TF = TW / 32;
+  static_assert(F::BOX <= STAGE && R >= 4 && R <= 8, "a stage holds a wave's sums");
   __shared__ __attribute__((aligned(1024))) int8_t lds0[STAGE];
   __shared__ __attribute__((aligned(1024))) int8_t lds1[STAGE];
   __shared__ __attribute__((aligned(1024))) int8_t lds2[STAGE];
   __shared__ __attribute__((aligned(1024))) int8_t lds3[STAGE];
-  __shared__ __attribute__((aligned(1024))) int8_t lds4[R > 4 ? STAGE : 1024];
-  __shared__ __attribute__((aligned(1024))) int8_t lds5[R > 5 ? STAGE : 1024];
+  __shared__ __attribute__((aligned(1024))) int8_t lds4[R > 4 ? STAGE : 1];
+  __shared__ __attribute__((aligned(1024))) int8_t lds5[R > 5 ? STAGE : 1];
+  __shared__ __attribute__((aligned(1024))) int8_t lds6[R > 6 ? STAGE : 1];
+  __shared__ __attribute__((aligned(1024))) int8_t lds7[R > 7 ? STAGE : 1];
   __shared__ __attribute__((aligned(16))) float channel[3][TC];
+  auto ring = [&](auto index) -> int8_t* {
+    constexpr int i = decltype(index)::value % R;
+    return i == 0 ? lds0 : i == 1 ? lds1 : i == 2 ? lds2 : i == 3 ? lds3 : i == 4 ? lds4 : i == 5 ? lds5 : i == 6 ? lds6 : lds7;
+  };
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-  const int part = wave >> 1, wt = wave & 1;  // of the features, and of the tokens
+  const int part = wave >> 1, share = wave & 1;
   const uint32_t tile = (blockIdx.x & 7) * a.tiles_xcd + (blockIdx.x >> 3);
   if (tile >= a.tiles) return;
-  const Tile t = tile_at<TC, TALL, 8>(a, tile);
+  const Tile t = tile_at<TC, TT, 8>(a, tile);
   const Set& s = a.set[t.set];
   load_channels<F16, QKV>(a, s, t.c0, channel);
   // Loads as in the wide kernel.
@@ -455,248 +599,130 @@ __global__ __launch_bounds__(512, 2) void int8_tile_kernel(Args a) {
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) {
     const int r = 8 * (8 * j + wave) + (lane >> 3);
-    const int row = 64 * j < TC ? min(r, a.columns - 1 - t.c0) : (int)min((uint32_t)(r - TC), s.tokens - 1 - t.t0);
-    offset[j] = row * a.padded + chunk * 16;
+    const bool there = r < TC ? r < a.columns - t.c0 : (uint32_t)(r - TC) < s.tokens - t.t0;
+    offset[j] = there ? (r < TC ? r : r - TC) * a.padded + chunk * 16 : (int)0x80000000;
   }
-  const int stages = (a.padded + STEP - 1) / STEP;
+  const int stages = (a.padded + 127) / 128;
   const Ends ends(a.padded, chunk);
+  const bool all = 8 * (LOADS - 1) + wave < F::GROUPS;  // (the last loads are not every wave's)
   auto load = [&](int8_t* dst, int stage, int j, int past) {
-    load_lds16(64 * j < TC ? wbase : qbase, dst + 1024 * (8 * j + wave), offset[j] | past, uniform(stage * STEP));
+    const int group = 8 * j + wave;
+    if (j < LOADS - 1 || all)
+      load_lds16(group * 8 < TC ? wbase : qbase, dst + 1024 * group, offset[j] | past, uniform(stage * 128));
   };
-  const int read = col * STEP + ((col >> 1 & 7) ^ (2 * part + half)) * 16;
-  i32x4 w[2][CF], x[2][2];
+  auto arrivals = [&] {
+    if (F::GROUPS % 8 == 0 || all) wait_arrivals<(R - 3) * LOADS>();
+    else wait_arrivals<(R - 3) * (LOADS - 1)>();
+  };
+  const int read = col * 128 + ((col >> 1 & 7) ^ (2 * part + half)) * 16;
+  const int wread = read + (TT > 32 ? 0 : share * CW * 128), xread = read + (TC + (TT > 32 ? share * TW : 0)) * 128;
+  i32x4 w[2][CF], x[2][TF];
   auto fetch = [&](const int8_t* src, int to) {
 #pragma unroll
-    for (int i = 0; i < CF; ++i) w[to][i] = *(const i32x4*)(src + i * 32 * STEP + read);
+    for (int i = 0; i < CF; ++i) w[to][i] = *(const i32x4*)(src + wread + i * 4096);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) x[to][j] = *(const i32x4*)(src + (TC + (wt * 2 + j) * 32) * STEP + read);
+    for (int j = 0; j < TF; ++j) x[to][j] = *(const i32x4*)(src + xread + j * 4096);
     __builtin_amdgcn_sched_barrier(0);
   };
-  i32x16 acc[2][CF] = {};
-  // Stage n's operands are in w[from], x[from], or on their way, and stage n + 1 is in `next`.  `free`, whose
-  // reads ended in the last step, takes stage n + R - 1.  Before the barrier stage n + 2 is there.
-  auto step = [&](const int8_t* next, int8_t* free, int n, int from) {
+  i32x16 acc[TF][CF] = {};
+  // Stage n's operands are in w, x, or on their way; stage n + 1 is in LDS.  The stage whose reads ended in
+  // the last step takes n + R - 1.  Before the barrier stage n + 2 is there.
+  int n = 0;
+  auto step = [&](auto index) {
+    constexpr int I = decltype(index)::value;
+    int8_t* const free = ring(std::integral_constant<int, I + R - 1>());
     const int past = ends.past(uniform(n + R - 1));
-    int done = 0, asked = 0;
+    int asked = 0, done = 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < TF; ++j)
 #pragma unroll
       for (int i = 0; i < CF; ++i) {
-        acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[from][i], x[from][j], acc[j][i], 0, 0, 0);
-        for (++done; asked * PRODUCTS < done * LOADS; ++asked) {
+        acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[I & 1][i], x[I & 1][j], acc[j][i], 0, 0, 0);
+        for (++done; asked * TF * CF < done * LOADS; ++asked) {
           __builtin_amdgcn_sched_barrier(0);
           load(free, n + R - 1, asked, past);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
     __builtin_amdgcn_sched_barrier(0);
-    fetch(next, from ^ 1);
-    wait_arrivals<(R - 3) * LOADS>();
+    fetch(ring(std::integral_constant<int, I + 1>()), ~I & 1);
+    arrivals();
     barrier();
+    return ++n == stages;
   };
-  auto begin = [&](int8_t* dst, int stage) {
+  // (Zeros into the last stage, so that the compiler, which tracks what is on its way to which array, has met them
+  // all before the loop: otherwise it waits for everything each time around.)
+  load(ring(std::integral_constant<int, R - 1>()), 0, 0, (int)0x80000000);
+  auto begin = [&](auto index) {
+    constexpr int I = decltype(index)::value;
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) load(dst, stage, j, ends.past(stage));
+    for (int j = 0; j < LOADS; ++j) load(ring(index), I, j, ends.past(I));
   };
-  // (Zeros into the last stage, so that the compiler, which tracks what is on its way to which array, has met
-  // them all before the loop: otherwise it waits for everything each time around.)
-  load(R == 6 ? lds5 : lds3, 0, 0, (int)0x80000000);
-  begin(lds0, 0);
-  begin(lds1, 1);
-  begin(lds2, 2);
-  if (R == 6) {
-    begin(lds3, 3);
-    begin(lds4, 4);
-  }
-  wait_arrivals<(R - 3) * LOADS>();
+  begin_all(begin, std::make_integer_sequence<int, R - 1>());
+  arrivals();
   barrier();
   fetch(lds0, 0);
-  for (int n = 0;;) {
-    step(lds1, R == 6 ? lds5 : lds3, n, 0);
-    if (++n == stages) break;
-    step(lds2, lds0, n, 1);
-    if (++n == stages) break;
-    step(lds3, lds1, n, 0);
-    if (++n == stages) break;
-    step(R == 6 ? lds4 : lds0, lds2, n, 1);
-    if (++n == stages) break;
-    if (R == 6) {
-      step(lds5, lds3, n, 0);
-      if (++n == stages) break;
-      step(lds0, lds4, n, 1);
-      if (++n == stages) break;
-    }
-  }
+  while (!step_all(step, std::make_integer_sequence<int, R % 2 ? 2 * R : R>())) {}
   wait_loads<0>();  // (nothing is on its way to LDS any more)
   barrier();
-  // Parts 2 and 3 hand their sums to 0 and 1, which then exchange the second and first 32 tokens and finish
-  // the ones they keep: 16 bytes a lane at a time, as they lie in registers.
-  auto hand = [&](int8_t* to, int j) {
+  // Parts 2 and 3 hand their sums to 0 and 1, which add their own: token-major, four channels a unit, units in an
+  // order of the token's, so that neighbouring tokens' lie in different banks.
+  auto box = [&](int k, int h) -> int8_t* { return k ? (h ? lds3 : lds2) : (h ? lds1 : lds0); };
+  auto unit = [&](int token, int c) { return (token * CW + (c ^ (token & 7) * 4)) * 4; };
+  auto hand = [&](bool add) {
+    int8_t* const to = box(part & 1, share);
 #pragma unroll
-    for (int i = 0; i < CF; ++i)
+    for (int j = 0; j < TF; ++j)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *(i32x4*)(to + ((i * 4 + g) * 64 + lane) * 16) = i32x4{acc[j][i][4 * g], acc[j][i][4 * g + 1], acc[j][i][4 * g + 2], acc[j][i][4 * g + 3]};
-  };
-  auto take = [&](const int8_t* from, int j) {
+      for (int i = 0; i < CF; ++i)
 #pragma unroll
-    for (int i = 0; i < CF; ++i)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const i32x4 v = *(const i32x4*)(from + ((i * 4 + g) * 64 + lane) * 16);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[j][i][4 * g + k] += v[k];
-      }
-  };
-  constexpr int SUMS = CF * 4096;  // bytes of a wave's sums of 32 tokens
-  static_assert(2 * SUMS <= STAGE, "a stage holds the sums of 64 tokens");
-  int8_t* const box = (part & 1) ? (wt ? lds3 : lds2) : (wt ? lds1 : lds0);
-  if (part >= 2) {
-    hand(box, 0);
-    hand(box + SUMS, 1);
-  }
-  __syncthreads();
-  if (part < 2) {
-    take(box, 0);
-    take(box + SUMS, 1);
-  }
-  __syncthreads();
-  if (part == 0) hand(box, 1);
-  if (part == 1) hand(box, 0);
-  __syncthreads();
-  if (part >= 2) return;
-  int8_t* const other = part ? (wt ? lds1 : lds0) : (wt ? lds3 : lds2);
-  const uint32_t t0 = t.t0 + (wt * 2 + part) * 32;
-  const float scale = s.scale[min(t0 + col, s.tokens - 1)];
-  if (part == 0) {
-    take(other, 0);
-    finish<F16, QKV, GELU, CF, TC>(a, s, acc[0], scale, channel[0], t.c0, t0);
-  } else {
-    take(other, 1);
-    finish<F16, QKV, GELU, CF, TC>(a, s, acc[1], scale, channel[0], t.c0, t0);
-  }
-}
-
-// ------------------------------------------------------------------ a few rows
-// Bound by the read of the weights.  Waves read 16 WF channels each straight into the operands of
-// v_mfma_i32_16x16x64_i8 (whose columns are 16 TF tokens), 64 bytes of a row a lane quartet, and split the
-// features between them; the partial sums meet in LDS.  CG channel groups and KS feature splits a workgroup.
-template <bool F16, bool QKV, bool GELU, int TF, int WF, int CG, int KS>
-__global__ __launch_bounds__(64 * CG * KS) void int8_rows_product_kernel(Args a) {
-  constexpr int TC = 16 * WF * CG, TT = 16 * TF, THREADS = 64 * CG * KS;
-  // (a row of sums is four ints longer, so that rows start in different banks)
-  __shared__ __attribute__((aligned(16))) int partial[KS][TT][TC + 4];
-  __shared__ __attribute__((aligned(16))) float channel[3][TC];
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, quarter = lane >> 4;
-  const int cg = wave % CG, ks = wave / CG;
-  uint32_t tile = blockIdx.x;
-  const int set = tile >= a.tiles0;
-  if (set) tile -= a.tiles0;
-  const Set& s = a.set[set];
-  const uint32_t tt = tile / a.channel_tiles, t0 = tt * TT;
-  const int c0 = (int)(tile - tt * a.channel_tiles) * TC;
-  const int8_t* wp[WF];
-#pragma unroll
-  for (int i = 0; i < WF; ++i)
-    wp[i] = s.w + (int64_t)min(c0 + (cg * WF + i) * 16 + col, a.columns - 1) * a.padded + quarter * 16;
-  const int8_t* xp[TF];
-#pragma unroll
-  for (int j = 0; j < TF; ++j) xp[j] = s.q + (int64_t)min(t0 + j * 16 + col, s.tokens - 1) * a.padded + quarter * 16;
-  i32x4 acc[TF][WF] = {};
-  // (a split is a whole number of 128-byte lines)
-  const int steps = a.padded / 64, each = ((steps + KS - 1) / KS + 1) & ~1;
-  const int begin = min(ks * each, steps), end = min(begin + each, steps);
-  int n = begin;
-  auto walk = [&](auto steps_at_once) {
-    constexpr int D = decltype(steps_at_once)::value;
-    i32x4 w[D][WF], x[D][TF];
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-#pragma unroll
-      for (int i = 0; i < WF; ++i) w[d][i] = *(const i32x4*)(wp[i] + (n + d) * 64);
-#pragma unroll
-      for (int j = 0; j < TF; ++j) x[d][j] = *(const i32x4*)(xp[j] + (n + d) * 64);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-#pragma unroll
-      for (int j = 0; j < TF; ++j)
-#pragma unroll
-        for (int i = 0; i < WF; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d][i], x[d][j], acc[j][i], 0, 0, 0);
-    n += D;
-  };
-  // (as many steps' loads as possible in flight together)
-  constexpr int MOST = TF * WF >= 4 ? 4 : 8;
-  while (n + MOST <= end) walk(std::integral_constant<int, MOST>());
-  if (MOST > 4 && n + 6 <= end) walk(std::integral_constant<int, 6>());
-  if (MOST > 4 && n + 4 <= end) walk(std::integral_constant<int, 4>());
-  if (n + 2 <= end) walk(std::integral_constant<int, 2>());
-  if (n < end) walk(std::integral_constant<int, 1>());
-  load_channels<F16, QKV>(a, s, c0, channel);
-  // a lane's sums: token col, channels 4 quarter .. + 3 of each 16
-#pragma unroll
-  for (int j = 0; j < TF; ++j)
-#pragma unroll
-    for (int i = 0; i < WF; ++i) *(i32x4*)&partial[ks][j * 16 + col][(cg * WF + i) * 16 + quarter * 4] = acc[j][i];
-  __syncthreads();
-  // eight channels of a token a thread; 16 lanes hold a head
-  const int plane = QKV ? c0 / (a.heads * HEAD) : 2;
-  for (int e = threadIdx.x; e < TT * (TC / 8); e += THREADS) {
-    const int token = e / (TC / 8), c = e % (TC / 8) * 8;
-    i32x4 sum[2] = {};
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) sum[h] += *(const i32x4*)&partial[k][token][c + 4 * h];
-    const uint32_t at = t0 + token;
-    const float scale = s.scale[min(at, s.tokens - 1)];
-    float v[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = (float)sum[k >> 2][k & 3] * scale * channel[0][c + k] + channel[1][c + k];
-    uint16_t* out = s.out + row_of(s, at) + c0 + c;
-    if (QKV) {
-      out += plane * a.out_p - plane * a.heads * HEAD;
-      if (plane < 2) {
-        float squares = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) squares += v[k] * v[k];
-#pragma unroll
-        for (int m = 8; m >= 1; m >>= 1) squares += __shfl_xor(squares, m, 16);
-        const float rms = __builtin_amdgcn_rsqf(squares * (1.f / HEAD) + a.eps);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] *= rms * channel[2][c + k];
-        const int64_t table = table_of(s, at) + c;
-        if (a.cos) {
-#pragma unroll
-          for (int g = 0; g < 8; g += 4)
-            rotate(v + g, *(const f32x4*)(a.cos + table + g), *(const f32x4*)(a.sin + table + g));
+        for (int g = 0; g < 4; ++g) {
+          i32x4* const at = (i32x4*)(to + unit(j * 32 + col, i * 32 + g * 8 + half * 4));
+          const i32x4 v = {acc[j][i][4 * g], acc[j][i][4 * g + 1], acc[j][i][4 * g + 2], acc[j][i][4 * g + 3]};
+          *at = add ? *at + v : v;
         }
-      }
-    } else if (GELU) {
+  };
+  if (part >= 2) hand(false);
+  __syncthreads();
+  if (part < 2) hand(true);
+  __syncthreads();
+  for (int e = threadIdx.x; e < TT * (TC / 8); e += 512) {
+    const int token = e / (TC / 8), c = e % (TC / 8) * 8;
+    const int h = TT > 32 ? token / TW : c / CW;
+    i32x4 sum[2];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = gelu(v[k]);
+    for (int g = 0; g < 2; ++g) {
+      const int at = unit(TT > 32 ? token % TW : token, (TT > 32 ? c : c % CW) + 4 * g);
+      sum[g] = *(const i32x4*)(box(0, h) + at) + *(const i32x4*)(box(1, h) + at);
     }
-    if (at < s.tokens) store8<QKV>(a, out, c0 + c, pack8<F16>(v));
+    finish8<F16, QKV, GELU, TC>(a, s, sum, channel, t.c0, t.t0 + token, c);
   }
 }
 
 // ------------------------------------------------------------------ launches
-enum Kernel { ROWS16, ROWS32, TILE64, TILE128, WIDE256, KERNELS };
+enum Kernel { T64x32, T32x64, T64x64, T96x64, T96x128, T128x32, T128x64, T128x128, WIDE256, WIDE_HEADS, KERNELS };
 
-// What a tile of each kernel covers, and what it takes in us on 256 CUs: a round of tiles, one a CU, is
-// `round` + stages of 128 features x `stage` + `full` (f) f, f the share of the CUs that have one (stages
-// slow each other down where many load).
+// What a tile of each kernel covers, and what it takes on 256 CUs, fitted to the times of 900 sizes of 1 to 6000
+// rows: `launch`, and for a round of tiles, one a CU, `round` + stages of 128 features x (`stage` + `full` f^2)
+// us, f the share of the CUs that have one (stages slow each other down where many load).
 struct Shape {
   int tc, tt;
-  float round, stage, full;
+  float launch, round, stage, full;
 };
 constexpr Shape SHAPES[KERNELS] = {
-    {16, 16, 0.f, 0.f, 0.f},
-    {32, 32, 0.f, 0.f, 0.f},
-    {64, 128, 2.6f, 0.26f, 0.10f},
-    {128, 128, 5.0f, 0.34f, 0.20f},
-    {256, 256, 6.7f, 1.06f, 0.60f},
+    // linear
+    {64, 32, 2.65f, 1.30f, 0.148f, 0.021f},
+    {32, 64, 1.72f, 2.38f, 0.144f, 0.060f},
+    {64, 64, 1.70f, 2.86f, 0.147f, 0.129f},
+    {96, 64, 1.67f, 3.78f, 0.189f, 0.133f},
+    {96, 128, 0.95f, 5.82f, 0.258f, 0.234f},
+    // qkv (a head's channels stay together)
+    {128, 32, 1.91f, 3.63f, 0.174f, 0.138f},
+    {128, 64, 1.96f, 4.70f, 0.195f, 0.249f},
+    {128, 128, 1.91f, 6.67f, 0.304f, 0.349f},
+    // the wide kernel, linear and qkv
+    {256, 256, 5.9f, 3.0f, 0.99f, 0.70f},
+    {256, 256, 7.0f, 8.2f, 1.00f, 0.70f},
 };
 
 // Tiles of TC x TT of both sets.
@@ -707,17 +733,12 @@ int64_t tiles_of(const Args& a, int count, int tc, int tt) {
   return tiles;
 }
 
-// A head's channels stay together.
-int channels_of(Kernel k, bool qkv) { return qkv && SHAPES[k].tc < HEAD ? HEAD : SHAPES[k].tc; }
-
 // What a kernel takes for the sets, in us.
-float estimate(const Args& a, int count, Kernel k, bool qkv) {
+float estimate(const Args& a, int count, Kernel k) {
   const Shape& s = SHAPES[k];
-  const int tc = channels_of(k, qkv);
-  const float tiles = (float)tiles_of(a, count, tc, s.tt), stages = (float)((a.padded + 127) / 128), cus = 256.f;
-  if (k <= ROWS32) return 3.f + tiles * (float)(tc + s.tt) * (float)a.padded / 6.5e6f;
-  const float rounds = std::floor(tiles / cus), rest = tiles / cus - rounds;
-  return 2.3f + rounds * (s.round + stages * (s.stage + s.full)) +
+  const float rounds = (float)tiles_of(a, count, s.tc, s.tt) / 256.f, whole = std::floor(rounds), rest = rounds - whole;
+  const float stages = (float)((a.padded + 127) / 128);
+  return s.launch + whole * (s.round + stages * (s.stage + s.full)) +
          (rest > 0.f ? s.round + stages * (s.stage + s.full * rest * rest) : 0.f);
 }
 
@@ -726,35 +747,32 @@ struct Choice {
   float us;
 };
 
-// The kernel whose estimate is the least.  Up to 16 tokens a set it is the first; measured, rows x features x
-// columns, us: 1 x 3072 x 18432 12.6 (32 x 32 blocks 15.7, 64 x 128 tiles 21.5), 16 x 3072 x 9216 11.2 (11.7,
-// 11.3).  The others, 32 x 32 blocks / 64 x 128 / 128 x 128 / 256 x 256 tiles: 64 x 3072 x 3072 8.5 / 10.6 / 14.7 /
-// 32.4; 200 x 1024 x 1024 4.6 / 6.8 / 9.3 / 15.6; 128 x 3072 x 12288 37 / 13.6 / 17.0 / 32.7; 512 x 12288 x 3072 128 /
-// 33 / 41 / 111; 256 x 3072 x 9216 56 / 24 / 17.4 / 34; 512 x 3072 x 9216 101 / 35 / 34 / 36; 4096 x 3072 x 3072 - / 70 /
-// 57 / 42; 16384 x 256 x 256 - / 10.7 / 8.4 / 10.3.  Blocks are as long as the bytes they read, at 6.5 TB/s.
+// The kernel whose estimate is the least: over those sizes 0.7% (linear) and 0.4% (qkv) slower than always the
+// fastest.  Measured, rows x features x columns, us for 64 x 32 / 32 x 64 / 64 x 64 / 96 x 64 / 96 x 128 / 256 x 256
+// tiles: 77 x 4096 x 3072 9.1 / 9.2 / 9.4 / 11.4 / 14.7 / 40; 128 x 3072 x 12288 18.9 / 23 / 18.4 / 14.0 / 16.5 / 33;
+// 512 x 12288 x 3072 56 / 62 / 50 / 31 / 39 / 110; 256 x 3072 x 9216 27 / 36 / 25 / 22 / 16.6 / 34; 4096 x 3072 x 3072
+// - / - / 96 / 79 / 64 / 43; 1 x 3072 x 18432 13.7 / 22 / 18.8 / 13.1 / 14.6 / 33.  qkv, rows x features, 24 heads, us
+// for 128 x 32 / 128 x 64 / 128 x 128 / 256 x 256: 1 x 3072 11 / 13 / 17 / 39; 128 x 3072 21 / 15 / 20 / 43;
+// 512 x 3072 48 / 39 / 38 / 45; 512 + 4096 x 3072 368 / 246 / 202 / 147.
 Choice choose(const Args& a, int count, bool qkv) {
-  uint32_t tokens = 0;
-  for (int i = 0; i < count; ++i) tokens = std::max(tokens, a.set[i].tokens);
-  // (a grid holds fewer than 2^32 threads)
-  const auto fits = [&](Kernel k) { return tiles_of(a, count, channels_of(k, qkv), SHAPES[k].tt) < (1 << 21); };
-  if (tokens <= 16 && fits(ROWS16)) return {ROWS16, 0.f};
-  Choice best = {WIDE256, estimate(a, count, WIDE256, qkv)};
-  for (int i = ROWS32; i < WIDE256; ++i) {
+  const Kernel wide = qkv ? WIDE_HEADS : WIDE256;
+  Choice best = {wide, estimate(a, count, wide)};
+  for (int i = qkv ? T128x32 : T64x32; i <= (qkv ? T128x128 : T96x128); ++i) {
     const Kernel k = (Kernel)i;
-    if ((k == TILE64 && qkv) || !fits(k)) continue;
-    const float us = estimate(a, count, k, qkv);
+    if (tiles_of(a, count, SHAPES[k].tc, SHAPES[k].tt) >= (1 << 21)) continue;  // (a grid holds fewer than 2^32 threads)
+    const float us = estimate(a, count, k);
     if (us < best.us) best = {k, us};
   }
   return best;
 }
 
 // The last rows of the last set that are better off in a launch of their own, because the tiles before them
-// fill whole rounds of the CUs: 16896 x 15360 x 3072, 792 tiles of 256 x 256, 934 us at once, and 728 as
+// fill whole rounds of the CUs: 16896 x 15360 x 3072, 792 tiles of 256 x 256, 788 us at once, and 675 as
 // 768 of them and 512 rows apart.
 uint32_t apart(const Args& a, int count, const Choice& whole, bool qkv) {
   const Set& s = a.set[count - 1];
   const int64_t across = (a.columns + 255) / 256, tiles = tiles_of(a, count, 256, 256);
-  if (whole.kernel != WIDE256 || tiles < 256 || tiles % 256 == 0) return 0;
+  if (whole.kernel < WIDE256 || tiles < 256 || tiles % 256 == 0) return 0;
   // token tiles to take off, so that what is left is the most that fits the whole rounds
   const int64_t off = (tiles % 256 + across - 1) / across, token_tiles = (s.tokens + 255) / 256;
   if (off >= token_tiles) return 0;
@@ -763,32 +781,44 @@ uint32_t apart(const Args& a, int count, const Choice& whole, bool qkv) {
   main.set[count - 1].tokens = keep;
   rest.set[0] = s;
   rest.set[0].tokens = s.tokens - keep;
-  return estimate(main, count, WIDE256, qkv) + choose(rest, 1, qkv).us + 5.f < whole.us ? s.tokens - keep : 0;
+  return estimate(main, count, whole.kernel) + choose(rest, 1, qkv).us + 5.f < whole.us ? s.tokens - keep : 0;
 }
 
 template <bool F16, bool QKV, bool GELU>
 int launch_kernel(Args& a, int count, Kernel kernel, hipStream_t st) {
-  const int tc = channels_of(kernel, QKV), tt = SHAPES[kernel].tt;
+  const int tc = SHAPES[kernel].tc, tt = SHAPES[kernel].tt;
   const int64_t tiles = tiles_of(a, count, tc, tt);
   HB_REQUIRE(tiles < (1ll << 30), "too many output tiles for one launch");
   a.channel_tiles = (uint32_t)((a.columns + tc - 1) / tc);
   a.tiles0 = (uint32_t)tiles_of(a, 1, tc, tt);
   a.tiles = (uint32_t)tiles;
   a.tiles_xcd = (a.tiles + 7) / 8;
-  const dim3 blocks(a.tiles), each(8 * a.tiles_xcd), eight(512);
+  const dim3 each(8 * a.tiles_xcd), eight(512);
   switch (kernel) {
-    case ROWS16:
-      if constexpr (QKV) hipLaunchKernelGGL((int8_rows_product_kernel<F16, QKV, GELU, 1, 2, 4, 4>), blocks, dim3(1024), 0, st, a);
-      else hipLaunchKernelGGL((int8_rows_product_kernel<F16, QKV, GELU, 1, 1, 1, 8>), blocks, eight, 0, st, a);
+    case T64x32:
+      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 64, 32, 6>), each, eight, 0, st, a);
       break;
-    case ROWS32:
-      if constexpr (QKV) hipLaunchKernelGGL((int8_rows_product_kernel<F16, QKV, GELU, 2, 2, 4, 4>), blocks, dim3(1024), 0, st, a);
-      else hipLaunchKernelGGL((int8_rows_product_kernel<F16, QKV, GELU, 2, 2, 1, 8>), blocks, eight, 0, st, a);
+    case T32x64:
+      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 32, 64, 8>), each, eight, 0, st, a);
       break;
-    case TILE64:
-      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 2, 6>), each, eight, 0, st, a);
+    case T64x64:
+      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 64, 64, 8>), each, eight, 0, st, a);
       break;
-    case TILE128: hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 4, 4>), each, eight, 0, st, a); break;
+    case T96x64:
+      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 96, 64, 7>), each, eight, 0, st, a);
+      break;
+    case T96x128:
+      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 96, 128, 5>), each, eight, 0, st, a);
+      break;
+    case T128x32:
+      if constexpr (QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 128, 32, 7>), each, eight, 0, st, a);
+      break;
+    case T128x64:
+      if constexpr (QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 128, 64, 6>), each, eight, 0, st, a);
+      break;
+    case T128x128:
+      if constexpr (QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 128, 128, 4>), each, eight, 0, st, a);
+      break;
     default: {
       const uint32_t per_xcd = std::max(1, device_cu_count() / 8);
       hipLaunchKernelGGL((int8_wide_kernel<F16, QKV, GELU>), dim3(8 * std::min(a.tiles_xcd, per_xcd)), eight, 0, st, a);
@@ -810,7 +840,7 @@ int launch_type(Args& a, int count, hipStream_t st) {
   s.q += (int64_t)s.start * a.padded;
   s.scale += s.start;
   s.tokens = rest;
-  const int rc = launch_kernel<F16, QKV, GELU>(a, count, WIDE256, st);
+  const int rc = launch_kernel<F16, QKV, GELU>(a, count, whole.kernel, st);
   return rc ? rc : launch_kernel<F16, QKV, GELU>(b, 1, choose(b, 1, QKV).kernel, st);
 }
 

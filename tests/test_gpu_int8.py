@@ -114,6 +114,31 @@ def test_rows_of_little_nothing_and_not_numbers():
             assert torch.isnan(out[1]).all() and torch.isfinite(out[[0, 2]]).all()
 
 
+def test_rows_larger_than_the_caches():
+    """What is read past the caches is the same."""
+    gen = _gen(5)
+    for features in (1000, 9000):
+        x = _randn(gen, (1 << 27) // features, features, dtype=FP16)
+        r = quantize_rows(x)
+        assert all(torch.equal(r.q[at:at + 1000, :features].long(), O.quantize(x[at:at + 1000])[0])
+                   for at in range(0, len(x), 1000))
+        assert not r.q[:, features:].any()
+
+
+def test_adaln_larger_than_the_caches():
+    gen = _gen(6)
+    for C in (640, 3072):
+        M = (1 << 26) // C
+        x, y, mod = _randn(gen, 1, M, C), _randn(gen, 1, M, C), _randn(gen, 1, 3 * C, std=0.3)
+        shift, scale, gate = mod.chunk(3, 1)
+        out = torch.empty_like(x)
+        r = adaln_quantize(x, shift, scale, y=y, gate=gate, x_out=out)
+        for at in range(0, M, 5000):
+            part, one = slice(at, at + 5000), torch.empty_like(x[:, at:at + 5000])
+            few = adaln_quantize(x[:, part], shift, scale, y=y[:, part], gate=gate, x_out=one)
+            assert torch.equal(few.q, r.q[:, part]) and torch.equal(few.scale, r.scale[:, part]) and torch.equal(one, out[:, part])
+
+
 def test_rows_by_strides():
     gen = _gen(5)
     big = _randn(gen, 3, 50, 400)
@@ -233,6 +258,47 @@ def test_linear_of_real_sizes(rows, features, columns):
     _check_linear(int8_linear(x, w, b, gelu=True), x, w, b, True)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,features,columns", [(1, 1122, 53), (2739, 1141, 135), (135, 1110, 3307), (335, 1106, 2721),
+                                                   (2703, 1091, 485), (833, 1098, 3489), (14, 1122, 256), (700, 1200, 3010)])
+def test_linear_over_tiles(rows, features, columns, dtype):
+    """Each shape of tile, its ring of stages walked past its end, ragged on every side."""
+    gen = _gen(rows)
+    x, w = _rows(gen, rows, features, dtype), _weight(gen, columns, features)
+    b = _randn(gen, columns, dtype=dtype)
+    for gelu in (False, True):
+        _check_linear(int8_linear(x, w, b, gelu=gelu), x, w, b, gelu)
+
+
+@pytest.mark.parametrize("features", [1400, 15360])
+def test_last_rows_apart(features):
+    """Tiles that fill whole rounds of the CUs, and the rows after them: 66 x 12 of 256 x 256."""
+    gen = _gen(features)
+    M, N = 16896 - 77, 12 * 256 - 8
+    x, w = _rows(gen, (3, M // 3), features), _weight(gen, N, features)
+    out, again = (int8_linear(x, w) for _ in range(2))
+    assert torch.equal(out, again)
+    flat = Int8Rows(x.q.flatten(0, 1), x.scale.flatten(), features, BF16)
+    for at in (slice(0, 40), slice(16300, 16420), slice(M // 3 * 3 - 40, M)):
+        part = Int8Rows(flat.q[at], flat.scale[at], features, BF16)
+        _check_linear(out.flatten(0, 1)[at], part, w, None)
+    assert torch.equal(out.flatten(0, 1)[16000:], int8_linear(flat._replace(q=flat.q[16000:], scale=flat.scale[16000:]), w))
+
+
+@pytest.mark.parametrize("offset", range(8))
+def test_linear_into_rows_that_start_anywhere(offset):
+    """Output rows at every alignment of whole elements, odd strides among them; what is around them stays."""
+    gen = _gen(offset)
+    for M, K, N in ((50, 192, 100), (130, 192, 264), (40, 64, 7)):
+        x, w = _rows(gen, M, K), _weight(gen, N, K)
+        want = int8_linear(x, w)
+        for pad in (8, 9, 10):
+            buf = torch.full((M, N + pad + offset), 5.0, dtype=BF16, device="cuda")
+            int8_linear(x, w, out=buf[:, offset:offset + N])
+            assert torch.equal(buf[:, offset:offset + N], want)
+            assert (buf[:, :offset] == 5).all() and (buf[:, offset + N:] == 5).all()
+
+
 def test_linear_takes_16_bit_rows():
     gen = _gen(3)
     x, weight, b = _randn(gen, 2, 50, 333, dtype=FP16), _randn(gen, 90, 333, dtype=FP16, std=0.05), _randn(gen, 90, dtype=FP16)
@@ -320,7 +386,8 @@ def _tables(T, n):
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("B,T,n,heads,K", [(1, 0, 1, 1, 64), (1, 0, 1, 24, 3072), (2, 1, 1, 3, 128), (1, 5, 30, 2, 200),
                                            (3, 77, 51, 5, 648), (1, 130, 260, 4, 512), (2, 0, 129, 3, 320),
-                                           (1, 33, 600, 2, 1024), (1, 512, 1024, 24, 3072)])
+                                           (1, 33, 600, 2, 1024), (1, 512, 1024, 24, 3072), (1, 4, 13, 1, 1126),
+                                           (1, 163, 97, 9, 1110), (2, 3, 193, 11, 1167), (1, 145, 1170, 12, 1102)])
 def test_qkv(B, T, n, heads, K, dtype):
     gen = _gen(n + heads)
     sets = ([_qkv_set(gen, B, T, K, heads, dtype)] if T else []) + [_qkv_set(gen, B, n, K, heads, dtype)]
