@@ -59,9 +59,9 @@ struct Args {
 };
 
 __device__ __forceinline__ float gelu(float v) {
-  // v (1 + tanh u) / 2 = v / (1 + exp(-2u)),  u = sqrt(2 / pi) (v + 0.044715 v^3)
-  const float u = v * (0.7978845608028654f + 0.035677408136300125f * v * v);
-  return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.885390081777927f * u));
+  // v (1 + tanh u) / 2 = v / (1 + exp(-2u)),  u = sqrt(2 / pi) (v + 0.044715 v^3);  -2u / ln 2 by its powers
+  const float e = v * (-2.302208198144325f - 0.1029432395800235f * v * v);
+  return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(e));
 }
 
 // Four values of this lane's token, channels c .. c + 3 with c = 8g + 4 (lane / 32), of quarters g = 2p
@@ -267,13 +267,13 @@ __device__ __forceinline__ bool step_all(Step& step, std::integer_sequence<int, 
 // The epilogue of a wave's 32 tokens from t0 on and one head from c0 on (qkv).  Lanes l and l + 32 hold token
 // t0 + l % 32, and would read its rotary rows and write its output 32 bytes at a time.  So 16 tokens at a time go
 // through the wave's own part of a stage, eight pieces of 1 KB, and come back as four tokens of 16 lanes each,
-// whose reads and writes are whole lines (512 + 16384 rows x 3072, 24 heads: 511 -> 484 us).  `channel` are the head's values, TC apart.
+// whose reads and writes are whole lines (512 + 16384 rows x 3072, 24 heads: 511 -> 479 us).  `channel` are the head's values, TC apart.
 template <bool F16, bool TURN, int TC>
 __device__ __forceinline__ void finish_head(const Args& a, const Set& s, const i32x16 (&acc)[4], float scale,
                                             const float* channel, int c0, uint32_t t0, int8_t* box) {
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, c = (lane & 15) * 8;
   const int plane = c0 / (a.heads * HEAD);
-  const bool heads = TURN || plane < 2;
+  const bool heads = TURN || plane < 2, one = s.start + s.tokens <= s.rows;  // (one batch element: no division)
   uint16_t* const out = s.out + plane * a.out_p + (c0 - plane * a.heads * HEAD) + c;
   auto place = [&](int token) { return (token >> 1) * 8192 + (token & 1) * 512; };
   float ws[8], bias[8], norm[8];
@@ -288,7 +288,8 @@ __device__ __forceinline__ void finish_head(const Args& a, const Set& s, const i
   auto ask = [&](int m) {
     Ahead to;
     to.at = t0 + m * 4 + (lane >> 4);
-    const uint32_t token = s.start + min(to.at, s.tokens - 1), b = token / s.rows, n = token - b * s.rows;
+    uint32_t n = s.start + min(to.at, s.tokens - 1), b = 0;
+    if (!one) b = n / s.rows, n -= b * s.rows;
     to.row = b * s.out_b + (int64_t)n * s.out_n;
     if (TURN) {
       const int64_t table = (int64_t)(s.first + n) * HEAD + c;
