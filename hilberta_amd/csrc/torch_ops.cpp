@@ -356,6 +356,33 @@ void check_written(const Tensor& out, const char* name, std::initializer_list<co
   }
 }
 
+// Whether two views of rows may share a value: no where their bytes lie apart, or where row ranges or column
+// blocks of one buffer do.
+bool may_overlap(const Tensor& a, const Tensor& b) {
+  if (!a.numel() || !b.numel()) return false;
+  const auto [a0, a1] = bytes_of(a);
+  const auto [b0, b1] = bytes_of(b);
+  if (a1 <= b0 || b1 <= a0) return false;
+  const Rows ra = rows_of(a, "rows"), rb = rows_of(b, "rows");
+  const int64_t size = a.element_size(), delta = b0 - a0;
+  if (b.element_size() != size || delta % size) return true;
+  // Within a period of both views, one takes its first `na` elements and the other `nb` from d on.
+  const auto apart = [&](int64_t period, int64_t na, int64_t nb) {
+    const int64_t d = ((delta / size) % period + period) % period;
+    return d >= na && d + nb <= period;
+  };
+  const bool many = a.dim() == 3 && b.dim() == 3 && (ra.batch > 1 || rb.batch > 1);
+  const int64_t row = ra.row_stride, all = many ? ra.batch_stride : 0;
+  if (rb.row_stride != row || row <= 0 || (many && (rb.batch_stride != all || all <= 0))) return true;
+  if ((!many || all % row == 0) && apart(row, a.size(-1), b.size(-1))) return false;
+  return !(many && apart(all, (ra.rows - 1) * row + a.size(-1), (rb.rows - 1) * row + b.size(-1)));
+}
+
+// Whether two views of one shape are the same places in the same order.
+bool same_places(const Tensor& a, const Tensor& b) {
+  return a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides();
+}
+
 // Checks of 8-bit rows [.., padded] with their scales; returns padded.
 int64_t check_int8(const Tensor& q, const Tensor& scale, const char* name) {
   TORCH_CHECK_VALUE(q.dim() >= 2 && q.scalar_type() == at::kChar && q.is_contiguous() && q.size(-1) > 0 &&
@@ -430,7 +457,18 @@ std::array<Tensor, 4> int8_adaln_sets(std::initializer_list<AdaSet> sets, double
     TORCH_CHECK_VALUE(batch == 1 || s.shift.stride(0) == s.scale.stride(0), "shift and scale must share one batch stride");
     const Rows rx = rows_of(s.x, "x"), ry = y.defined() ? rows_of(y, "y") : Rows{},
                ro = x_out.defined() ? rows_of(x_out, "x_out") : Rows{};
-    if (x_out.defined()) check_written(x_out, "x_out", {&s.shift, &s.scale, &gate});
+    if (x_out.defined()) {
+      check_written(x_out, "x_out", {&s.shift, &s.scale, &gate});
+      for (const AdaSet& other : sets) {
+        // (a row is read before it is written, by one wave: x_out may be this set's x or y)
+        const bool own = &other == &s;
+        for (const Tensor* t : {&other.x, &value_or_none(other.y)})
+          TORCH_CHECK_VALUE(!t->defined() || (own && same_places(x_out, *t)) || !may_overlap(x_out, *t),
+                            "x_out must be x itself or lie apart from the rows read");
+        TORCH_CHECK_VALUE(own || !other.x_out.has_value() || !may_overlap(x_out, *other.x_out),
+                          "both sets' x_out must lie apart");
+      }
+    }
     one_device(s0.x, {&s.x, &s.shift, &s.scale, &y, &gate, &x_out});
     void* p[8] = {pointer(s.x), pointer(y), pointer(gate), pointer(x_out), pointer(s.shift), pointer(s.scale), nullptr, nullptr};
     // (a stride of a dimension of one says nothing)
@@ -508,7 +546,10 @@ void int8_linear_sets(std::initializer_list<LinearSet> sets, bool gelu) {
     TORCH_CHECK_VALUE(s.q.sizes().slice(0, s.q.dim() - 1) == s.out.sizes().slice(0, s.out.dim() - 1),
                       "out must have the rows' leading dimensions");
     check_weight(s.weight, s.weight_scale, bias, padded, s.out.size(-1), s.out.scalar_type());
-    check_written(s.out, "out", {&s.q, &s.scale, &s.weight, &s.weight_scale, &bias});
+    for (const LinearSet& o : sets) {
+      check_written(s.out, "out", {&o.q, &o.scale, &o.weight, &o.weight_scale, &value_or_none(o.bias)});
+      TORCH_CHECK_VALUE(&o == &s || !may_overlap(s.out, o.out), "both outputs must lie apart");
+    }
     one_device(s0.q, {&s.q, &s.scale, &s.weight, &s.weight_scale, &bias, &s.out});
     void* p[6] = {pointer(s.q), pointer(s.scale), pointer(s.weight), pointer(s.weight_scale), pointer(bias), pointer(s.out)};
     std::copy(p, p + 6, pointers + 6 * i);

@@ -541,6 +541,32 @@ def test_graph_replays():
             assert torch.equal(a, b)
 
 
+def test_two_launches_in_a_graph():
+    """A product whose last rows go apart, captured and replayed among eager calls on new rows."""
+    gen = _gen(31)
+    M, N, K = 16819, 3064, 1400
+    w, b = _weight(gen, N, K), _randn(gen, N)
+    x = _rows(gen, M, K)
+    out = torch.empty(M, N, dtype=BF16, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        int8_linear(x, w, b, gelu=True, out=out)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            int8_linear(x, w, b, gelu=True, out=out)
+        for _ in range(3):
+            q, scale = _int8(gen, M, K)
+            x.q.copy_(q)
+            x.scale.copy_(scale)
+            out.zero_()
+            graph.replay()
+            want = int8_linear(x, w, b, gelu=True)
+            stream.synchronize()
+            assert torch.equal(out, want)
+
+
 def test_the_same_twice():
     s = _chain_state(34)
     a, b = _chain(s), _chain(s)

@@ -78,6 +78,18 @@ def test_adaln_refusals():
     call("non-overlapping", y=x, gate=v, x_out=torch.zeros(1, 3, 64, dtype=BF16).expand(2, 3, 64))
     call("cannot alias", y=x, gate=v, shift=x.view(6, 64)[:2], scale=x.view(6, 64)[:2], x_out=x)
     call("Inference only", shift=v.clone().requires_grad_())
+    # the residual goes over x or y, or apart from both
+    h = torch.zeros(2, 8, 64, dtype=BF16)
+    call(ON_DEVICE, y=x, gate=v, x=h[:, :3], x_out=h[:, 3:6])
+    call(ON_DEVICE, y=h[:, 5:], x=h[:, :3], gate=v, x_out=h[:, 5:])
+    call("x itself", y=x, gate=v, x=h[:, :3], x_out=h[:, 2:5])
+    call("x itself", y=h[:, 2:5], gate=v, x_out=h[:, :3])
+    call("x itself", y=x[:1], gate=v[:1], x=h[:1, :3], x_out=h[:1, 1:4], shift=v[:1], scale=v[:1])
+    row = dict(shift=v, scale=v, gate=v)
+    t, i = dict(x=h[:, :3], y=x, x_out=h[:, :3], **row), dict(x=h[:, 3:], y=h[:, 3:], x_out=h[:, 3:], **row)
+    _refused(ON_DEVICE, f.adaln_quantize_pair, t, i)
+    _refused("x itself", f.adaln_quantize_pair, {**t, "x_out": h[:, 3:6]}, i)
+    _refused("must lie apart", f.adaln_quantize_pair, {**t, "x": x, "x_out": h[:, :3]}, {**i, "x": x, "y": x, "x_out": h[:, 2:5]})
     a, b = dict(x=x, shift=v, scale=v), dict(x=x[:, :1], shift=v, scale=v)
     _refused(ON_DEVICE, f.adaln_quantize_pair, a, b)
     _refused("one batch", f.adaln_quantize_pair, a, dict(x=x[:1], shift=v[:1], scale=v[:1]))
@@ -117,6 +129,13 @@ def test_linear_refusals():
     call("cannot alias", b=shared[3:8], out=shared[:30].view(2, 3, 5))
     call("Inference only", b=b.clone().requires_grad_())
     call("Inference only", x=torch.zeros(2, 3, 70, dtype=BF16, requires_grad=True))
+    buf = torch.zeros(2, 9, 12, dtype=BF16)
+    for first, second in ((buf[:, :3, :5], buf[:, 3:6, :5]), (buf[:, :3, :5], buf[:, :3, 5:10]), (buf[:, 3:6, 7:], buf[:, :3, 7:])):
+        _refused(ON_DEVICE, f.int8_linear_pair, dict(x=x, weight=w, out=first), dict(x=x, weight=w, out=second))
+    for first, second in ((buf[:, :3, :5], buf[:, 2:5, :5]), (buf[:, :3, :5], buf[:, :3, 4:9]), (out, out)):
+        _refused("lie apart", f.int8_linear_pair, dict(x=x, weight=w, out=first), dict(x=x, weight=w, out=second))
+    _refused("cannot alias", f.int8_linear_pair, dict(x=x, weight=w, out=shared[:30].view(2, 3, 5)),
+             dict(x=x, weight=w, bias=shared[10:15]))
     a = dict(x=x, weight=w, bias=b)
     _refused(ON_DEVICE, f.int8_linear_pair, a, dict(x=_rows(2, 9), weight=w))
     _refused("must share", f.int8_linear_pair, a, dict(x=_rows(1, 9), weight=w))
@@ -177,7 +196,8 @@ def test_entry_points_reject_before_any_launch():
         return (x, bs, rs, batch, rows, features, padded, dtype, q, scale, None)
 
     for match, over in (("null", dict(x=None)), ("null", dict(scale=None)), ("positive", dict(rows=0)),
-                        ("2^31", dict(batch=1 << 16, rows=1 << 16)), ("features", dict(features=0)),
+                        ("2^31", dict(batch=1 << 16, rows=1 << 16)), ("too many", dict(batch=2, rows=1 << 25)),
+                        ("too many", dict(rows=1 << 24, features=3073, padded=3136)), ("features", dict(features=0)),
                         ("features", dict(features=(1 << 17) + 1)), ("padded", dict(padded=63)), ("padded", dict(features=65)),
                         ("dtype", dict(dtype=2)), ("aligned", dict(x=17)), ("aligned", dict(q=264)), ("strides", dict(rs=-1))):
         _einval(match, "hb_int8_rows", *rows(**over))
@@ -189,6 +209,7 @@ def test_entry_points_reject_before_any_launch():
     p = (16, None, None, None, 16, 16, 16, 16)
     for match, over in (("count", dict(count=3)), ("hidden", dict(hidden=60)), ("hidden", dict(hidden=8200, padded=8256)),
                         ("padded", dict(padded=72)), ("dtype", dict(dtype=9)), ("eps", dict(eps=0.0)), ("positive", dict(batch=0)),
+                        ("too many", dict(batch=4, rows=(1 << 24,))),
                         ("null", dict(pointers=(None,) + p[1:])), ("given together", dict(pointers=(16, 16) + p[2:])),
                         ("residual", dict(pointers=(16, None, None, 16) + p[4:])), ("16-byte", dict(pointers=(24,) + p[1:])),
                         ("4-byte", dict(pointers=p[:7] + (18,))), ("multiples of 8", dict(strides=(4,) + (64,) * 7))):
