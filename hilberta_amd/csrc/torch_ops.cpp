@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <ATen/DeviceGuard.h>
 #include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/variable.h>
@@ -397,13 +398,20 @@ int64_t check_int8(const Tensor& q, const Tensor& scale, const char* name) {
 // Columns of 8-bit rows of `features` values.
 int64_t padded_features(int64_t features) { return (features + 63) / 64 * 64; }
 
+// An unwritten tensor on x's device.  (Not through the dispatcher: it takes as long as the allocation does, and
+// the short calls here are the host's.)
+Tensor new_tensor(const Tensor& x, at::IntArrayRef sizes, at::ScalarType dtype) {
+  if (!x.is_cuda()) return at::empty(sizes, x.options().dtype(dtype));
+  return Tensor(at::detail::empty_cuda(sizes, dtype, x.device(), std::nullopt));
+}
+
 // Unwritten 8-bit rows for x [.., features], and their scales.
 std::tuple<Tensor, Tensor> new_int8_rows(const Tensor& x) {
-  auto sizes = x.sizes().vec();
+  c10::SmallVector<int64_t, 3> sizes(x.sizes().begin(), x.sizes().end());
   sizes.back() = padded_features(sizes.back());
-  Tensor q = at::empty(sizes, x.options().dtype(at::kChar));
+  Tensor q = new_tensor(x, sizes, at::kChar);
   sizes.pop_back();
-  return {std::move(q), at::empty(sizes, x.options().dtype(at::kFloat))};
+  return {std::move(q), new_tensor(x, sizes, at::kFloat)};
 }
 
 // hb_int8_rows: 16-bit rows to 8-bit rows and their scales.
@@ -575,9 +583,9 @@ Tensor int8_linear(const Tensor& q, const Tensor& scale, const Tensor& weight, c
   type_of(dtype, "rows");
   TORCH_CHECK_VALUE((q.dim() == 2 || q.dim() == 3) && weight.dim() == 2,
                     "rows must be [rows, padded] or [B, rows, padded] and weight [columns, padded]");
-  auto sizes = q.sizes().vec();
+  c10::SmallVector<int64_t, 3> sizes(q.sizes().begin(), q.sizes().end());
   sizes.back() = weight.size(0);
-  Tensor out = at::empty(sizes, q.options().dtype(dtype));
+  Tensor out = new_tensor(q, sizes, dtype);
   int8_linear_out(q, scale, weight, weight_scale, bias, out, gelu);
   return out;
 }
