@@ -553,26 +553,28 @@ __global__ __launch_bounds__(512, 2) void int8_wide_kernel(Args a) {
 }
 
 // ------------------------------------------------------------------ fewer rows
-// TC channels x TT tokens a workgroup of eight waves, in tiles so small that most CUs have one.  What is on its
-// way to a CU bounds it: some 80 bytes a ns and CU with 100 to 140 KB asked for ahead.  So the operands go to LDS by
+// TC channels x TT tokens a workgroup, in tiles so small that most CUs have one.  What is on its way to a CU
+// bounds it: some 70 to 100 bytes a ns and CU with 60 to 140 KB asked for ahead.  So the operands go to LDS by
 // direct loads, into a ring of R stages of 128 features, as many as there is room for (straight into registers,
-// which hold less: 1 x 3072 x 9216 qkv 15.3 us, so 10.9; 77 x 4096 x 3072 12.4 -> 9.5), the loads spread over the
-// products.  Four waves share a stage's features, 32 each, and two of each the tokens (of 32 tokens: the channels),
-// so that LDS is read by few.  The sums meet in LDS, and a thread finishes eight channels of a token: neighbouring
-// lanes read and write whole lines (a wave finishing 32 tokens as they lie in registers: 512 + 1024 x 3072 qkv
-// 88 us of 128 x 128 tiles, so 77).  Rows past the operands' ends are zeros that nothing reads.
-template <int TC, int TT>
+// which hold less: 1 x 3072 x 9216 qkv 15.3 us, so 10.9; 77 x 4096 x 3072 12.4 -> 9.6), the loads spread over the
+// products.  A stage's features are in four parts of 32, a wave each in the smallest tiles (77 x 4096 x 3072 10.3 us
+// with two), or two waves that share the tokens (of 32 tokens: the channels), whose epilogue is shorter
+// (512 x 3072 x 9216 28.8 us, with one 33.6).  The sums meet in LDS, and a thread finishes eight channels of a
+// token: neighbouring lanes read and write whole lines (a wave finishing 32 tokens as they lie in registers:
+// 512 + 1024 x 3072 qkv 88 us of 128 x 128 tiles, so 73).  Rows past the operands' ends are zeros that nothing reads.
+template <int TC, int TT, int WAVES>
 struct Ring {
-  static constexpr int STAGE = (TC + TT) * 128, GROUPS = STAGE / 1024, LOADS = (GROUPS + 7) / 8;
-  static constexpr int CW = TT > 32 ? TC : TC / 2, TW = TT > 32 ? TT / 2 : TT;  // of a wave
-  static constexpr int BOX = TW * CW * 4;                                       // bytes of a wave's sums
+  static constexpr int STAGE = (TC + TT) * 128, GROUPS = STAGE / 1024, LOADS = (GROUPS + WAVES - 1) / WAVES;
+  static constexpr int CW = TT > 32 ? TC : TC / 2, TW = TT > 32 ? TT / 2 : TT;  // of half the sums
+  static constexpr int BOX = TW * CW * 4;
+  static constexpr int CF = (WAVES > 4 ? CW : TC) / 32, TF = (WAVES > 4 ? TW : TT) / 32;  // of a wave
 };
 
-template <bool F16, bool QKV, bool GELU, int TC, int TT, int R>
-__global__ __launch_bounds__(512, 2) void int8_tile_kernel(Args a) {
-  typedef Ring<TC, TT> F;
-  constexpr int STAGE = F::STAGE, LOADS = F::LOADS, CW = F::CW, TW = F::TW, CF = CW / 32, TF = TW / 32;
-  static_assert(F::BOX <= STAGE && R >= 4 && R <= 8, "a stage holds a wave's sums");
+template <bool F16, bool QKV, bool GELU, int TC, int TT, int R, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void int8_tile_kernel(Args a) {
+  typedef Ring<TC, TT, WAVES> F;
+  constexpr int STAGE = F::STAGE, LOADS = F::LOADS, CW = F::CW, TW = F::TW, CF = F::CF, TF = F::TF;
+  static_assert(F::BOX <= STAGE && R >= 4 && R <= 8, "a stage holds half a part's sums");
   __shared__ __attribute__((aligned(1024))) int8_t lds0[STAGE];
   __shared__ __attribute__((aligned(1024))) int8_t lds1[STAGE];
   __shared__ __attribute__((aligned(1024))) int8_t lds2[STAGE];
@@ -587,7 +589,7 @@ __global__ __launch_bounds__(512, 2) void int8_tile_kernel(Args a) {
     return i == 0 ? lds0 : i == 1 ? lds1 : i == 2 ? lds2 : i == 3 ? lds3 : i == 4 ? lds4 : i == 5 ? lds5 : i == 6 ? lds6 : lds7;
   };
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-  const int part = wave >> 1, share = wave & 1;
+  const int part = WAVES > 4 ? wave >> 1 : wave, share = WAVES > 4 ? wave & 1 : 0;
   const uint32_t tile = (blockIdx.x & 7) * a.tiles_xcd + (blockIdx.x >> 3);
   if (tile >= a.tiles) return;
   const Tile t = tile_at<TC, TT, 8>(a, tile);
@@ -599,20 +601,20 @@ __global__ __launch_bounds__(512, 2) void int8_tile_kernel(Args a) {
   int offset[LOADS];
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) {
-    const int r = 8 * (8 * j + wave) + (lane >> 3);
+    const int r = 8 * (WAVES * j + wave) + (lane >> 3);
     const bool there = r < TC ? r < a.columns - t.c0 : (uint32_t)(r - TC) < s.tokens - t.t0;
     offset[j] = there ? (r < TC ? r : r - TC) * a.padded + chunk * 16 : (int)0x80000000;
   }
   const int stages = (a.padded + 127) / 128;
   const Ends ends(a.padded, chunk);
-  const bool all = 8 * (LOADS - 1) + wave < F::GROUPS;  // (the last loads are not every wave's)
+  const bool all = WAVES * (LOADS - 1) + wave < F::GROUPS;  // (the last loads are not every wave's)
   auto load = [&](int8_t* dst, int stage, int j, int past) {
-    const int group = 8 * j + wave;
-    if (j < LOADS - 1 || all)
+    const int group = WAVES * j + wave;
+    if (F::GROUPS % WAVES == 0 || j < LOADS - 1 || all)
       load_lds16(group * 8 < TC ? wbase : qbase, dst + 1024 * group, offset[j] | past, uniform(stage * 128));
   };
   auto arrivals = [&] {
-    if (F::GROUPS % 8 == 0 || all) wait_arrivals<(R - 3) * LOADS>();
+    if (F::GROUPS % WAVES == 0 || all) wait_arrivals<(R - 3) * LOADS>();
     else wait_arrivals<(R - 3) * (LOADS - 1)>();
   };
   const int read = col * 128 + ((col >> 1 & 7) ^ (2 * part + half)) * 16;
@@ -671,14 +673,15 @@ __global__ __launch_bounds__(512, 2) void int8_tile_kernel(Args a) {
   auto box = [&](int k, int h) -> int8_t* { return k ? (h ? lds3 : lds2) : (h ? lds1 : lds0); };
   auto unit = [&](int token, int c) { return (token * CW + (c ^ (token & 7) * 4)) * 4; };
   auto hand = [&](bool add) {
-    int8_t* const to = box(part & 1, share);
 #pragma unroll
     for (int j = 0; j < TF; ++j)
 #pragma unroll
       for (int i = 0; i < CF; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          i32x4* const at = (i32x4*)(to + unit(j * 32 + col, i * 32 + g * 8 + half * 4));
+          const int h = WAVES > 4 ? share : TT > 32 ? j * 32 / TW : i * 32 / CW;
+          const int token = TT > 32 ? j * 32 % TW : j * 32, c = TT > 32 ? i * 32 : i * 32 % CW;
+          i32x4* const at = (i32x4*)(box(part & 1, h) + unit(token + col, c + g * 8 + half * 4));
           const i32x4 v = {acc[j][i][4 * g], acc[j][i][4 * g + 1], acc[j][i][4 * g + 2], acc[j][i][4 * g + 3]};
           *at = add ? *at + v : v;
         }
@@ -687,7 +690,7 @@ __global__ __launch_bounds__(512, 2) void int8_tile_kernel(Args a) {
   __syncthreads();
   if (part < 2) hand(true);
   __syncthreads();
-  for (int e = threadIdx.x; e < TT * (TC / 8); e += 512) {
+  for (int e = threadIdx.x; e < TT * (TC / 8); e += 64 * WAVES) {
     const int token = e / (TC / 8), c = e % (TC / 8) * 8;
     const int h = TT > 32 ? token / TW : c / CW;
     i32x4 sum[2];
@@ -712,9 +715,9 @@ struct Shape {
 };
 constexpr Shape SHAPES[KERNELS] = {
     // linear
-    {64, 32, 2.65f, 1.30f, 0.148f, 0.021f},
-    {32, 64, 1.72f, 2.38f, 0.144f, 0.060f},
-    {64, 64, 1.70f, 2.86f, 0.147f, 0.129f},
+    {64, 32, 2.97f, 1.34f, 0.102f, 0.065f},
+    {32, 64, 1.81f, 2.61f, 0.096f, 0.088f},
+    {64, 64, 1.74f, 2.84f, 0.127f, 0.134f},
     {96, 64, 1.67f, 3.78f, 0.189f, 0.133f},
     {96, 128, 0.95f, 5.82f, 0.258f, 0.234f},
     // qkv (a head's channels stay together)
@@ -748,13 +751,13 @@ struct Choice {
   float us;
 };
 
-// The kernel whose estimate is the least: over those sizes 0.7% (linear) and 0.4% (qkv) slower than always the
-// fastest.  Measured, rows x features x columns, us for 64 x 32 / 32 x 64 / 64 x 64 / 96 x 64 / 96 x 128 / 256 x 256
-// tiles: 77 x 4096 x 3072 9.1 / 9.2 / 9.4 / 11.4 / 14.7 / 40; 128 x 3072 x 12288 18.9 / 23 / 18.4 / 14.0 / 16.5 / 33;
-// 512 x 12288 x 3072 56 / 62 / 50 / 31 / 39 / 110; 256 x 3072 x 9216 27 / 36 / 25 / 22 / 16.6 / 34; 4096 x 3072 x 3072
-// - / - / 96 / 79 / 64 / 43; 1 x 3072 x 18432 13.7 / 22 / 18.8 / 13.1 / 14.6 / 33.  qkv, rows x features, 24 heads, us
-// for 128 x 32 / 128 x 64 / 128 x 128 / 256 x 256: 1 x 3072 11 / 13 / 17 / 39; 128 x 3072 21 / 15 / 20 / 43;
-// 512 x 3072 48 / 39 / 38 / 45; 512 + 4096 x 3072 368 / 246 / 202 / 147.
+// The kernel whose estimate is the least: over those sizes 0.5% slower than always the fastest.  Measured, rows x
+// features x columns, us for 64 x 32 / 32 x 64 / 64 x 64 / 96 x 64 / 96 x 128 / 256 x 256 tiles: 77 x 4096 x 3072 9.5 /
+// 9.0 / 10.1 / 12.2 / 15.3 / 40; 128 x 3072 x 12288 18 / 21 / 17 / 12.1 / 15.5 / 32; 512 x 12288 x 3072 45 / 54 / 45 /
+// 28.8 / 37 / 108; 666 x 1000 x 777 6.9 / 8.9 / 6.4 / 7.4 / 9.6 / 18; 256 x 3072 x 9216 25 / 32 / 23 / 20 / 15.4 / 33;
+// 4096 x 3072 x 3072 96 / 141 / 86 / 74 / 56 / 38; 1 x 3072 x 18432 13.4 / 19.5 / 17.0 / 12.8 / 14.1 / 31.  qkv, rows x
+// features, 24 heads, us for 128 x 32 / 128 x 64 / 128 x 128 / 256 x 256: 1 x 3072 11.2 / 12.0 / 15.9 / 37; 128 x 3072
+// 21 / 14.7 / 19.3 / 41; 512 x 3072 48 / 37 / 36 / 43; 512 + 4096 x 3072 365 / 236 / 192 / 141.
 Choice choose(const Args& a, int count, bool qkv) {
   const Kernel wide = qkv ? WIDE_HEADS : WIDE256;
   Choice best = {wide, estimate(a, count, wide)};
@@ -794,31 +797,31 @@ int launch_kernel(Args& a, int count, Kernel kernel, hipStream_t st) {
   a.tiles0 = (uint32_t)tiles_of(a, 1, tc, tt);
   a.tiles = (uint32_t)tiles;
   a.tiles_xcd = (a.tiles + 7) / 8;
-  const dim3 each(8 * a.tiles_xcd), eight(512);
+  const dim3 each(8 * a.tiles_xcd), four(256), eight(512);
   switch (kernel) {
     case T64x32:
-      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 64, 32, 6>), each, eight, 0, st, a);
+      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 64, 32, 6, 4>), each, four, 0, st, a);
       break;
     case T32x64:
-      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 32, 64, 8>), each, eight, 0, st, a);
+      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 32, 64, 8, 4>), each, four, 0, st, a);
       break;
     case T64x64:
-      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 64, 64, 8>), each, eight, 0, st, a);
+      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 64, 64, 8, 8>), each, eight, 0, st, a);
       break;
     case T96x64:
-      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 96, 64, 7>), each, eight, 0, st, a);
+      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 96, 64, 7, 8>), each, eight, 0, st, a);
       break;
     case T96x128:
-      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 96, 128, 5>), each, eight, 0, st, a);
+      if constexpr (!QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 96, 128, 5, 8>), each, eight, 0, st, a);
       break;
     case T128x32:
-      if constexpr (QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 128, 32, 7>), each, eight, 0, st, a);
+      if constexpr (QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 128, 32, 7, 8>), each, eight, 0, st, a);
       break;
     case T128x64:
-      if constexpr (QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 128, 64, 6>), each, eight, 0, st, a);
+      if constexpr (QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 128, 64, 6, 8>), each, eight, 0, st, a);
       break;
     case T128x128:
-      if constexpr (QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 128, 128, 4>), each, eight, 0, st, a);
+      if constexpr (QKV) hipLaunchKernelGGL((int8_tile_kernel<F16, QKV, GELU, 128, 128, 4, 8>), each, eight, 0, st, a);
       break;
     default: {
       const uint32_t per_xcd = std::max(1, device_cu_count() / 8);
