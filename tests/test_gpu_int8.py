@@ -285,6 +285,18 @@ def test_last_rows_apart(features):
     assert torch.equal(out.flatten(0, 1)[16000:], int8_linear(flat._replace(q=flat.q[16000:], scale=flat.scale[16000:]), w))
 
 
+def test_last_rows_of_the_second_set_apart():
+    gen = _gen(17)
+    K, N = 1400, 3064
+    sets = [dict(x=_rows(gen, (2, rows), K), weight=_weight(gen, N, K), bias=_randn(gen, N)) for rows in (256, 8192 - 77)]
+    for out, s in zip(int8_linear_pair(*sets), sets):
+        assert torch.equal(out, torch.cat([int8_linear(s["x"]._replace(q=s["x"].q[b:b + 1], scale=s["x"].scale[b:b + 1]),
+                                                       s["weight"], s["bias"]) for b in range(2)]))
+        for at in (slice(0, 30), slice(-30, None)):
+            x = Int8Rows(s["x"].q[1, at], s["x"].scale[1, at], K, BF16)
+            _check_linear(out[1, at], x, s["weight"], s["bias"])
+
+
 @pytest.mark.parametrize("offset", range(8))
 def test_linear_into_rows_that_start_anywhere(offset):
     """Output rows at every alignment of whole elements, odd strides among them; what is around them stays."""
@@ -397,6 +409,23 @@ def test_qkv(B, T, n, heads, K, dtype):
                    norms=((t and t["q"], i["q"]), (t and t["k"], i["k"])), cos=cos, sin=sin)
     assert out.shape == (3, B, T + n, heads, 128) and out.dtype == dtype and out.is_contiguous()
     _check_qkv(out, sets, heads, cos, sin)
+
+
+@pytest.mark.parametrize("B,T,n", [(1, 0, 14587), (1, 500, 14060), (2, 250, 7030)])
+def test_qkv_last_rows_apart(B, T, n):
+    gen = _gen(n)
+    heads, K = 24, 1400
+    sets = ([_qkv_set(gen, B, T, K, heads, BF16)] if T else []) + [_qkv_set(gen, B, n, K, heads, BF16)]
+    cos, sin = _tables(T, n)
+    t, i = (sets[0] if T else None), sets[-1]
+    out = int8_qkv(t and t["x"], i["x"], heads=heads, weights=(t and t["w"], i["w"]), biases=(t and t["b"], i["b"]),
+                   norms=((t and t["q"], i["q"]), (t and t["k"], i["k"])), cos=cos, sin=sin)
+    for at in (slice(0, 20), slice(n - 300, n - 240), slice(n - 30, n)):  # (of the image rows)
+        part = {**i, "x": Int8Rows(i["x"].q[:, at].contiguous(), i["x"].scale[:, at].contiguous(), K, BF16)}
+        place = slice(T + at.start, T + at.stop)
+        _check_qkv(out[:, :, place], [part], heads, cos[place], sin[place])
+    if T:
+        _check_qkv(out[:, :, :T], [t], heads, cos[:T], sin[:T])
 
 
 def test_qkv_parts_may_be_missing():
