@@ -426,10 +426,12 @@ class FluxTransformer:
             return h, hn
         return None, adaln_modulate(h[:, T:], shift, scale, y=p[:, T:], gate=gate, eps=s.eps)
 
-    def _blocks(self, x, c, cos, sin, attention, double_mods, single_mods, out_mods):
-        """All blocks on embedded image rows x and text rows c; the image rows as the output norm modulates
-        them."""
+    def _blocks(self, streams, cos, sin, attention, double_mods, single_mods, out_mods):
+        """All blocks on ``streams`` = [image rows, text rows], embedded, which it takes out of the list, so that
+        they end with the double blocks; the image rows as the output norm modulates them."""
         s = self.shape
+        x, c = streams
+        streams.clear()
         (B, n, _), T = x.shape, c.shape[1]
         (sx, scx, *_), (sc, scc, *_) = double_mods[0]
         xn, cn = adaln_modulate_pair(dict(x=x, shift=sx, scale=scx), dict(x=c, shift=sc, scale=scc), eps=s.eps)
@@ -531,9 +533,10 @@ class FluxTransformer:
             return h, adaln_quantize(h, shift, scale, y=p, gate=mods[2], x_out=h, eps=s.eps)
         return None, adaln_modulate(h[:, T:], shift, scale, y=p[:, T:], gate=mods[2], eps=s.eps)
 
-    def _blocks_int8(self, x, c, cos, sin, attention, double_mods, single_mods, out_mods):
-        """All blocks on embedded image rows x and text rows c; the image rows as the output norm modulates
-        them (16 bits)."""
+    def _blocks_int8(self, streams, cos, sin, attention, double_mods, single_mods, out_mods):
+        """_blocks in 8 bits; the image rows as the output norm modulates them are 16-bit."""
+        x, c = streams
+        streams.clear()
         s, T = self.shape, c.shape[1]
         last = len(self.double) - 1
         # each block's first (shift, scale) for image and text rows; after the double blocks one for both
@@ -548,6 +551,7 @@ class FluxTransformer:
         if not self.single:  # (the output layer takes 16-bit rows)
             return adaln_modulate(h[:, T:], *out_mods, eps=s.eps)
         hn = (cn, xn)
+        del x, xn, c, cn
         for j, w in enumerate(self.single):
             nxt = single_mods[j + 1][:2] if j + 1 < len(self.single) else out_mods
             h, hn = self._single_block_int8(w, single_mods[j], h, hn, T, cos, sin, attention, s.num_layers + j, nxt)
@@ -593,9 +597,9 @@ class FluxTransformer:
         cos, sin = rotary_tables(torch.cat([txt_ids, img_ids]).to(self.device))
         double_mods, single_mods, out_mods = self._modulations(self.temb(timestep, guidance,
                                                                          pooled_projections, silu=True))
-        x = _linear(hidden_states.to(self.dtype), *self.x_embedder)
-        c = _linear(encoder_hidden_states.to(self.dtype), *self.context_embedder)
-        hn = (self._blocks_int8 if self.int8 else self._blocks)(x, c, cos, sin, attention, double_mods, single_mods,
+        streams = [_linear(hidden_states.to(self.dtype), *self.x_embedder),
+                   _linear(encoder_hidden_states.to(self.dtype), *self.context_embedder)]
+        hn = (self._blocks_int8 if self.int8 else self._blocks)(streams, cos, sin, attention, double_mods, single_mods,
                                                                 out_mods)
         out = _linear(hn, *self.proj_out)
         if layout is not None and layout_scope == "transformer":
