@@ -71,6 +71,10 @@ SIGNATURES = {
     "hb_int8_rows": (_c_int, [_p, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p, _p]),
     "hb_int8_adaln": (_c_int, [_c_int, _c_int, _p, _c_int, _c_int, _c_int, _c_f32, _p, _p, _p]),
     "hb_int8_linear": (_c_int, [_c_int, _c_int, _p, _c_int, _c_int, _c_int, _c_int, _p, _p, _p]),
+    "hb_int8_linear_rows": (
+        _c_int,
+        [_p, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p, _p, _p, _c_i64, _c_i64, _p],
+    ),
     "hb_int8_qkv": (
         _c_int,
         [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f32, _p, _p, _p, _p, _c_i64, _c_i64, _c_i64, _p],

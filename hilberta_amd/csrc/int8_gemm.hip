@@ -18,7 +18,7 @@
 #include <type_traits>
 #include <utility>
 
-#include "common.h"
+#include "int8_common.h"
 #include "../../include/hilberta_hip.h"
 
 namespace hb {
@@ -27,7 +27,6 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int MAX_FEATURES = 1 << 17;
 constexpr int HEAD = 128;
 
 // One set of rows with its weight.  Two sets (a block's text and image rows) share a launch.
@@ -156,8 +155,12 @@ __device__ __forceinline__ void store8(const Args& a, uint16_t* out, int c, cons
 
 // The sum over 16 neighbouring lanes, in each of them: of pairs, of quads, of the mirrored half row and row.
 template <int CONTROL>
+__device__ __forceinline__ uint32_t moved_bits(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, 0xf, 0xf, true);
+}
+template <int CONTROL>
 __device__ __forceinline__ float moved(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CONTROL, 0xf, 0xf, true));
+  return __builtin_bit_cast(float, moved_bits<CONTROL>(__builtin_bit_cast(uint32_t, v)));
 }
 __device__ __forceinline__ float sum16(float v) {
   v += moved<0xb1>(v);
@@ -221,12 +224,11 @@ __device__ __forceinline__ void finish(const Args& a, const Set& s, const i32x16
   }
 }
 
-// Channels c0 + c .. + 7 of token `at`, of its sums (qkv: 16 neighbouring lanes hold a head).
+// Channels c0 + c .. + 7 of token `at`, of its sums and scale (qkv: 16 neighbouring lanes hold a head).
 template <bool F16, bool QKV, bool GELU, int TC>
-__device__ __forceinline__ void finish8(const Args& a, const Set& s, const i32x4 (&sum)[2], const float (&channel)[3][TC],
-                                        int c0, uint32_t at, int c) {
+__device__ __forceinline__ void finish8(const Args& a, const Set& s, const i32x4 (&sum)[2], float scale,
+                                        const float (&channel)[3][TC], int c0, uint32_t at, int c) {
   const int plane = QKV ? c0 / (a.heads * HEAD) : 2;
-  const float scale = s.scale[min(at, s.tokens - 1)];
   float v[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = (float)sum[k >> 2][k & 3] * scale * channel[0][c + k] + channel[1][c + k];
@@ -699,7 +701,193 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void int8_tile_kernel(Args a
       const int at = unit(TT > 32 ? token % TW : token, (TT > 32 ? c : c % CW) + 4 * g);
       sum[g] = *(const i32x4*)(box(0, h) + at) + *(const i32x4*)(box(1, h) + at);
     }
-    finish8<F16, QKV, GELU, TC>(a, s, sum, channel, t.c0, t.t0 + token, c);
+    const uint32_t to = t.t0 + token;
+    finish8<F16, QKV, GELU, TC>(a, s, sum, s.scale[min(to, s.tokens - 1)], channel, t.c0, to, c);
+  }
+}
+
+// ------------------------------------------------------------------ a few rows of 16 bits
+// Linear layer of rows that are quantized here, by every workgroup for itself: few enough that this hides behind
+// the first weights' way to it, and saves a launch.  TC channels a workgroup of four waves, a part of a stage's
+// features each; a ring of R stages of the weight alone, three workgroups a CU.  Bound by the weight's read: 1 x 3072 x
+// 18432 (57 MB) 11.5 us, 4.9 TB/s (64 channels, six stages: 12.3; 32768 values of rows in LDS, two workgroups a CU:
+// 17.1); small ones by the launch, 1 x 512 x 2048 6.0.
+constexpr int FEW_ROWS = 32, FEW_VALUES = HB_INT8_FEW_VALUES;
+
+struct FewArgs {
+  Args a;  // (its one set has neither q nor scale)
+  const uint16_t* x;
+  int64_t x_b, x_n;
+  int32_t features;
+};
+
+template <bool F16, bool GELU, int TC, int R>
+__global__ __launch_bounds__(256, 2) void int8_few_kernel(FewArgs f) {
+  constexpr int STAGE = TC * 128, LOADS = STAGE / 4096, CF = TC / 32, VECTORS = FEW_VALUES / 2048;
+  static_assert(R == 6 || R == 8, "an even ring");
+  __shared__ __attribute__((aligned(1024))) int8_t lds0[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds1[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds2[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds3[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds4[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds5[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds6[R > 6 ? STAGE : 1];
+  __shared__ __attribute__((aligned(1024))) int8_t lds7[R > 7 ? STAGE : 1];
+  __shared__ __attribute__((aligned(16))) int8_t rows[FEW_VALUES];
+  __shared__ __attribute__((aligned(16))) float channel[3][TC];
+  __shared__ uint32_t groups[FEW_VALUES / 64], tops[FEW_ROWS];
+  __shared__ float scales[FEW_ROWS];
+  auto ring = [&](auto index) -> int8_t* {
+    constexpr int i = decltype(index)::value % R;
+    return i == 0 ? lds0 : i == 1 ? lds1 : i == 2 ? lds2 : i == 3 ? lds3 : i == 4 ? lds4 : i == 5 ? lds5 : i == 6 ? lds6 : lds7;
+  };
+  const Args& a = f.a;
+  const Set& s = a.set[0];
+  const int lane = threadIdx.x & 63, part = uniform(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+  const int c0 = blockIdx.x * TC;
+  // The rows' values, asked for before any weights: eight at a time, a row's after the one's before it.
+  const int padded = a.padded, row_bytes = (padded + 127) & ~127;  // (in LDS)
+  const uint32_t each = (uint32_t)padded / 8, all = s.tokens * each;
+  auto row_at = [&](uint32_t r) {
+    const uint32_t b = r / s.rows;
+    return f.x + b * f.x_b + (int64_t)(r - b * s.rows) * f.x_n;
+  };
+  u32x4 raw[VECTORS];
+  uint32_t row[VECTORS];
+#pragma unroll
+  for (int v = 0; v < VECTORS; ++v) {
+    const uint32_t at = v * 256 + threadIdx.x;
+    row[v] = at / each;
+    raw[v] = u32x4{0, 0, 0, 0};
+    const int c = (int)(at - row[v] * each) * 8;
+    if (at < all) raw[v] = *(const any_u32x4*)(row_at(row[v]) + min(c, f.features - 8));
+  }
+  // (load_channels, whose loads have to be asked for before those to LDS too)
+  const int mine = min(c0 + (int)threadIdx.x % TC, a.columns - 1);
+  const float weight_scale = s.w_scale[mine];
+  const uint16_t bias = (s.bias ? s.bias : (const uint16_t*)s.w_scale)[mine];  // (a value unused; no branch to wait at)
+  // Loads of the weight as in the tile kernel.
+  const int8_t* const wbase = s.w + (int64_t)c0 * padded;
+  const int chunk = (lane & 7) ^ ((4 * part + (lane >> 4)) & 7);
+  int offset[LOADS];
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int r = 8 * (4 * j + part) + (lane >> 3);
+    offset[j] = r < a.columns - c0 ? r * padded + chunk * 16 : (int)0x80000000;
+  }
+  const int stages = (padded + 127) / 128;
+  const Ends ends(padded, chunk);
+  auto load = [&](int8_t* dst, int stage, int j, int past) {
+    load_lds16(wbase, dst + 1024 * (4 * j + part), offset[j] | past, uniform(stage * 128));
+  };
+  // (Zeros into the last stage as above.)
+  load(ring(std::integral_constant<int, R - 1>()), 0, 0, (int)0x80000000);
+  auto begin = [&](auto index) {
+    constexpr int I = decltype(index)::value;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) load(ring(index), I, j, ends.past(I));
+  };
+  begin_all(begin, std::make_integer_sequence<int, R - 1>());
+  // The rows' largest patterns: of eight lanes, which are always of one row, then of a row's groups of those.
+#pragma unroll
+  for (int v = 0; v < VECTORS; ++v) {
+    const int c = (int)(v * 256 + threadIdx.x - row[v] * each) * 8, past = c + 8 - f.features;
+    if (past > 0) raw[v] = drop_values(raw[v], min(past, 8));  // (what lies before a row's last values)
+    uint32_t top = fp32_bits<F16>(max_pairs(u16x2{0, 0}, raw[v]));
+    top = max(top, moved_bits<0xb1>(top));
+    top = max(top, moved_bits<0x4e>(top));
+    top = max(top, moved_bits<0x141>(top));
+    if ((lane & 7) == 0) groups[v * 32 + (threadIdx.x >> 3)] = top;
+  }
+  if (threadIdx.x < TC) {
+    channel[0][threadIdx.x] = weight_scale;
+    channel[1][threadIdx.x] = s.bias ? to_f<F16>(bias) : 0.f;
+  }
+  wait_loads<63>();
+  barrier();
+  for (uint32_t m = part; m < s.tokens; m += 4) {
+    uint32_t top = 0;
+    for (uint32_t k = lane; k < each / 8; k += 64) top = max(top, groups[m * (each / 8) + k]);
+    top = max(top, moved_bits<0xb1>(top));
+    top = max(top, moved_bits<0x4e>(top));
+    top = max(top, moved_bits<0x141>(top));
+    top = max(top, moved_bits<0x140>(top));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    if (lane == 0) tops[m] = top;
+  }
+  wait_loads<63>();
+  barrier();
+  // Their whole numbers: chunks of 16 bytes, each 128 bytes' in an order of the row's, so that rows lie in
+  // different banks.
+#pragma unroll
+  for (int v = 0; v < VECTORS; ++v) {
+    const uint32_t at = v * 256 + threadIdx.x;
+    if (at < all) {
+      const Scaler scaler(tops[row[v]]);
+      const int c = (int)(at - row[v] * each) * 8;
+      float values[8];
+      unpack8<F16>(raw[v], values);
+      *(u32x2*)(rows + row[v] * row_bytes + (c & ~127) + ((c >> 4 & 7) ^ (row[v] & 7)) * 16 + (c & 8)) = pack_row8(scaler, values);
+      if (c == 0) scales[row[v]] = scaler.scale;
+    }
+  }
+  wait_loads<63>();
+  wait_arrivals<(R - 3) * LOADS>();
+  barrier();
+  const int read = col * 128 + ((col >> 1 & 7) ^ (2 * part + half)) * 16;
+  const int token = min(col, (int)s.tokens - 1), xread = token * row_bytes + ((2 * part + half) ^ (token & 7)) * 16;
+  i32x4 w[2][CF], x[2];
+  auto fetch = [&](const int8_t* src, int stage, int to) {
+#pragma unroll
+    for (int i = 0; i < CF; ++i) w[to][i] = *(const i32x4*)(src + read + i * 4096);
+    x[to] = *(const i32x4*)(rows + xread + min(stage, stages - 1) * 128);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  i32x16 acc[CF] = {};
+  int n = 0;
+  auto step = [&](auto index) {
+    constexpr int I = decltype(index)::value;
+    int8_t* const free = ring(std::integral_constant<int, I + R - 1>());
+    const int past = ends.past(uniform(n + R - 1));
+#pragma unroll
+    for (int i = 0; i < CF; ++i) {
+      acc[i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[I & 1][i], x[I & 1], acc[i], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      load(free, n + R - 1, i, past);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    fetch(ring(std::integral_constant<int, I + 1>()), n + 1, ~I & 1);
+    wait_arrivals<(R - 3) * LOADS>();
+    barrier();
+    return ++n == stages;
+  };
+  static_assert(LOADS == CF, "a load a product");
+  fetch(lds0, 0, 0);
+  while (!step_all(step, std::make_integer_sequence<int, R>())) {}
+  wait_loads<0>();  // (nothing is on its way to LDS any more)
+  barrier();
+  // The four parts' sums, [token][channel], each in a stage.
+  int8_t* const box = part == 0 ? lds0 : part == 1 ? lds1 : part == 2 ? lds2 : lds3;
+  if (col < (int)s.tokens) {
+#pragma unroll
+    for (int i = 0; i < CF; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(i32x4*)(box + (col * TC + ((i * 32 + g * 8 + half * 4) ^ (col & 7) * 4)) * 4) =
+            i32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
+  }
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < s.tokens * (TC / 8); e += 256) {
+    const uint32_t to = e / (TC / 8);
+    const int c = e % (TC / 8) * 8;
+    i32x4 sum[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int at = (to * TC + ((c + 4 * g) ^ (to & 7) * 4)) * 4;
+      sum[g] = *(const i32x4*)(lds0 + at) + *(const i32x4*)(lds1 + at) + *(const i32x4*)(lds2 + at) + *(const i32x4*)(lds3 + at);
+    }
+    finish8<F16, false, GELU, TC>(a, s, sum, scales[to], channel, c0, to, c);
   }
 }
 
@@ -858,6 +1046,13 @@ int launch(Args& a, int count, int32_t dtype, hipStream_t st) {
     return a.gelu ? launch_type<false, false, true>(a, count, st) : launch_type<false, false, false>(a, count, st);
 }
 
+template <bool F16, bool GELU>
+int launch_few(const FewArgs& f, hipStream_t st) {
+  hipLaunchKernelGGL((int8_few_kernel<F16, GELU, 32, 8>), dim3((f.a.columns + 31) / 32), dim3(256), 0, st, f);
+  HB_HIP(hipGetLastError());
+  return HB_OK;
+}
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // The checks both entry points make of a set's rows and weight.
@@ -901,6 +1096,37 @@ extern "C" int hb_int8_linear(int32_t count, int32_t batch, const int32_t* rows,
     a.vectors &= aligned16(s.out) && s.out_b % 8 == 0 && s.out_n % 8 == 0;
   }
   return launch<false>(a, count, dtype, stream);
+}
+
+extern "C" int hb_int8_linear_rows(const void* x, int64_t batch_stride, int64_t row_stride, int32_t batch, int32_t rows,
+                                   int32_t features, int32_t columns, int32_t padded, int32_t dtype, int32_t gelu,
+                                   const int8_t* weight, const float* weight_scale, const void* bias, void* out,
+                                   int64_t out_batch_stride, int64_t out_row_stride, hb_stream_t stream) {
+  HB_REQUIRE(x && weight && weight_scale && out, "null pointer argument");
+  HB_REQUIRE(batch > 0 && rows > 0 && batch <= FEW_ROWS && rows <= FEW_ROWS && batch * rows <= FEW_ROWS, "batch and rows must be positive, with at most %d rows in all", FEW_ROWS);
+  HB_REQUIRE(features >= 8, "at least 8 features");
+  HB_REQUIRE(padded >= features && padded % 64 == 0 && padded <= FEW_VALUES, "padded must be a multiple of 64, no smaller than features");
+  HB_REQUIRE(batch * rows * ((padded + 127) / 128 * 128) <= FEW_VALUES, "at most %d values of rows in all", FEW_VALUES);
+  HB_REQUIRE(columns > 0 && columns < (1 << 28), "columns must be positive (and below 2^28)");
+  HB_REQUIRE(dtype == HB_DTYPE_BF16 || dtype == HB_DTYPE_F16, "dtype must be bf16 or fp16");
+  HB_REQUIRE(gelu == 0 || gelu == 1, "gelu must be 0 or 1");
+  HB_REQUIRE((((uintptr_t)x | (uintptr_t)bias | (uintptr_t)out) & 1) == 0 && aligned16(weight) && ((uintptr_t)weight_scale & 3) == 0,
+             "x, bias and out must be 2-byte, the weight 16-byte and its scales 4-byte aligned");
+  HB_REQUIRE(batch_stride >= 0 && row_stride >= 0 && out_batch_stride >= 0 && out_row_stride >= 0, "strides must be non-negative");
+  FewArgs f = {};
+  f.x = (const uint16_t*)x;
+  f.x_b = batch_stride;
+  f.x_n = row_stride;
+  f.features = features;
+  Args& a = f.a;
+  a.columns = columns;
+  a.padded = padded;
+  a.gelu = gelu;
+  a.vectors = aligned16(out) && out_batch_stride % 8 == 0 && out_row_stride % 8 == 0;
+  a.set[0] = {nullptr, nullptr, weight, weight_scale, (const uint16_t*)bias, (uint16_t*)out, {nullptr, nullptr},
+              out_batch_stride, out_row_stride, (uint32_t)rows, (uint32_t)(batch * rows), 0, 0};
+  if (dtype == HB_DTYPE_F16) return gelu ? launch_few<true, true>(f, stream) : launch_few<true, false>(f, stream);
+  return gelu ? launch_few<false, true>(f, stream) : launch_few<false, false>(f, stream);
 }
 
 extern "C" int hb_int8_qkv(int32_t batch, int32_t text_tokens, int32_t tokens, int32_t heads, int32_t padded,

@@ -590,8 +590,37 @@ Tensor int8_linear(const Tensor& q, const Tensor& scale, const Tensor& weight, c
   return out;
 }
 
+// Whether a few 16-bit rows take one launch (hb_int8_linear_rows): where its workgroups, which quantize the rows each
+// for itself, run all at once, and ask for the weight as fast as the product of 8-bit rows does: a weight up to 48 MB,
+// or enough workgroups.  Rows x features x columns, us for two launches and one: 1 x 512 x 2048 12.4, 6.0; 1 x 3072 x
+// 18432 16.1, 11.5; 5 x 3072 x 18432 16.5, 12.8; 32 x 512 x 18432 12.3, 11.2; 1 x 12288 x 3072 21.7, 14.9; on the other
+// side 1 x 8192 x 8192 17.4, 20.7; 30 x 512 x 30000 12.3, 16.4.
+bool one_launch(int64_t rows, int64_t features, int64_t columns) {
+  return rows <= 32 && features >= 8 && rows * ((features + 127) / 128 * 128) <= HB_INT8_FEW_VALUES && columns <= 24576 &&
+         (padded_features(features) * columns <= (48 << 20) || columns >= 14336);
+}
+
 // int8_rows and int8_linear in one call: a short layer's time is the host's.
 Tensor int8_linear_rows(const Tensor& x, const Tensor& weight, const Tensor& weight_scale, const Maybe& bias, bool gelu) {
+  const int64_t count = x.dim() ? x.numel() / std::max<int64_t>(x.size(-1), 1) : 0, features = x.dim() ? x.size(-1) : 0;
+  if (x.is_cuda() && count > 0 && weight.dim() == 2 && weight.size(0) > 0 && one_launch(count, features, weight.size(0))) {
+    const int32_t dtype = type_of(x.scalar_type(), "rows");
+    const Rows r = rows_of(x, "rows");
+    const Tensor& b = value_or_none(bias);
+    const int64_t columns = weight.size(0), padded = padded_features(features);
+    check_weight(weight, weight_scale, b, padded, columns, x.scalar_type());
+    one_device(x, {&weight, &weight_scale, &b});
+    const at::OptionalDeviceGuard guard(x.device());
+    c10::SmallVector<int64_t, 3> sizes(x.sizes().begin(), x.sizes().end());
+    sizes.back() = columns;
+    Tensor out = new_tensor(x, sizes, x.scalar_type());
+    check(hb_int8_linear_rows(x.data_ptr(), r.batch_stride, r.row_stride, i32(r.batch, "batch"), i32(r.rows, "rows"),
+                              i32(features, "features"), i32(columns, "columns"), i32(padded, "padded"), dtype, gelu,
+                              static_cast<int8_t*>(weight.data_ptr()), static_cast<float*>(weight_scale.data_ptr()),
+                              pointer(b), out.data_ptr(), r.rows * columns, columns, stream_of(x.device())),
+          "hb_int8_linear_rows");
+    return out;
+  }
   const auto [q, scale] = int8_rows(x);
   return int8_linear(q, scale, weight, weight_scale, bias, x.scalar_type(), gelu);
 }

@@ -252,6 +252,16 @@ int hb_int8_linear(int32_t count, int32_t batch, const int32_t* rows, int32_t co
                    int32_t padded, int32_t dtype, int32_t gelu, void* const* pointers,
                    const int64_t* strides, hb_stream_t stream);
 
+/* hb_int8_rows and hb_int8_linear of a few 16-bit rows [batch, rows, features] in one launch, with the same
+ * results: at least 8 features, at most 32 rows, and rows x (padded rounded up to 128) at most
+ * HB_INT8_FEW_VALUES.  x and out by element strides, any alignment of whole elements. */
+#define HB_INT8_FEW_VALUES 16384
+int hb_int8_linear_rows(const void* x, int64_t batch_stride, int64_t row_stride, int32_t batch,
+                        int32_t rows, int32_t features, int32_t columns, int32_t padded,
+                        int32_t dtype, int32_t gelu, const int8_t* weight,
+                        const float* weight_scale, const void* bias, void* out,
+                        int64_t out_batch_stride, int64_t out_row_stride, hb_stream_t stream);
+
 /* Joint Q/K/V projection of 8-bit rows with the heads' RMSNorm and rotation in the same pass:
  *   p = as hb_int8_linear with columns [Q | K | V] of heads * 128 each
  *   out[0], out[1] (Q, K): p * rsqrt(mean(p^2) + eps) * norm over each head, pairs (2i, 2i + 1) rotated by

@@ -329,6 +329,38 @@ def test_linear_takes_16_bit_rows():
     O.held(out, ref, step * 1.01)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("lead,features,columns", [((1,), 8, 1), ((1,), 3072, 18432), ((1,), 16384, 100), ((2,), 8192, 33),
+                                                   ((2,), 8129, 65), ((32,), 512, 300), ((31,), 500, 129), ((3, 2), 777, 64),
+                                                   ((1, 5), 2049, 4100), ((4, 8), 9, 40), ((2, 1), 64, 12290),
+                                                   ((7,), 2111, 13000), ((1,), 65, 31), ((33,), 100, 50), ((2,), 8193, 40)])
+def test_linear_of_a_few_16_bit_rows(lead, features, columns, dtype):
+    """One launch gives what two do, to the bit: up to 32 rows and 16384 values, and past that."""
+    gen = _gen(features)
+    big = _randn(gen, *lead, features + 11, dtype=dtype)
+    b = _randn(gen, columns, dtype=dtype)
+    w = _weight(gen, columns, features)
+    for x in (big[..., :features].contiguous(), big[..., 3:features + 3]):
+        rows = quantize_rows(x)
+        for gelu, bias in ((False, None), (True, b)):
+            got = int8_linear(x, w, bias, gelu=gelu)
+            assert got.shape == (*lead, columns) and torch.equal(got, int8_linear(rows, w, bias, gelu=gelu))
+    _check_linear(got, rows, w, b, True)
+
+
+def test_a_few_bad_rows():
+    gen = _gen(4)
+    x = _randn(gen, 5, 300)
+    x[1] = 0
+    x[2, 7], x[3, 299], x[4, 0] = float("inf"), float("nan"), 3e38
+    w, b = _weight(gen, 70, 300), _randn(gen, 70)
+    got = int8_linear(x, w, b)
+    assert torch.equal(got[:2], int8_linear(quantize_rows(x[:2]), w, b)) and torch.equal(got[1], b)
+    assert torch.isnan(got[2:4]).all() and torch.equal(got[4], int8_linear(quantize_rows(x), w, b)[4])
+    empty = int8_linear(x[:0], w, b)
+    assert empty.shape == (0, 70)
+
+
 def test_largest_sums():
     """Every product 127 * 127 over 2^17 features: the sum fits 32 bits."""
     K = 1 << 17

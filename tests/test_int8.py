@@ -219,6 +219,18 @@ def test_entry_points_reject_before_any_launch():
                strides=(0, 40, 0, 40)):
         return (count, batch, (I32 * 2)(*rows), columns, padded, dtype, gelu, (P * 12)(*pointers), (I64 * 4)(*strides), None)
 
+    def few(x=16, bs=0, rs=64, batch=1, rows=4, features=60, columns=40, padded=64, dtype=0, gelu=0, w=256, ws=256, bias=None,
+            out=256, ob=0, on=40):
+        return (x, bs, rs, batch, rows, features, columns, padded, dtype, gelu, w, ws, bias, out, ob, on, None)
+
+    for match, over in (("null", dict(x=None)), ("null", dict(w=None)), ("null", dict(out=None)), ("positive", dict(rows=0)),
+                        ("32 rows", dict(rows=33)), ("32 rows", dict(batch=8, rows=5)), ("8 features", dict(features=7)),
+                        ("padded", dict(padded=72)), ("padded", dict(features=65)), ("padded", dict(padded=16448)),
+                        ("16384 values", dict(rows=3, features=8000, padded=8000)), ("columns", dict(columns=0)),
+                        ("dtype", dict(dtype=2)), ("gelu", dict(gelu=2)), ("aligned", dict(w=264)), ("aligned", dict(x=17)),
+                        ("aligned", dict(ws=258)), ("strides", dict(on=-1))):
+        _einval(match, "hb_int8_linear_rows", *few(**over))
+
     p = (256, 256, 256, 256, None, 256)
     for match, over in (("count", dict(count=0)), ("columns", dict(columns=0)), ("padded", dict(padded=72)),
                         ("padded", dict(padded=1 << 18)), ("dtype", dict(dtype=2)), ("gelu", dict(gelu=2)),
