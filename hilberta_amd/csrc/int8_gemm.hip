@@ -10,9 +10,11 @@
 // once, to the 16-bit output.
 //
 // The weight's channels are the rows of the matrix instruction (v_mfma_i32_32x32x32_i8) and the tokens its
-// columns: a lane then holds one token's values, 4 consecutive channels an accumulator quarter, so that a
-// token's scale is one register, a rotated pair lies in one lane, and a head's 128 channels in the lanes l
-// and l + 32.
+// columns: a lane then holds one token's values, 4 consecutive channels an accumulator quarter, so that they move
+// 16 bytes at a time and a token's scale is one register.
+//
+// Three kernels: many rows (int8_wide_kernel), fewer (int8_tile_kernel), and a few that come in 16 bits and are
+// quantized in the same launch (int8_few_kernel, linear only).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

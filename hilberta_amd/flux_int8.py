@@ -106,7 +106,8 @@ def _check_features(weight, features):
 
 def int8_linear(x, weight, bias=None, *, gelu=False, out=None):
     """act(x @ weight^T + bias) for x Int8Rows, or 16-bit rows that are quantized first, and an Int8Weight;
-    act is GELU(tanh) with ``gelu``.  bias [out_features] in the rows' dtype.  ``out`` [..., rows,
+    act is GELU(tanh) with ``gelu``.  (A few 16-bit rows are quantized in the product's launch, to the same
+    result.)  bias [out_features] in the rows' dtype.  ``out`` [..., rows,
     out_features] may be a row range or a column block of a larger buffer."""
     if out is not None:
         args, out = _linear(x, weight, bias, out)
