@@ -631,11 +631,21 @@ void int8_linear_pair_out(const Tensor& q, const Tensor& scale, const Tensor& we
   int8_linear_sets({{q, scale, weight, weight_scale, bias, out}, {q2, scale2, weight2, weight_scale2, bias2, out2}}, gelu);
 }
 
-// The text set's tensors are given together or not at all (its bias and norms may be missing).
-void int8_qkv_out(const Maybe& text_q, const Maybe& text_scale, const Maybe& text_weight, const Maybe& text_weight_scale,
+// The text set's tensors are given together or not at all (its bias and norms may be missing).  An undefined `out` is
+// made here, for `heads` heads in `type`.
+void int8_qkv_into(const Maybe& text_q, const Maybe& text_scale, const Maybe& text_weight, const Maybe& text_weight_scale,
               const Maybe& text_bias, const Maybe& text_norm_q, const Maybe& text_norm_k, const Tensor& q,
               const Tensor& scale, const Tensor& weight, const Tensor& weight_scale, const Maybe& bias,
-              const Maybe& norm_q, const Maybe& norm_k, const Maybe& cos, const Maybe& sin, Tensor out, double eps) {
+              const Maybe& norm_q, const Maybe& norm_k, const Maybe& cos, const Maybe& sin, Tensor& out, int64_t heads_of_new,
+              at::ScalarType type, double eps) {
+  if (!out.defined()) {
+    type_of(type, "rows");
+    TORCH_CHECK_VALUE(q.dim() == 3 && q.size(0) && q.size(1), "image must be nonempty [B, n, features] rows");
+    TORCH_CHECK_VALUE(heads_of_new > 0, "heads must be positive");
+    const Tensor& t = value_or_none(text_q);
+    TORCH_CHECK_VALUE(!t.defined() || t.dim() == 3, "text must be [B, T, features] rows");
+    out = new_tensor(q, {3, q.size(0), q.size(1) + (t.defined() ? t.size(1) : 0), heads_of_new, 128}, type);
+  }
   TORCH_CHECK_VALUE(out.dim() == 5 && out.size(0) == 3 && out.size(3) > 0 && out.size(4) == 128,
                     "out must be [3, B, N, heads, 128]");
   const int32_t dtype = type_of(out.scalar_type(), "out");
@@ -687,18 +697,39 @@ void int8_qkv_out(const Maybe& text_q, const Maybe& text_scale, const Maybe& tex
         "hb_int8_qkv");
 }
 
+void int8_qkv_out(const Maybe& text_q, const Maybe& text_scale, const Maybe& text_weight, const Maybe& text_weight_scale,
+                  const Maybe& text_bias, const Maybe& text_norm_q, const Maybe& text_norm_k, const Tensor& q,
+                  const Tensor& scale, const Tensor& weight, const Tensor& weight_scale, const Maybe& bias,
+                  const Maybe& norm_q, const Maybe& norm_k, const Maybe& cos, const Maybe& sin, Tensor out, double eps) {
+  int8_qkv_into(text_q, text_scale, text_weight, text_weight_scale, text_bias, text_norm_q, text_norm_k, q, scale, weight,
+                weight_scale, bias, norm_q, norm_k, cos, sin, out, 0, out.scalar_type(), eps);
+}
+
+Tensor int8_qkv(const Maybe& text_q, const Maybe& text_scale, const Maybe& text_weight, const Maybe& text_weight_scale,
+                const Maybe& text_bias, const Maybe& text_norm_q, const Maybe& text_norm_k, const Tensor& q,
+                const Tensor& scale, const Tensor& weight, const Tensor& weight_scale, const Maybe& bias,
+                const Maybe& norm_q, const Maybe& norm_k, const Maybe& cos, const Maybe& sin, at::ScalarType dtype,
+                int64_t heads, double eps) {
+  Tensor out;
+  int8_qkv_into(text_q, text_scale, text_weight, text_weight_scale, text_bias, text_norm_q, text_norm_k, q, scale, weight,
+                weight_scale, bias, norm_q, norm_k, cos, sin, out, heads, dtype, eps);
+  return out;
+}
+
 // The attention operators and the 8-bit ones return nothing and write `out` and `lse` (and the like),
 // which torch's own boxed fallbacks overlook: they look after returned tensors only.
 
 // (the 8-bit operators that return their results write nothing)
 constexpr const char* WRITING[] = {"paired_fwd", "sparse_fwd", "int8_adaln", "int8_adaln_pair", "int8_linear_out",
                                    "int8_linear_pair_out", "int8_qkv_out"};
-constexpr const char* RETURNING[] = {"int8_rows", "int8_linear", "int8_linear_rows"};
+constexpr const char* RETURNING[] = {"int8_rows", "int8_linear", "int8_linear_rows", "int8_qkv"};
 
 // No derivative is recorded (the entry points refuse inputs that need one); a transform that takes one
 // is refused, as torch refuses an autograd.Function in one, for it would get zeros.
 void no_derivative(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
   const size_t count = op.schema().arguments().size();
+  // (the attention operators' entry points look for gradients themselves; the 8-bit ones leave it to this)
+  const bool refuse = at::GradMode::is_enabled() && op.schema().name().rfind("hilberta_hip::int8_", 0) == 0;
   // (included for as long as any torch.func transform is active)
   const bool transformed = at::GradMode::is_enabled() &&
                            c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerBackMode);
@@ -707,6 +738,7 @@ void no_derivative(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torc
     const Tensor& t = value.toTensor();
     TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), "Trying to use forward AD with ",
                                 op.schema().name(), " that does not support it.");
+    TORCH_CHECK_VALUE(!(refuse && !transformed && t.requires_grad()), "Inference only; disable autograd");
     TORCH_CHECK(!(transformed && t.requires_grad()), op.schema().name(), " has no derivative for torch.func transforms");
   }
   const at::AutoDispatchBelowAutograd below;
@@ -760,10 +792,11 @@ TORCH_LIBRARY(hilberta_hip, m) {
   m.def("int8_linear_rows(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias, bool gelu) -> Tensor", tags);
   m.def(("int8_linear_out(" + set(linear, "") + "bool gelu) -> ()").c_str(), tags);
   m.def(("int8_linear_pair_out(" + set(linear, "") + set(linear, "2") + "bool gelu) -> ()").c_str(), tags);
-  m.def("int8_qkv_out(Tensor? text_q, Tensor? text_scale, Tensor? text_weight, Tensor? text_weight_scale, "
-        "Tensor? text_bias, Tensor? text_norm_q, Tensor? text_norm_k, Tensor q, Tensor scale, Tensor weight, "
-        "Tensor weight_scale, Tensor? bias, Tensor? norm_q, Tensor? norm_k, Tensor? cos, Tensor? sin, "
-        "Tensor(a16!) out, float eps) -> ()", tags);
+  const std::string qkv = "Tensor? text_q, Tensor? text_scale, Tensor? text_weight, Tensor? text_weight_scale, "
+                          "Tensor? text_bias, Tensor? text_norm_q, Tensor? text_norm_k, Tensor q, Tensor scale, Tensor weight, "
+                          "Tensor weight_scale, Tensor? bias, Tensor? norm_q, Tensor? norm_k, Tensor? cos, Tensor? sin, ";
+  m.def(("int8_qkv(" + qkv + "ScalarType dtype, SymInt heads, float eps) -> Tensor").c_str(), tags);
+  m.def(("int8_qkv_out(" + qkv + "Tensor(a16!) out, float eps) -> ()").c_str(), tags);
   m.def("_attention_workspace(Device device, int need) -> Tensor");
   m.def("_workspace_keys() -> int[]");
   m.def("_clear_workspaces() -> ()");
@@ -786,6 +819,7 @@ void int8_operators(torch::Library& m) {
   m.impl("int8_linear_rows", int8_linear_rows);
   m.impl("int8_linear_out", int8_linear_out);
   m.impl("int8_linear_pair_out", int8_linear_pair_out);
+  m.impl("int8_qkv", int8_qkv);
   m.impl("int8_qkv_out", int8_qkv_out);
 }
 TORCH_LIBRARY_IMPL(hilberta_hip, CUDA, int8_hip) { int8_operators(int8_hip); }

@@ -54,16 +54,8 @@ class Int8Weight(NamedTuple):
     features: int
 
 
-def _inference(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError("Inference only; disable autograd")
-
-
 def quantize_rows(x):
     """Int8Rows of 16-bit rows x [rows, features] or [B, rows, features] (contiguous last dimension)."""
-    _inference(x)
     q, scale = ops.int8_rows(x)
     return Int8Rows(q, scale, x.shape[-1], x.dtype)
 
@@ -80,7 +72,6 @@ def adaln_quantize(x, shift, scale, *, y=None, gate=None, x_out=None, eps=1e-6):
     """Int8Rows of shift + LayerNorm(r) * (1 + scale), r = x + gate * y, in one pass; r is stored in
     ``x_out`` (which may be x) rounded, and normalised before that rounding.  Arguments as
     flux_norm.adaln_modulate's; hidden is any multiple of 8 up to 8192."""
-    _inference(x, shift, scale, y, gate, x_out)
     q, row_scale = ops.int8_adaln(x, shift, scale, y, gate, x_out, eps)
     return Int8Rows(q, row_scale, x.shape[-1], x.dtype)
 
@@ -89,7 +80,6 @@ def adaln_quantize_pair(first, second, *, eps=1e-6):
     """adaln_quantize of two row sets in one launch: ``first`` and ``second`` are its arguments as dicts, of
     one batch, hidden size, dtype and device.  Returns both Int8Rows."""
     sets = [(s["x"], s["shift"], s["scale"], s.get("y"), s.get("gate"), s.get("x_out")) for s in (first, second)]
-    _inference(*sets[0], *sets[1])
     q, scale, q2, scale2 = ops.int8_adaln_pair(*sets[0], *sets[1], eps)
     x, x2 = first["x"], second["x"]
     return Int8Rows(q, scale, x.shape[-1], x.dtype), Int8Rows(q2, scale2, x2.shape[-1], x2.dtype)
@@ -115,12 +105,10 @@ def int8_linear(x, weight, bias=None, *, gelu=False, out=None):
         return out
     w, w_scale, features = weight
     if isinstance(x, Int8Rows):
-        _inference(bias)
         q, scale, n, dtype = x
         if n != features:
             _check_features(weight, n)
         return ops.int8_linear(q, scale, w, w_scale, bias, dtype, gelu)
-    _inference(x, bias)
     if x.shape[-1] != features:
         _check_features(weight, x.shape[-1])
     return ops.int8_linear_rows(x, w, w_scale, bias, gelu)
@@ -128,7 +116,6 @@ def int8_linear(x, weight, bias=None, *, gelu=False, out=None):
 
 def _linear(x, weight, bias=None, out=None):
     """Arguments of one row set for the operators that write ``out``, and it."""
-    _inference(bias, out)
     q, scale, features, dtype = _rows(x)
     _check_features(weight, features)
     if out is None:
@@ -155,25 +142,20 @@ def int8_qkv(text, image, *, heads, weights, biases=(None, None), norms=((None, 
     that are quantized first; ``weights`` and ``biases`` = (text, image) are Int8Weights and biases of the
     columns [Q | K | V], heads * 128 each; ``norms`` = ((q_text, q_image), (k_text, k_image)) the RMSNorm
     weights [128] (None: no weight); cos/sin float32 [T + n, 128] in token order (None: no rotation)."""
-    image = _rows(image)
-    if text is not None:
-        text = _rows(text)
-        if text.features != image.features or text.dtype != image.dtype:
-            raise ValueError("text and image rows must share features and dtype")
-        if not text.q.shape[-2]:
-            text = None
+    q, scale, features, dtype = _rows(image)
     (wt, wi), (bt, bi), ((qt, qi), (kt, ki)) = weights, biases, norms
-    if any([w.features != image.features for w in (wi,) + ((wt,) if text is not None else ())]):
+    t = (None,) * 7
+    if text is not None:
+        text_q, text_scale, text_features, text_dtype = _rows(text)
+        if text_features != features or text_dtype != dtype:
+            raise ValueError("text and image rows must share features and dtype")
+        if text_q.size(-2):
+            t = (text_q, text_scale, wt.q, wt.scale, bt, qt, kt)
+    if wi.features != features or (t[0] is not None and wt.features != features):
         raise ValueError("the weights must take the rows' features")
-    _inference(bt, bi, qt, qi, kt, ki, cos, sin, out)
-    if image.q.ndim != 3 or not image.q.shape[0] or not image.q.shape[1]:
-        raise ValueError("image must be nonempty [B, n, features] rows")
-    B, n = image.q.shape[:2]
-    N = n + (0 if text is None else text.q.shape[-2])
     if out is None:
-        out = torch.empty(3, B, N, heads, HEAD_DIM, dtype=image.dtype, device=image.q.device)
-    elif out.dtype != image.dtype:
+        return ops.int8_qkv(*t, q, scale, wi.q, wi.scale, bi, qi, ki, cos, sin, dtype, heads, eps)
+    if out.dtype != dtype:
         raise ValueError("out must have the rows' dtype")
-    t = (None,) * 7 if text is None else (text.q, text.scale, wt.q, wt.scale, bt, qt, kt)
-    ops.int8_qkv_out(*t, image.q, image.scale, wi.q, wi.scale, bi, qi, ki, cos, sin, out, eps)
+    ops.int8_qkv_out(*t, q, scale, wi.q, wi.scale, bi, qi, ki, cos, sin, out, eps)
     return out

@@ -21,6 +21,7 @@ implementation for tracing and, for pair_rows alone, a CPU one:
   hilberta_hip::int8_qkv_out(text_q?, text_scale?, text_weight?, text_weight_scale?, text_bias?, text_norm_q?,
                              text_norm_k?, q, scale, weight, weight_scale, bias?, norm_q?, norm_k?, cos?, sin?,
                              out!, eps) -> ()
+  hilberta_hip::int8_qkv(.. as int8_qkv_out up to sin?, dtype, heads, eps) -> Tensor [3, B, N, heads, 128]
   hilberta_hip::int8_adaln_pair, int8_linear_pair_out: two row sets' arguments (the second's names end in 2)
 
 The attention ops write into caller-provided outputs (declared mutated), as the reference's
@@ -78,6 +79,12 @@ def _fake_int8_linear_rows(x, weight, weight_scale, bias, gelu):
     return x.new_empty((*x.shape[:-1], weight.shape[0]))
 
 
+def _fake_int8_qkv(text_q, text_scale, text_weight, text_weight_scale, text_bias, text_norm_q, text_norm_k, q, scale,
+                   weight, weight_scale, bias, norm_q, norm_k, cos, sin, dtype, heads, eps):
+    tokens = q.shape[1] + (0 if text_q is None else text_q.shape[1])
+    return q.new_empty((3, q.shape[0], tokens, heads, 128), dtype=dtype)
+
+
 def _pair_rows_cpu(kv_indices: Tensor, kv_counts: Tensor, total_blocks: int, key_block_size: int,
                    paired_width: int) -> tuple[Tensor, Tensor, Tensor]:
     """pair_rows of CPU tensors by hb_pair_rows_host."""
@@ -114,7 +121,7 @@ def _load():
                  gather_rows=_fake_gather_rows, int8_rows=_fake_int8_rows, int8_adaln=_fake_int8_rows,
                  int8_adaln_pair=_fake_int8_adaln_pair, int8_linear=_fake_int8_linear,
                  int8_linear_rows=_fake_int8_linear_rows, int8_linear_out=_fake_none,
-                 int8_linear_pair_out=_fake_none, int8_qkv_out=_fake_none)
+                 int8_linear_pair_out=_fake_none, int8_qkv=_fake_int8_qkv, int8_qkv_out=_fake_none)
     for name, fake in fakes.items():
         torch.library.register_fake(f"{_NS}::{name}", fake)
     torch.library.impl(f"{_NS}::pair_rows", "cpu", _pair_rows_cpu)
@@ -123,11 +130,11 @@ def _load():
 
 _NAMES = ("paired_fwd", "sparse_fwd", "pair_rows", "gather_rows", "_attention_workspace",
           "_workspace_keys", "_clear_workspaces", "int8_rows", "int8_adaln", "int8_adaln_pair", "int8_linear",
-          "int8_linear_rows", "int8_linear_out", "int8_linear_pair_out", "int8_qkv_out")
+          "int8_linear_rows", "int8_linear_out", "int8_linear_pair_out", "int8_qkv", "int8_qkv_out")
 try:
     _bound = _load()
 except (RuntimeError, OSError) as e:  # the package still imports, so that it can be (re)built
     _bound = [_Missing(name, str(e)) for name in _NAMES]
 (paired_fwd, sparse_fwd, pair_rows, gather_rows, attention_workspace, workspace_keys, clear_workspaces,
  int8_rows, int8_adaln, int8_adaln_pair, int8_linear, int8_linear_rows, int8_linear_out, int8_linear_pair_out,
- int8_qkv_out) = _bound
+ int8_qkv, int8_qkv_out) = _bound
