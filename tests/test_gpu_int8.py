@@ -646,6 +646,27 @@ def test_operators_are_traceable():
                      (hip.int8_adaln_pair, (s["x"], s["sh"], s["sc"], s["y"], s["g"], s["xo"],
                                             s["c"], s["sh"], s["sc"], None, None, None, 1e-6))):
         torch.library.opcheck(op.default, args, test_utils=checks)
+    t, (wt, wi), ((qt, qi), (kt, ki)) = quantize_rows(s["c"]), s["w"], s["norms"]
+    sets = (t.q, t.scale, wt.q, wt.scale, None, qt, kt, x.q, x.scale, wi.q, wi.scale, None, qi, ki, s["cos"], s["sin"])
+    qkv = torch.empty(3, 2, s["cos"].shape[0], s["heads"], 128, dtype=BF16, device="cuda")
+    torch.library.opcheck(hip.int8_qkv.default, (*sets, BF16, s["heads"], 1e-6), test_utils=checks)
+    torch.library.opcheck(hip.int8_qkv_out.default, (*sets, qkv, 1e-6), test_utils=checks)
+    torch.library.opcheck(hip.int8_linear_rows.default, (s["x"][:1, :3], w.q, w.scale, s["bo"], True), test_utils=checks)
+    assert torch.equal(hip.int8_qkv.default(*sets, BF16, s["heads"], 1e-6), hip.int8_qkv_out.default(*sets, qkv, 1e-6) or qkv)
+
+
+def test_gradients_are_refused():
+    s = _chain_state(37)
+    w, b = s["wo"], s["bo"].clone().requires_grad_()
+    for call in (lambda: int8_linear(s["x"][:1, :3], w, b), lambda: int8_linear(s["x"], w, b),
+                 lambda: quantize_rows(s["x"].clone().requires_grad_()),
+                 lambda: int8_linear(s["x"], w, out=torch.empty(2, 100, 300, dtype=BF16, device="cuda", requires_grad=True))):
+        with pytest.raises(ValueError, match="Inference only"):
+            call()
+    with torch.no_grad():
+        assert torch.equal(int8_linear(s["x"], w, b), int8_linear(s["x"], w, b.detach()))
+    with torch.inference_mode():
+        assert int8_linear(s["x"], w, b).shape == (2, 100, 300)
 
 
 def test_writes_count_for_autograd():
