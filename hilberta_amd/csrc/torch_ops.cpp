@@ -466,8 +466,8 @@ std::array<Tensor, 4> int8_adaln_sets(std::initializer_list<AdaSet> sets, double
     const Rows rx = rows_of(s.x, "x"), ry = y.defined() ? rows_of(y, "y") : Rows{},
                ro = x_out.defined() ? rows_of(x_out, "x_out") : Rows{};
     if (x_out.defined()) {
-      check_written(x_out, "x_out", {&s.shift, &s.scale, &gate});
       for (const AdaSet& other : sets) {
+        check_written(x_out, "x_out", {&other.shift, &other.scale, &value_or_none(other.gate)});
         // (a row is read before it is written, by one wave: x_out may be this set's x or y)
         const bool own = &other == &s;
         for (const Tensor* t : {&other.x, &value_or_none(other.y)})
