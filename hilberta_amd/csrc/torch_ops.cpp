@@ -669,16 +669,16 @@ void int8_qkv_into(const Maybe& text_q, const Maybe& text_scale, const Maybe& te
     void** p = pointers + 7 * part;
     void* values[5] = {pointer(r), pointer(rs), pointer(w), pointer(ws), pointer(b)};
     std::copy(values, values + 5, p);
-    for (int k = 0; k < 2; ++k) {
-      const Tensor& n = value_or_none(part ? (k ? norm_k : norm_q) : (k ? text_norm_k : text_norm_q));
-      TORCH_CHECK_VALUE(!n.defined() || (n.dim() == 1 && n.size(0) == 128 && n.is_contiguous() &&
-                                         n.scalar_type() == out.scalar_type()),
+    const Tensor& nq = value_or_none(part ? norm_q : text_norm_q);
+    const Tensor& nk = value_or_none(part ? norm_k : text_norm_k);
+    for (const Tensor* n : {&nq, &nk})
+      TORCH_CHECK_VALUE(!n->defined() || (n->dim() == 1 && n->size(0) == 128 && n->is_contiguous() &&
+                                          n->scalar_type() == out.scalar_type()),
                         "norm weights are contiguous [128] tensors of out's dtype");
-      p[5 + k] = pointer(n);
-      one_device(q, {&n});
-    }
-    one_device(q, {&r, &rs, &w, &ws, &b});
-    check_written(out, "out", {&r, &rs, &w, &ws, &b});
+    p[5] = pointer(nq);
+    p[6] = pointer(nk);
+    one_device(q, {&r, &rs, &w, &ws, &b, &nq, &nk});
+    check_written(out, "out", {&r, &rs, &w, &ws, &b, &nq, &nk});
   }
   TORCH_CHECK_VALUE(text + q.size(1) == tokens, "out must hold the text rows and then the image rows");
   TORCH_CHECK_VALUE(co.defined() == si.defined(), "cos and sin must be given together");

@@ -34,3 +34,20 @@ def test_adaln_residual_over_the_other_sets_vectors(writer, read):
     _refused("cannot alias", f.adaln_quantize_pair, *sets)
     sets[1 - writer][read] = torch.zeros(B, C, dtype=BF16)
     _refused(ON_DEVICE, f.adaln_quantize_pair, *sets)
+
+
+@pytest.mark.parametrize("which", ["text_norm_q", "text_norm_k", "norm_q", "norm_k"])
+def test_qkv_output_over_a_heads_norm(which):
+    B, T, n, H = 2, 3, 5, 2
+    rows = lambda k: f.Int8Rows(torch.zeros(B, k, 128, dtype=torch.int8), torch.zeros(B, k), 70, BF16)  # noqa: E731
+    w = f.Int8Weight(torch.zeros(3 * H * 128, 128, dtype=torch.int8), torch.zeros(3 * H * 128), 70)
+    out = torch.zeros(3, B, T + n, H, 128, dtype=BF16)
+    norms = {k: torch.zeros(128, dtype=BF16) for k in ("text_norm_q", "text_norm_k", "norm_q", "norm_k")}
+
+    def call(match):
+        _refused(match, f.int8_qkv, rows(T), rows(n), heads=H, weights=(w, w), out=out,
+                 norms=((norms["text_norm_q"], norms["norm_q"]), (norms["text_norm_k"], norms["norm_k"])))
+
+    call(ON_DEVICE)
+    norms[which] = out[1, 1, 4, 1]
+    call("cannot alias")
