@@ -12,7 +12,7 @@
 namespace hb {
 namespace {
 
-constexpr uint32_t GRID_BLOCKS = 1 << 24;  // (a grid holds fewer than 2^32 threads)
+constexpr uint32_t GRID_BLOCKS = (1 << 24) - 1;  // of 256 threads (a grid holds fewer than 2^32)
 constexpr int WAVE_FEATURES = 3072;        // a row up to here is a wave's, a longer one a workgroup's
 
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
@@ -224,7 +224,7 @@ extern "C" int hb_int8_rows(const void* x, int64_t batch_stride, int64_t row_str
   HB_REQUIRE(((uintptr_t)x & 1) == 0 && aligned16(q) && ((uintptr_t)scale & 3) == 0, "x must be 2-byte, q 16-byte and scale 4-byte aligned");
   HB_REQUIRE(batch_stride >= 0 && row_stride >= 0, "strides must be non-negative");
   const uint32_t total = (uint32_t)(batch * rows);
-  HB_REQUIRE(total < (padded <= WAVE_FEATURES ? GRID_BLOCKS * 4 : GRID_BLOCKS), "too many rows for one launch");
+  HB_REQUIRE(total <= (padded <= WAVE_FEATURES ? GRID_BLOCKS * 4 : GRID_BLOCKS), "too many rows for one launch");
   const RowArgs a = {(const uint16_t*)x, batch_stride, row_stride, q, scale, (uint32_t)rows, total, features, padded};
   const bool repeats = (batch > 1 && batch_stride == 0) || (rows > 1 && row_stride == 0);
   const bool stream_in = (int64_t)total * features * 3 > CACHE_BYTES && !repeats;
@@ -256,7 +256,7 @@ extern "C" int hb_int8_adaln(int32_t count, int32_t batch, const int32_t* rows, 
     const int64_t* s = strides + 8 * i;
     HB_REQUIRE(batch > 0 && rows[i] > 0, "batch and rows must be positive");
     total += (int64_t)batch * rows[i];
-    HB_REQUIRE(total < GRID_BLOCKS * 4, "too many rows for one launch");
+    HB_REQUIRE(total <= GRID_BLOCKS * 4, "too many rows for one launch");
     HB_REQUIRE(q[0] && q[4] && q[5] && q[6] && q[7], "null pointer argument");
     HB_REQUIRE((q[1] == nullptr) == (q[2] == nullptr), "y and gate are given together");
     HB_REQUIRE(!q[3] || q[1], "x_out is written only with a residual update");

@@ -223,8 +223,8 @@ int hb_adaln_modulate_pair(int32_t batch, const int32_t* rows, int32_t hidden, i
  * 16-bit rows to 8-bit rows: scale = max|x| / 127, q = rint(127 x / max|x|) (ties to even; a row of zeros
  * is all zero with scale 0; a row with an infinity or a NaN gets the scale NaN).  x is [batch, rows,
  * features] by element strides, last dimension contiguous, any alignment; q [batch * rows, padded] and
- * scale [batch * rows] contiguous, q 16-byte aligned; features up to 2^17, rows in all below 2^26 (2^24 of
- * more than 3072 features). */
+ * scale [batch * rows] contiguous, q 16-byte aligned; features up to 2^17, rows in all up to 2^26 - 4 (2^24 - 1
+ * where padded is past 3072). */
 int hb_int8_rows(const void* x, int64_t batch_stride, int64_t row_stride, int32_t batch,
                  int32_t rows, int32_t features, int32_t padded, int32_t dtype, int8_t* q,
                  float* scale, hb_stream_t stream);
@@ -236,7 +236,7 @@ int hb_int8_rows(const void* x, int64_t batch_stride, int64_t row_stride, int32_
  * all in fp32: unlike hb_adaln_modulate nothing on the way to q is rounded to 16 bits.  Host arrays, set
  * after set: rows [count]; pointers [count x 8] {x, y, gate, x_out, shift, scale, q, row_scale}; strides
  * [count x 8] {x batch, x row, y batch, y row, gate batch, x_out batch, x_out row, shift and scale batch}.
- * hidden a multiple of 8 up to 8192; fewer than 2^26 rows; pointers 16-byte aligned; strides multiples of 8. */
+ * hidden a multiple of 8 up to 8192; up to 2^26 - 4 rows; pointers 16-byte aligned; strides multiples of 8. */
 int hb_int8_adaln(int32_t count, int32_t batch, const int32_t* rows, int32_t hidden,
                   int32_t padded, int32_t dtype, float eps, void* const* pointers,
                   const int64_t* strides, hb_stream_t stream);
