@@ -340,6 +340,7 @@ std::pair<const char*, const char*> bytes_of(const Tensor& t) {
 
 // What is written has places of its own: no two of its values share one, and no input lies among them.
 void check_written(const Tensor& out, const char* name, std::initializer_list<const Tensor*> inputs) {
+  if (!out.numel()) return;
   c10::SmallVector<std::pair<int64_t, int64_t>, 5> dims;
   for (int64_t d = 0; d < out.dim(); ++d)
     if (out.size(d) > 1) dims.emplace_back(out.stride(d), out.size(d));
@@ -478,6 +479,7 @@ std::array<Tensor, 4> int8_adaln_sets(std::initializer_list<AdaSet> sets, double
       }
     }
     one_device(s0.x, {&s.x, &s.shift, &s.scale, &y, &gate, &x_out});
+    if (!s.x.numel()) continue;  // (a set without rows takes no part in the launch)
     void* p[8] = {pointer(s.x), pointer(y), pointer(gate), pointer(x_out), pointer(s.shift), pointer(s.scale), nullptr, nullptr};
     // (a stride of a dimension of one says nothing)
     const int64_t one = batch == 1 ? 0 : 1;
@@ -490,15 +492,18 @@ std::array<Tensor, 4> int8_adaln_sets(std::initializer_list<AdaSet> sets, double
   }
   require_hip(s0.x);
   const at::OptionalDeviceGuard guard(s0.x.device());
+  int count = 0;
   i = 0;
   for (const AdaSet& s : sets) {
     std::tie(made[2 * i], made[2 * i + 1]) = new_int8_rows(s.x);
-    pointers[8 * i + 6] = made[2 * i].data_ptr();
-    pointers[8 * i + 7] = made[2 * i + 1].data_ptr();
+    if (s.x.numel()) {
+      pointers[8 * count + 6] = made[2 * i].data_ptr();
+      pointers[8 * count++ + 7] = made[2 * i + 1].data_ptr();
+    }
     ++i;
   }
-  if (i == 1 && !made[1].numel()) return made;
-  check(hb_int8_adaln(i, i32(batch, "batch"), rows, i32(hidden, "hidden"), i32(padded, "padded"), dtype,
+  if (!count) return made;
+  check(hb_int8_adaln(count, i32(batch, "batch"), rows, i32(hidden, "hidden"), i32(padded, "padded"), dtype,
                       static_cast<float>(eps), pointers, strides, stream_of(s0.x.device())),
         "hb_int8_adaln");
   return made;
@@ -559,6 +564,7 @@ void int8_linear_sets(std::initializer_list<LinearSet> sets, bool gelu) {
       TORCH_CHECK_VALUE(&o == &s || !may_overlap(s.out, o.out), "both outputs must lie apart");
     }
     one_device(s0.q, {&s.q, &s.scale, &s.weight, &s.weight_scale, &bias, &s.out});
+    if (!s.out.numel()) continue;  // (a set without rows takes no part in the launch)
     void* p[6] = {pointer(s.q), pointer(s.scale), pointer(s.weight), pointer(s.weight_scale), pointer(bias), pointer(s.out)};
     std::copy(p, p + 6, pointers + 6 * i);
     strides[2 * i] = batch == 1 ? 0 : r.batch_stride;
@@ -566,6 +572,7 @@ void int8_linear_sets(std::initializer_list<LinearSet> sets, bool gelu) {
     rows[i++] = i32(r.rows, "rows");
   }
   require_hip(s0.q);
+  if (!i) return;
   const at::OptionalDeviceGuard guard(s0.q.device());
   check(hb_int8_linear(i, i32(batch, "batch"), rows, i32(s0.out.size(-1), "columns"), i32(padded, "padded"), dtype, gelu,
                        pointers, strides, stream_of(s0.q.device())),
@@ -574,7 +581,6 @@ void int8_linear_sets(std::initializer_list<LinearSet> sets, bool gelu) {
 
 void int8_linear_out(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
                      const Maybe& bias, Tensor out, bool gelu) {
-  if (!out.numel() && out.is_cuda()) return;
   int8_linear_sets({{q, scale, weight, weight_scale, bias, out}}, gelu);
 }
 

@@ -78,7 +78,7 @@ def adaln_quantize(x, shift, scale, *, y=None, gate=None, x_out=None, eps=1e-6):
 
 def adaln_quantize_pair(first, second, *, eps=1e-6):
     """adaln_quantize of two row sets in one launch: ``first`` and ``second`` are its arguments as dicts, of
-    one batch, hidden size, dtype and device.  Returns both Int8Rows."""
+    one batch, hidden size, dtype and device; either may have no rows.  Returns both Int8Rows."""
     sets = [(s["x"], s["shift"], s["scale"], s.get("y"), s.get("gate"), s.get("x_out")) for s in (first, second)]
     q, scale, q2, scale2 = ops.int8_adaln_pair(*sets[0], *sets[1], eps)
     x, x2 = first["x"], second["x"]
@@ -127,7 +127,7 @@ def _linear(x, weight, bias=None, out=None):
 
 def int8_linear_pair(first, second, *, gelu=False):
     """int8_linear of two row sets in one launch: ``first`` and ``second`` are dicts of x, weight, bias and
-    out, of one batch, layer shape, dtype and device.  Returns both outputs."""
+    out, of one batch, layer shape, dtype and device; either may have no rows.  Returns both outputs."""
     a, out_a = _linear(**first)
     b, out_b = _linear(**second)
     ops.int8_linear_pair_out(*a, *b, gelu)
