@@ -480,7 +480,7 @@ class FluxTransformer:
     def _double_block_int8(self, w, mods, x, xn, c, cn, cos, sin, attention, layer, next_mods, joint_out):
         """_double_block with xn, cn Int8Rows.  With ``joint_out`` = h [B, N, C] the residual streams end
         there; returns (x, xn, c, cn), the first and third None then.  ``next_mods`` are the (shift, scale)
-        pairs of the image and text rows."""
+        pairs of the image and text rows.  Of the last block of all only xn is made, the image rows in 16 bits."""
         s, H = self.shape, self.shape.heads
         T = c.shape[1]
         (_, _, gx, sx2, scx2, gx2), (_, _, gc, sc2, scc2, gc2) = mods
@@ -502,6 +502,8 @@ class FluxTransformer:
                                   gelu=True)
         fx, fc = int8_linear_pair(dict(x=fx, weight=w2x[0], bias=w2x[1]), dict(x=fc, weight=w2c[0], bias=w2c[1]))
         (nsx, nscx), (nsc, nscc) = next_mods
+        if layer == s.blocks - 1:  # (the output layer takes 16-bit rows, the image's alone)
+            return None, adaln_modulate(x, nsx, nscx, y=fx, gate=gx2, eps=s.eps), None, None
         hx, hc = (x, c) if joint_out is None else (joint_out[:, T:], joint_out[:, :T])
         xn, cn = adaln_quantize_pair(dict(x=x, shift=nsx, scale=nscx, y=fx, gate=gx2, x_out=hx),
                                      dict(x=c, shift=nsc, scale=nscc, y=fc, gate=gc2, x_out=hc), eps=s.eps)
@@ -544,12 +546,12 @@ class FluxTransformer:
         first.append((single_mods[0][:2],) * 2 if self.single else (out_mods,) * 2)
         (sx, scx), (sc, scc) = first[0]
         xn, cn = adaln_quantize_pair(dict(x=x, shift=sx, scale=scx), dict(x=c, shift=sc, scale=scc), eps=s.eps)
-        h = x.new_empty(x.shape[0], T + x.shape[1], s.hidden)
+        h = x.new_empty(x.shape[0], T + x.shape[1], s.hidden) if self.single else None
         for i, w in enumerate(self.double):
             x, xn, c, cn = self._double_block_int8(w, double_mods[i], x, xn, c, cn, cos, sin, attention, i,
                                                    first[i + 1], h if i == last else None)
-        if not self.single:  # (the output layer takes 16-bit rows)
-            return adaln_modulate(h[:, T:], *out_mods, eps=s.eps)
+        if not self.single:
+            return xn
         hn = (cn, xn)
         del x, xn, c, cn
         for j, w in enumerate(self.single):

@@ -5,6 +5,7 @@ tests/test_int8_blocks.py shows that each mistake in their wiring is further off
 import pytest
 import torch
 
+from hilberta_amd.flux_int8 import Int8Rows
 from oracle import int8_blocks as B
 from oracle import int8_ops as O
 from tests.helpers import say
@@ -38,8 +39,6 @@ def _inputs(model, grid, text, batch):
 
 def _value(rows):
     """What Int8Rows stand for; of a pair the joint rows."""
-    from hilberta_amd.flux_int8 import Int8Rows
-
     if not isinstance(rows, Int8Rows):
         return torch.cat([_value(r) for r in rows], 1)
     return rows.q[..., :rows.features].double() * rows.scale.double()[..., None]
@@ -180,3 +179,35 @@ def test_quantized_weights_are_the_layers():
         same(a["qkv"], *b["qkv"])
         same(a["mlp"], *b["mlp"])
         same(a["out"], torch.cat([b["out_attn"][0], b["out_mlp"][0]], 1), b["out_attn"][1])
+
+
+@pytest.mark.parametrize("layers", [(2, 0), (1, 1), (2, 2)])
+def test_every_8_bit_row_that_is_made_is_read(layers, monkeypatch):
+    from hilberta_amd import flux_model
+
+    model, made, read = _model(layers, raised=False).quantize(), [], []
+
+    def rows_of(value):
+        if isinstance(value, Int8Rows):
+            return [value.q.data_ptr()]
+        if isinstance(value, dict):
+            value = list(value.values())
+        return [p for v in value for p in rows_of(v)] if isinstance(value, (tuple, list)) else []
+
+    def spy(name, into, of):
+        call = getattr(flux_model, name)
+
+        def spied(*args, **kwargs):
+            done = call(*args, **kwargs)
+            into.extend(rows_of(done if of == "done" else args))
+            kept.append((args, done))  # (so that no address comes twice)
+            return done
+        monkeypatch.setattr(flux_model, name, spied)
+
+    kept = []
+    for name in ("adaln_quantize", "adaln_quantize_pair"):
+        spy(name, made, "done")
+    for name in ("int8_linear", "int8_linear_pair", "int8_qkv"):
+        spy(name, read, "args")
+    model(**_inputs(model, 8, 13, 2))
+    assert made and set(made) == set(read)
