@@ -1,10 +1,15 @@
 // 16-bit values to 8-bit whole numbers by their row's largest, as the row kernels and the products of a few rows
 // need them.
 //
-// q is exact: 127 x_k and top are whole multiples of powers of two with 15 and 11 significant bits at most,
-// so a quotient that is not a tie is at least 2^-19 of itself away from one, far more than its fp32 error
-// (an exact tie comes out as that tie).  The largest value is found on the bit patterns without
-// the sign, in which an infinity is above every number and a NaN above that.
+// Of 16-bit rows q is exact.  A value is a 2^i and the top b 2^j, i <= j, with a, b < 2^11 (fp16's significand;
+// bf16's has 8 bits): the quotient 127 x / top = 127 a / (b 2^(j - i)) is off a tie, k + 1/2, by |254 a - (2k + 1)
+// b 2^(j - i)| / (2 b 2^(j - i)), a whole number over that: nothing, and the tie comes out as itself, or at least 1
+// / (254 a) > 2^-19 of the quotient, far more than its fp32 error.  127 x itself, of 18 bits at most, is exact in
+// fp32.  Rows of fp32 values (the AdaLN pass) have no such margin: there a quotient within fp32's error of a tie
+// may go either way.
+//
+// The largest value is found on the bit patterns without the sign, in which an infinity is above every number and a
+// NaN above that.
 #pragma once
 #include "common.h"
 

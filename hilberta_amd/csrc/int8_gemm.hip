@@ -184,9 +184,14 @@ __device__ __forceinline__ void rotate(float* v, const f32x4& cos, const f32x4& 
 // The epilogue of a wave's 32 tokens from t0 on and 32 CF channels from c0 on (linear); `channel` are those
 // channels' values, TC apart.  Lanes l and l + 32 hold token t0 + l % 32.  After pack_pair a 32-channel block of
 // a token is four 16-byte chunks, two in each of those lanes; exchanged with the lane 16 on, four lanes hold a
-// token's four chunks, and a store writes 64 bytes a row (32 without: 16896 x 3072 x 12288 586 -> 580 us).  The
-// stores bypass the caches (580 -> 571): the output is larger than they are, and what they hold is wanted by
-// the tiles to come.
+// token's four chunks, and a store writes 64 bytes a row (32 without: 16896 x 3072 x 12288 586 -> 580 us).
+//
+// Stores of 16 bytes, here and below, bypass the caches at every size, which leaves those to the operands.  Measured
+// alone and with int8_rows reading the output next, us past the caches / through them: 16384 x 3072 x 12288 with GELU
+// (403 MB) 555, 665 / 584, 680; 8192 rows 286, 328 / 292, 335; 16384 x 3072 x 3072 (101 MB) 149, 182 / 162, 181; 4096
+// rows 46, 54.6 / 46, 54.4; 512 x 3072 x 12288 (13 MB) 39.6, 45.2 / 40.6, 45.6; 77 x 4096 x 3072 8.1, 11.9 / 8.1, 11.6;
+// qkv of 512 + 16384 tokens 476, 554 / 494, 555, of 512 + 1024 57.5, 63.3 / 56.3, 64.3.  Where it loses is one row that
+// is read next: 1 x 3072 x 18432 13.7, 22.9 / 13.9, 21.2.
 template <bool F16, bool GELU, int CF, int TC>
 __device__ __forceinline__ void finish(const Args& a, const Set& s, const i32x16 (&acc)[CF], float scale,
                                        const float* channel, int c0, uint32_t t0) {
@@ -896,9 +901,10 @@ __global__ __launch_bounds__(256, 2) void int8_few_kernel(FewArgs f) {
 // ------------------------------------------------------------------ launches
 enum Kernel { T64x32, T32x64, T64x64, T96x64, T96x128, T128x32, T128x64, T128x128, WIDE256, WIDE_HEADS, KERNELS };
 
-// What a tile of each kernel covers, and what it takes on 256 CUs, fitted to the times of 900 sizes of 1 to 6000
-// rows: `launch`, and for a round of tiles, one a CU, `round` + stages of 128 features x (`stage` + `full` f^2)
-// us, f the share of the CUs that have one (stages slow each other down where many load).
+// What a tile of each kernel covers, and what it takes on 256 CUs, a whole MI355X (on a partition of one the results are
+// the same, the choice untimed), fitted to the times of 694 linear and 30 Q/K/V sizes of 1 to 6000 rows: `launch`,
+// and for a round of tiles, one a CU, `round` + stages of 128 features x (`stage` + `full` f^2) us, f the share of the
+// CUs that have one (stages slow each other down where many load).
 struct Shape {
   int tc, tt;
   float launch, round, stage, full;
@@ -941,13 +947,14 @@ struct Choice {
   float us;
 };
 
-// The kernel whose estimate is the least: over those sizes 0.5% slower than always the fastest.  Measured, rows x
-// features x columns, us for 64 x 32 / 32 x 64 / 64 x 64 / 96 x 64 / 96 x 128 / 256 x 256 tiles: 77 x 4096 x 3072 9.5 /
-// 9.0 / 10.1 / 12.2 / 15.3 / 40; 128 x 3072 x 12288 18 / 21 / 17 / 12.1 / 15.5 / 32; 512 x 12288 x 3072 45 / 54 / 45 /
-// 28.8 / 37 / 108; 666 x 1000 x 777 6.9 / 8.9 / 6.4 / 7.4 / 9.6 / 18; 256 x 3072 x 9216 25 / 32 / 23 / 20 / 15.4 / 33;
-// 4096 x 3072 x 3072 96 / 141 / 86 / 74 / 56 / 38; 1 x 3072 x 18432 13.4 / 19.5 / 17.0 / 12.8 / 14.1 / 31.  qkv, rows x
-// features, 24 heads, us for 128 x 32 / 128 x 64 / 128 x 128 / 256 x 256: 1 x 3072 11.2 / 12.0 / 15.9 / 37; 128 x 3072
-// 21 / 14.7 / 19.3 / 41; 512 x 3072 48 / 37 / 36 / 43; 512 + 4096 x 3072 365 / 236 / 192 / 141.
+// The kernel whose estimate is the least: over the linear sizes 0.5% slower than always the fastest, at worst 21%
+// (30 x 8760 x 4433); for all 30 Q/K/V sizes it is the fastest, few as they are.  Measured, rows x features x
+// columns, us for 64 x 32 / 32 x 64 / 64 x 64 / 96 x 64 / 96 x 128 / 256 x 256 tiles: 77 x 4096 x 3072 9.5 / 9.0 /
+// 10.1 / 12.2 / 15.3 / 40; 128 x 3072 x 12288 18 / 21 / 17 / 12.1 / 15.5 / 32; 512 x 12288 x 3072 45 / 54 / 45 /
+// 28.8 / 37 / 108; 666 x 1000 x 777 6.9 / 8.9 / 6.4 / 7.4 / 9.6 / 18; 256 x 3072 x 9216 25 / 32 / 23 / 20 / 15.4 /
+// 33; 4096 x 3072 x 3072 96 / 141 / 86 / 74 / 56 / 38; 1 x 3072 x 18432 13.4 / 19.5 / 17.0 / 12.8 / 14.1 / 31.
+// qkv, rows x features, 24 heads, us for 128 x 32 / 128 x 64 / 128 x 128 / 256 x 256: 1 x 3072 11.2 / 12.0 / 15.9 /
+// 37; 128 x 3072 21 / 14.7 / 19.3 / 41; 512 x 3072 48 / 37 / 36 / 43; 512 + 4096 x 3072 365 / 236 / 192 / 141.
 Choice choose(const Args& a, int count, bool qkv) {
   const Kernel wide = qkv ? WIDE_HEADS : WIDE256;
   Choice best = {wide, estimate(a, count, wide)};
