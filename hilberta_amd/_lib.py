@@ -145,8 +145,9 @@ def load():
             )
         for name, (restype, argtypes) in SIGNATURES.items():
             fn = getattr(lib, name, None)
-            if fn is None:
-                continue
+            if fn is None:  # (an entry point that came without a new version)
+                raise RuntimeError(f"{LIB_PATH} lacks {name}, which include/hilberta_hip.h declares: rebuild the HIP "
+                                   "library (python -m hilberta_amd.build)")
             fn.restype = restype
             fn.argtypes = argtypes
         _lib = lib

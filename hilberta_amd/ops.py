@@ -117,6 +117,9 @@ def _load():
         raise RuntimeError(f"{TORCH_LIB_PATH} was built for {f'ABI {built}' if built else 'an older ABI'} but "
                            f"include/hilberta_hip.h declares ABI {declared}: rebuild the libraries "
                            "(python -m hilberta_amd.build)")
+    for name in _NAMES:
+        if not hasattr(getattr(torch.ops, _NS), name):
+            raise RuntimeError(f"{TORCH_LIB_PATH} lacks {name}: rebuild the libraries (python -m hilberta_amd.build)")
     fakes = dict(paired_fwd=_fake_none, sparse_fwd=_fake_none, pair_rows=_fake_pair_rows,
                  gather_rows=_fake_gather_rows, int8_rows=_fake_int8_rows, int8_adaln=_fake_int8_rows,
                  int8_adaln_pair=_fake_int8_adaln_pair, int8_linear=_fake_int8_linear,
