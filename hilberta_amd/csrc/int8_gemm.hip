@@ -20,6 +20,7 @@
 #include <type_traits>
 #include <utility>
 
+#include "gemm_common.h"
 #include "int8_common.h"
 #include "../../include/hilberta_hip.h"
 
@@ -59,12 +60,6 @@ struct Args {
   float eps;
 };
 
-__device__ __forceinline__ float gelu(float v) {
-  // v (1 + tanh u) / 2 = v / (1 + exp(-2u)),  u = sqrt(2 / pi) (v + 0.044715 v^3);  -2u / ln 2 by its powers
-  const float e = v * (-2.302208198144325f - 0.1029432395800235f * v * v);
-  return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(e));
-}
-
 // Four values of this lane's token, channels c .. c + 3 with c = 8g + 4 (lane / 32), of quarters g = 2p
 // (`even`) and 2p + 1 (`odd`) of a 32-channel accumulator, to 16 bits and exchanged with the other half of
 // the wave: lanes below 32 then hold channels 16p .. 16p + 7 of their token, the others 16p + 8 .. 16p + 15.
@@ -74,40 +69,6 @@ __device__ __forceinline__ u32x4 pack_pair(const float (&even)[4], const float (
   const auto lo = __builtin_amdgcn_permlane32_swap(two(even[0], even[1]), two(odd[0], odd[1]), false, false);
   const auto hi = __builtin_amdgcn_permlane32_swap(two(even[2], even[3]), two(odd[2], odd[3]), false, false);
   return u32x4{lo[0], hi[0], lo[1], hi[1]};
-}
-
-typedef __attribute__((address_space(3))) void* lds_ptr;
-
-// word 3 of a raw buffer resource (32-bit data format, no swizzle)
-constexpr int BUFFER_WORD3 = 0x00020000;
-
-// 16 bytes a lane from base + voffset + soffset into LDS at dst + 16 lane.  (The buffer resource type exists
-// for the device target only; the host pass sees an empty body.)
-__device__ __forceinline__ void load_lds16(const void* base, void* dst, int voffset, int soffset) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  const __amdgpu_buffer_rsrc_t rsrc =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, BUFFER_WORD3);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)dst, 16, voffset, soffset, 0, 0);
-#endif
-}
-
-// s_waitcnt vmcnt(N): all but the last N loads have arrived.
-template <int N>
-__device__ __forceinline__ void wait_arrivals() {
-  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);
-}
-
-// The same, and this wave's reads of LDS.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0070);
-}
-
-// A barrier that no access to LDS is moved across.
-__device__ __forceinline__ void barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
 }
 
 // ------------------------------------------------------------------ what every kernel does with its sums
@@ -153,22 +114,6 @@ __device__ __forceinline__ void store8(const Args& a, uint16_t* out, int c, cons
     for (int k = 0; k < 8; ++k)
       if (c + k < a.columns) out[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
   }
-}
-
-// The sum over 16 neighbouring lanes, in each of them: of pairs, of quads, of the mirrored half row and row.
-template <int CONTROL>
-__device__ __forceinline__ uint32_t moved_bits(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, 0xf, 0xf, true);
-}
-template <int CONTROL>
-__device__ __forceinline__ float moved(float v) {
-  return __builtin_bit_cast(float, moved_bits<CONTROL>(__builtin_bit_cast(uint32_t, v)));
-}
-__device__ __forceinline__ float sum16(float v) {
-  v += moved<0xb1>(v);
-  v += moved<0x4e>(v);
-  v += moved<0x141>(v);
-  return v + moved<0x140>(v);
 }
 
 // Two pairs (2i, 2i + 1) turned by cos and sin.
@@ -263,16 +208,6 @@ __device__ __forceinline__ void finish8(const Args& a, const Set& s, const i32x4
   if (at < s.tokens) store8<QKV>(a, out, c0 + c, pack8<F16>(v));
 }
 
-template <typename Begin, int... I>
-__device__ __forceinline__ void begin_all(Begin& begin, std::integer_sequence<int, I...>) {
-  (begin(std::integral_constant<int, I>()), ...);
-}
-// Whether one of the steps was the last.
-template <typename Step, int... I>
-__device__ __forceinline__ bool step_all(Step& step, std::integer_sequence<int, I...>) {
-  return (step(std::integral_constant<int, I>()) || ...);
-}
-
 // The epilogue of a wave's 32 tokens from t0 on and one head from c0 on (qkv).  Lanes l and l + 32 hold token
 // t0 + l % 32, and would read its rotary rows and write its output 32 bytes at a time.  So 16 tokens at a time go
 // through the wave's own part of a stage, eight pieces of 1 KB, and come back as four tokens of 16 lanes each,
@@ -357,24 +292,6 @@ __device__ __forceinline__ void finish_head(const Args& a, const Set& s, const i
   }
 }
 
-// Which tile a workgroup takes.
-struct Tile {
-  int set, c0;
-  uint32_t t0;
-};
-
-// Tiles walk bands of `BAND` token tiles, channel tile by channel tile.
-template <int TC, int TT, int BAND>
-__device__ __forceinline__ Tile tile_at(const Args& a, uint32_t tile) {
-  const int set = tile >= a.tiles0;
-  if (set) tile -= a.tiles0;
-  const uint32_t token_tiles = (a.set[set].tokens + TT - 1) / TT;
-  const uint32_t band = tile / (BAND * a.channel_tiles), in_band = tile - band * (BAND * a.channel_tiles);
-  const uint32_t height = min((uint32_t)BAND, token_tiles - band * BAND);
-  const uint32_t c = in_band / height;
-  return {set, (int)c * TC, (band * BAND + in_band - c * height) * TT};
-}
-
 // Where rows end.  A stage is 128 features, and rows a multiple of 64: what a lane's load asks for past the row
 // (its chunk of a last half stage, or a stage after the last) is moved outside the buffer, from where a load
 // brings zeros and reads nothing.
@@ -405,11 +322,6 @@ struct Ends {
 constexpr int WIDE = 256, WIDE_STEP = 128, WIDE_BAND = 4;
 constexpr int WIDE_STAGE = 2 * WIDE * WIDE_STEP;     // 64 KB
 constexpr int WIDE_LOADS = WIDE_STAGE / 1024 / 8;    // 1 KB loads of a wave and stage
-
-__device__ __forceinline__ const int8_t* uniform_pointer(const int8_t* p) {
-  const uint64_t v = (uint64_t)p;
-  return (const int8_t*)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
-}
 
 template <bool F16, bool QKV, bool GELU>
 __global__ __launch_bounds__(512, 2) void int8_wide_kernel(Args a) {

@@ -1,0 +1,934 @@
+// Linear layers of 16-bit rows with what follows them in the same pass.
+//
+//   out[m, n] = residual[m, n] + gate[b, n] * act(sum_k x[m, k] w[n, k] + bias[n])
+//
+// act: none, GELU(tanh) or SiLU; bias, residual and gate where they are given.  The sums are fp32 and so is what
+// follows, rounded once to the 16-bit output.
+//
+// The weight's channels are the rows of the matrix instruction and the tokens its columns, as in the 8-bit products: a
+// lane then holds one token's values, 4 consecutive channels an accumulator quarter.
+//
+// Three kernels: many rows (linear_wide_kernel), fewer (linear_tile_kernel) and a few (linear_few_kernel); rows that
+// direct loads cannot take are copied first (pad_rows_kernel).
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+#include <utility>
+
+#include "gemm_common.h"
+#include "rows16.h"
+#include "../../include/hilberta_hip.h"
+
+namespace hb {
+namespace {
+
+enum Act { NONE, GELU, SILU };
+
+// One set of rows with its weight.  Two sets (a block's text and image rows) share a launch.
+struct Set {
+  const uint16_t* x;         // [tokens, features]
+  const uint16_t* w;         // [columns, features]
+  const uint16_t* bias;      // [columns] or null
+  const uint16_t* residual;  // [tokens, columns] or null
+  const uint16_t* gate;      // [batch, columns] or null
+  uint16_t* out;
+  int64_t x_b, x_n, w_n, r_b, r_n, g_b, out_b, out_n;  // strides of a batch element and a row
+  uint32_t rows, tokens;     // rows of a batch element, and of all
+  uint32_t start;            // rows of the set before these (which another launch takes)
+};
+
+struct Args {
+  Set set[2];
+  int32_t columns, features;
+  uint32_t tiles0, tiles, tiles_xcd;  // tiles of set 0, of all, and of an XCD
+  uint32_t channel_tiles;             // tiles along the channels
+  int32_t act;
+  int32_t vectors;                    // every output row takes 16-byte stores
+};
+
+template <bool F16>
+__device__ __forceinline__ f32x16 multiply32(const u32x4& w, const u32x4& x, const f32x16& acc) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, x), acc, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x), acc, 0, 0, 0);
+}
+template <bool F16>
+__device__ __forceinline__ f32x4 multiply16(const u32x4& w, const u32x4& x, const f32x4& acc) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, x), acc, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x), acc, 0, 0, 0);
+}
+
+// The same with the sums in accumulation registers and the operands in the others: where 256 sums take all of the former,
+// the compiler left to itself moves some to and fro in every stage (16384 x 12288 x 3072 846 -> 1070 us by a change in the
+// order of loads).  It does not know these for matrix instructions and adds none of their waits, so whatever reads a sum
+// next comes late enough by itself: the next product on it 64 products later, moved_out after settle.
+template <bool F16>
+__device__ __forceinline__ void accumulate16(const u32x4& w, const u32x4& x, f32x4& acc) {
+  if constexpr (F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(w), "v"(x));
+  else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(w), "v"(x));
+}
+template <bool F16>
+__device__ __forceinline__ void begin16(const u32x4& w, const u32x4& x, f32x4& acc) {
+  if constexpr (F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, 0" : "=a"(acc) : "v"(w), "v"(x));
+  else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=a"(acc) : "v"(w), "v"(x));
+}
+// The last product's sums are there (18 cycles after a product of 8 passes).
+__device__ __forceinline__ void settle() {
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ float moved_out(float acc) {
+  float v;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(acc));
+  return v;
+}
+__device__ __forceinline__ f32x4 moved_out(const f32x4& acc) {
+  return f32x4{moved_out(acc[0]), moved_out(acc[1]), moved_out(acc[2]), moved_out(acc[3])};
+}
+
+// ------------------------------------------------------------------ what every kernel does with its sums
+__device__ __forceinline__ float silu(float v) {
+  return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+}
+
+__device__ __forceinline__ void activate(float (&v)[8], int act) {  // (act: of a known value, or uniform)
+  if (act == GELU) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = gelu(v[k]);
+  } else if (act == SILU) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = silu(v[k]);
+  }
+}
+
+// A token of a set: its batch element and its row there.
+struct Place {
+  uint32_t b, n;
+};
+__device__ __forceinline__ Place place_of(const Set& s, uint32_t at) {
+  uint32_t n = s.start + min(at, s.tokens - 1), b = 0;
+  if (s.start + s.tokens > s.rows) b = n / s.rows, n -= b * s.rows;  // (one batch element: no division)
+  return {b, n};
+}
+
+// Values p[0 .. 7] of channels c .. c + 7, those of them that there are.
+__device__ __forceinline__ u32x4 load8(const uint16_t* p, int c, int columns) {
+  if (c + 8 <= columns) return *(const any_u32x4*)p;
+  u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < 7; ++k)
+    if (c + k < columns) v[k >> 1] |= (uint32_t)p[k] << (16 * (k & 1));
+  return v;
+}
+
+// Eight values of channels c .. c + 7 to `out`, those of them that there are.  (A row that begins between words takes a
+// word-aligned 12 bytes and two ends: 16-byte stores across words are slower.)
+__device__ __forceinline__ void store8(const Args& a, uint16_t* out, int c, const u32x4& v) {
+  typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint32_t words3 __attribute__((ext_vector_type(3), aligned(4)));
+  if (c + 8 <= a.columns) {
+    if (a.vectors) {
+      __builtin_nontemporal_store(v, (u32x4*)out);
+    } else if ((uintptr_t)out & 2) {
+      out[0] = (uint16_t)v[0];
+      *(words3*)(out + 1) = words3{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16};
+      out[7] = (uint16_t)(v[3] >> 16);
+    } else {
+      *(words4*)out = v;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + k < a.columns) out[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
+  }
+}
+
+// What a token's eight channels need from memory besides their sums.
+struct Epilogue {
+  uint16_t* out;
+  u32x4 residual, gate;
+};
+
+// (c: the first channel; nothing is read where there are none)
+__device__ __forceinline__ Epilogue ask(const Args& a, const Set& s, uint32_t at, int c) {
+  const Place p = place_of(s, at);
+  Epilogue e = {s.out + p.b * s.out_b + (int64_t)p.n * s.out_n + c, {}, {}};
+  if (c < a.columns) {
+    if (s.residual) e.residual = load8(s.residual + p.b * s.r_b + (int64_t)p.n * s.r_n + c, c, a.columns);
+    if (s.gate) e.gate = load8(s.gate + p.b * s.g_b + c, c, a.columns);
+  }
+  return e;
+}
+
+// v: the sums with their bias.
+template <bool F16>
+__device__ __forceinline__ void finish8(const Args& a, const Set& s, float (&v)[8], const Epilogue& e, uint32_t at, int c) {
+  activate(v, a.act);
+  if (s.gate) {
+    float g[8];
+    unpack8<F16>(e.gate, g);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= g[k];
+  }
+  if (s.residual) {
+    float r[8];
+    unpack8<F16>(e.residual, r);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] += r[k];
+  }
+  if (at < s.tokens) store8(a, e.out, c, pack8<F16>(v));
+}
+
+// The epilogue's bias of a tile's channels, in LDS.
+template <bool F16, int TC>
+__device__ __forceinline__ void load_bias(const Args& a, const Set& s, int c0, float (&bias)[TC]) {
+  const int i = threadIdx.x;
+  if (i < TC) bias[i] = s.bias ? to_f<F16>(s.bias[min(c0 + i, a.columns - 1)]) : 0.f;
+}
+
+// Where rows end.  A stage is 64 features, 128 bytes: what a lane's load asks for past the row (a multiple of 16 bytes)
+// is moved outside the buffer, from where a load brings zeros and reads nothing.
+struct RowEnd {
+  int full, beyond;  // whole stages, and what the stage after them adds to this lane's offset
+  __device__ RowEnd(int features, int chunk)
+      : full(features >> 6), beyond(chunk * 8 < (features & 63) ? 0 : (int)0x80000000) {}
+  __device__ int past(int stage) const {
+    return stage < full ? 0 : stage == full ? beyond : (int)0x80000000;
+  }
+};
+
+// ------------------------------------------------------------------ many rows
+// 256 channels x 256 tokens a workgroup of four waves, 128 x 128 each; one workgroup a CU, which walks its tiles.
+//  * Two stages of 64 KB in LDS, 64 features of every row (a row's 128 bytes are one request to the L2), by direct loads.
+//  * A stage's two steps of 32 features each have registers of their own.  Everyone has read a stage when a quarter of its
+//    products are done, and its place takes the stage after the next from then on: a load has at least 100 products' time
+//    until it is waited for, enough for one that misses the L2.
+//  * What is asked of memory and LDS is spread among the products: asked for together it holds up their issue.
+//  * The stages of consecutive tiles follow one another; what comes after a tile's sums works in registers while the next
+//    tile's first stages arrive.
+//  * An XCD takes a run of the tiles, four token tiles by all channel tiles at a time, so that its L2 serves both
+//    operands.
+constexpr int WIDE = 256, WIDE_BAND = 4, WIDE_WAVES = 4;
+constexpr int WIDE_STAGE = 2 * WIDE * 128;                  // 64 KB
+constexpr int WIDE_LOADS = WIDE_STAGE / 1024 / WIDE_WAVES;  // 1 KB loads of a wave and stage
+
+// What the epilogue does.  All but ANY are for whole tiles, each of one batch element, with aligned outputs, and work on
+// the sums in registers; ANY takes them through LDS.  (One kernel for both kinds of tile keeps too much in registers.)
+enum Mode { PLAIN, ACT_GELU, ACT_SILU, RESIDUAL, GATED, ANY };
+
+// A wave's 128 x 128 sums: acc[i][j] are channels 16 i + 4 (lane / 16) .. + 3 of token 16 j + lane % 16.
+struct Sums {
+  f32x4 v[8][8];
+};
+
+// Four words of two neighbouring 16-channel blocks of a token, four channels of each, exchanged among the four lanes of a
+// token so that each has eight channels in a row: chunk 2 (q % 2) + q / 2 of the blocks' four, q = lane / 16.  Undoes
+// itself.
+__device__ __forceinline__ u32x4 cross(const u32x4& v) {
+  const auto lo = __builtin_amdgcn_permlane16_swap(v[0], v[2], false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(v[1], v[3], false, false);
+  return u32x4{lo[0], hi[0], lo[1], hi[1]};
+}
+
+// Chunks of two such pairs of blocks, `a` of channels 0 .. 31 and `b` of 32 .. 63 of tokens 0 .. 15, exchanged among lanes 8
+// apart so that eight lanes have the 64 channels of a token, tokens 0 .. 7 in a and 8 .. 15 in b.  Undoes itself.
+__device__ __forceinline__ void halves(u32x4& a, u32x4& b) {
+  const bool upper = threadIdx.x & 8;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t other = moved_bits<0x128>(upper ? a[k] : b[k]);  // (of the lane 8 on, around 16)
+    if (upper) a[k] = other;
+    else b[k] = other;
+  }
+}
+
+// The epilogue of a whole tile of one batch element, a wave's part: tokens from t0 and channels from c0 on; `bias` and
+// `gate` are theirs, in LDS.  A store moves 128 bytes, whole lines, of 8 rows (64 of 16 rows: 16384 x 3072 x 12288 892
+// us, so 867).
+template <bool F16, int MODE>
+__device__ __forceinline__ void finish_wide(const Set& s, const Sums& acc, const float* bias, const float* gate, int c0,
+                                            uint32_t t0) {
+  constexpr bool ADD = MODE == RESIDUAL || MODE == GATED;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (or addresses stay in registers from tile to tile)
+  const int q = lane >> 4, c = c0 + (lane >> 3 & 1) * 32 + (q & 1) * 16 + (q >> 1) * 8;
+  const Place p = place_of(s, t0 + (lane & 7));
+  uint16_t* const out = s.out + p.b * s.out_b + (int64_t)p.n * s.out_n + c;
+  const uint16_t* const from = s.residual + p.b * s.r_b + (int64_t)p.n * s.r_n + c;
+  constexpr int AHEAD = 2;
+  u32x4 res[AHEAD + 1][4];
+  auto ask = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) res[j % (AHEAD + 1)][i] = *(const any_u32x4*)(from + (j * 16 + (i & 1) * 8) * s.r_n + (i >> 1) * 64);
+  };
+  if (ADD) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) ask(j);
+  }
+  f32x4 b[8], g[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    b[i] = *(const f32x4*)(bias + i * 16 + q * 4);
+    if (MODE == GATED) g[i] = *(const f32x4*)(gate + i * 16 + q * 4);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (ADD && j + AHEAD < 8) ask(j + AHEAD);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // 64 channels
+      u32x4* const r = &res[j % (AHEAD + 1)][2 * h];
+      if (ADD) halves(r[0], r[1]);
+      u32x4 packed[2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {  // 32 channels
+        const int i = 4 * h + 2 * m;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = moved_out(acc.v[i + (k >> 2)][j][k & 3]) + b[i + (k >> 2)][k & 3];
+        activate(v, MODE == ACT_GELU ? GELU : MODE == ACT_SILU ? SILU : NONE);
+        if (ADD) {
+          float add[8];
+          unpack8<F16>(cross(r[m]), add);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = (MODE == GATED ? v[k] * g[i + (k >> 2)][k & 3] : v[k]) + add[k];
+        }
+        packed[m] = cross(pack8<F16>(v));
+      }
+      halves(packed[0], packed[1]);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) __builtin_nontemporal_store(packed[m], (u32x4*)(out + (j * 16 + m * 8) * s.out_n + h * 64));
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (all at once take more registers than there are)
+  }
+}
+
+// The epilogue of any tile: a wave's 32 tokens from t0 on and 128 channels from c0 on, whose sums lie in `box`, the
+// wave's sixteen pieces of 1 KB, 4 KB apart.  They come back as four tokens of 16 lanes each.
+template <bool F16>
+__device__ __forceinline__ void finish_any(const Args& a, const Set& s, const float* bias, int c0, uint32_t t0, const int8_t* box) {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (as above)
+  const int c = (lane & 15) * 8;
+  if (c0 + c >= a.columns) return;
+  f32x4 b[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) b[g] = *(const f32x4*)(bias + c + 4 * g);
+  Epilogue next = ask(a, s, t0 + (lane >> 4), c0 + c);  // (asked for four tokens ahead)
+#pragma unroll 1
+  for (int q = 0; q < 8; ++q) {
+    const Epilogue now = next;
+    const int token = q * 4 + (lane >> 4);
+    if (q < 7) next = ask(a, s, t0 + token + 4, c0 + c);
+    float v[8];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const f32x4 sum = *(const f32x4*)(box + (token >> 1) * 4096 + (token & 1) * 512 + (((lane & 15) ^ (token & 15)) + 16 * g) * 16) + b[g];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[4 * g + k] = sum[k];
+    }
+    finish8<F16>(a, s, v, now, t0 + token, c0 + c);
+  }
+}
+
+// The sums of 32 of a wave's tokens, blocks j and j + 1, to its box.  (Units of four channels: even ones in the first half
+// of a token's 512 bytes, odd ones in the second, in an order of the token's, so that neither the lanes that write together
+// nor those that read together share a bank.)
+template <int J>
+__device__ __forceinline__ void fill_box(const Sums& acc, int8_t* box) {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (as above)
+  const int q = lane >> 4, token = lane & 15;
+  int8_t* const to = box + (token >> 1) * 4096 + (token & 1) * 512 + (q & 1) * 256;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *(f32x4*)(to + j * 8 * 4096 + ((i * 2 + (q >> 1)) ^ token) * 16) = moved_out(acc.v[i][J + j]);
+}
+
+template <bool F16, int MODE>
+__global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds0[WIDE_STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds1[WIDE_STAGE];
+  __shared__ __attribute__((aligned(16))) float bias[2][WIDE], gate[2][WIDE];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), row = lane & 15, quarter = lane >> 4;
+  const int wc = wave & 1, wt = wave >> 1;
+  const int stages = max((a.features + 127) / 128 * 2, 4);  // (an even number)
+  // (workgroups go to the eight XCDs in turn)
+  const uint32_t first = (blockIdx.x & 7) * a.tiles_xcd, stride = gridDim.x >> 3;
+  uint32_t slot = blockIdx.x >> 3;
+  if (slot >= a.tiles_xcd || first + slot >= a.tiles) return;
+  // Loads: a wave's load j fills LDS rows 8 (4 j + wave) .. + 7, eight lanes a row; rows below WIDE are
+  // channels, the others tokens (rows past the operands' ends: the last ones again).  The lane at slot p of
+  // row r loads chunk p ^ (r / 2 % 8), so that the chunks that 16 rows' lanes read together lie in
+  // different banks.
+  const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+  const RowEnd ends(a.features, chunk);
+  const int8_t *wbase, *xbase;
+  int offset[WIDE_LOADS];
+  int aimed = -1;  // the set that `offset` is of
+  auto aim = [&](const Tile& t) {
+    const Set& s = a.set[t.set];
+    const Place begin = place_of(s, t.t0);
+    wbase = uniform_pointer((const int8_t*)(s.w + t.c0 * s.w_n));
+    xbase = uniform_pointer((const int8_t*)(s.x + begin.b * s.x_b + begin.n * s.x_n));
+    if (MODE != ANY && aimed == t.set) return;  // (whole tiles differ by where they begin)
+    aimed = t.set;
+#pragma unroll
+    for (int j = 0; j < WIDE_LOADS; ++j) {
+      const int r = 8 * (WIDE_WAVES * j + wave) + (lane >> 3);
+      if (j < WIDE_LOADS / 2) {
+        offset[j] = (MODE == ANY ? min(r, a.columns - 1 - t.c0) : r) * (int)s.w_n * 2 + chunk * 16;
+      } else if (MODE == ANY) {
+        const Place p = place_of(s, t.t0 + (r - WIDE));
+        offset[j] = (int)(((p.b - begin.b) * s.x_b + ((int64_t)p.n - begin.n) * s.x_n) * 2) + chunk * 16;
+      } else {
+        offset[j] = (r - WIDE) * (int)s.x_n * 2 + chunk * 16;
+      }
+    }
+  };
+  auto load = [&](int8_t* dst, int stage, int j, int past) {
+    load_lds16(j < WIDE_LOADS / 2 ? wbase : xbase, dst + 1024 * (WIDE_WAVES * j + wave), offset[j] | past, uniform(stage * 128));
+  };
+  // Operands: lane l holds bytes 16 (l / 16) .. + 15 of a 64-byte step of row l % 16.
+  const int read = row * 128 + ((row >> 1 & 7) ^ quarter) * 16;
+  u32x4 w[2][8], x[2][8];
+  // (k of sixteen, as the products need them)
+  auto fetch = [&](const int8_t* src, int u, int k) {
+    const int at = read ^ (u * 64);
+    if (k == 0 || k > 8) {
+      const int j = k ? k - 8 : 0;
+      x[u][j] = *(const u32x4*)(src + (WIDE + wt * 128 + j * 16) * 128 + at);
+    } else {
+      w[u][k - 1] = *(const u32x4*)(src + (wc * 128 + (k - 1) * 16) * 128 + at);
+    }
+  };
+  Sums acc;
+  // The 128 products of the stage in `cur`, whose first step is in registers or on its way there; the first step of the one
+  // in `next` is fetched (at a tile's end the epilogue needs the registers), and `after` is asked for into `cur`.
+  constexpr std::false_type no;
+  constexpr std::true_type yes;
+  auto step = [&](auto first_one, auto last, int8_t* cur, int8_t* next, int after) {
+    constexpr bool FIRST = decltype(first_one)::value, LAST = decltype(last)::value;
+    const int past = ends.past(uniform(after));
+    auto product = [&](auto index) {
+      constexpr int k = decltype(index)::value, u = k >> 6, j = k >> 3 & 7, i = k & 7;
+      if (FIRST && u == 0) begin16<F16>(w[u][i], x[u][j], acc.v[i][j]);
+      else accumulate16<F16>(w[u][i], x[u][j], acc.v[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (k < 16) fetch(cur, 1, k);
+      if (k == 29) {
+        wait_loads<63>();
+        barrier();  // nobody reads `cur` any more
+      }
+      if (!(LAST && MODE == ANY) && k >= 30 && (k - 30) % 6 == 0 && (k - 30) / 6 < WIDE_LOADS) load(cur, after, (k - 30) / 6, past);
+      if (k == 86) {
+        wait_arrivals<LAST && MODE == ANY ? 0 : 10>();  // (what this stage has asked for by now)
+        barrier();                                      // `next` is there
+      }
+      if (!LAST && k >= 88 && k % 2 == 0 && (k - 88) / 2 < 16) fetch(next, 0, (k - 88) / 2);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    begin_all(product, std::make_integer_sequence<int, 128>());
+  };
+  // The epilogue's values of channel c0 + threadIdx.x of a tile.
+  auto ask_channel = [&](const Tile& t, uint16_t& b, uint16_t& g) {
+    const Set& s = a.set[t.set];
+    const int c = min(t.c0 + (int)threadIdx.x, a.columns - 1);
+    b = s.bias ? s.bias[c] : 0;
+    if (MODE == GATED) g = s.gate[place_of(s, t.t0).b * s.g_b + c];
+  };
+  Tile t = tile_at<WIDE, WIDE, WIDE_BAND>(a, first + slot);
+  aim(t);
+  uint16_t bias_value, gate_value;
+  ask_channel(t, bias_value, gate_value);
+#pragma unroll
+  for (int j = 0; j < WIDE_LOADS; ++j) load(lds0, 0, j, ends.past(0));
+#pragma unroll
+  for (int j = 0; j < WIDE_LOADS; ++j) load(lds1, 1, j, ends.past(1));
+  wait_loads<WIDE_LOADS>();
+  barrier();
+  for (int parity = 0;; parity ^= 1) {
+    const Tile done = t;
+    const Set& s = a.set[done.set];
+    bias[parity][threadIdx.x] = to_f<F16>(bias_value);  // (read after the next barriers)
+    if (MODE == GATED) gate[parity][threadIdx.x] = to_f<F16>(gate_value);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) fetch(lds0, 0, k);
+    step(yes, no, lds0, lds1, 2);
+    step(no, no, lds1, lds0, 3);
+    for (int n = 4; n < stages; n += 2) {
+      step(no, no, lds0, lds1, n);
+      step(no, no, lds1, lds0, n + 1);
+    }
+    slot += stride;
+    const bool more = slot < a.tiles_xcd && first + slot < a.tiles;
+    if (more) t = tile_at<WIDE, WIDE, WIDE_BAND>(a, first + slot);
+    aim(t);  // (after the last tile: its own first stages once more, never multiplied)
+    ask_channel(t, bias_value, gate_value);  // (before the stores, which a load after them would wait for)
+    step(no, no, lds0, lds1, 0);
+    step(no, yes, lds1, lds0, 1);
+    settle();
+    const int c0 = done.c0 + wc * 128;
+    const uint32_t t0 = done.t0 + wt * 128;
+    if constexpr (MODE != ANY) {
+      finish_wide<F16, MODE>(s, acc, &bias[parity][wc * 128], &gate[parity][wc * 128], c0, t0);
+    } else {
+      int8_t* const box = lds1 + 1024 * wave;
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j) {
+        if (j == 0) fill_box<0>(acc, box);
+        else if (j == 1) fill_box<2>(acc, box);
+        else if (j == 2) fill_box<4>(acc, box);
+        else fill_box<6>(acc, box);
+        finish_any<F16>(a, s, &bias[parity][wc * 128], c0, t0 + j * 32, box);
+      }
+      wait_loads<63>();  // (into the pieces that this wave's own epilogue has read)
+#pragma unroll
+      for (int j = 0; j < WIDE_LOADS; ++j) load(lds1, 1, j, ends.past(1));
+    }
+    if (!more) break;
+  }
+  wait_loads<0>();  // (nothing may still be on its way to LDS when the workgroup ends)
+}
+
+// ------------------------------------------------------------------ fewer rows
+// TC channels x TT tokens a workgroup, in tiles so small that most CUs have one.  What is on its way to a CU
+// bounds it, so the operands go to LDS by direct loads, into a ring of R stages of 64 features, the loads spread over
+// the products.  A stage's features are in four parts of 16, a wave each in the smallest tiles, or two waves that
+// share the tokens (of 32 tokens: the channels), whose epilogue is shorter.  The sums meet in LDS, and a thread
+// finishes eight channels of a token: neighbouring lanes read and write whole lines.  Rows past the operands' ends are
+// zeros that nothing reads.
+template <int TC, int TT, int WAVES>
+struct Ring {
+  static constexpr int STAGE = (TC + TT) * 128, GROUPS = STAGE / 1024, LOADS = (GROUPS + WAVES - 1) / WAVES;
+  static constexpr int CW = TT > 32 ? TC : TC / 2, TW = TT > 32 ? TT / 2 : TT;  // of half the sums
+  static constexpr int BOX = TW * CW * 4;
+  static constexpr int CF = (WAVES > 4 ? CW : TC) / 32, TF = (WAVES > 4 ? TW : TT) / 32;  // of a wave
+};
+
+template <bool F16, int TC, int TT, int R, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_tile_kernel(Args a) {
+  typedef Ring<TC, TT, WAVES> F;
+  constexpr int STAGE = F::STAGE, LOADS = F::LOADS, CW = F::CW, TW = F::TW, CF = F::CF, TF = F::TF;
+  static_assert(F::BOX <= STAGE && R >= 4 && R <= 8, "a stage holds half a part's sums");
+  __shared__ __attribute__((aligned(1024))) int8_t lds0[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds1[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds2[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds3[STAGE];
+  __shared__ __attribute__((aligned(1024))) int8_t lds4[R > 4 ? STAGE : 1];
+  __shared__ __attribute__((aligned(1024))) int8_t lds5[R > 5 ? STAGE : 1];
+  __shared__ __attribute__((aligned(1024))) int8_t lds6[R > 6 ? STAGE : 1];
+  __shared__ __attribute__((aligned(1024))) int8_t lds7[R > 7 ? STAGE : 1];
+  __shared__ __attribute__((aligned(16))) float bias[TC];
+  auto ring = [&](auto index) -> int8_t* {
+    constexpr int i = decltype(index)::value % R;
+    return i == 0 ? lds0 : i == 1 ? lds1 : i == 2 ? lds2 : i == 3 ? lds3 : i == 4 ? lds4 : i == 5 ? lds5 : i == 6 ? lds6 : lds7;
+  };
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+  const int part = WAVES > 4 ? wave >> 1 : wave, share = WAVES > 4 ? wave & 1 : 0;
+  const uint32_t tile = (blockIdx.x & 7) * a.tiles_xcd + (blockIdx.x >> 3);
+  if (tile >= a.tiles) return;
+  const Tile t = tile_at<TC, TT, 8>(a, tile);
+  const Set& s = a.set[t.set];
+  load_bias<F16>(a, s, t.c0, bias);
+  // Loads as in the wide kernel.
+  const Place begin = place_of(s, t.t0);
+  const int8_t *wbase = (const int8_t*)(s.w + t.c0 * s.w_n), *xbase = (const int8_t*)(s.x + begin.b * s.x_b + begin.n * s.x_n);
+  const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+  int offset[LOADS];
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int r = 8 * (WAVES * j + wave) + (lane >> 3);
+    if (r < TC) {
+      offset[j] = r < a.columns - t.c0 ? r * (int)s.w_n * 2 + chunk * 16 : (int)0x80000000;
+    } else {
+      const Place p = place_of(s, t.t0 + (r - TC));
+      offset[j] = (uint32_t)(r - TC) < s.tokens - t.t0
+                      ? (int)(((p.b - begin.b) * s.x_b + ((int64_t)p.n - begin.n) * s.x_n) * 2) + chunk * 16
+                      : (int)0x80000000;
+    }
+  }
+  const int stages = (a.features + 63) / 64;
+  const RowEnd ends(a.features, chunk);
+  const bool all = WAVES * (LOADS - 1) + wave < F::GROUPS;  // (the last loads are not every wave's)
+  auto load = [&](int8_t* dst, int stage, int j, int past) {
+    const int group = WAVES * j + wave;
+    if (F::GROUPS % WAVES == 0 || j < LOADS - 1 || all)
+      load_lds16(group * 8 < TC ? wbase : xbase, dst + 1024 * group, offset[j] | past, uniform(stage * 128));
+  };
+  auto arrivals = [&] {
+    if (F::GROUPS % WAVES == 0 || all) wait_arrivals<(R - 3) * LOADS>();
+    else wait_arrivals<(R - 3) * (LOADS - 1)>();
+  };
+  const int read = col * 128 + ((col >> 1 & 7) ^ (2 * part + half)) * 16;
+  const int wread = read + (TT > 32 ? 0 : share * CW * 128), xread = read + (TC + (TT > 32 ? share * TW : 0)) * 128;
+  u32x4 w[2][CF], x[2][TF];
+  auto fetch = [&](const int8_t* src, int to) {
+#pragma unroll
+    for (int i = 0; i < CF; ++i) w[to][i] = *(const u32x4*)(src + wread + i * 4096);
+#pragma unroll
+    for (int j = 0; j < TF; ++j) x[to][j] = *(const u32x4*)(src + xread + j * 4096);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  f32x16 acc[TF][CF] = {};
+  // Stage n's operands are in w, x, or on their way; stage n + 1 is in LDS.  The stage whose reads ended in
+  // the last step takes n + R - 1.  Before the barrier stage n + 2 is there.
+  int n = 0;
+  auto step = [&](auto index) {
+    constexpr int I = decltype(index)::value;
+    int8_t* const free = ring(std::integral_constant<int, I + R - 1>());
+    const int past = ends.past(uniform(n + R - 1));
+    int asked = 0, done = 0;
+#pragma unroll
+    for (int j = 0; j < TF; ++j)
+#pragma unroll
+      for (int i = 0; i < CF; ++i) {
+        acc[j][i] = multiply32<F16>(w[I & 1][i], x[I & 1][j], acc[j][i]);
+        for (++done; asked * TF * CF < done * LOADS; ++asked) {
+          __builtin_amdgcn_sched_barrier(0);
+          load(free, n + R - 1, asked, past);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(ring(std::integral_constant<int, I + 1>()), ~I & 1);
+    arrivals();
+    barrier();
+    return ++n == stages;
+  };
+  // (Zeros into the last stage, so that the compiler, which tracks what is on its way to which array, has met them
+  // all before the loop: otherwise it waits for everything each time around.)
+  load(ring(std::integral_constant<int, R - 1>()), 0, 0, (int)0x80000000);
+  auto begin_stage = [&](auto index) {
+    constexpr int I = decltype(index)::value;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) load(ring(index), I, j, ends.past(I));
+  };
+  begin_all(begin_stage, std::make_integer_sequence<int, R - 1>());
+  arrivals();
+  barrier();
+  fetch(lds0, 0);
+  while (!step_all(step, std::make_integer_sequence<int, R % 2 ? 2 * R : R>())) {}
+  wait_loads<0>();  // (nothing is on its way to LDS any more)
+  barrier();
+  // Parts 2 and 3 hand their sums to 0 and 1, which add their own: token-major, four channels a unit, units in an
+  // order of the token's, so that neighbouring tokens' lie in different banks.
+  auto box = [&](int k, int h) -> int8_t* { return k ? (h ? lds3 : lds2) : (h ? lds1 : lds0); };
+  auto unit = [&](int token, int c) { return (token * CW + (c ^ (token & 7) * 4)) * 4; };
+  auto hand = [&](bool add) {
+#pragma unroll
+    for (int j = 0; j < TF; ++j)
+#pragma unroll
+      for (int i = 0; i < CF; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int h = WAVES > 4 ? share : TT > 32 ? j * 32 / TW : i * 32 / CW;
+          const int token = TT > 32 ? j * 32 % TW : j * 32, c = TT > 32 ? i * 32 : i * 32 % CW;
+          f32x4* const at = (f32x4*)(box(part & 1, h) + unit(token + col, c + g * 8 + half * 4));
+          const f32x4 v = {acc[j][i][4 * g], acc[j][i][4 * g + 1], acc[j][i][4 * g + 2], acc[j][i][4 * g + 3]};
+          *at = add ? *at + v : v;
+        }
+  };
+  if (part >= 2) hand(false);
+  __syncthreads();
+  if (part < 2) hand(true);
+  __syncthreads();
+  for (int e = threadIdx.x; e < TT * (TC / 8); e += 64 * WAVES) {
+    const int token = e / (TC / 8), c = e % (TC / 8) * 8;
+    const int h = TT > 32 ? token / TW : c / CW;
+    const uint32_t to = t.t0 + token;
+    if (to >= s.tokens || t.c0 + c >= a.columns) continue;
+    const Epilogue more = ask(a, s, to, t.c0 + c);
+    float v[8];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int at = unit(TT > 32 ? token % TW : token, (TT > 32 ? c : c % CW) + 4 * g);
+      const f32x4 sum = *(const f32x4*)(box(0, h) + at) + *(const f32x4*)(box(1, h) + at) + *(const f32x4*)(bias + c + 4 * g);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[4 * g + k] = sum[k];
+    }
+    finish8<F16>(a, s, v, more, to, t.c0 + c);
+  }
+}
+
+// ------------------------------------------------------------------ a few rows
+// 16 channels by up to 16 tokens a workgroup; its eight waves take turns at 128 features, straight from memory into the
+// matrix instruction's registers, and their sums meet in LDS.  Rows may lie at any address.  Bound by the weight's
+// read.
+constexpr int FEW_ROWS = 16, FEW_WAVES = 8;
+
+template <bool F16>
+__global__ __launch_bounds__(64 * FEW_WAVES) void linear_few_kernel(Args a) {
+  __shared__ float sums[FEW_WAVES][16][17];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), r = lane & 15, quarter = lane >> 4;
+  const int set = blockIdx.x >= a.tiles0;
+  const Set& s = a.set[set];
+  const int c0 = (int)(blockIdx.x - (set ? a.tiles0 : 0)) * 16;
+  const uint16_t* const w = s.w + min(c0 + r, a.columns - 1) * s.w_n;
+  const Place p = place_of(s, r);
+  const uint16_t* const x = s.x + p.b * s.x_b + p.n * s.x_n;
+  f32x4 acc[2] = {};
+  const int whole = a.features & ~127;
+  for (int k0 = wave * 128; k0 < whole; k0 += FEW_WAVES * 128) {
+    u32x4 wv[4], xv[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) wv[u] = __builtin_nontemporal_load((const any_u32x4*)(w + k0 + u * 32 + quarter * 8));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) xv[u] = *(const any_u32x4*)(x + k0 + u * 32 + quarter * 8);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) acc[u & 1] = multiply16<F16>(wv[u], xv[u], acc[u & 1]);
+  }
+  if (whole < a.features && wave == whole / 128 % FEW_WAVES) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      acc[u & 1] = multiply16<F16>(load_row8<false>(w, whole + u * 32 + quarter * 8, a.features),
+                                   load_row8<false>(x, whole + u * 32 + quarter * 8, a.features), acc[u & 1]);
+  }
+  // (lane: channels 4 quarter .. + 3 of token r)
+#pragma unroll
+  for (int k = 0; k < 4; ++k) sums[wave][r][quarter * 4 + k] = acc[0][k] + acc[1][k];
+  __syncthreads();
+  const int token = threadIdx.x >> 4, c = c0 + (threadIdx.x & 15);
+  if (threadIdx.x >= 256 || (uint32_t)token >= s.tokens || c >= a.columns) return;
+  float v = 0.f;
+#pragma unroll
+  for (int k = 0; k < FEW_WAVES; ++k) v += sums[k][token][threadIdx.x & 15];
+  if (s.bias) v += to_f<F16>(s.bias[c]);
+  if (a.act == GELU) v = gelu(v);
+  else if (a.act == SILU) v = silu(v);
+  const Place at = place_of(s, token);
+  if (s.gate) v *= to_f<F16>(s.gate[at.b * s.g_b + c]);
+  if (s.residual) v += to_f<F16>(s.residual[at.b * s.r_b + (int64_t)at.n * s.r_n + c]);
+  s.out[at.b * s.out_b + (int64_t)at.n * s.out_n + c] = from_f<F16>(v);
+}
+
+// ------------------------------------------------------------------ rows that direct loads cannot take
+// Direct loads to LDS bring 16 bytes from a multiple of 16, and a row's last 16 must not reach into what follows.
+// Other rows (an odd length, an odd column of a wider buffer) are copied into rows of a multiple of 64 values, zeros
+// after their own.
+struct PadArgs {
+  struct Matrix {
+    const uint16_t* from;
+    uint16_t* to;
+    int64_t b, n;
+    uint32_t rows, all;  // rows of a batch element, and of all
+  } m[4];
+  uint32_t first[5];  // workgroups up to each matrix
+  int32_t features, padded;
+};
+
+constexpr uint32_t PAD_GROUPS = 1 << 16;
+
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
+  for (uint32_t group = blockIdx.x; group < p.first[4]; group += gridDim.x) {
+    int i = 0;
+    while (group >= p.first[i + 1]) ++i;
+    const PadArgs::Matrix& m = p.m[i];
+    // a wave a row
+    const uint32_t row = (group - p.first[i]) * 4 + (threadIdx.x >> 6);
+    if (row >= m.all) continue;
+    const uint32_t b = row / m.rows;
+    const uint16_t* const from = m.from + b * m.b + (int64_t)(row - b * m.rows) * m.n;
+    uint16_t* const to = m.to + (int64_t)row * p.padded;
+    for (int c = (threadIdx.x & 63) * 8; c < p.padded; c += 512) *(u32x4*)(to + c) = load_row8<false>(from, c, p.features);
+  }
+}
+
+// ------------------------------------------------------------------ launches
+enum Kernel { T64x32, T32x64, T64x64, T96x64, T96x128, WIDE256, KERNELS };
+
+struct Shape {
+  int tc, tt;
+  float launch, round, stage, full;
+};
+constexpr Shape SHAPES[KERNELS] = {
+    {64, 32, 2.97f, 1.34f, 0.102f, 0.065f},  {32, 64, 1.81f, 2.61f, 0.096f, 0.088f},   {64, 64, 1.74f, 2.84f, 0.127f, 0.134f},
+    {96, 64, 1.67f, 3.78f, 0.189f, 0.133f},  {96, 128, 0.95f, 5.82f, 0.258f, 0.234f}, {256, 256, 5.9f, 3.0f, 0.99f, 0.70f},
+};
+
+// Tiles of TC x TT of both sets.
+int64_t tiles_of(const Args& a, int count, int tc, int tt) {
+  int64_t tiles = 0;
+  for (int i = 0; i < count; ++i)
+    tiles += ((a.set[i].tokens + (int64_t)tt - 1) / tt) * ((a.columns + (int64_t)tc - 1) / tc);
+  return tiles;
+}
+
+// What a kernel takes for the sets, in us.
+float estimate(const Args& a, int count, Kernel k) {
+  const Shape& s = SHAPES[k];
+  const float rounds = (float)tiles_of(a, count, s.tc, s.tt) / 256.f, whole = std::floor(rounds), rest = rounds - whole;
+  const float stages = (float)((a.features + 63) / 64);
+  return s.launch + whole * (s.round + stages * (s.stage + s.full)) +
+         (rest > 0.f ? s.round + stages * (s.stage + s.full * rest * rest) : 0.f);
+}
+
+struct Choice {
+  Kernel kernel;
+  float us;
+};
+
+Choice choose(const Args& a, int count) {
+  Choice best = {WIDE256, estimate(a, count, WIDE256)};
+  for (int i = 0; i < WIDE256; ++i) {
+    const Kernel k = (Kernel)i;
+    if (tiles_of(a, count, SHAPES[k].tc, SHAPES[k].tt) >= (1 << 21)) continue;  // (a grid holds fewer than 2^32 threads)
+    const float us = estimate(a, count, k);
+    if (us < best.us) best = {k, us};
+  }
+  return best;
+}
+
+// The wide kernel's epilogue for these sets.
+Mode mode_of(const Args& a, int count) {
+  const bool residual = a.set[0].residual, gate = a.set[0].gate;
+  bool whole = a.vectors && a.columns % WIDE == 0;
+  for (int i = 0; i < count; ++i)
+    whole &= a.set[i].rows % WIDE == 0 && residual == !!a.set[i].residual && gate == !!a.set[i].gate;
+  if (!whole || (a.act != NONE && residual)) return ANY;
+  return a.act == GELU ? ACT_GELU : a.act == SILU ? ACT_SILU : gate ? GATED : residual ? RESIDUAL : PLAIN;
+}
+
+template <bool F16>
+int launch_kernel(Args& a, int count, Kernel kernel, hipStream_t st) {
+  const int tc = SHAPES[kernel].tc, tt = SHAPES[kernel].tt;
+  const int64_t tiles = tiles_of(a, count, tc, tt);
+  HB_REQUIRE(tiles < (1ll << 30), "too many output tiles for one launch");
+  a.channel_tiles = (uint32_t)((a.columns + tc - 1) / tc);
+  a.tiles0 = (uint32_t)tiles_of(a, 1, tc, tt);
+  a.tiles = (uint32_t)tiles;
+  a.tiles_xcd = (a.tiles + 7) / 8;
+  const dim3 each(8 * a.tiles_xcd), four(256), eight(512);
+  switch (kernel) {
+    case T64x32: hipLaunchKernelGGL((linear_tile_kernel<F16, 64, 32, 6, 4>), each, four, 0, st, a); break;
+    case T32x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 32, 64, 8, 4>), each, four, 0, st, a); break;
+    case T64x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 64, 64, 8, 8>), each, eight, 0, st, a); break;
+    case T96x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 96, 64, 7, 8>), each, eight, 0, st, a); break;
+    case T96x128: hipLaunchKernelGGL((linear_tile_kernel<F16, 96, 128, 5, 8>), each, eight, 0, st, a); break;
+    default: {
+      const uint32_t per_xcd = std::max(1, device_cu_count() / 8);
+      const dim3 grid(8 * std::min(a.tiles_xcd, per_xcd)), block(64 * WIDE_WAVES);
+      switch (mode_of(a, count)) {
+        case PLAIN: hipLaunchKernelGGL((linear_wide_kernel<F16, PLAIN>), grid, block, 0, st, a); break;
+        case ACT_GELU: hipLaunchKernelGGL((linear_wide_kernel<F16, ACT_GELU>), grid, block, 0, st, a); break;
+        case ACT_SILU: hipLaunchKernelGGL((linear_wide_kernel<F16, ACT_SILU>), grid, block, 0, st, a); break;
+        case RESIDUAL: hipLaunchKernelGGL((linear_wide_kernel<F16, RESIDUAL>), grid, block, 0, st, a); break;
+        case GATED: hipLaunchKernelGGL((linear_wide_kernel<F16, GATED>), grid, block, 0, st, a); break;
+        default: hipLaunchKernelGGL((linear_wide_kernel<F16, ANY>), grid, block, 0, st, a);
+      }
+    }
+  }
+  HB_HIP(hipGetLastError());
+  return HB_OK;
+}
+
+template <bool F16>
+int launch(Args& a, int count, hipStream_t st) {
+  bool few = true;
+  for (int i = 0; i < count; ++i) few &= a.set[i].tokens <= FEW_ROWS;
+  if (few) {
+    a.tiles0 = (uint32_t)((a.columns + 15) / 16);
+    hipLaunchKernelGGL((linear_few_kernel<F16>), dim3(a.tiles0 * count), dim3(64 * FEW_WAVES), 0, st, a);
+    HB_HIP(hipGetLastError());
+    return HB_OK;
+  }
+  return launch_kernel<F16>(a, count, choose(a, count).kernel, st);
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Whether direct loads take a matrix of `features` columns: rows of whole 16 bytes, and 256 of them, in order, within
+// what a load's offset reaches (2^31 bytes, the row itself among them).
+bool direct(const void* p, int64_t batch, int64_t rows, int64_t b, int64_t n, int32_t features) {
+  if (features % 8 || !aligned16(p) || (rows > 1 && n % 8) || (batch > 1 && b % 8)) return false;
+  const int64_t last = (rows - 1) * n;
+  if (batch > 1 && b < last) return false;  // (a later row would lie before a tile's first)
+  const int64_t batches = std::min(batch - 1, 255 / rows + 1);
+  return (batches * b + std::min<int64_t>(255, rows - 1) * n) * 2 + features * 2ll < (1ll << 31) - 4096;
+}
+
+// Whether a set's rows take the kernel of a few, which loads them as they lie.
+bool few_rows(int count, int32_t batch, const int32_t* rows) {
+  for (int i = 0; i < count; ++i)
+    if ((int64_t)batch * rows[i] > FEW_ROWS) return false;
+  return true;
+}
+
+int64_t padded_bytes(int64_t rows, int32_t features) { return rows * ((features + 63ll) / 64 * 64) * 2; }
+
+constexpr int MAX_DEPTH = 1 << 20;
+
+}  // namespace
+}  // namespace hb
+
+using namespace hb;
+
+extern "C" int64_t hb_linear_workspace_bytes(int32_t count, int32_t batch, const int32_t* rows, int32_t columns,
+                                             int32_t features, void* const* pointers, const int64_t* strides) {
+  if (!rows || !pointers || !strides || count < 1 || count > 2 || batch < 1 || columns < 1 || features < 1) return -1;
+  if (few_rows(count, batch, rows)) return 0;
+  int64_t bytes = 0;
+  for (int i = 0; i < count; ++i) {
+    if (rows[i] < 1) return -1;
+    const int64_t* st = strides + 8 * i;
+    if (!direct(pointers[6 * i], batch, rows[i], st[0], st[1], features)) bytes += padded_bytes((int64_t)batch * rows[i], features);
+    if (!direct(pointers[6 * i + 1], 1, columns, 0, st[2], features)) bytes += padded_bytes(columns, features);
+  }
+  return bytes;
+}
+
+extern "C" int hb_linear(int32_t count, int32_t batch, const int32_t* rows, int32_t columns, int32_t features,
+                         int32_t dtype, int32_t act, void* const* pointers, const int64_t* strides, void* workspace,
+                         int64_t workspace_bytes, hb_stream_t stream) {
+  HB_REQUIRE(count == 1 || count == 2, "count must be 1 or 2");
+  HB_REQUIRE(rows && pointers && strides, "null pointer argument");
+  HB_REQUIRE(columns > 0 && columns < (1 << 28), "columns must be positive (and below 2^28)");
+  HB_REQUIRE(features > 0 && features <= MAX_DEPTH, "features must be in [1, %d] (got %d)", MAX_DEPTH, features);
+  HB_REQUIRE(dtype == HB_DTYPE_BF16 || dtype == HB_DTYPE_F16, "dtype must be bf16 or fp16");
+  HB_REQUIRE(act >= 0 && act <= 2, "act must be 0 (none), 1 (GELU) or 2 (SiLU)");
+  Args a = {};
+  a.columns = columns;
+  a.features = features;
+  a.act = act;
+  a.vectors = 1;
+  const bool few = few_rows(count, batch, rows);
+  PadArgs pad = {};
+  pad.features = features;
+  pad.padded = (features + 63) / 64 * 64;
+  int copies = 0;
+  int64_t used = 0;
+  for (int i = 0; i < count; ++i) {
+    void* const* p = pointers + 6 * i;
+    const int64_t* st = strides + 8 * i;
+    HB_REQUIRE(batch > 0 && rows[i] > 0 && (int64_t)batch * rows[i] < (1ll << 31), "batch and rows must be positive, with fewer than 2^31 rows in all");
+    HB_REQUIRE(p[0] && p[1] && p[5], "null pointer argument");
+    HB_REQUIRE(!p[4] || p[3], "a gate needs its residual");
+    for (int k = 0; k < 6; ++k) HB_REQUIRE(((uintptr_t)p[k] & 1) == 0, "every pointer must be 2-byte aligned");
+    for (int k = 0; k < 8; ++k) HB_REQUIRE(st[k] >= 0, "strides must be non-negative");
+    Set& s = a.set[i];
+    s = {(const uint16_t*)p[0], (const uint16_t*)p[1], (const uint16_t*)p[2], (const uint16_t*)p[3], (const uint16_t*)p[4],
+         (uint16_t*)p[5], st[0], st[1], st[2], st[3], st[4], st[5], st[6], st[7], (uint32_t)rows[i], (uint32_t)(batch * rows[i]), 0};
+    a.vectors &= aligned16(s.out) && s.out_b % 8 == 0 && s.out_n % 8 == 0;
+    if (few) continue;
+    auto copy = [&](const uint16_t*& from, int64_t& b, int64_t& n, uint32_t rows_of_one, uint32_t all) {
+      uint16_t* const to = (uint16_t*)((char*)workspace + used);
+      used += padded_bytes(all, features);
+      pad.m[copies] = {from, to, b, n, rows_of_one, all};
+      pad.first[copies + 1] = pad.first[copies] + (all + 3) / 4;
+      ++copies;
+      from = to;
+      n = pad.padded;
+      b = n * rows_of_one;
+    };
+    if (!direct(s.x, batch, rows[i], s.x_b, s.x_n, features)) copy(s.x, s.x_b, s.x_n, s.rows, s.tokens);
+    int64_t none = 0;
+    if (!direct(s.w, 1, columns, 0, s.w_n, features)) copy(s.w, none, s.w_n, (uint32_t)columns, (uint32_t)columns);
+  }
+  if (copies) {
+    HB_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= used, "the workspace must hold %lld bytes, 16-byte aligned", (long long)used);
+    for (int i = copies; i < 4; ++i) pad.first[i + 1] = pad.first[copies];
+    if (features % 8) a.features = pad.padded;  // (then every matrix is a copy)
+    hipLaunchKernelGGL(pad_rows_kernel, dim3(std::min(pad.first[copies], PAD_GROUPS)), dim3(256), 0, stream, pad);
+    HB_HIP(hipGetLastError());
+  }
+  return dtype == HB_DTYPE_F16 ? launch<true>(a, count, stream) : launch<false>(a, count, stream);
+}

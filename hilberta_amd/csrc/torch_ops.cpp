@@ -39,6 +39,8 @@ constexpr int64_t PAIR_MAX_BLOCKS = 16384;
 constexpr int64_t MIN_WORKSPACE = 1 << 16;
 // Features of 8-bit rows: a sum of so many products fits 32 bits.
 constexpr int64_t MAX_FEATURES = 1 << 17;
+// Features of 16-bit rows (hb_linear).
+constexpr int64_t MAX_DEPTH = 1 << 20;
 
 void check(int rc, const char* name) {
   if (rc == 0) return;
@@ -722,20 +724,116 @@ Tensor int8_qkv(const Maybe& text_q, const Maybe& text_scale, const Maybe& text_
   return out;
 }
 
-// The attention operators and the 8-bit ones return nothing and write `out` and `lse` (and the like),
+// ------------------------------------------------------------------ 16-bit linear layers
+struct DenseSet {
+  const Tensor &x, &weight;
+  const Maybe&bias, &residual, &gate;
+  const Tensor& out;
+};
+
+// hb_linear of one or two row sets.
+void linear_sets(std::initializer_list<DenseSet> sets, int64_t act) {
+  void* pointers[12];
+  int64_t strides[16];
+  int32_t rows[2];
+  const DenseSet& s0 = *sets.begin();
+  const at::ScalarType type = s0.x.scalar_type();
+  const int32_t dtype = type_of(type, "rows");
+  TORCH_CHECK_VALUE(act >= 0 && act <= 2, "act must be 0 (none), 1 (GELU) or 2 (SiLU)");
+  const int64_t batch = s0.x.dim() == 3 ? s0.x.size(0) : 1, features = s0.x.dim() ? s0.x.size(-1) : 0;
+  const int64_t columns = s0.weight.dim() == 2 ? s0.weight.size(0) : 0;
+  int i = 0;
+  for (const DenseSet& s : sets) {
+    const Tensor &bias = value_or_none(s.bias), &residual = value_or_none(s.residual), &gate = value_or_none(s.gate);
+    const Rows x = rows_of(s.x, "x"), out = rows_of(s.out, "out"),
+               res = residual.defined() ? rows_of(residual, "residual") : Rows{};
+    TORCH_CHECK_VALUE(s.weight.dim() == 2 && s.weight.size(1) == s.x.size(-1) && s.x.size(-1) > 0 &&
+                          s.x.size(-1) <= MAX_DEPTH && (features <= 1 || s.weight.stride(1) == 1),
+                      "weight must be [out_features, features] with a contiguous last dimension, of the rows' 1 to ",
+                      MAX_DEPTH, " features");
+    TORCH_CHECK_VALUE(x.batch == batch && s.x.size(-1) == features && s.weight.size(0) == columns &&
+                          s.x.scalar_type() == type,
+                      "both row sets must share batch, features, out_features and dtype");
+    TORCH_CHECK_VALUE(s.out.sizes().slice(0, s.out.dim() - 1) == s.x.sizes().slice(0, s.x.dim() - 1) &&
+                          s.out.size(-1) == columns,
+                      "out must be [..., rows, out_features]");
+    TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == columns && bias.is_contiguous()),
+                      "bias must be a contiguous [out_features] tensor");
+    TORCH_CHECK_VALUE(!residual.defined() || residual.sizes() == s.out.sizes(), "residual must be like out");
+    TORCH_CHECK_VALUE(!gate.defined() || residual.defined(), "a gate needs its residual");
+    TORCH_CHECK_VALUE(!gate.defined() || (gate.dim() == 2 && gate.size(0) == batch && gate.size(1) == columns &&
+                                          (columns <= 1 || gate.stride(1) == 1)),
+                      "gate must be [B, out_features] with a contiguous last dimension");
+    for (const Tensor* t : {&s.weight, &bias, &residual, &gate, &s.out})
+      TORCH_CHECK_VALUE(!t->defined() || t->scalar_type() == type, "all tensors must have the rows' dtype");
+    for (const DenseSet& o : sets) {
+      const Tensor& other = value_or_none(o.residual);
+      check_written(s.out, "out", {&o.weight, &value_or_none(o.bias), &value_or_none(o.gate)});
+      TORCH_CHECK_VALUE(!may_overlap(s.out, o.x), "out must lie apart from the rows");
+      // (a value is read before it is written, by one lane: out may be this set's residual)
+      TORCH_CHECK_VALUE(!other.defined() || (&o == &s && same_places(s.out, other)) || !may_overlap(s.out, other),
+                        "out must be the residual itself or lie apart from it");
+      TORCH_CHECK_VALUE(&o == &s || !may_overlap(s.out, o.out), "both outputs must lie apart");
+    }
+    one_device(s0.x, {&s.x, &s.weight, &bias, &residual, &gate, &s.out});
+    if (!s.out.numel()) continue;  // (a set without rows takes no part in the launch)
+    void* p[6] = {pointer(s.x), pointer(s.weight), pointer(bias), pointer(residual), pointer(gate), pointer(s.out)};
+    // (a stride of a dimension of one says nothing)
+    const int64_t b = batch == 1 ? 0 : 1, n = x.rows == 1 ? 0 : 1;
+    const int64_t st[8] = {b * x.batch_stride, n * x.row_stride, columns == 1 ? 0 : s.weight.stride(0), b * res.batch_stride,
+                           n * res.row_stride, gate.defined() ? b * gate.stride(0) : 0, b * out.batch_stride, n * out.row_stride};
+    std::copy(p, p + 6, pointers + 6 * i);
+    std::copy(st, st + 8, strides + 8 * i);
+    rows[i++] = i32(x.rows, "rows");
+  }
+  require_hip(s0.x);
+  if (!i) return;
+  const at::OptionalDeviceGuard guard(s0.x.device());
+  const int32_t b = i32(batch, "batch"), n = i32(columns, "out_features"), k = i32(features, "features");
+  const int64_t bytes = hb_linear_workspace_bytes(i, b, rows, n, k, pointers, strides);
+  Tensor workspace;  // (freed in the stream's order, after this launch)
+  if (bytes > 0) workspace = new_tensor(s0.x, {bytes}, at::kByte);
+  check(hb_linear(i, b, rows, n, k, dtype, static_cast<int32_t>(act), pointers, strides, pointer(workspace), bytes,
+                  stream_of(s0.x.device())),
+        "hb_linear");
+}
+
+void linear_out(const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& residual, const Maybe& gate,
+                Tensor out, int64_t act) {
+  linear_sets({{x, weight, bias, residual, gate, out}}, act);
+}
+
+Tensor linear(const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& residual, const Maybe& gate, int64_t act) {
+  TORCH_CHECK_VALUE((x.dim() == 2 || x.dim() == 3) && weight.dim() == 2,
+                    "x must be [rows, features] or [B, rows, features] and weight [out_features, features]");
+  c10::SmallVector<int64_t, 3> sizes(x.sizes().begin(), x.sizes().end());
+  sizes.back() = weight.size(0);
+  Tensor out = new_tensor(x, sizes, x.scalar_type());
+  linear_out(x, weight, bias, residual, gate, out, act);
+  return out;
+}
+
+void linear_pair_out(const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& residual, const Maybe& gate,
+                     Tensor out, const Tensor& x2, const Tensor& weight2, const Maybe& bias2, const Maybe& residual2,
+                     const Maybe& gate2, Tensor out2, int64_t act) {
+  linear_sets({{x, weight, bias, residual, gate, out}, {x2, weight2, bias2, residual2, gate2, out2}}, act);
+}
+
+// The attention operators and the layers' return nothing and write `out` and `lse` (and the like),
 // which torch's own boxed fallbacks overlook: they look after returned tensors only.
 
-// (the 8-bit operators that return their results write nothing)
+// (the layers' operators that return their results write nothing)
 constexpr const char* WRITING[] = {"paired_fwd", "sparse_fwd", "int8_adaln", "int8_adaln_pair", "int8_linear_out",
-                                   "int8_linear_pair_out", "int8_qkv_out"};
-constexpr const char* RETURNING[] = {"int8_rows", "int8_linear", "int8_linear_rows", "int8_qkv"};
+                                   "int8_linear_pair_out", "int8_qkv_out", "linear_out", "linear_pair_out"};
+constexpr const char* RETURNING[] = {"int8_rows", "int8_linear", "int8_linear_rows", "int8_qkv", "linear"};
 
 // No derivative is recorded (the entry points refuse inputs that need one); a transform that takes one
 // is refused, as torch refuses an autograd.Function in one, for it would get zeros.
 void no_derivative(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
   const size_t count = op.schema().arguments().size();
-  // (the attention operators' entry points look for gradients themselves; the 8-bit ones leave it to this)
-  const bool refuse = at::GradMode::is_enabled() && op.schema().name().rfind("hilberta_hip::int8_", 0) == 0;
+  // (the attention operators' entry points look for gradients themselves; the layers' leave it to this)
+  const std::string& name = op.schema().name();
+  const bool refuse = at::GradMode::is_enabled() && name != "hilberta_hip::paired_fwd" && name != "hilberta_hip::sparse_fwd";
   // (included for as long as any torch.func transform is active)
   const bool transformed = at::GradMode::is_enabled() &&
                            c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerBackMode);
@@ -803,6 +901,11 @@ TORCH_LIBRARY(hilberta_hip, m) {
                           "Tensor weight_scale, Tensor? bias, Tensor? norm_q, Tensor? norm_k, Tensor? cos, Tensor? sin, ";
   m.def(("int8_qkv(" + qkv + "ScalarType dtype, SymInt heads, float eps) -> Tensor").c_str(), tags);
   m.def(("int8_qkv_out(" + qkv + "Tensor(a16!) out, float eps) -> ()").c_str(), tags);
+  const std::string dense = "Tensor x$, Tensor weight$, Tensor? bias$, Tensor? residual$, Tensor? gate$, ";
+  m.def(("linear(" + set(dense, "") + "SymInt act) -> Tensor").c_str(), tags);
+  const std::string into = dense + "Tensor(o$!) out$, ";
+  m.def(("linear_out(" + set(into, "") + "SymInt act) -> ()").c_str(), tags);
+  m.def(("linear_pair_out(" + set(into, "") + set(into, "2") + "SymInt act) -> ()").c_str(), tags);
   m.def("_attention_workspace(Device device, int need) -> Tensor");
   m.def("_workspace_keys() -> int[]");
   m.def("_clear_workspaces() -> ()");
@@ -816,8 +919,11 @@ TORCH_LIBRARY_IMPL(hilberta_hip, CUDA, m) {
   m.impl("gather_rows", gather_rows);
 }
 
-// (on CPU tensors the 8-bit operators make their checks and refuse)
-void int8_operators(torch::Library& m) {
+// (on CPU tensors the layers' operators make their checks and refuse)
+void layer_operators(torch::Library& m) {
+  m.impl("linear", linear);
+  m.impl("linear_out", linear_out);
+  m.impl("linear_pair_out", linear_pair_out);
   m.impl("int8_rows", int8_rows);
   m.impl("int8_adaln", int8_adaln);
   m.impl("int8_adaln_pair", int8_adaln_pair);
@@ -828,8 +934,8 @@ void int8_operators(torch::Library& m) {
   m.impl("int8_qkv", int8_qkv);
   m.impl("int8_qkv_out", int8_qkv_out);
 }
-TORCH_LIBRARY_IMPL(hilberta_hip, CUDA, int8_hip) { int8_operators(int8_hip); }
-TORCH_LIBRARY_IMPL(hilberta_hip, CPU, int8_cpu) { int8_operators(int8_cpu); }
+TORCH_LIBRARY_IMPL(hilberta_hip, CUDA, layers_hip) { layer_operators(layers_hip); }
+TORCH_LIBRARY_IMPL(hilberta_hip, CPU, layers_cpu) { layer_operators(layers_cpu); }
 
 TORCH_LIBRARY_IMPL(hilberta_hip, CompositeExplicitAutograd, m) {
   m.impl("_attention_workspace", attention_workspace);

@@ -214,6 +214,24 @@ int hb_adaln_modulate_pair(int32_t batch, const int32_t* rows, int32_t hidden, i
                            float eps, void* const* pointers, const int64_t* strides,
                            hb_stream_t stream);
 
+/* ---------------------------------------------------------------- 16-bit linear layers
+ * No counterpart in the reference, whose linear layers are library calls with passes around them (in the
+ * transformer that hilberta/flux_adapter.py wraps).  For one or two row sets (count) of one batch and layer
+ * shape in one launch:
+ *   out[b, m, n] = residual[b, m, n] + gate[b, n] * act(sum_k x[b, m, k] weight[n, k] + bias[n])
+ * act: 0 none, 1 GELU(tanh), 2 SiLU; sums and epilogue in fp32, one rounding.  Host arrays, set after set: rows
+ * [count]; pointers [count x 6] {x, weight, bias or NULL, residual or NULL, gate or NULL (else with a residual), out};
+ * strides [count x 8] {x batch, x row, weight row, residual batch, residual row, gate batch, out batch, out row},
+ * elements, last dimensions contiguous.  out may be the residual itself; it may lie over nothing else that is read.
+ * features up to 2^20.  Rows may begin at any element; x and weights whose rows are no multiples of 16 bytes, or lie too
+ * far apart, are copied into `workspace` first (hb_linear_workspace_bytes, -1 where the sizes are rejected; 16-byte
+ * aligned, contents irrelevant before and after), unless both sets have at most 16 rows. */
+int64_t hb_linear_workspace_bytes(int32_t count, int32_t batch, const int32_t* rows, int32_t columns,
+                                  int32_t features, void* const* pointers, const int64_t* strides);
+int hb_linear(int32_t count, int32_t batch, const int32_t* rows, int32_t columns, int32_t features,
+              int32_t dtype, int32_t act, void* const* pointers, const int64_t* strides,
+              void* workspace, int64_t workspace_bytes, hb_stream_t stream);
+
 /* ---------------------------------------------------------------- 8-bit linear layers
  * No counterpart in the reference, which runs the linear layers of the transformer that
  * hilberta/flux_adapter.py wraps in 16 bits.  Rows and weights are held as int8 [rows, padded], padded the

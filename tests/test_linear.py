@@ -1,0 +1,123 @@
+"""flux_linear on the CPU: what its operators refuse, and that they run nowhere but on the GPU.
+
+The operators make their checks on any device and refuse CPU tensors last: a call that passes every check ends with
+that refusal.
+"""
+
+import pytest
+import torch
+
+from hilberta_amd import flux_linear as f
+from hilberta_amd import ops
+
+BF16, HALF = torch.bfloat16, torch.float16
+ON_DEVICE = "device tensors"
+B, M, K, N = 2, 3, 24, 40
+
+
+def _args(**changes):
+    a = dict(x=torch.zeros(B, M, K, dtype=BF16), weight=torch.zeros(N, K, dtype=BF16), bias=torch.zeros(N, dtype=BF16),
+             residual=torch.zeros(B, M, N, dtype=BF16), gate=torch.zeros(B, N, dtype=BF16))
+    return {k: v for k, v in (a | changes).items() if v is not None or k in ("bias", "residual", "gate")}
+
+
+def _refused(match, **changes):
+    with pytest.raises(ValueError, match=match):
+        f.linear(**_args(**changes))
+
+
+def test_a_call_that_passes_every_check_needs_the_gpu():
+    for changes in ({}, dict(bias=None), dict(gate=None), dict(gate=None, residual=None), dict(act="gelu"), dict(act="silu"),
+                    dict(out=torch.zeros(B, M, N, dtype=BF16)),
+                    dict(x=torch.zeros(M, K, dtype=BF16), residual=torch.zeros(M, N, dtype=BF16), gate=torch.zeros(1, N, dtype=BF16)),
+                    dict(x=torch.zeros(B, 0, K, dtype=BF16), residual=torch.zeros(B, 0, N, dtype=BF16)),
+                    dict(x=torch.zeros(B, M, K + 8, dtype=BF16)[..., 3:3 + K], weight=torch.zeros(N, K + 5, dtype=BF16)[:, 1:1 + K])):
+        _refused(ON_DEVICE, **changes)
+
+
+def test_shapes_and_types():
+    zeros = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype)  # noqa: E731
+    _refused("act must be", act="relu")
+    _refused("act must be", act=True)
+    _refused("x must be", x=zeros(K))
+    _refused("x must be", weight=zeros(N))
+    _refused("x must be", x=zeros(B, 1, M, K))
+    _refused("weight must be", weight=zeros(N, K + 1))
+    _refused("weight must be", weight=zeros(K, N).T)
+    _refused("weight must be", x=zeros(B, M, 0), weight=zeros(N, 0))
+    _refused("contiguous last dimension", x=zeros(B, K, M).transpose(1, 2))
+    _refused("bias must be", bias=zeros(N + 1))
+    _refused("bias must be", bias=zeros(2 * N)[::2])
+    _refused("residual must be like out", residual=zeros(B, M, N + 1))
+    _refused("residual must have a contiguous", residual=zeros(B, N, M).transpose(1, 2))
+    _refused("needs its residual", residual=None)
+    _refused("gate must be", gate=zeros(B + 1, N))
+    _refused("gate must be", gate=zeros(N))
+    _refused("gate must be", gate=zeros(N, B).T)
+    _refused("out must be", out=zeros(B, M, N + 1))
+    for name, shape in (("weight", (N, K)), ("bias", (N,)), ("residual", (B, M, N)), ("gate", (B, N)), ("out", (B, M, N))):
+        _refused("rows' dtype", **{name: zeros(*shape, dtype=HALF)})
+    _refused("bf16 or fp16", x=zeros(B, M, K, dtype=torch.float32))
+    with pytest.raises(ValueError, match="act must be 0"):
+        ops.linear(zeros(B, M, K), zeros(N, K), None, None, None, 3)
+
+
+def test_what_is_written_lies_apart():
+    buffer = torch.zeros(B, M, K + N, dtype=BF16)
+    _refused(ON_DEVICE, out=buffer[..., K:])
+    _refused(ON_DEVICE, x=buffer[..., :K], out=buffer[..., K:])
+    _refused("apart from the rows", x=buffer[..., 1:K + 1], out=buffer[..., K:])
+    _refused("non-overlapping", out=torch.zeros(1, M, N, dtype=BF16).expand(B, M, N))
+    res = torch.zeros(B, M, N, dtype=BF16)
+    _refused(ON_DEVICE, residual=res, out=res)
+    wide = torch.zeros(B, M, N + 1, dtype=BF16)
+    _refused("residual itself", residual=wide[..., 1:], out=wide[..., :N])
+    _refused(ON_DEVICE, residual=torch.zeros(B, M, 2 * N, dtype=BF16)[..., :N], out=res)
+    both = torch.zeros(B, M, 2 * N, dtype=BF16)
+    _refused(ON_DEVICE, residual=both[..., :N], out=both[..., N:])
+    flat = torch.zeros(B * N, dtype=BF16)
+    _refused("cannot alias", gate=flat.view(B, N), residual=torch.zeros(B, 1, N, dtype=BF16),
+             x=torch.zeros(B, 1, K, dtype=BF16), out=flat.view(B, 1, N))
+
+
+def test_pairs():
+    a, b = _args(), _args(x=torch.zeros(B, 5, K, dtype=BF16), residual=torch.zeros(B, 5, N, dtype=BF16))
+
+    def pair(match, **changes):
+        with pytest.raises(ValueError, match=match):
+            f.linear_pair(a, b | changes)
+
+    pair(ON_DEVICE)
+    pair(ON_DEVICE, x=torch.zeros(B, 0, K, dtype=BF16), residual=None, gate=None)
+    pair("share batch", x=torch.zeros(B + 1, 5, K, dtype=BF16), residual=None, gate=None)
+    pair("share batch", weight=torch.zeros(N + 8, K, dtype=BF16), bias=None, residual=None, gate=None)
+    pair("share batch", x=torch.zeros(B, 5, K + 8, dtype=BF16), weight=torch.zeros(N, K + 8, dtype=BF16))
+    out = torch.zeros(B, 8, N, dtype=BF16)
+    with pytest.raises(ValueError, match=ON_DEVICE):
+        f.linear_pair(a | dict(out=out[:, :3]), b | dict(out=out[:, 3:]))
+    with pytest.raises(ValueError, match="lie apart"):
+        f.linear_pair(a | dict(out=out[:, :3]), b | dict(out=out[:, 2:7]))
+    with pytest.raises(ValueError, match="residual itself"):  # (one set's output over the other's residual)
+        f.linear_pair(a | dict(out=b["residual"][:, :3]), b)
+
+
+def test_gradients_are_refused():
+    a = _args(weight=torch.zeros(N, K, dtype=BF16, requires_grad=True))
+    with pytest.raises(ValueError, match="Inference only"):
+        f.linear(**a)
+    with torch.no_grad(), pytest.raises(ValueError, match=ON_DEVICE):
+        f.linear(**a)
+    with pytest.raises(RuntimeError, match="linear has no derivative for torch.func"):
+        torch.func.grad(lambda w: f.linear(_args()["x"], w).float().sum())(_args()["weight"])
+    with pytest.raises(NotImplementedError, match="does not support it"):
+        torch.func.jvp(lambda w: f.linear(_args()["x"], w), (_args()["weight"],), (_args()["weight"],))
+
+
+def test_shapes_of_traced_calls():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x, w = torch.empty(2, 5, 24, dtype=HALF, device="cuda"), torch.empty(40, 24, dtype=HALF, device="cuda")
+        y = f.linear(x, w, act="silu")
+        assert y.shape == (2, 5, 40) and y.dtype == HALF and y.device.type == "cuda"
+        assert [t.shape[1] for t in f.linear_pair(dict(x=x, weight=w), dict(x=x[:, :3], weight=w))] == [5, 3]
