@@ -68,6 +68,11 @@ SIGNATURES = {
          _p, _c_i64, _c_i64, _p, _p, _c_i64, _p, _c_i64, _c_i64, _p],
     ),
     "hb_adaln_modulate_pair": (_c_int, [_c_int, _p, _c_int, _c_int, _c_f32, _p, _p, _p]),
+    "hb_group_norm_workspace_bytes": (_c_i64, [_c_int, _c_i64, _c_int, _c_int, _c_int]),
+    "hb_group_norm": (
+        _c_int,
+        [_c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_f32, _p, _c_i64, _c_i64, _p, _p, _p, _c_i64, _c_i64, _p, _c_i64, _p],
+    ),
     "hb_linear_workspace_bytes": (_c_i64, [_c_int, _c_int, _p, _c_int, _c_int, _p, _p]),
     "hb_linear": (_c_int, [_c_int, _c_int, _p, _c_int, _c_int, _c_int, _c_int, _p, _p, _p, _c_i64, _p]),
     "hb_int8_rows": (_c_int, [_p, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p, _p]),

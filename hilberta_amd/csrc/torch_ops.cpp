@@ -819,13 +819,85 @@ void linear_pair_out(const Tensor& x, const Tensor& weight, const Maybe& bias, c
   linear_sets({{x, weight, bias, residual, gate, out}, {x2, weight2, bias2, residual2, gate2, out2}}, act);
 }
 
+// ------------------------------------------------------------------ group norm
+// An image batch whose channels lie last in memory: [B, pixels, C], or [B, C, ...] with one to three dimensions of pixels,
+// which one stride walks.
+struct Image {
+  int64_t batch, pixels, channels, batch_stride, pixel_stride;
+};
+Image image_of(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.dim() >= 3 && t.dim() <= 5, name, " must be [B, pixels, C], [B, C, H, W] or [B, C, T, H, W]");
+  const int64_t channel = t.dim() == 3 ? 2 : 1, first = t.dim() == 3 ? 1 : 2, last = t.dim() == 3 ? 1 : t.dim() - 1;
+  Image m{t.size(0), 1, t.size(channel), t.size(0) > 1 ? t.stride(0) : 0, 0};
+  bool fits = t.size(channel) <= 1 || t.stride(channel) == 1;
+  int64_t step = -1;  // what the next dimension outwards must advance by
+  for (int64_t d = last; d >= first; --d) {
+    m.pixels *= t.size(d);
+    if (t.size(d) <= 1) continue;
+    if (step < 0) m.pixel_stride = t.stride(d);
+    else fits &= t.stride(d) == step;
+    step = t.stride(d) * t.size(d);
+  }
+  TORCH_CHECK_VALUE(fits || !t.numel(), name, " must hold its channels last in memory (torch.channels_last), its pixels evenly apart");
+  return m;
+}
+
+void group_norm_out(const Tensor& x, int64_t groups, const Maybe& weight, const Maybe& bias, Tensor out, bool silu, double eps) {
+  const Tensor &w = value_or_none(weight), &b = value_or_none(bias);
+  const at::ScalarType type = x.scalar_type();
+  TORCH_CHECK_VALUE(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "x must be bf16, fp16 or fp32");
+  const Image m = image_of(x, "x");
+  TORCH_CHECK_VALUE(m.channels > 0 && m.channels <= 8192, "x must have 1 to 8192 channels");
+  TORCH_CHECK_VALUE(groups > 0 && m.channels % groups == 0, "groups must divide the channels");
+  TORCH_CHECK_VALUE(eps > 0, "eps must be positive");
+  for (const Tensor* t : {&w, &b})
+    TORCH_CHECK_VALUE(!t->defined() || (t->dim() == 1 && t->size(0) == m.channels && t->is_contiguous() && t->scalar_type() == type),
+                      "weight and bias must be contiguous [C] tensors of x's dtype");
+  TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == type, "out must be like x");
+  const Image o = image_of(out, "out");
+  check_written(out, "out", {&w, &b});
+  // (a value is read before it is written, by one lane, and the statistics before that: out may be x)
+  if (!same_places(out, x)) check_written(out, "out", {&x});
+  one_device(x, {&w, &b, &out});
+  require_hip(x);
+  if (!x.numel()) return;
+  const at::OptionalDeviceGuard guard(x.device());
+  const int32_t dtype = type == at::kFloat ? HB_DTYPE_F32 : type == at::kHalf ? HB_DTYPE_F16 : HB_DTYPE_BF16;
+  const int32_t batch = i32(m.batch, "batch"), channels = i32(m.channels, "channels"), g = i32(groups, "groups");
+  const int64_t bytes = hb_group_norm_workspace_bytes(batch, m.pixels, channels, g, dtype);
+  Tensor workspace;  // (freed in the stream's order, after this launch)
+  if (bytes > 0) workspace = new_tensor(x, {bytes}, at::kByte);
+  check(hb_group_norm(batch, m.pixels, channels, g, dtype, silu, static_cast<float>(eps), x.data_ptr(), m.batch_stride,
+                      m.pixel_stride, pointer(w), pointer(b), out.data_ptr(), o.batch_stride, o.pixel_stride,
+                      pointer(workspace), bytes, stream_of(x.device())),
+        "hb_group_norm");
+}
+
+Tensor group_norm(const Tensor& x, int64_t groups, const Maybe& weight, const Maybe& bias, bool silu, double eps) {
+  const Image m = image_of(x, "x");
+  // x's sizes, its channels last in memory
+  c10::SmallVector<int64_t, 5> strides(x.dim());
+  int64_t step = x.dim() == 3 ? 1 : m.channels;
+  if (x.dim() == 3) {
+    strides = {m.pixels * m.channels, m.channels, 1};
+  } else {
+    strides[1] = 1;
+    for (int64_t d = x.dim() - 1; d >= 2; --d) strides[d] = step, step *= x.size(d);
+    strides[0] = step;
+  }
+  Tensor out = x.is_cuda() ? Tensor(at::detail::empty_strided_cuda(x.sizes(), strides, x.scalar_type(), x.device()))
+                           : at::empty_strided(x.sizes(), strides, x.options());
+  group_norm_out(x, groups, weight, bias, out, silu, eps);
+  return out;
+}
+
 // The attention operators and the layers' return nothing and write `out` and `lse` (and the like),
 // which torch's own boxed fallbacks overlook: they look after returned tensors only.
 
 // (the layers' operators that return their results write nothing)
 constexpr const char* WRITING[] = {"paired_fwd", "sparse_fwd", "int8_adaln", "int8_adaln_pair", "int8_linear_out",
-                                   "int8_linear_pair_out", "int8_qkv_out", "linear_out", "linear_pair_out"};
-constexpr const char* RETURNING[] = {"int8_rows", "int8_linear", "int8_linear_rows", "int8_qkv", "linear"};
+                                   "int8_linear_pair_out", "int8_qkv_out", "linear_out", "linear_pair_out", "group_norm_out"};
+constexpr const char* RETURNING[] = {"int8_rows", "int8_linear", "int8_linear_rows", "int8_qkv", "linear", "group_norm"};
 
 // No derivative is recorded (the entry points refuse inputs that need one); a transform that takes one
 // is refused, as torch refuses an autograd.Function in one, for it would get zeros.
@@ -906,6 +978,8 @@ TORCH_LIBRARY(hilberta_hip, m) {
   const std::string into = dense + "Tensor(o$!) out$, ";
   m.def(("linear_out(" + set(into, "") + "SymInt act) -> ()").c_str(), tags);
   m.def(("linear_pair_out(" + set(into, "") + set(into, "2") + "SymInt act) -> ()").c_str(), tags);
+  m.def("group_norm(Tensor x, SymInt groups, Tensor? weight, Tensor? bias, bool silu, float eps) -> Tensor", tags);
+  m.def("group_norm_out(Tensor x, SymInt groups, Tensor? weight, Tensor? bias, Tensor(a4!) out, bool silu, float eps) -> ()", tags);
   m.def("_attention_workspace(Device device, int need) -> Tensor");
   m.def("_workspace_keys() -> int[]");
   m.def("_clear_workspaces() -> ()");
@@ -921,6 +995,8 @@ TORCH_LIBRARY_IMPL(hilberta_hip, CUDA, m) {
 
 // (on CPU tensors the layers' operators make their checks and refuse)
 void layer_operators(torch::Library& m) {
+  m.impl("group_norm", group_norm);
+  m.impl("group_norm_out", group_norm_out);
   m.impl("linear", linear);
   m.impl("linear_out", linear_out);
   m.impl("linear_pair_out", linear_pair_out);

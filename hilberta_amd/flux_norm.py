@@ -1,12 +1,16 @@
-"""Gated residual + AdaLN modulation of the FLUX blocks in one HIP pass (csrc/adaln.hip).
+"""The norms: gated residual + AdaLN modulation of the FLUX blocks, and the image decoder's group norm.
 
-``adaln_modulate(x, shift, scale, y=y, gate=gate, x_out=x)`` computes, per token row,
+``adaln_modulate(x, shift, scale, y=y, gate=gate, x_out=x)`` (csrc/adaln.hip, one pass) computes, per token row,
 
     r = x + gate * y;  x_out = r;  out = shift + LayerNorm(r) * (1 + scale)
 
 which the FLUX blocks (diffusers 0.36.0 FluxTransformerBlock / FluxSingleTransformerBlock with
 AdaLayerNormZero / AdaLayerNormZeroSingle / AdaLayerNormContinuous) run as separate torch passes:
 ``torch.addcmul`` for the gated residual, ``layer_norm``, ``1 + scale`` and another ``addcmul``.
+
+``group_norm(x, groups, weight, bias, act="silu")`` (csrc/group_norm.hip) is what precedes every convolution of the
+decoder that turns a sampling loop's latents into an image, on images whose channels lie last in memory: the norm
+over a group's channels and all pixels, and the activation, which torch runs as two or three passes.
 """
 
 from __future__ import annotations
@@ -15,7 +19,7 @@ import ctypes
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
@@ -98,3 +102,19 @@ def adaln_modulate_pair(first, second, *, eps=1e-6):
         (ctypes.c_int64 * 20)(*sa, *sb), _lib.stream_ptr(device))
     _lib.check(rc, "hb_adaln_modulate_pair")
     return out_a, out_b
+
+
+def group_norm(x, groups, weight=None, bias=None, *, act=None, eps=1e-6, out=None):
+    """act((x - mean) / sqrt(var + eps) * weight + bias), mean and variance of each batch element's ``groups`` groups of
+    neighbouring channels over all pixels.
+
+    x [B, pixels, C], [B, C, H, W] or [B, C, T, H, W], its channels last in memory (torch.channels_last,
+    channels_last_3d) and its pixels evenly apart; bf16, fp16 or fp32, up to 8192 channels; weight and bias [C] of x's
+    dtype; act None or "silu".  Statistics and values are fp32, rounded once.  ``out`` is like x and may be x itself.
+    Inference only; asynchronous on the current stream, and can be captured into a graph."""
+    if act not in (None, "silu"):
+        raise ValueError('act must be None or "silu"')
+    if out is None:
+        return ops.group_norm(x, groups, weight, bias, act == "silu", eps)
+    ops.group_norm_out(x, groups, weight, bias, out, act == "silu", eps)
+    return out

@@ -26,6 +26,8 @@ implementation for tracing and, for pair_rows alone, a CPU one:
   hilberta_hip::linear(x, weight, bias?, residual?, gate?, act) -> Tensor
   hilberta_hip::linear_out(.. as linear up to gate?, out!, act) -> ()
   hilberta_hip::linear_pair_out: two row sets' arguments (the second's names end in 2)
+  hilberta_hip::group_norm(x, groups, weight?, bias?, silu, eps) -> Tensor
+  hilberta_hip::group_norm_out(x, groups, weight?, bias?, out!, silu, eps) -> ()
 
 The attention ops write into caller-provided outputs (declared mutated), as the reference's
 launches write into ``out``.  Argument checks with the reference's messages stay in the Python
@@ -33,7 +35,7 @@ entry points (paired_attention, sparse_attention) and run before the op; the lib
 cheap ones and reports them as ValueError.  The attention and gather ops have no CPU kernel: on
 CPU tensors they raise.  pair_rows is plan setup and also runs on CPU tensors, through the
 library's host table builder (hb_pair_rows_host, bit-identical to the device kernel).  The layers' ops
-(flux_int8.py, flux_linear.py) check their arguments on any device and refuse CPU tensors.  Without the
+(flux_int8.py, flux_linear.py, flux_norm.group_norm) check their arguments on any device and refuse CPU tensors.  Without the
 built library the operators do not exist and every use of one raises.
 """
 
@@ -92,6 +94,12 @@ def _fake_linear(x, weight, bias, residual, gate, act):
     return x.new_empty((*x.shape[:-1], weight.shape[0]))
 
 
+def _fake_group_norm(x, groups, weight, bias, silu, eps):
+    if x.ndim == 3:
+        return x.new_empty(x.shape)
+    return torch.empty_like(x, memory_format=torch.channels_last if x.ndim == 4 else torch.channels_last_3d)
+
+
 def _pair_rows_cpu(kv_indices: Tensor, kv_counts: Tensor, total_blocks: int, key_block_size: int,
                    paired_width: int) -> tuple[Tensor, Tensor, Tensor]:
     """pair_rows of CPU tensors by hb_pair_rows_host."""
@@ -132,7 +140,8 @@ def _load():
                  int8_adaln_pair=_fake_int8_adaln_pair, int8_linear=_fake_int8_linear,
                  int8_linear_rows=_fake_int8_linear_rows, int8_linear_out=_fake_none,
                  int8_linear_pair_out=_fake_none, int8_qkv=_fake_int8_qkv, int8_qkv_out=_fake_none,
-                 linear=_fake_linear, linear_out=_fake_none, linear_pair_out=_fake_none)
+                 linear=_fake_linear, linear_out=_fake_none, linear_pair_out=_fake_none,
+                 group_norm=_fake_group_norm, group_norm_out=_fake_none)
     for name, fake in fakes.items():
         torch.library.register_fake(f"{_NS}::{name}", fake)
     torch.library.impl(f"{_NS}::pair_rows", "cpu", _pair_rows_cpu)
@@ -142,11 +151,11 @@ def _load():
 _NAMES = ("paired_fwd", "sparse_fwd", "pair_rows", "gather_rows", "_attention_workspace",
           "_workspace_keys", "_clear_workspaces", "int8_rows", "int8_adaln", "int8_adaln_pair", "int8_linear",
           "int8_linear_rows", "int8_linear_out", "int8_linear_pair_out", "int8_qkv", "int8_qkv_out",
-          "linear", "linear_out", "linear_pair_out")
+          "linear", "linear_out", "linear_pair_out", "group_norm", "group_norm_out")
 try:
     _bound = _load()
 except (RuntimeError, OSError) as e:  # the package still imports, so that it can be (re)built
     _bound = [_Missing(name, str(e)) for name in _NAMES]
 (paired_fwd, sparse_fwd, pair_rows, gather_rows, attention_workspace, workspace_keys, clear_workspaces,
  int8_rows, int8_adaln, int8_adaln_pair, int8_linear, int8_linear_rows, int8_linear_out, int8_linear_pair_out,
- int8_qkv, int8_qkv_out, linear, linear_out, linear_pair_out) = _bound
+ int8_qkv, int8_qkv_out, linear, linear_out, linear_pair_out, group_norm, group_norm_out) = _bound

@@ -20,6 +20,7 @@ extern "C" {
 #define HB_ABI_VERSION 5
 #define HB_DTYPE_BF16 0
 #define HB_DTYPE_F16 1
+#define HB_DTYPE_F32 2
 
 typedef struct ihipStream_t* hb_stream_t;
 
@@ -213,6 +214,23 @@ int hb_adaln_modulate(int32_t batch, int32_t rows, int32_t hidden, int32_t dtype
 int hb_adaln_modulate_pair(int32_t batch, const int32_t* rows, int32_t hidden, int32_t dtype,
                            float eps, void* const* pointers, const int64_t* strides,
                            hb_stream_t stream);
+
+/* ---------------------------------------------------------------- group norm
+ * No counterpart in the reference: the norm of the image decoder that its pipeline ends with, there separate library
+ * passes.  Per batch element and group of channels:
+ *   out = act((x - mean) / sqrt(var + eps) * weight[c] + bias[c])
+ * mean and var (of n, not n - 1) over the element's pixels and the group's channels; silu = 1: act is SiLU, else none;
+ * statistics and values in fp32, one rounding.  x and out are [batch, pixels, channels] by element strides, channels
+ * contiguous; groups divide the channels, which are up to 8192; dtype may be HB_DTYPE_F32; weight and bias [channels] of
+ * that type, or NULL.  out may be x itself.  `workspace`: hb_group_norm_workspace_bytes (0 for small groups, -1 where the
+ * sizes are rejected), 8-byte aligned, contents irrelevant before and after. */
+int64_t hb_group_norm_workspace_bytes(int32_t batch, int64_t pixels, int32_t channels,
+                                      int32_t groups, int32_t dtype);
+int hb_group_norm(int32_t batch, int64_t pixels, int32_t channels, int32_t groups, int32_t dtype,
+                  int32_t silu, float eps, const void* x, int64_t x_batch_stride,
+                  int64_t x_pixel_stride, const void* weight, const void* bias, void* out,
+                  int64_t out_batch_stride, int64_t out_pixel_stride, void* workspace,
+                  int64_t workspace_bytes, hb_stream_t stream);
 
 /* ---------------------------------------------------------------- 16-bit linear layers
  * No counterpart in the reference, whose linear layers are library calls with passes around them (in the
