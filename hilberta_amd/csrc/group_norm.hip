@@ -22,10 +22,10 @@ namespace hb {
 namespace {
 
 constexpr int V = 8;                  // channels of a thread
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, MAX_THREADS = 1024;
 constexpr int MAX_CHANNELS = 8192;
-constexpr int64_t CHUNK_BYTES = 64 << 10;
-constexpr int MAX_CHUNKS = 512;       // of a launch
+constexpr int64_t CHUNK_BYTES = 16 << 10;
+constexpr int64_t LARGE_BYTES = 512ll << 20;
 
 struct Args {
   const void* x;
@@ -65,10 +65,14 @@ template <int DT>
 struct Raw {
   u32x4 v[DT == HB_DTYPE_F32 ? 2 : 1];
 };
-template <int DT, bool EDGE, bool STREAM>
+// How rows divide into vectors: evenly; with a last vector that begins eight channels before the row's end and shares some
+// with the one before; not at all, where there are fewer than eight channels (`there` of them).
+enum Edge { EVEN, SHARED, SHORT };
+
+template <int DT, int EDGE, bool STREAM>
 __device__ __forceinline__ Raw<DT> load(const typename Type<DT>::T* p, int there) {
   Raw<DT> r = {};
-  if (EDGE && there < V) {
+  if (EDGE == SHORT) {
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       if (k >= there) continue;
@@ -98,12 +102,13 @@ __device__ __forceinline__ void unpack(const Raw<DT>& r, float (&x)[V]) {
     unpack8<DT == HB_DTYPE_F16>(r.v[0], x);
   }
 }
-template <int DT, bool EDGE, bool STREAM>
-__device__ __forceinline__ void store(typename Type<DT>::T* p, const float (&x)[V], int there) {
-  if (EDGE && there < V) {
+// (skip: the first channels that the vector before this one stores)
+template <int DT, int EDGE, bool STREAM>
+__device__ __forceinline__ void store(typename Type<DT>::T* p, const float (&x)[V], int skip, int there) {
+  if (EDGE == SHORT || (EDGE == SHARED && skip)) {
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      if (k >= there) continue;
+      if (k < skip || k >= there) continue;
       if constexpr (DT == HB_DTYPE_F32) p[k] = x[k];
       else p[k] = from_f<DT == HB_DTYPE_F16>(x[k]);
     }
@@ -137,14 +142,14 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
 }
 
 // ------------------------------------------------------------------ statistics of a chunk
-template <int DT, bool EDGE>
+template <int DT, int EDGE>
 __global__ void group_norm_sums_kernel(Args a) {
   typedef typename Type<DT>::T T;
   extern __shared__ float lds[];  // [2][rows][vectors * V]
   const int width = a.vectors * V, tx = threadIdx.x % a.vectors, ty = threadIdx.x / a.vectors;
   const uint32_t p0 = blockIdx.x * a.chunk, p1 = min(a.pixels, p0 + a.chunk), rows = a.rows;
-  const int there = a.channels - tx * V;
-  const T* const x = (const T*)a.x + blockIdx.y * a.x_b + tx * V;
+  const int first = EDGE == SHARED ? min(tx * V, a.channels - V) : tx * V, there = a.channels;
+  const T* const x = (const T*)a.x + blockIdx.y * a.x_b + first;
   float mean[V] = {}, squares[V] = {}, n = 0.f;
   auto take = [&](uint32_t p, auto whole) {
     constexpr bool WHOLE = decltype(whole)::value;
@@ -180,115 +185,161 @@ __global__ void group_norm_sums_kernel(Args a) {
   if (p < p1) take(p, std::false_type());
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    lds[ty * width + tx * V + k] = mean[k];
-    lds[(rows + ty) * width + tx * V + k] = squares[k];
+    lds[ty * width + first + k] = mean[k];  // (channels that two vectors share: the same values twice)
+    lds[(rows + ty) * width + first + k] = squares[k];
   }
   __syncthreads();
-  // Eight lanes a group: its mean, then the squares about it.
-  const int lanes = blockDim.x / 8, lane = threadIdx.x & 7, taken = p1 - p0;
-  for (int g = threadIdx.x / 8; g < a.groups && (int)threadIdx.x < lanes * 8; g += lanes) {
-    float sum = 0.f;
-    for (uint32_t r = 0; r < rows; ++r) {
-      const float count = (float)((taken - (int)r + (int)rows - 1) / (int)rows);
-      for (int c = lane; c < a.per; c += 8) sum += count * lds[r * width + g * a.per + c];
-    }
-#pragma unroll
-    for (int m = 1; m < 8; m <<= 1) sum += __shfl_xor(sum, m, 64);
-    const float center = sum / ((float)taken * (float)a.per);
-    float square = 0.f;
-    for (uint32_t r = 0; r < rows; ++r) {
-      const float count = (float)((taken - (int)r + (int)rows - 1) / (int)rows);
-      for (int c = lane; c < a.per; c += 8) {
-        const float d = lds[r * width + g * a.per + c] - center;
-        square += lds[(rows + r) * width + g * a.per + c] + count * d * d;
+  // `lanes` neighbouring threads a group: its mean, then the squares about it.
+  int lanes = 64;
+  while (lanes > 1 && lanes * a.groups > (int)blockDim.x) lanes >>= 1;
+  const int together = blockDim.x / lanes, lane = threadIdx.x & (lanes - 1), taken = p1 - p0, values = rows * a.per;
+  // (the pixels of a row of threads: base, and one more of the first; where a lane begins, and its step)
+  const int more = taken % (int)rows, r0 = lane / a.per, c0 = lane - r0 * a.per, dr = lanes / a.per, dc = lanes - dr * a.per;
+  const float base = (float)(taken / (int)rows);
+  for (int g = threadIdx.x / lanes; g < a.groups && (int)threadIdx.x < together * lanes; g += together) {
+    auto sum_of = [&](auto term) {
+      float sum = 0.f;
+      int r = r0, c = c0;
+#pragma unroll 4
+      for (int e = lane; e < values; e += lanes) {
+        sum += term(base + (r < more ? 1.f : 0.f), r * width + g * a.per + c);
+        r += dr;
+        c += dc;
+        if (c >= a.per) c -= a.per, ++r;
       }
-    }
-#pragma unroll
-    for (int m = 1; m < 8; m <<= 1) square += __shfl_xor(square, m, 64);
+      for (int m = 1; m < lanes; m <<= 1) sum += __shfl_xor(sum, m, 64);
+      return sum;
+    };
+    const float center = sum_of([&](float count, int at) { return count * lds[at]; }) / ((float)taken * (float)a.per);
+    const float square = sum_of([&](float count, int at) {
+      const float d = lds[at] - center;
+      return lds[rows * width + at] + count * d * d;
+    });
     if (lane == 0) a.sums[((int64_t)blockIdx.y * a.chunks + blockIdx.x) * a.groups + g] = {center, square};
   }
 }
 
 // ------------------------------------------------------------------ the values of a chunk
-template <int DT, bool EDGE, bool STREAM>
-__global__ void group_norm_kernel(Args a) {
-  typedef typename Type<DT>::T T;
-  extern __shared__ float lds[];  // [2][groups] mean and 1 / deviation
-  const int tx = threadIdx.x % a.vectors, ty = threadIdx.x / a.vectors;
-  int lanes = 64;  // that share a group
-  while (lanes > 1 && lanes * a.groups > (int)blockDim.x) lanes >>= 1;
-  const int together = blockDim.x / lanes, lane = threadIdx.x & (lanes - 1);
+// The element's means and 1 / deviations of all groups: neighbouring threads take neighbouring groups, whose sums lie
+// together, `lanes` threads a group its chunks in turn, eight loads at a time; what they have meets in LDS.
+__device__ __forceinline__ void join_chunks(const Args& a, float* lds) {
+  __shared__ Sums part[MAX_THREADS];
+  int lanes = 1;
+  while (2 * lanes * a.groups <= (int)blockDim.x && lanes < (int)a.chunks) lanes *= 2;
   const float2* const sums = a.sums + (int64_t)blockIdx.y * a.chunks * a.groups;
-  for (int g = threadIdx.x / lanes; g < a.groups && (int)threadIdx.x < together * lanes; g += together) {
+  const float each = (float)a.chunk * (float)a.per;
+  for (int g0 = 0; g0 < a.groups; g0 += blockDim.x) {
+    const int here = min(a.groups - g0, (int)blockDim.x), lane = threadIdx.x / here, g = g0 + threadIdx.x - lane * here;
     Sums all = {0.f, 0.f, 0.f};
-    for (uint32_t c = lane; c < a.chunks; c += lanes) {
-      const float2 s = sums[(int64_t)c * a.groups + g];
-      all = join(all, {(float)(min(a.pixels, (c + 1) * a.chunk) - c * a.chunk) * (float)a.per, s.x, s.y});
+    if (lane < lanes) {
+      for (uint32_t c = lane; c < a.chunks; c += 8 * lanes) {
+        float2 s[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = sums[(int64_t)min(c + i * lanes, a.chunks - 1) * a.groups + g];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t at = c + i * lanes;
+          const float n = at >= a.chunks ? 0.f : at + 1 < a.chunks ? each : (float)(a.pixels - at * a.chunk) * (float)a.per;
+          all = join(all, {n, s[i].x, at < a.chunks ? s[i].y : 0.f});
+        }
+      }
     }
-    for (int m = 1; m < lanes; m <<= 1)
-      all = join(all, {__shfl_xor(all.n, m, 64), __shfl_xor(all.mean, m, 64), __shfl_xor(all.squares, m, 64)});
+    for (int half = lanes / 2; half; half /= 2) {
+      if (lane >= half && lane < 2 * half) part[threadIdx.x - half * here] = all;
+      __syncthreads();
+      if (lane < half) all = join(all, part[threadIdx.x]);
+      __syncthreads();
+    }
     if (lane == 0) {
       lds[g] = all.mean;
       lds[a.groups + g] = __builtin_amdgcn_rsqf(all.squares / all.n + a.eps);
     }
   }
   __syncthreads();
-  const int c0 = tx * V, there = a.channels - c0;
-  float mean[V], scale[V], shift[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const int c = min(c0 + k, a.channels - 1), g = c / a.per;
-    mean[k] = lds[g];
-    scale[k] = lds[a.groups + g] * (a.weight ? value<DT>((const T*)a.weight + c) : 1.f);
-    shift[k] = a.bias ? value<DT>((const T*)a.bias + c) : 0.f;
-  }
+}
+
+template <int DT, int EDGE, bool STREAM>
+__global__ void group_norm_kernel(Args a) {
+  typedef typename Type<DT>::T T;
+  extern __shared__ float lds[];  // [2][groups] mean and 1 / deviation
+  const int tx = threadIdx.x % a.vectors, ty = threadIdx.x / a.vectors, there = a.channels;
+  const int c0 = EDGE == SHARED ? min(tx * V, a.channels - V) : tx * V;
   const T* const x = (const T*)a.x + blockIdx.y * a.x_b + c0;
   T* const out = (T*)a.out + blockIdx.y * a.out_b + c0;
   const uint32_t p0 = blockIdx.x * a.chunk, p1 = min(a.pixels, p0 + a.chunk), rows = a.rows;
-  constexpr int AT_ONCE = 4;
-  // (backwards: the thread's last pixels first)
-  for (int i = ((int)(p1 - p0) - ty + (int)rows - 1) / (int)rows - 1; i >= 0; i -= AT_ONCE) {
-    Raw<DT> raw[AT_ONCE];
+  // What needs no statistics is asked for before them.  (Backwards: the thread's last pixels first.)
+  constexpr int AT_ONCE = DT == HB_DTYPE_F32 ? 4 : 8;
+  Raw<DT> raw[AT_ONCE];
+  auto ask = [&](int i) {
 #pragma unroll
-    for (int r = 0; r < AT_ONCE; ++r) raw[r] = load<DT, EDGE, STREAM>(x + (int64_t)(p0 + ty + max(i - r, 0) * rows) * a.x_n, there);
+    for (int r = 0; r < AT_ONCE; ++r) raw[r] = load<DT, EDGE, STREAM>(x + (int64_t)(p0 + min(ty + (uint32_t)max(i - r, 0) * rows, p1 - p0 - 1)) * a.x_n, there);
+  };
+  int i = ((int)(p1 - p0) - ty + (int)rows - 1) / (int)rows - 1;
+  ask(i);
+  float mean[V], scale[V], shift[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) scale[k] = 1.f, shift[k] = 0.f;
+  if (a.weight) unpack(load<DT, EDGE, false>((const T*)a.weight + c0, there), scale);
+  if (a.bias) unpack(load<DT, EDGE, false>((const T*)a.bias + c0, there), shift);
+  join_chunks(a, lds);
+  int g = c0 / a.per, c = c0 - g * a.per;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    mean[k] = lds[g];
+    scale[k] *= lds[a.groups + g];
+    if (++c == a.per && g + 1 < a.groups) c = 0, ++g;
+  }
+  while (i >= 0) {
+    float v[AT_ONCE][V];
+#pragma unroll
+    for (int r = 0; r < AT_ONCE; ++r) unpack(raw[r], v[r]);
+    const int done = i;
+    i -= AT_ONCE;
+    if (i >= 0) ask(i);
 #pragma unroll
     for (int r = 0; r < AT_ONCE; ++r) {
-      if (i < r) break;
-      float v[V];
-      unpack(raw[r], v);
+      if (done < r) break;
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] = activate((v[k] - mean[k]) * scale[k] + shift[k], a.silu);
-      store<DT, EDGE, STREAM>(out + (int64_t)(p0 + ty + (i - r) * rows) * a.out_n, v, there);
+      for (int k = 0; k < V; ++k) v[r][k] = activate((v[r][k] - mean[k]) * scale[k] + shift[k], a.silu);
+      store<DT, EDGE, STREAM>(out + (int64_t)(p0 + ty + (done - r) * rows) * a.out_n, v[r], tx * V - c0, there);
     }
   }
 }
 
 // ------------------------------------------------------------------ groups that fit a workgroup
-// W channels a load, up to UNITS loads a thread.
-constexpr int UNITS = 8, FEW_THREADS = 1024;
+// W channels a load, up to UNITS loads a thread.  A few loads' and two barriers' time: 1 x 256 pixels x 512 channels, 32 groups
+// 4.8 us.
+constexpr int UNITS = 2, FEW_THREADS = 1024;
 
 template <int DT, int W>
 __global__ __launch_bounds__(FEW_THREADS) void group_norm_few_kernel(Args a) {
   typedef typename Type<DT>::T T;
   __shared__ float parts[2][FEW_THREADS / 64];
-  const int g = blockIdx.x, wave = threadIdx.x >> 6, waves = (blockDim.x + 63) >> 6;
+  const int g = blockIdx.x, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const uint32_t across = a.per / W, all = a.pixels * across;  // loads of a pixel, and of the group
   const T* const x = (const T*)a.x + blockIdx.y * a.x_b + g * a.per;
   T* const out = (T*)a.out + blockIdx.y * a.out_b + g * a.per;
   typedef T Unit __attribute__((ext_vector_type(W), aligned(sizeof(T))));
-  float v[UNITS][W];
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < UNITS; ++i) {
-    const uint32_t at = i * blockDim.x + threadIdx.x, p = at / across, c = (at - p * across) * W;
-    Unit u = {};
-    if (at < all) u = *(const Unit*)(x + (int64_t)p * a.x_n + c);
+  auto widen = [](const Unit& u, float (&v)[W]) {
 #pragma unroll
     for (int k = 0; k < W; ++k) {
-      if constexpr (DT == HB_DTYPE_F32) v[i][k] = u[k];
-      else v[i][k] = to_f<DT == HB_DTYPE_F16>(u[k]);
-      sum += v[i][k];  // (zeros past the group's values)
+      const T t = u[k];
+      if constexpr (DT == HB_DTYPE_F32) v[k] = t;
+      else v[k] = to_f<DT == HB_DTYPE_F16>(t);
     }
+  };
+  Unit raw[UNITS] = {}, weight[UNITS], bias[UNITS];
+  uint32_t pixel[UNITS], channel[UNITS];
+  bool there[UNITS];
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const uint32_t at = i * blockDim.x + threadIdx.x;
+    there[i] = at < all;
+    pixel[i] = at / across;
+    channel[i] = (at - pixel[i] * across) * W;
+    if (there[i]) raw[i] = *(const Unit*)(x + (int64_t)pixel[i] * a.x_n + channel[i]);
+    if (a.weight) weight[i] = *(const Unit*)((const T*)a.weight + g * a.per + channel[i]);
+    if (a.bias) bias[i] = *(const Unit*)((const T*)a.bias + g * a.per + channel[i]);
   }
   auto total = [&](float s, float (&part)[FEW_THREADS / 64]) {
 #pragma unroll
@@ -299,29 +350,33 @@ __global__ __launch_bounds__(FEW_THREADS) void group_norm_few_kernel(Args a) {
     for (int w = 0; w < waves; ++w) s += part[w];
     return s;
   };
+  float v[UNITS][W], sum = 0.f, squares = 0.f;
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    widen(raw[i], v[i]);
+#pragma unroll
+    for (int k = 0; k < W; ++k) sum += v[i][k];  // (zeros past the group's values)
+  }
   const float n = (float)all * W, mean = total(sum, parts[0]) / n;
-  float squares = 0.f;
 #pragma unroll
   for (int i = 0; i < UNITS; ++i)
-    if (i * blockDim.x + threadIdx.x < all) {
 #pragma unroll
-      for (int k = 0; k < W; ++k) squares += (v[i][k] - mean) * (v[i][k] - mean);
-    }
+    for (int k = 0; k < W; ++k) squares += there[i] ? (v[i][k] - mean) * (v[i][k] - mean) : 0.f;
   const float scale = __builtin_amdgcn_rsqf(total(squares, parts[1]) / n + a.eps);
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
-    const uint32_t at = i * blockDim.x + threadIdx.x, p = at / across, c = (at - p * across) * W;
-    if (at >= all) break;
+    if (!there[i]) continue;
+    float w[W], b[W];
+    widen(weight[i], w);
+    widen(bias[i], b);
     Unit u;
 #pragma unroll
     for (int k = 0; k < W; ++k) {
-      const float w = a.weight ? value<DT>((const T*)a.weight + g * a.per + c + k) : 1.f;
-      const float b = a.bias ? value<DT>((const T*)a.bias + g * a.per + c + k) : 0.f;
-      const float y = activate((v[i][k] - mean) * (scale * w) + b, a.silu);
+      const float y = activate((v[i][k] - mean) * (a.weight ? scale * w[k] : scale) + (a.bias ? b[k] : 0.f), a.silu);
       if constexpr (DT == HB_DTYPE_F32) u[k] = y;
       else u[k] = from_f<DT == HB_DTYPE_F16>(y);
     }
-    *(Unit*)(out + (int64_t)p * a.out_n + c) = u;
+    *(Unit*)(out + (int64_t)pixel[i] * a.out_n + channel[i]) = u;
   }
 }
 
@@ -331,18 +386,30 @@ int64_t size_of(int dtype) { return dtype == HB_DTYPE_F32 ? 4 : 2; }
 // Channels of a load of group_norm_few_kernel: the most that divide a group's.
 int few_width(int per) { return per % 8 == 0 ? 8 : per % 4 == 0 ? 4 : per % 2 == 0 ? 2 : 1; }
 
-// Whether a workgroup holds a group (and the launch all of them: a grid holds fewer than 2^32 threads).
+// Whether a workgroup holds a group (and the launch all of them: a grid holds fewer than 2^32 threads).  One launch and
+// two, 512 channels in 32 groups, us: 256 pixels 7.4, 10.6; 1024 8.7, 10.6; with groups twice and four times as large
+// as a workgroup holds now 13.7, 10.9 and 30.4, 11.5.
 bool few(int64_t batch, int64_t pixels, int groups, int per) {
-  return pixels * (per / few_width(per)) <= (int64_t)UNITS * FEW_THREADS / 4 && batch * groups < (1ll << 32) / FEW_THREADS;
+  return pixels * (per / few_width(per)) <= (int64_t)UNITS * FEW_THREADS && batch * groups < (1ll << 32) / FEW_THREADS;
 }
 
+// Chunks of at least 16 KB, up to as many as there are CUs, and twice as many of twice the threads past 512 MB: by the
+// element alone, so that an image's result is the same in every batch.
+// us of 256, 512 chunks of 256 threads, and of 512 threads: 65536 pixels x 512 channels bf16 45.2, 47.3, 47.4, 47.0; 262144 x
+// 256 fp32 142, 146, 150, 159, bf16 85, 88, 81, 87; 2048 x 2048 x 128 bf16 578, 550, 543, 534.  Of 16384 x 512 18.2, 20.4,
+// 17.0, 23.8; 128 chunks 22.4: every workgroup of the second launch joins all chunks of its element.
 struct Chunks {
   int64_t pixels, count;
+  int threads;
 };
 Chunks chunks_of(int64_t batch, int64_t pixels, int channels, int dtype) {
-  const int64_t row = channels * size_of(dtype), most = std::max<int64_t>(1, MAX_CHUNKS / batch);
-  const int64_t count = std::clamp<int64_t>(pixels * row / CHUNK_BYTES, 1, most), each = (pixels + count - 1) / count;
-  return {each, (pixels + each - 1) / each};
+  const int64_t row = channels * size_of(dtype);
+  const int large = pixels * row > LARGE_BYTES ? 2 : 1;
+  // (a grid holds fewer than 2^32 threads, of up to 1024 a workgroup)
+  const int64_t most = std::min<int64_t>(256 * large, std::max<int64_t>(1, ((1ll << 32) - 1) / MAX_THREADS / batch));
+  const int64_t count = std::clamp<int64_t>(pixels * row / CHUNK_BYTES, 1, most);
+  const int64_t each = (pixels + count - 1) / count;
+  return {each, (pixels + each - 1) / each, THREADS * large};
 }
 
 template <int DT, int W>
@@ -354,7 +421,7 @@ int launch_few(const Args& a, int32_t batch, hipStream_t st) {
   return HB_OK;
 }
 
-template <int DT, bool EDGE>
+template <int DT, int EDGE>
 int launch_chunks(const Args& a, int32_t batch, bool stream_values, hipStream_t st) {
   const dim3 grid(a.chunks, batch), block(a.vectors * a.rows);
   hipLaunchKernelGGL((group_norm_sums_kernel<DT, EDGE>), grid, block, block.x * V * 2 * sizeof(float), st, a);
@@ -377,7 +444,8 @@ int launch(Args& a, int32_t batch, hipStream_t st) {
     }
   }
   const bool stream_values = 2 * (int64_t)batch * a.pixels * a.channels * size_of(DT) > CACHE_BYTES;
-  return a.channels % V ? launch_chunks<DT, true>(a, batch, stream_values, st) : launch_chunks<DT, false>(a, batch, stream_values, st);
+  if (a.channels < V) return launch_chunks<DT, SHORT>(a, batch, stream_values, st);
+  return a.channels % V ? launch_chunks<DT, SHARED>(a, batch, stream_values, st) : launch_chunks<DT, EVEN>(a, batch, stream_values, st);
 }
 
 }  // namespace
@@ -421,7 +489,6 @@ extern "C" int hb_group_norm(int32_t batch, int64_t pixels, int32_t channels, in
   a.eps = eps;
   a.silu = silu;
   a.vectors = (channels + V - 1) / V;
-  a.rows = std::max(1, THREADS / a.vectors);
   const int64_t need = hb_group_norm_workspace_bytes(batch, pixels, channels, groups, dtype);
   if (need) {
     HB_REQUIRE(workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= need, "the workspace must hold %lld bytes, 8-byte aligned", (long long)need);
@@ -429,6 +496,7 @@ extern "C" int hb_group_norm(int32_t batch, int64_t pixels, int32_t channels, in
     a.sums = (float2*)workspace;
     a.chunk = (uint32_t)c.pixels;
     a.chunks = (uint32_t)c.count;
+    a.rows = std::max(1, c.threads / a.vectors);
   }
   switch (dtype) {
     case HB_DTYPE_BF16: return launch<HB_DTYPE_BF16>(a, batch, stream);
