@@ -34,7 +34,6 @@ struct Set {
   uint16_t* out;
   int64_t x_b, x_n, w_n, r_b, r_n, g_b, out_b, out_n;  // strides of a batch element and a row
   uint32_t rows, tokens;     // rows of a batch element, and of all
-  uint32_t start;            // rows of the set before these (which another launch takes)
 };
 
 struct Args {
@@ -44,6 +43,8 @@ struct Args {
   uint32_t channel_tiles;             // tiles along the channels
   int32_t act;
   int32_t vectors;                    // every output row takes 16-byte stores
+  int32_t splits, stages_each;        // parts of the features, and stages of each
+  float* sums;                        // [splits, tokens of both sets, columns rounded up to 8], with several parts
 };
 
 template <bool F16>
@@ -105,8 +106,8 @@ struct Place {
   uint32_t b, n;
 };
 __device__ __forceinline__ Place place_of(const Set& s, uint32_t at) {
-  uint32_t n = s.start + min(at, s.tokens - 1), b = 0;
-  if (s.start + s.tokens > s.rows) b = n / s.rows, n -= b * s.rows;  // (one batch element: no division)
+  uint32_t n = min(at, s.tokens - 1), b = 0;
+  if (s.tokens > s.rows) b = n / s.rows, n -= b * s.rows;  // (one batch element: no division)
   return {b, n};
 }
 
@@ -178,6 +179,10 @@ __device__ __forceinline__ void finish8(const Args& a, const Set& s, float (&v)[
   if (at < s.tokens) store8(a, e.out, c, pack8<F16>(v));
 }
 
+// Rows and columns of the sums of a layer's parts.
+__device__ __forceinline__ uint32_t all_tokens(const Args& a) { return a.set[0].tokens + a.set[1].tokens; }
+__device__ __forceinline__ uint32_t padded_columns(const Args& a) { return (uint32_t)(a.columns + 7) & ~7u; }
+
 // The epilogue's bias of a tile's channels, in LDS.
 template <bool F16, int TC>
 __device__ __forceinline__ void load_bias(const Args& a, const Set& s, int c0, float (&bias)[TC]) {
@@ -191,6 +196,9 @@ struct RowEnd {
   int full, beyond;  // whole stages, and what the stage after them adds to this lane's offset
   __device__ RowEnd(int features, int chunk)
       : full(features >> 6), beyond(chunk * 8 < (features & 63) ? 0 : (int)0x80000000) {}
+  __device__ void stop(int stage) {  // nothing from this stage on
+    if (stage <= full) full = stage, beyond = (int)0x80000000;
+  }
   __device__ int past(int stage) const {
     return stage < full ? 0 : stage == full ? beyond : (int)0x80000000;
   }
@@ -491,12 +499,13 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a)
 }
 
 // ------------------------------------------------------------------ fewer rows
-// TC channels x TT tokens a workgroup, in tiles so small that most CUs have one.  What is on its way to a CU
-// bounds it, so the operands go to LDS by direct loads, into a ring of R stages of 64 features, the loads spread over
-// the products.  A stage's features are in four parts of 16, a wave each in the smallest tiles, or two waves that
-// share the tokens (of 32 tokens: the channels), whose epilogue is shorter.  The sums meet in LDS, and a thread
-// finishes eight channels of a token: neighbouring lanes read and write whole lines.  Rows past the operands' ends are
-// zeros that nothing reads.
+// TC channels x TT tokens a workgroup, in tiles so small that most CUs have one.  What reaches a CU bounds it, some 58
+// bytes a ns in every size of tile; so the operands go to LDS by direct loads, into a ring of R stages of 64 features,
+// the loads spread over the products, and where the tiles are fewer than the CUs the features are split among
+// workgroups, whose sums meet in memory (join_kernel).  A stage's features are in four parts of 16, a wave each in the
+// smallest tiles, or two waves that share the tokens (of 32 tokens: the channels), whose epilogue is shorter.  The sums
+// meet in LDS, and a thread finishes eight channels of a token: neighbouring lanes read and write whole lines.  Rows
+// past the operands' ends are zeros that nothing reads.
 template <int TC, int TT, int WAVES>
 struct Ring {
   static constexpr int STAGE = (TC + TT) * 128, GROUPS = STAGE / 1024, LOADS = (GROUPS + WAVES - 1) / WAVES;
@@ -547,8 +556,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_tile_kernel(Args
                       : (int)0x80000000;
     }
   }
-  const int stages = (a.features + 63) / 64;
-  const RowEnd ends(a.features, chunk);
+  const int first = blockIdx.y * a.stages_each, last = min(first + a.stages_each, (a.features + 63) / 64);
+  RowEnd ends(a.features, chunk);
+  ends.stop(last);
   const bool all = WAVES * (LOADS - 1) + wave < F::GROUPS;  // (the last loads are not every wave's)
   auto load = [&](int8_t* dst, int stage, int j, int past) {
     const int group = WAVES * j + wave;
@@ -572,7 +582,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_tile_kernel(Args
   f32x16 acc[TF][CF] = {};
   // Stage n's operands are in w, x, or on their way; stage n + 1 is in LDS.  The stage whose reads ended in
   // the last step takes n + R - 1.  Before the barrier stage n + 2 is there.
-  int n = 0;
+  int n = first;
   auto step = [&](auto index) {
     constexpr int I = decltype(index)::value;
     int8_t* const free = ring(std::integral_constant<int, I + R - 1>());
@@ -593,7 +603,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_tile_kernel(Args
     fetch(ring(std::integral_constant<int, I + 1>()), ~I & 1);
     arrivals();
     barrier();
-    return ++n == stages;
+    return ++n == last;
   };
   // (Zeros into the last stage, so that the compiler, which tracks what is on its way to which array, has met them
   // all before the loop: otherwise it waits for everything each time around.)
@@ -601,7 +611,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_tile_kernel(Args
   auto begin_stage = [&](auto index) {
     constexpr int I = decltype(index)::value;
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) load(ring(index), I, j, ends.past(I));
+    for (int j = 0; j < LOADS; ++j) load(ring(index), first + I, j, ends.past(first + I));
   };
   begin_all(begin_stage, std::make_integer_sequence<int, R - 1>());
   arrivals();
@@ -637,17 +647,51 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_tile_kernel(Args
     const int h = TT > 32 ? token / TW : c / CW;
     const uint32_t to = t.t0 + token;
     if (to >= s.tokens || t.c0 + c >= a.columns) continue;
-    const Epilogue more = ask(a, s, to, t.c0 + c);
-    float v[8];
+    f32x4 sum[2];
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const int at = unit(TT > 32 ? token % TW : token, (TT > 32 ? c : c % CW) + 4 * g);
-      const f32x4 sum = *(const f32x4*)(box(0, h) + at) + *(const f32x4*)(box(1, h) + at) + *(const f32x4*)(bias + c + 4 * g);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[4 * g + k] = sum[k];
+      sum[g] = *(const f32x4*)(box(0, h) + at) + *(const f32x4*)(box(1, h) + at);
     }
+    if (a.splits > 1) {
+      f32x4* const parts = (f32x4*)(a.sums + ((int64_t)blockIdx.y * all_tokens(a) + (t.set ? a.set[0].tokens : 0) + to) * padded_columns(a) + t.c0 + c);
+      parts[0] = sum[0];
+      parts[1] = sum[1];
+      continue;
+    }
+    const Epilogue more = ask(a, s, to, t.c0 + c);
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = sum[k >> 2][k & 3] + bias[c + k];
     finish8<F16>(a, s, v, more, to, t.c0 + c);
   }
+}
+
+// The sums of a layer's parts, in their order, and the epilogue: a thread has eight channels of a token.
+template <bool F16>
+__global__ __launch_bounds__(256) void join_kernel(Args a) {
+  const uint32_t across = padded_columns(a) / 8, tokens = all_tokens(a);
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, row = i / across;
+  if (row >= tokens) return;
+  const int c = (int)(i - row * across) * 8;
+  const int set = row >= a.set[0].tokens;
+  const Set& s = a.set[set];
+  const uint32_t to = row - (set ? a.set[0].tokens : 0);
+  const Epilogue more = ask(a, s, to, c);
+  const u32x4 bias = s.bias ? load8(s.bias + c, c, a.columns) : u32x4{};
+  const f32x4* from = (const f32x4*)(a.sums + (int64_t)row * padded_columns(a) + c);
+  const int64_t step = (int64_t)tokens * padded_columns(a) / 4;
+  f32x4 sum[2] = {};
+#pragma unroll 4
+  for (int k = 0; k < a.splits; ++k, from += step) {
+    sum[0] += from[0];
+    sum[1] += from[1];
+  }
+  float v[8];
+  unpack8<F16>(bias, v);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] += sum[k >> 2][k & 3];
+  finish8<F16>(a, s, v, more, to, c);
 }
 
 // ------------------------------------------------------------------ a few rows
@@ -734,16 +778,23 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
 }
 
 // ------------------------------------------------------------------ launches
-enum Kernel { T64x32, T32x64, T64x64, T96x64, T96x128, WIDE256, KERNELS };
+enum Kernel { T64x32, T32x64, T64x64, T96x64, T96x128, T128x128, WIDE256, KERNELS };
 
+// A kernel's tile and what its time is made of, in us: the launch, a round of 256 workgroups, a round's stage of 64
+// features, what a stage takes longer when all CUs are at it, and each megabyte of rows and weight.  Fitted to 2140
+// times of 150 sizes, which they meet to 14% (one sigma).
 struct Shape {
   int tc, tt;
-  float launch, round, stage, full;
+  float launch, round, stage, full, megabyte;
 };
 constexpr Shape SHAPES[KERNELS] = {
-    {64, 32, 2.97f, 1.34f, 0.102f, 0.065f},  {32, 64, 1.81f, 2.61f, 0.096f, 0.088f},   {64, 64, 1.74f, 2.84f, 0.127f, 0.134f},
-    {96, 64, 1.67f, 3.78f, 0.189f, 0.133f},  {96, 128, 0.95f, 5.82f, 0.258f, 0.234f}, {256, 256, 5.9f, 3.0f, 0.99f, 0.70f},
+    {64, 32, 3.9f, 1.3f, 0.133f, 0.010f, 0.06f},  {32, 64, 2.35f, 2.5f, 0.132f, 0.035f, 0.06f},
+    {64, 64, 2.4f, 2.5f, 0.161f, 0.087f, 0.06f},  {96, 64, 1.7f, 3.7f, 0.218f, 0.074f, 0.06f},
+    {96, 128, 2.2f, 4.75f, 0.314f, 0.139f, 0.06f}, {128, 128, 3.9f, 4.4f, 0.333f, 0.236f, 0.06f},
+    {256, 256, 0.9f, 9.f, 0.97f, 0.270f, 0.04f},
 };
+constexpr float WIDE_ANY_ROUND = 24.f;  // (tiles that are not whole)
+constexpr float JOIN = 3.f, JOIN_BYTE = 4e-7f;
 
 // Tiles of TC x TT of both sets.
 int64_t tiles_of(const Args& a, int count, int tc, int tt) {
@@ -753,57 +804,84 @@ int64_t tiles_of(const Args& a, int count, int tc, int tt) {
   return tiles;
 }
 
-// What a kernel takes for the sets, in us.
-float estimate(const Args& a, int count, Kernel k) {
-  const Shape& s = SHAPES[k];
-  const float rounds = (float)tiles_of(a, count, s.tc, s.tt) / 256.f, whole = std::floor(rounds), rest = rounds - whole;
-  const float stages = (float)((a.features + 63) / 64);
-  return s.launch + whole * (s.round + stages * (s.stage + s.full)) +
-         (rest > 0.f ? s.round + stages * (s.stage + s.full * rest * rest) : 0.f);
-}
-
 struct Choice {
   Kernel kernel;
-  float us;
+  int splits;
 };
 
-Choice choose(const Args& a, int count) {
-  Choice best = {WIDE256, estimate(a, count, WIDE256)};
-  for (int i = 0; i < WIDE256; ++i) {
-    const Kernel k = (Kernel)i;
-    if (tiles_of(a, count, SHAPES[k].tc, SHAPES[k].tt) >= (1 << 21)) continue;  // (a grid holds fewer than 2^32 threads)
-    const float us = estimate(a, count, k);
-    if (us < best.us) best = {k, us};
-  }
-  return best;
+int64_t sums_bytes(const Args& a, int splits) {
+  return splits > 1 ? (int64_t)splits * ((int64_t)a.set[0].tokens + a.set[1].tokens) * ((a.columns + 7) & ~7) * 4 : 0;
+}
+
+// Whether all of the wide kernel's tiles are whole, of one batch element and stored in 16 bytes.
+bool whole_tiles(const Args& a, int count) {
+  bool whole = a.vectors && a.columns % WIDE == 0;
+  for (int i = 0; i < count; ++i) whole &= a.set[i].rows % WIDE == 0;
+  return whole;
 }
 
 // The wide kernel's epilogue for these sets.
 Mode mode_of(const Args& a, int count) {
   const bool residual = a.set[0].residual, gate = a.set[0].gate;
-  bool whole = a.vectors && a.columns % WIDE == 0;
-  for (int i = 0; i < count; ++i)
-    whole &= a.set[i].rows % WIDE == 0 && residual == !!a.set[i].residual && gate == !!a.set[i].gate;
+  bool whole = whole_tiles(a, count);
+  for (int i = 0; i < count; ++i) whole &= residual == !!a.set[i].residual && gate == !!a.set[i].gate;
   if (!whole || (a.act != NONE && residual)) return ANY;
   return a.act == GELU ? ACT_GELU : a.act == SILU ? ACT_SILU : gate ? GATED : residual ? RESIDUAL : PLAIN;
 }
 
+// What a kernel takes for the sets, in us (whatever the activation, so that the workspace is known without it).
+float estimate(const Args& a, int count, Kernel k, int splits) {
+  const Shape& s = SHAPES[k];
+  const float rounds = (float)(tiles_of(a, count, s.tc, s.tt) * splits) / 256.f, whole = std::floor(rounds), rest = rounds - whole;
+  const float stages = (float)(((a.features + 63) / 64 + splits - 1) / splits);
+  const float round = k == WIDE256 && !whole_tiles(a, count) ? WIDE_ANY_ROUND : s.round;
+  const float rows = (float)a.set[0].tokens + (float)a.set[1].tokens + (float)count * (float)a.columns;
+  return s.launch + whole * (round + stages * (s.stage + s.full)) +
+         (rest > 0.f ? round + stages * (s.stage + s.full * rest * rest) : 0.f) + s.megabyte * 2e-6f * rows * (float)a.features;
+}
+
+// The kernel, and the parts that it takes the features in, of the least estimate.  Parts pay where few tiles leave CUs
+// idle over many features; they are tried while all their workgroups fit the card at once with six stages each or
+// more, and taken where they promise 5% and 1 us.  Measured, one part / the parts: 126 x 13952 -> 27 33.9 / 10.3 us, 63 x 8120 -> 386
+// 27.8 / 12.1, 1283 x 10072 -> 450 48.4 / 37.4.  Over the 150
+// sizes the choice takes 1.9% more time than the best of all, and the best of one part 9.6%.
+Choice choose(const Args& a, int count) {
+  Choice best = {WIDE256, 1};
+  float least = estimate(a, count, WIDE256, 1);
+  const int stages = (a.features + 63) / 64;
+  for (int i = 0; i < WIDE256; ++i) {
+    const Kernel k = (Kernel)i;
+    const int64_t tiles = tiles_of(a, count, SHAPES[k].tc, SHAPES[k].tt);
+    if (tiles >= (1 << 21)) continue;  // (a grid holds fewer than 2^32 threads)
+    for (int splits = 1; splits <= 16; splits *= 2) {
+      if (splits > 1 && (tiles * splits > 256 || stages < 6 * splits)) break;
+      float us = estimate(a, count, k, splits);
+      if (splits > 1) us = 1.05f * (us + JOIN + JOIN_BYTE * (float)sums_bytes(a, splits)) + 1.f;
+      if (us < least) best = {k, splits}, least = us;
+    }
+  }
+  return best;
+}
+
 template <bool F16>
-int launch_kernel(Args& a, int count, Kernel kernel, hipStream_t st) {
-  const int tc = SHAPES[kernel].tc, tt = SHAPES[kernel].tt;
+int launch_kernel(Args& a, int count, const Choice& choice, hipStream_t st) {
+  const int tc = SHAPES[choice.kernel].tc, tt = SHAPES[choice.kernel].tt, stages = (a.features + 63) / 64;
   const int64_t tiles = tiles_of(a, count, tc, tt);
   HB_REQUIRE(tiles < (1ll << 30), "too many output tiles for one launch");
   a.channel_tiles = (uint32_t)((a.columns + tc - 1) / tc);
   a.tiles0 = (uint32_t)tiles_of(a, 1, tc, tt);
   a.tiles = (uint32_t)tiles;
   a.tiles_xcd = (a.tiles + 7) / 8;
-  const dim3 each(8 * a.tiles_xcd), four(256), eight(512);
-  switch (kernel) {
+  a.stages_each = (stages + choice.splits - 1) / choice.splits;
+  a.splits = (stages + a.stages_each - 1) / a.stages_each;
+  const dim3 each(8 * a.tiles_xcd, a.splits), four(256), eight(512);
+  switch (choice.kernel) {
     case T64x32: hipLaunchKernelGGL((linear_tile_kernel<F16, 64, 32, 6, 4>), each, four, 0, st, a); break;
     case T32x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 32, 64, 8, 4>), each, four, 0, st, a); break;
     case T64x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 64, 64, 8, 8>), each, eight, 0, st, a); break;
     case T96x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 96, 64, 7, 8>), each, eight, 0, st, a); break;
     case T96x128: hipLaunchKernelGGL((linear_tile_kernel<F16, 96, 128, 5, 8>), each, eight, 0, st, a); break;
+    case T128x128: hipLaunchKernelGGL((linear_tile_kernel<F16, 128, 128, 4, 8>), each, eight, 0, st, a); break;
     default: {
       const uint32_t per_xcd = std::max(1, device_cu_count() / 8);
       const dim3 grid(8 * std::min(a.tiles_xcd, per_xcd)), block(64 * WIDE_WAVES);
@@ -818,20 +896,12 @@ int launch_kernel(Args& a, int count, Kernel kernel, hipStream_t st) {
     }
   }
   HB_HIP(hipGetLastError());
-  return HB_OK;
-}
-
-template <bool F16>
-int launch(Args& a, int count, hipStream_t st) {
-  bool few = true;
-  for (int i = 0; i < count; ++i) few &= a.set[i].tokens <= FEW_ROWS;
-  if (few) {
-    a.tiles0 = (uint32_t)((a.columns + 15) / 16);
-    hipLaunchKernelGGL((linear_few_kernel<F16>), dim3(a.tiles0 * count), dim3(64 * FEW_WAVES), 0, st, a);
+  if (choice.kernel != WIDE256 && a.splits > 1) {
+    const int64_t threads = (int64_t)(a.set[0].tokens + a.set[1].tokens) * ((a.columns + 7) / 8);
+    hipLaunchKernelGGL((join_kernel<F16>), dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, st, a);
     HB_HIP(hipGetLastError());
-    return HB_OK;
   }
-  return launch_kernel<F16>(a, count, choose(a, count).kernel, st);
+  return HB_OK;
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -846,16 +916,87 @@ bool direct(const void* p, int64_t batch, int64_t rows, int64_t b, int64_t n, in
   return (batches * b + std::min<int64_t>(255, rows - 1) * n) * 2 + features * 2ll < (1ll << 31) - 4096;
 }
 
-// Whether a set's rows take the kernel of a few, which loads them as they lie.
-bool few_rows(int count, int32_t batch, const int32_t* rows) {
-  for (int i = 0; i < count; ++i)
-    if ((int64_t)batch * rows[i] > FEW_ROWS) return false;
-  return true;
-}
-
 int64_t padded_bytes(int64_t rows, int32_t features) { return rows * ((features + 63ll) / 64 * 64) * 2; }
 
 constexpr int MAX_DEPTH = 1 << 20;
+
+// A call, and what it takes: the launches and the workspace.
+struct Plan {
+  Args a;
+  PadArgs pad;
+  Choice choice;
+  bool few;
+  int copies;
+  int64_t bytes;  // of copied rows, and of all
+};
+
+int plan(Plan& p, int32_t count, int32_t batch, const int32_t* rows, int32_t columns, int32_t features, int32_t act,
+         void* const* pointers, const int64_t* strides, void* workspace) {
+  HB_REQUIRE(count == 1 || count == 2, "count must be 1 or 2");
+  HB_REQUIRE(rows && pointers && strides, "null pointer argument");
+  HB_REQUIRE(columns > 0 && columns < (1 << 28), "columns must be positive (and below 2^28)");
+  HB_REQUIRE(features > 0 && features <= MAX_DEPTH, "features must be in [1, %d] (got %d)", MAX_DEPTH, features);
+  p = {};
+  Args& a = p.a;
+  a.columns = columns;
+  a.features = features;
+  a.act = act;
+  a.vectors = 1;
+  p.few = true;
+  for (int i = 0; i < count; ++i) {
+    HB_REQUIRE(batch > 0 && rows[i] > 0 && (int64_t)batch * rows[i] < (1ll << 31), "batch and rows must be positive, with fewer than 2^31 rows in all");
+    p.few &= (int64_t)batch * rows[i] <= FEW_ROWS;
+  }
+  p.pad.features = features;
+  p.pad.padded = (features + 63) / 64 * 64;
+  for (int i = 0; i < count; ++i) {
+    void* const* q = pointers + 6 * i;
+    const int64_t* st = strides + 8 * i;
+    HB_REQUIRE(q[0] && q[1] && q[5], "null pointer argument");
+    HB_REQUIRE(!q[4] || q[3], "a gate needs its residual");
+    for (int k = 0; k < 6; ++k) HB_REQUIRE(((uintptr_t)q[k] & 1) == 0, "every pointer must be 2-byte aligned");
+    for (int k = 0; k < 8; ++k) HB_REQUIRE(st[k] >= 0, "strides must be non-negative");
+    Set& s = a.set[i];
+    s = {(const uint16_t*)q[0], (const uint16_t*)q[1], (const uint16_t*)q[2], (const uint16_t*)q[3], (const uint16_t*)q[4],
+         (uint16_t*)q[5], st[0], st[1], st[2], st[3], st[4], st[5], st[6], st[7], (uint32_t)rows[i], (uint32_t)(batch * rows[i])};
+    a.vectors &= aligned16(s.out) && s.out_b % 8 == 0 && s.out_n % 8 == 0;
+    if (p.few) continue;
+    auto copy = [&](const uint16_t*& from, int64_t& b, int64_t& n, uint32_t rows_of_one, uint32_t all) {
+      uint16_t* const to = (uint16_t*)((char*)workspace + p.bytes);
+      p.bytes += padded_bytes(all, features);
+      p.pad.m[p.copies] = {from, to, b, n, rows_of_one, all};
+      p.pad.first[p.copies + 1] = p.pad.first[p.copies] + (all + 3) / 4;
+      ++p.copies;
+      from = to;
+      n = p.pad.padded;
+      b = n * rows_of_one;
+    };
+    if (!direct(s.x, batch, rows[i], s.x_b, s.x_n, features)) copy(s.x, s.x_b, s.x_n, s.rows, s.tokens);
+    int64_t none = 0;
+    if (!direct(s.w, 1, columns, 0, s.w_n, features)) copy(s.w, none, s.w_n, (uint32_t)columns, (uint32_t)columns);
+  }
+  for (int i = p.copies; i < 4; ++i) p.pad.first[i + 1] = p.pad.first[p.copies];
+  if (p.copies && features % 8) a.features = p.pad.padded;  // (then every matrix is a copy)
+  if (!p.few) {
+    p.choice = choose(a, count);
+    a.sums = (float*)((char*)workspace + p.bytes);
+    p.bytes += sums_bytes(a, p.choice.splits);
+  }
+  return HB_OK;
+}
+
+template <bool F16>
+int launch(Plan& p, int count, hipStream_t st) {
+  if (p.copies) {
+    hipLaunchKernelGGL(pad_rows_kernel, dim3(std::min(p.pad.first[p.copies], PAD_GROUPS)), dim3(256), 0, st, p.pad);
+    HB_HIP(hipGetLastError());
+  }
+  if (!p.few) return launch_kernel<F16>(p.a, count, p.choice, st);
+  p.a.tiles0 = (uint32_t)((p.a.columns + 15) / 16);
+  hipLaunchKernelGGL((linear_few_kernel<F16>), dim3(p.a.tiles0 * count), dim3(64 * FEW_WAVES), 0, st, p.a);
+  HB_HIP(hipGetLastError());
+  return HB_OK;
+}
 
 }  // namespace
 }  // namespace hb
@@ -864,71 +1005,19 @@ using namespace hb;
 
 extern "C" int64_t hb_linear_workspace_bytes(int32_t count, int32_t batch, const int32_t* rows, int32_t columns,
                                              int32_t features, void* const* pointers, const int64_t* strides) {
-  if (!rows || !pointers || !strides || count < 1 || count > 2 || batch < 1 || columns < 1 || features < 1) return -1;
-  if (few_rows(count, batch, rows)) return 0;
-  int64_t bytes = 0;
-  for (int i = 0; i < count; ++i) {
-    if (rows[i] < 1) return -1;
-    const int64_t* st = strides + 8 * i;
-    if (!direct(pointers[6 * i], batch, rows[i], st[0], st[1], features)) bytes += padded_bytes((int64_t)batch * rows[i], features);
-    if (!direct(pointers[6 * i + 1], 1, columns, 0, st[2], features)) bytes += padded_bytes(columns, features);
-  }
-  return bytes;
+  Plan p;
+  return plan(p, count, batch, rows, columns, features, NONE, pointers, strides, nullptr) ? -1 : p.bytes;
 }
 
 extern "C" int hb_linear(int32_t count, int32_t batch, const int32_t* rows, int32_t columns, int32_t features,
                          int32_t dtype, int32_t act, void* const* pointers, const int64_t* strides, void* workspace,
                          int64_t workspace_bytes, hb_stream_t stream) {
-  HB_REQUIRE(count == 1 || count == 2, "count must be 1 or 2");
-  HB_REQUIRE(rows && pointers && strides, "null pointer argument");
-  HB_REQUIRE(columns > 0 && columns < (1 << 28), "columns must be positive (and below 2^28)");
-  HB_REQUIRE(features > 0 && features <= MAX_DEPTH, "features must be in [1, %d] (got %d)", MAX_DEPTH, features);
   HB_REQUIRE(dtype == HB_DTYPE_BF16 || dtype == HB_DTYPE_F16, "dtype must be bf16 or fp16");
   HB_REQUIRE(act >= 0 && act <= 2, "act must be 0 (none), 1 (GELU) or 2 (SiLU)");
-  Args a = {};
-  a.columns = columns;
-  a.features = features;
-  a.act = act;
-  a.vectors = 1;
-  const bool few = few_rows(count, batch, rows);
-  PadArgs pad = {};
-  pad.features = features;
-  pad.padded = (features + 63) / 64 * 64;
-  int copies = 0;
-  int64_t used = 0;
-  for (int i = 0; i < count; ++i) {
-    void* const* p = pointers + 6 * i;
-    const int64_t* st = strides + 8 * i;
-    HB_REQUIRE(batch > 0 && rows[i] > 0 && (int64_t)batch * rows[i] < (1ll << 31), "batch and rows must be positive, with fewer than 2^31 rows in all");
-    HB_REQUIRE(p[0] && p[1] && p[5], "null pointer argument");
-    HB_REQUIRE(!p[4] || p[3], "a gate needs its residual");
-    for (int k = 0; k < 6; ++k) HB_REQUIRE(((uintptr_t)p[k] & 1) == 0, "every pointer must be 2-byte aligned");
-    for (int k = 0; k < 8; ++k) HB_REQUIRE(st[k] >= 0, "strides must be non-negative");
-    Set& s = a.set[i];
-    s = {(const uint16_t*)p[0], (const uint16_t*)p[1], (const uint16_t*)p[2], (const uint16_t*)p[3], (const uint16_t*)p[4],
-         (uint16_t*)p[5], st[0], st[1], st[2], st[3], st[4], st[5], st[6], st[7], (uint32_t)rows[i], (uint32_t)(batch * rows[i]), 0};
-    a.vectors &= aligned16(s.out) && s.out_b % 8 == 0 && s.out_n % 8 == 0;
-    if (few) continue;
-    auto copy = [&](const uint16_t*& from, int64_t& b, int64_t& n, uint32_t rows_of_one, uint32_t all) {
-      uint16_t* const to = (uint16_t*)((char*)workspace + used);
-      used += padded_bytes(all, features);
-      pad.m[copies] = {from, to, b, n, rows_of_one, all};
-      pad.first[copies + 1] = pad.first[copies] + (all + 3) / 4;
-      ++copies;
-      from = to;
-      n = pad.padded;
-      b = n * rows_of_one;
-    };
-    if (!direct(s.x, batch, rows[i], s.x_b, s.x_n, features)) copy(s.x, s.x_b, s.x_n, s.rows, s.tokens);
-    int64_t none = 0;
-    if (!direct(s.w, 1, columns, 0, s.w_n, features)) copy(s.w, none, s.w_n, (uint32_t)columns, (uint32_t)columns);
-  }
-  if (copies) {
-    HB_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= used, "the workspace must hold %lld bytes, 16-byte aligned", (long long)used);
-    for (int i = copies; i < 4; ++i) pad.first[i + 1] = pad.first[copies];
-    if (features % 8) a.features = pad.padded;  // (then every matrix is a copy)
-    hipLaunchKernelGGL(pad_rows_kernel, dim3(std::min(pad.first[copies], PAD_GROUPS)), dim3(256), 0, stream, pad);
-    HB_HIP(hipGetLastError());
-  }
-  return dtype == HB_DTYPE_F16 ? launch<true>(a, count, stream) : launch<false>(a, count, stream);
+  Plan p;
+  const int rc = plan(p, count, batch, rows, columns, features, act, pointers, strides, workspace);
+  if (rc) return rc;
+  HB_REQUIRE(!p.bytes || (workspace && aligned16(workspace) && workspace_bytes >= p.bytes),
+             "the workspace must hold %lld bytes, 16-byte aligned", (long long)p.bytes);
+  return dtype == HB_DTYPE_F16 ? launch<true>(p, count, stream) : launch<false>(p, count, stream);
 }

@@ -39,7 +39,7 @@ SIZES = [
     (1, 1, 1), (1, 8, 16), (1, 7, 5), (3, 127, 33), (5, 129, 16), (16, 1024, 100), (16, 3, 1000), (1, 5000, 24), (2, 100, 4097),
     (17, 1, 1), (17, 64, 32), (33, 65, 31), (100, 200, 64), (40, 1000, 3000), (77, 320, 1000), (130, 72, 129), (256, 512, 96),
     (500, 136, 1500), (640, 640, 640), (1000, 1000, 1001), (1025, 64, 2049), (300, 4096, 300), (512, 2048, 96),
-    (4096, 64, 2048), (4095, 72, 4097), (5000, 8, 4000), (4096, 1024, 4096), (2500, 130, 8000),
+    (2048, 640, 2048), (1000, 1096, 4001), (4096, 64, 2048), (4095, 72, 4097), (5000, 8, 4000), (4096, 1024, 4096), (2500, 130, 8000),
 ]
 
 
@@ -82,6 +82,82 @@ def test_long_sums():
         got = linear(x, **layer)
         exact, _ = L.linear(x, **layer)
         assert L.relative(got, exact) <= torch.finfo(BF16).eps / 2
+
+
+# few tiles over many features, which several workgroups share
+PARTS = [(126, 13952, 27), (383, 5200, 5024), (127, 8104, 5270), (17, 1543, 16), (20, 3001, 100), (100, 12345, 300), (1000, 8192, 520)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, HALF])
+@pytest.mark.parametrize("rows, K, N", PARTS)
+def test_features_in_parts(rows, K, N, dtype):
+    x, layer = _normal(rows, K, dtype=dtype), _layer(K, N, dtype)
+    _check(linear(x, **layer), x=x, **layer)
+
+
+@pytest.mark.parametrize("act, bias, more", EPILOGUES)
+def test_epilogues_of_parts(act, bias, more):
+    batch, rows, K, N = 3, 23, 4096, 203
+    x, layer = _normal(batch, rows, K), _layer(K, N, bias=bias)
+    if more:
+        layer["residual"] = _normal(batch, rows, N, seed=5)
+    if more == "gate":
+        layer["gate"] = _normal(batch, N, std=0.5, seed=6)
+    _check(linear(x, act=act, **layer), act=act, x=x, **layer)
+
+
+@pytest.mark.parametrize("text, image", [(1, 30), (30, 1), (77, 100), (0, 40)])
+def test_pairs_in_parts(text, image):
+    sets = []
+    for i, rows in enumerate((text, image)):
+        s = dict(x=_normal(2, rows, 6000, seed=i), **_layer(6000, 200, seed=10 * i))
+        if i:
+            s |= dict(residual=_normal(2, rows, 200, seed=31), gate=_normal(2, 200, seed=41))
+        sets.append(s)
+    for out, s in zip(linear_pair(*sets), sets):
+        if s["x"].numel():
+            _check(out, **s)
+
+
+def test_parts_into_a_wider_buffer_and_in_place():
+    x, layer, gate = _normal(2, 40, 8000), _layer(8000, 93), _normal(2, 93, seed=3)
+    held = _normal(2, 44, 200, seed=9)
+    before = held.clone()
+    out = held[:, 2:42, 11:104]
+    linear(x, **layer, residual=out, gate=gate, out=out)
+    _check(out, x=x, **layer, residual=before[:, 2:42, 11:104], gate=gate)
+    out.copy_(before[:, 2:42, 11:104])
+    assert torch.equal(held, before)
+
+
+def test_parts_on_two_streams_and_in_a_graph():
+    """Calls in flight together have workspaces of their own, and one input's are the same again."""
+    x, layer = [_normal(60, 9000, seed=i) for i in range(4)], _layer(9000, 100)
+    want = [linear(v, **layer) for v in x]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None] * 4
+    for i in range(4):
+        with torch.cuda.stream(streams[i % 2]):
+            got[i] = linear(x[i], **layer)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, held = [], []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(linear(x[i], **layer))
+        graphs.append(graph)
+    for _ in range(3):
+        for i in range(2):
+            x[i].copy_(_normal(60, 9000, seed=i))
+        for h in held:
+            h.zero_()
+        for g in graphs:
+            g.replay()
+        linear(x[2], **layer)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
 
 
 @pytest.mark.parametrize("rows", [1, 9, 40, 600, 4096])

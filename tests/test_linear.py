@@ -4,11 +4,13 @@ The operators make their checks on any device and refuse CPU tensors last: a cal
 that refusal.
 """
 
+import ctypes
+
 import pytest
 import torch
 
+from hilberta_amd import _lib, ops
 from hilberta_amd import flux_linear as f
-from hilberta_amd import ops
 
 BF16, HALF = torch.bfloat16, torch.float16
 ON_DEVICE = "device tensors"
@@ -121,3 +123,49 @@ def test_shapes_of_traced_calls():
         y = f.linear(x, w, act="silu")
         assert y.shape == (2, 5, 40) and y.dtype == HALF and y.device.type == "cuda"
         assert [t.shape[1] for t in f.linear_pair(dict(x=x, weight=w), dict(x=x[:, :3], weight=w))] == [5, 3]
+
+
+# ------------------------------------------------------------------ the C entry (addresses that nothing reads)
+HELD = 1 << 40
+
+
+def _workspace(rows, columns, features, *, x=HELD, row=None, count=1, batch=1):
+    pointers = (ctypes.c_void_p * 12)(*([x, HELD, None, None, None, HELD] * 2))
+    row = features if row is None else row
+    strides = (ctypes.c_int64 * 16)(*([rows * row, row, features, 0, 0, 0, rows * columns, columns] * 2))
+    call = (count, batch, (ctypes.c_int32 * 2)(rows, rows), columns, features)
+    return _lib.load().hb_linear_workspace_bytes(*call, pointers, strides), call, pointers, strides
+
+
+def test_workspaces():
+    # whole tiles, or enough of them: nothing
+    for rows, columns, features in ((4096, 9216, 3072), (512, 9216, 3072), (1, 18432, 3072), (16, 5, 12345), (77, 64, 64)):
+        assert _workspace(rows, columns, features)[0] == 0
+    # few tiles over many features: the sums of 2, 4, 8 or 16 parts of them
+    for rows, columns, features in ((126, 32, 13952), (100, 304, 12288)):
+        parts = _workspace(rows, columns, features)[0] / (rows * columns * 4)
+        assert parts in (2, 4, 8, 16)
+    assert _workspace(126, 27, 13952)[0] % (126 * 32 * 4) == 0
+    # rows and weights that are no multiple of 16 bytes
+    assert _workspace(300, 1000, 60)[0] == 1300 * 64 * 2
+    assert _workspace(300, 1000, 64, x=HELD + 2)[0] == 300 * 64 * 2
+    assert _workspace(300, 1000, 64, row=67)[0] == 300 * 64 * 2
+    assert _workspace(300, 1000, 60, count=2)[0] == 2 * 1300 * 64 * 2
+    # rows too far apart for one load's offset
+    assert _workspace(300, 1000, 64, row=1 << 23)[0] == 300 * 64 * 2
+    for bad in (dict(rows=0), dict(columns=0), dict(features=0), dict(features=(1 << 20) + 1), dict(count=0), dict(count=3), dict(batch=0),
+                dict(x=None), dict(x=HELD + 1), dict(row=-8)):
+        assert _workspace(**(dict(rows=300, columns=1000, features=64) | bad))[0] == -1
+
+
+def test_a_workspace_too_small_is_refused():
+    for sizes in ((126, 32, 13952), (300, 1000, 60)):
+        bytes, call, pointers, strides = _workspace(*sizes)
+        assert bytes > 0
+        for workspace, held in ((None, bytes), (HELD, bytes - 1), (HELD + 8, bytes)):
+            assert _lib.load().hb_linear(*call, 0, 0, pointers, strides, workspace, held, None) == 1
+            assert b"the workspace must hold" in _lib.load().hb_last_error()
+    for dtype, act, match in ((2, 0, b"dtype must be"), (0, 3, b"act must be")):
+        bytes, call, pointers, strides = _workspace(1, 8, 8)
+        assert _lib.load().hb_linear(*call, dtype, act, pointers, strides, None, 0, None) == 1
+        assert match in _lib.load().hb_last_error()
