@@ -219,9 +219,10 @@ constexpr int WIDE = 256, WIDE_BAND = 4, WIDE_WAVES = 4;
 constexpr int WIDE_STAGE = 2 * WIDE * 128;                  // 64 KB
 constexpr int WIDE_LOADS = WIDE_STAGE / 1024 / WIDE_WAVES;  // 1 KB loads of a wave and stage
 
-// What the epilogue does.  All but ANY are for whole tiles, each of one batch element, with aligned outputs, and work on
-// the sums in registers; ANY takes them through LDS.  (One kernel for both kinds of tile keeps too much in registers.)
-enum Mode { PLAIN, ACT_GELU, ACT_SILU, RESIDUAL, GATED, ANY };
+// What the epilogue does.  All up to GATED are for whole tiles, each of one batch element, with aligned outputs, and work
+// on the sums in registers; ANY takes them through LDS, and PARTS, for a part of the features of any tile, stores the sums
+// themselves.  (One kernel for several kinds of tile keeps too much in registers.)
+enum Mode { PLAIN, ACT_GELU, ACT_SILU, RESIDUAL, GATED, ANY, PARTS };
 
 // A wave's 128 x 128 sums: acc[i][j] are channels 16 i + 4 (lane / 16) .. + 3 of token 16 j + lane % 16.
 struct Sums {
@@ -352,6 +353,23 @@ __device__ __forceinline__ void fill_box(const Sums& acc, int8_t* box) {
     for (int i = 0; i < 8; ++i) *(f32x4*)(to + j * 8 * 4096 + ((i * 2 + (q >> 1)) ^ token) * 16) = moved_out(acc.v[i][J + j]);
 }
 
+// A wave's sums of the part blockIdx.y of a tile, from channel c0 and token t0 on, for join_kernel.
+__device__ __forceinline__ void keep_sums(const Args& a, int set, const Sums& acc, int c0, uint32_t t0) {
+  const int lane = threadIdx.x & 63, c = c0 + (lane >> 4) * 4, across = padded_columns(a);
+  const uint32_t tokens = a.set[set].tokens;
+  t0 += lane & 15;
+  float* const to = a.sums + ((int64_t)blockIdx.y * all_tokens(a) + (set ? a.set[0].tokens : 0) + t0) * across + c;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const f32x4 v = moved_out(acc.v[i][j]);
+      if (t0 + j * 16 < tokens && c + i * 16 < across) *(f32x4*)(to + (int64_t)j * 16 * across + i * 16) = v;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 template <bool F16, int MODE>
 __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) int8_t lds0[WIDE_STAGE];
@@ -359,7 +377,10 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a)
   __shared__ __attribute__((aligned(16))) float bias[2][WIDE], gate[2][WIDE];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), row = lane & 15, quarter = lane >> 4;
   const int wc = wave & 1, wt = wave >> 1;
-  const int stages = max((a.features + 127) / 128 * 2, 4);  // (an even number)
+  constexpr bool WHOLE = MODE < ANY;
+  const int start = MODE == PARTS ? blockIdx.y * a.stages_each : 0;
+  const int stop = MODE == PARTS ? min(start + a.stages_each, (a.features + 63) / 64) : (a.features + 63) / 64;
+  const int stages = max((stop - start + 1) / 2 * 2, 4);  // (an even number)
   // (workgroups go to the eight XCDs in turn)
   const uint32_t first = (blockIdx.x & 7) * a.tiles_xcd, stride = gridDim.x >> 3;
   uint32_t slot = blockIdx.x >> 3;
@@ -369,7 +390,8 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a)
   // row r loads chunk p ^ (r / 2 % 8), so that the chunks that 16 rows' lanes read together lie in
   // different banks.
   const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
-  const RowEnd ends(a.features, chunk);
+  RowEnd ends(a.features, chunk);
+  if (MODE == PARTS) ends.stop(stop);
   const int8_t *wbase, *xbase;
   int offset[WIDE_LOADS];
   int aimed = -1;  // the set that `offset` is of
@@ -378,24 +400,25 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a)
     const Place begin = place_of(s, t.t0);
     wbase = uniform_pointer((const int8_t*)(s.w + t.c0 * s.w_n));
     xbase = uniform_pointer((const int8_t*)(s.x + begin.b * s.x_b + begin.n * s.x_n));
-    if (MODE != ANY && aimed == t.set) return;  // (whole tiles differ by where they begin)
+    if (WHOLE && aimed == t.set) return;  // (whole tiles differ by where they begin)
     aimed = t.set;
 #pragma unroll
     for (int j = 0; j < WIDE_LOADS; ++j) {
       const int r = 8 * (WIDE_WAVES * j + wave) + (lane >> 3);
       if (j < WIDE_LOADS / 2) {
-        offset[j] = (MODE == ANY ? min(r, a.columns - 1 - t.c0) : r) * (int)s.w_n * 2 + chunk * 16;
-      } else if (MODE == ANY) {
+        offset[j] = (WHOLE ? r : min(r, a.columns - 1 - t.c0)) * (int)s.w_n * 2 + chunk * 16;
+      } else if (WHOLE) {
+        offset[j] = (r - WIDE) * (int)s.x_n * 2 + chunk * 16;
+      } else {
         const Place p = place_of(s, t.t0 + (r - WIDE));
         offset[j] = (int)(((p.b - begin.b) * s.x_b + ((int64_t)p.n - begin.n) * s.x_n) * 2) + chunk * 16;
-      } else {
-        offset[j] = (r - WIDE) * (int)s.x_n * 2 + chunk * 16;
       }
     }
   };
   auto load = [&](int8_t* dst, int stage, int j, int past) {
-    load_lds16(j < WIDE_LOADS / 2 ? wbase : xbase, dst + 1024 * (WIDE_WAVES * j + wave), offset[j] | past, uniform(stage * 128));
+    load_lds16(j < WIDE_LOADS / 2 ? wbase : xbase, dst + 1024 * (WIDE_WAVES * j + wave), offset[j] | past, uniform((start + stage) * 128));
   };
+  auto past = [&](int stage) { return ends.past(start + stage); };
   // Operands: lane l holds bytes 16 (l / 16) .. + 15 of a 64-byte step of row l % 16.
   const int read = row * 128 + ((row >> 1 & 7) ^ quarter) * 16;
   u32x4 w[2][8], x[2][8];
@@ -416,7 +439,7 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a)
   constexpr std::true_type yes;
   auto step = [&](auto first_one, auto last, int8_t* cur, int8_t* next, int after) {
     constexpr bool FIRST = decltype(first_one)::value, LAST = decltype(last)::value;
-    const int past = ends.past(uniform(after));
+    const int after_past = past(uniform(after));
     auto product = [&](auto index) {
       constexpr int k = decltype(index)::value, u = k >> 6, j = k >> 3 & 7, i = k & 7;
       if (FIRST && u == 0) begin16<F16>(w[u][i], x[u][j], acc.v[i][j]);
@@ -427,7 +450,7 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a)
         wait_loads<63>();
         barrier();  // nobody reads `cur` any more
       }
-      if (!(LAST && MODE == ANY) && k >= 30 && (k - 30) % 6 == 0 && (k - 30) / 6 < WIDE_LOADS) load(cur, after, (k - 30) / 6, past);
+      if (!(LAST && MODE == ANY) && k >= 30 && (k - 30) % 6 == 0 && (k - 30) / 6 < WIDE_LOADS) load(cur, after, (k - 30) / 6, after_past);
       if (k == 86) {
         wait_arrivals<LAST && MODE == ANY ? 0 : 10>();  // (what this stage has asked for by now)
         barrier();                                      // `next` is there
@@ -447,17 +470,17 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a)
   Tile t = tile_at<WIDE, WIDE, WIDE_BAND>(a, first + slot);
   aim(t);
   uint16_t bias_value, gate_value;
-  ask_channel(t, bias_value, gate_value);
+  if (MODE != PARTS) ask_channel(t, bias_value, gate_value);
 #pragma unroll
-  for (int j = 0; j < WIDE_LOADS; ++j) load(lds0, 0, j, ends.past(0));
+  for (int j = 0; j < WIDE_LOADS; ++j) load(lds0, 0, j, past(0));
 #pragma unroll
-  for (int j = 0; j < WIDE_LOADS; ++j) load(lds1, 1, j, ends.past(1));
+  for (int j = 0; j < WIDE_LOADS; ++j) load(lds1, 1, j, past(1));
   wait_loads<WIDE_LOADS>();
   barrier();
   for (int parity = 0;; parity ^= 1) {
     const Tile done = t;
     const Set& s = a.set[done.set];
-    bias[parity][threadIdx.x] = to_f<F16>(bias_value);  // (read after the next barriers)
+    if (MODE != PARTS) bias[parity][threadIdx.x] = to_f<F16>(bias_value);  // (read after the next barriers)
     if (MODE == GATED) gate[parity][threadIdx.x] = to_f<F16>(gate_value);
 #pragma unroll
     for (int k = 0; k < 16; ++k) fetch(lds0, 0, k);
@@ -468,16 +491,18 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a)
       step(no, no, lds1, lds0, n + 1);
     }
     slot += stride;
-    const bool more = slot < a.tiles_xcd && first + slot < a.tiles;
+    const bool more = MODE != PARTS && slot < a.tiles_xcd && first + slot < a.tiles;
     if (more) t = tile_at<WIDE, WIDE, WIDE_BAND>(a, first + slot);
     aim(t);  // (after the last tile: its own first stages once more, never multiplied)
-    ask_channel(t, bias_value, gate_value);  // (before the stores, which a load after them would wait for)
+    if (MODE != PARTS) ask_channel(t, bias_value, gate_value);  // (before the stores, which a load after them would wait for)
     step(no, no, lds0, lds1, 0);
     step(no, yes, lds1, lds0, 1);
     settle();
     const int c0 = done.c0 + wc * 128;
     const uint32_t t0 = done.t0 + wt * 128;
-    if constexpr (MODE != ANY) {
+    if constexpr (MODE == PARTS) {
+      keep_sums(a, done.set, acc, c0, t0);
+    } else if constexpr (WHOLE) {
       finish_wide<F16, MODE>(s, acc, &bias[parity][wc * 128], &gate[parity][wc * 128], c0, t0);
     } else {
       int8_t* const box = lds1 + 1024 * wave;
@@ -491,7 +516,7 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a)
       }
       wait_loads<63>();  // (into the pieces that this wave's own epilogue has read)
 #pragma unroll
-      for (int j = 0; j < WIDE_LOADS; ++j) load(lds1, 1, j, ends.past(1));
+      for (int j = 0; j < WIDE_LOADS; ++j) load(lds1, 1, j, past(1));
     }
     if (!more) break;
   }
@@ -781,20 +806,20 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
 enum Kernel { T64x32, T32x64, T64x64, T96x64, T96x128, T128x128, WIDE256, KERNELS };
 
 // A kernel's tile and what its time is made of, in us: the launch, a round of 256 workgroups, a round's stage of 64
-// features, what a stage takes longer when all CUs are at it, and each megabyte of rows and weight.  Fitted to 2140
-// times of 150 sizes, which they meet to 14% (one sigma).
+// features, what a stage takes longer when all CUs are at it, each megabyte of rows and weight, and, in parts, the join and
+// each megabyte of their sums.  Fitted to 2523 times of 175 sizes whose operands come from memory, which they meet to 13%
+// (one sigma).
 struct Shape {
   int tc, tt;
-  float launch, round, stage, full, megabyte;
+  float launch, round, stage, full, megabyte, join, sums;
 };
 constexpr Shape SHAPES[KERNELS] = {
-    {64, 32, 3.9f, 1.3f, 0.133f, 0.010f, 0.06f},  {32, 64, 2.35f, 2.5f, 0.132f, 0.035f, 0.06f},
-    {64, 64, 2.4f, 2.5f, 0.161f, 0.087f, 0.06f},  {96, 64, 1.7f, 3.7f, 0.218f, 0.074f, 0.06f},
-    {96, 128, 2.2f, 4.75f, 0.314f, 0.139f, 0.06f}, {128, 128, 3.9f, 4.4f, 0.333f, 0.236f, 0.06f},
-    {256, 256, 0.9f, 9.f, 0.97f, 0.270f, 0.04f},
+    {64, 32, 3.25f, 1.7f, 0.158f, 0.000f, 0.173f, 3.7f, 0.35f},  {32, 64, 2.3f, 3.1f, 0.153f, 0.043f, 0.143f, 3.5f, 0.53f},
+    {64, 64, 2.35f, 3.3f, 0.200f, 0.066f, 0.155f, 3.0f, 0.58f},  {96, 64, 2.6f, 5.1f, 0.261f, 0.055f, 0.143f, 1.3f, 0.77f},
+    {96, 128, 2.2f, 7.8f, 0.393f, 0.053f, 0.132f, 0.1f, 0.68f},  {128, 128, 4.3f, 6.75f, 0.435f, 0.142f, 0.124f, 0.0f, 0.51f},
+    {256, 256, 8.45f, 2.9f, 1.122f, 0.224f, 0.071f, 0.0f, 0.37f},
 };
-constexpr float WIDE_ANY_ROUND = 24.f;  // (tiles that are not whole)
-constexpr float JOIN = 3.f, JOIN_BYTE = 4e-7f;
+constexpr float WIDE_ANY_ROUND = 36.f;  // (tiles that are not whole)
 
 // Tiles of TC x TT of both sets.
 int64_t tiles_of(const Args& a, int count, int tc, int tt) {
@@ -834,29 +859,30 @@ float estimate(const Args& a, int count, Kernel k, int splits) {
   const Shape& s = SHAPES[k];
   const float rounds = (float)(tiles_of(a, count, s.tc, s.tt) * splits) / 256.f, whole = std::floor(rounds), rest = rounds - whole;
   const float stages = (float)(((a.features + 63) / 64 + splits - 1) / splits);
-  const float round = k == WIDE256 && !whole_tiles(a, count) ? WIDE_ANY_ROUND : s.round;
+  const float round = k == WIDE256 && splits == 1 && !whole_tiles(a, count) ? WIDE_ANY_ROUND : s.round;
   const float rows = (float)a.set[0].tokens + (float)a.set[1].tokens + (float)count * (float)a.columns;
-  return s.launch + whole * (round + stages * (s.stage + s.full)) +
-         (rest > 0.f ? round + stages * (s.stage + s.full * rest * rest) : 0.f) + s.megabyte * 2e-6f * rows * (float)a.features;
+  float us = s.launch + whole * (round + stages * (s.stage + s.full)) +
+             (rest > 0.f ? round + stages * (s.stage + s.full * rest * rest) : 0.f) + s.megabyte * 2e-6f * rows * (float)a.features;
+  if (splits > 1) us += s.join + s.sums * 1e-6f * (float)sums_bytes(a, splits);
+  return us;
 }
 
 // The kernel, and the parts that it takes the features in, of the least estimate.  Parts pay where few tiles leave CUs
-// idle over many features; they are tried while all their workgroups fit the card at once with six stages each or
-// more, and taken where they promise 5% and 1 us.  Measured, one part / the parts: 126 x 13952 -> 27 33.9 / 10.3 us, 63 x 8120 -> 386
-// 27.8 / 12.1, 1283 x 10072 -> 450 48.4 / 37.4.  Over the 150
-// sizes the choice takes 1.9% more time than the best of all, and the best of one part 9.6%.
+// idle over many features; they are tried while all their workgroups fit the card at once, with four stages each or more.
+// Measured, the best of one part / the parts: 99 x 8472 -> 64 30.4 / 9.9 us, 512 x 12288 -> 3072 72.8 / 60 (eight of the
+// wide kernel), 1280 x 13824 -> 5120 251 / 171 (two of it).  Over the 175 sizes the choice takes 1.9% more time than the
+// best of all, and the best of one part 13.9%.
 Choice choose(const Args& a, int count) {
   Choice best = {WIDE256, 1};
   float least = estimate(a, count, WIDE256, 1);
   const int stages = (a.features + 63) / 64;
-  for (int i = 0; i < WIDE256; ++i) {
+  for (int i = 0; i < KERNELS; ++i) {
     const Kernel k = (Kernel)i;
     const int64_t tiles = tiles_of(a, count, SHAPES[k].tc, SHAPES[k].tt);
     if (tiles >= (1 << 21)) continue;  // (a grid holds fewer than 2^32 threads)
-    for (int splits = 1; splits <= 16; splits *= 2) {
-      if (splits > 1 && (tiles * splits > 256 || stages < 6 * splits)) break;
-      float us = estimate(a, count, k, splits);
-      if (splits > 1) us = 1.05f * (us + JOIN + JOIN_BYTE * (float)sums_bytes(a, splits)) + 1.f;
+    for (int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      if (splits > 1 && (tiles * splits > 256 || stages < 4 * splits)) break;
+      const float us = estimate(a, count, k, splits);
       if (us < least) best = {k, splits}, least = us;
     }
   }
@@ -873,6 +899,7 @@ int launch_kernel(Args& a, int count, const Choice& choice, hipStream_t st) {
   a.tiles = (uint32_t)tiles;
   a.tiles_xcd = (a.tiles + 7) / 8;
   a.stages_each = (stages + choice.splits - 1) / choice.splits;
+  if (choice.kernel == WIDE256) a.stages_each = (a.stages_each + 1) & ~1;  // (which it takes in twos)
   a.splits = (stages + a.stages_each - 1) / a.stages_each;
   const dim3 each(8 * a.tiles_xcd, a.splits), four(256), eight(512);
   switch (choice.kernel) {
@@ -885,7 +912,8 @@ int launch_kernel(Args& a, int count, const Choice& choice, hipStream_t st) {
     default: {
       const uint32_t per_xcd = std::max(1, device_cu_count() / 8);
       const dim3 grid(8 * std::min(a.tiles_xcd, per_xcd)), block(64 * WIDE_WAVES);
-      switch (mode_of(a, count)) {
+      if (a.splits > 1) hipLaunchKernelGGL((linear_wide_kernel<F16, PARTS>), each, block, 0, st, a);
+      else switch (mode_of(a, count)) {
         case PLAIN: hipLaunchKernelGGL((linear_wide_kernel<F16, PLAIN>), grid, block, 0, st, a); break;
         case ACT_GELU: hipLaunchKernelGGL((linear_wide_kernel<F16, ACT_GELU>), grid, block, 0, st, a); break;
         case ACT_SILU: hipLaunchKernelGGL((linear_wide_kernel<F16, ACT_SILU>), grid, block, 0, st, a); break;
@@ -896,7 +924,7 @@ int launch_kernel(Args& a, int count, const Choice& choice, hipStream_t st) {
     }
   }
   HB_HIP(hipGetLastError());
-  if (choice.kernel != WIDE256 && a.splits > 1) {
+  if (a.splits > 1) {
     const int64_t threads = (int64_t)(a.set[0].tokens + a.set[1].tokens) * ((a.columns + 7) / 8);
     hipLaunchKernelGGL((join_kernel<F16>), dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, st, a);
     HB_HIP(hipGetLastError());

@@ -85,7 +85,8 @@ def test_long_sums():
 
 
 # few tiles over many features, which several workgroups share
-PARTS = [(126, 13952, 27), (383, 5200, 5024), (127, 8104, 5270), (17, 1543, 16), (20, 3001, 100), (100, 12345, 300), (1000, 8192, 520)]
+PARTS = [(126, 13952, 27), (383, 5200, 5024), (127, 8104, 5270), (17, 1543, 16), (20, 3001, 100), (100, 12345, 300), (1000, 8192, 520),
+         (512, 12288, 3072), (700, 9001, 1500), (1100, 8200, 1001), (513, 6000, 2048)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, HALF])
@@ -95,9 +96,9 @@ def test_features_in_parts(rows, K, N, dtype):
     _check(linear(x, **layer), x=x, **layer)
 
 
+@pytest.mark.parametrize("batch, rows, K, N", [(3, 23, 4096, 203), (3, 171, 12000, 2001)])
 @pytest.mark.parametrize("act, bias, more", EPILOGUES)
-def test_epilogues_of_parts(act, bias, more):
-    batch, rows, K, N = 3, 23, 4096, 203
+def test_epilogues_of_parts(batch, rows, K, N, act, bias, more):
     x, layer = _normal(batch, rows, K), _layer(K, N, bias=bias)
     if more:
         layer["residual"] = _normal(batch, rows, N, seed=5)
@@ -106,13 +107,14 @@ def test_epilogues_of_parts(act, bias, more):
     _check(linear(x, act=act, **layer), act=act, x=x, **layer)
 
 
-@pytest.mark.parametrize("text, image", [(1, 30), (30, 1), (77, 100), (0, 40)])
-def test_pairs_in_parts(text, image):
+@pytest.mark.parametrize("text, image, K, N", [(1, 30, 6000, 200), (30, 1, 6000, 200), (77, 100, 6000, 200), (0, 40, 6000, 200),
+                                               (77, 256, 12288, 2048), (300, 33, 9999, 1999)])
+def test_pairs_in_parts(text, image, K, N):
     sets = []
     for i, rows in enumerate((text, image)):
-        s = dict(x=_normal(2, rows, 6000, seed=i), **_layer(6000, 200, seed=10 * i))
+        s = dict(x=_normal(2, rows, K, seed=i), **_layer(K, N, seed=10 * i))
         if i:
-            s |= dict(residual=_normal(2, rows, 200, seed=31), gate=_normal(2, 200, seed=41))
+            s |= dict(residual=_normal(2, rows, N, seed=31), gate=_normal(2, N, seed=41))
         sets.append(s)
     for out, s in zip(linear_pair(*sets), sets):
         if s["x"].numel():
