@@ -453,8 +453,18 @@ int launch(Args& a, int32_t batch, hipStream_t st) {
 
 using namespace hb;
 
+namespace {
+int check_sizes(int32_t batch, int64_t pixels, int32_t channels, int32_t groups, int32_t dtype) {
+  HB_REQUIRE(batch > 0 && batch <= 65535 && pixels > 0 && pixels < (1ll << 31), "batch must be in [1, 65535] and pixels in [1, 2^31)");
+  HB_REQUIRE(channels > 0 && channels <= MAX_CHANNELS, "channels must be in [1, %d] (got %d)", MAX_CHANNELS, channels);
+  HB_REQUIRE(groups > 0 && channels % groups == 0, "groups must divide the channels");
+  HB_REQUIRE(dtype == HB_DTYPE_BF16 || dtype == HB_DTYPE_F16 || dtype == HB_DTYPE_F32, "dtype must be bf16, fp16 or fp32");
+  return HB_OK;
+}
+}  // namespace
+
 extern "C" int64_t hb_group_norm_workspace_bytes(int32_t batch, int64_t pixels, int32_t channels, int32_t groups, int32_t dtype) {
-  if (batch < 1 || pixels < 1 || channels < 1 || groups < 1 || channels % groups || dtype < 0 || dtype > HB_DTYPE_F32) return -1;
+  if (check_sizes(batch, pixels, channels, groups, dtype) != HB_OK) return -1;
   if (few(batch, pixels, groups, channels / groups)) return 0;
   return batch * chunks_of(batch, pixels, channels, dtype).count * groups * (int64_t)sizeof(float2);
 }
@@ -464,10 +474,8 @@ extern "C" int hb_group_norm(int32_t batch, int64_t pixels, int32_t channels, in
                              const void* bias, void* out, int64_t out_batch_stride, int64_t out_pixel_stride,
                              void* workspace, int64_t workspace_bytes, hb_stream_t stream) {
   HB_REQUIRE(x && out, "null pointer argument");
-  HB_REQUIRE(batch > 0 && batch <= 65535 && pixels > 0 && pixels < (1ll << 31), "batch must be in [1, 65535] and pixels in [1, 2^31)");
-  HB_REQUIRE(channels > 0 && channels <= MAX_CHANNELS, "channels must be in [1, %d] (got %d)", MAX_CHANNELS, channels);
-  HB_REQUIRE(groups > 0 && channels % groups == 0, "groups must divide the channels");
-  HB_REQUIRE(dtype == HB_DTYPE_BF16 || dtype == HB_DTYPE_F16 || dtype == HB_DTYPE_F32, "dtype must be bf16, fp16 or fp32");
+  const int rc = check_sizes(batch, pixels, channels, groups, dtype);
+  if (rc) return rc;
   HB_REQUIRE(silu == 0 || silu == 1, "silu must be 0 or 1");
   HB_REQUIRE(eps > 0.f, "eps must be positive");
   const uintptr_t size = (uintptr_t)size_of(dtype);

@@ -221,7 +221,7 @@ int hb_adaln_modulate_pair(int32_t batch, const int32_t* rows, int32_t hidden, i
  *   out = act((x - mean) / sqrt(var + eps) * weight[c] + bias[c])
  * mean and var (of n, not n - 1) over the element's pixels and the group's channels; silu = 1: act is SiLU, else none;
  * statistics and values in fp32, one rounding.  x and out are [batch, pixels, channels] by element strides, channels
- * contiguous; groups divide the channels, which are up to 8192; dtype may be HB_DTYPE_F32; weight and bias [channels] of
+ * contiguous; groups divide the channels, which are up to 8192; batch up to 65535, pixels below 2^31; dtype may be HB_DTYPE_F32; weight and bias [channels] of
  * that type, or NULL.  out may be x itself.  `workspace`: hb_group_norm_workspace_bytes (0 for small groups, -1 where the
  * sizes are rejected), 8-byte aligned, contents irrelevant before and after. */
 int64_t hb_group_norm_workspace_bytes(int32_t batch, int64_t pixels, int32_t channels,
@@ -241,10 +241,10 @@ int hb_group_norm(int32_t batch, int64_t pixels, int32_t channels, int32_t group
  * [count]; pointers [count x 6] {x, weight, bias or NULL, residual or NULL, gate or NULL (else with a residual), out};
  * strides [count x 8] {x batch, x row, weight row, residual batch, residual row, gate batch, out batch, out row},
  * elements, last dimensions contiguous.  out may be the residual itself; it may lie over nothing else that is read.
- * features up to 2^20.  Rows may begin at any element.  `workspace` (hb_linear_workspace_bytes, 0 where none is needed
- * and -1 where the sizes are rejected; 16-byte aligned, contents irrelevant before and after) holds x and weights whose
- * rows are no multiples of 16 bytes or lie too far apart, copied first unless both sets have at most 16 rows, and the
- * sums of the parts that the features of few rows and columns are taken in. */
+ * features up to 2^20, columns up to 2^25.  Rows may begin at any element.  `workspace` (hb_linear_workspace_bytes, 0
+ * where none is needed and -1 where the sizes are rejected; 16-byte aligned, contents irrelevant before and after) holds x
+ * and weights whose rows are no multiples of 16 bytes or lie too far apart, copied first unless both sets have at most 16
+ * rows, and the sums of the parts that the features of few rows and columns are taken in. */
 int64_t hb_linear_workspace_bytes(int32_t count, int32_t batch, const int32_t* rows, int32_t columns,
                                   int32_t features, void* const* pointers, const int64_t* strides);
 int hb_linear(int32_t count, int32_t batch, const int32_t* rows, int32_t columns, int32_t features,

@@ -76,3 +76,28 @@ def test_shapes_of_traced_calls():
         y = group_norm(torch.empty(2, 8, 4, 6, device="cuda", memory_format=torch.channels_last), 4, act="silu")
         assert y.shape == (2, 8, 4, 6) and y.is_contiguous(memory_format=torch.channels_last)
         assert group_norm(torch.empty(2, 24, 8, device="cuda"), 4).shape == (2, 24, 8)
+
+
+# ------------------------------------------------------------------ the C entry (addresses that nothing reads)
+def test_workspaces():
+    import ctypes
+
+    from hilberta_amd import _lib
+
+    lib, held = _lib.load(), ctypes.c_void_p(1 << 40)
+
+    def call(sizes, workspace, bytes):
+        batch, pixels, channels, *_ = sizes
+        return lib.hb_group_norm(*sizes, 0, 1e-6, held, pixels * channels, channels, None, None, held, pixels * channels, channels,
+                                 workspace, bytes, None)
+
+    assert lib.hb_group_norm_workspace_bytes(1, 256, 512, 32, 0) == 0  # (a workgroup holds a group)
+    sizes = (2, 16384, 512, 32, 0)
+    need = lib.hb_group_norm_workspace_bytes(*sizes)
+    assert need > 0 and need == 2 * lib.hb_group_norm_workspace_bytes(1, *sizes[1:])
+    for workspace, bytes in ((None, need), (held, need - 1), (ctypes.c_void_p((1 << 40) + 4), need)):
+        assert call(sizes, workspace, bytes) == 1 and b"the workspace must hold" in lib.hb_last_error()
+    for sizes in ((0, 9, 8, 4, 0), (65536, 9, 8, 4, 0), (1, 0, 8, 4, 0), (1, 1 << 31, 8, 4, 0), (1, 9, 8193, 1, 0), (1, 9, 0, 1, 0),
+                  (1, 9, 8, 3, 0), (1, 9, 8, 0, 0), (1, 9, 8, 4, 3), (1, 9, 8, 4, -1)):
+        assert lib.hb_group_norm_workspace_bytes(*sizes) == -1
+        assert call(sizes, held, 1 << 20) == 1

@@ -153,7 +153,7 @@ def test_workspaces():
     assert _workspace(300, 1000, 60, count=2)[0] == 2 * 1300 * 64 * 2
     # rows too far apart for one load's offset
     assert _workspace(300, 1000, 64, row=1 << 23)[0] == 300 * 64 * 2
-    for bad in (dict(rows=0), dict(columns=0), dict(features=0), dict(features=(1 << 20) + 1), dict(count=0), dict(count=3), dict(batch=0),
+    for bad in (dict(rows=0), dict(columns=0), dict(features=0), dict(features=(1 << 20) + 1), dict(columns=(1 << 25) + 1), dict(count=0), dict(count=3), dict(batch=0),
                 dict(x=None), dict(x=HELD + 1), dict(row=-8)):
         assert _workspace(**(dict(rows=300, columns=1000, features=64) | bad))[0] == -1
 
