@@ -549,6 +549,8 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a)
 // meet in LDS, and a thread finishes eight channels of a token: neighbouring lanes read and write whole lines.  Rows
 // past the operands' ends are zeros that nothing reads.  77 x 4096 -> 3072 13.4 us, 23 with the weight from memory; 2048 x
 // 2048 -> 2048 (128 x 128) 21, 0.8 PFLOP/s.
+// AHEAD > 0: rows at any address, by registers that AHEAD stages are on their way to, then into the ring: 0.3 us a stage of
+// 64 x 64, where direct loads take 0.2, but no copies.
 template <int TC, int TT, int WAVES>
 struct Ring {
   static constexpr int STAGE = (TC + TT) * 128, GROUPS = STAGE / 1024, LOADS = (GROUPS + WAVES - 1) / WAVES;
@@ -557,7 +559,7 @@ struct Ring {
   static constexpr int CF = (WAVES > 4 ? CW : TC) / 32, TF = (WAVES > 4 ? TW : TT) / 32;  // of a wave
 };
 
-template <bool F16, int TC, int TT, int R, int WAVES>
+template <bool F16, int TC, int TT, int R, int WAVES, int AHEAD = 0>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_tile_kernel(Args a) {
   typedef Ring<TC, TT, WAVES> F;
   constexpr int STAGE = F::STAGE, LOADS = F::LOADS, CW = F::CW, TW = F::TW, CF = F::CF, TF = F::TF;
@@ -586,11 +588,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_tile_kernel(Args
   const Place begin = place_of(s, t.t0);
   const int8_t *wbase = (const int8_t*)(s.w + t.c0 * s.w_n), *xbase = (const int8_t*)(s.x + begin.b * s.x_b + begin.n * s.x_n);
   const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
-  int offset[LOADS];
+  int offset[LOADS];  // (of direct loads)
+  const uint16_t* row[LOADS];  // (of the others)
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) {
     const int r = 8 * (WAVES * j + wave) + (lane >> 3);
-    if (r < TC) {
+    if (AHEAD) {
+      const Place p = place_of(s, t.t0 + (r - TC));
+      row[j] = r < TC ? s.w + min(t.c0 + r, a.columns - 1) * s.w_n : s.x + p.b * s.x_b + p.n * s.x_n;
+    } else if (r < TC) {
       offset[j] = r < a.columns - t.c0 ? r * (int)s.w_n * 2 + chunk * 16 : (int)0x80000000;
     } else {
       const Place p = place_of(s, t.t0 + (r - TC));
@@ -603,6 +609,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_tile_kernel(Args
   RowEnd ends(a.features, chunk);
   ends.stop(last);
   const bool all = WAVES * (LOADS - 1) + wave < F::GROUPS;  // (the last loads are not every wave's)
+  // (rows at any address: by registers)
+  u32x4 held[AHEAD ? AHEAD : 1][LOADS];
+  auto ask_rows = [&](u32x4& to, int stage, int j) { to = *(const any_u32x4*)(row[j] + min(stage * 64 + chunk * 8, a.features - 8)); };
+  auto hand_in = [&](int8_t* dst, u32x4 v, int stage, int j) {
+    if (stage * 64 + 64 > a.features) v = drop_values(v, min(max(stage * 64 + chunk * 8 - (a.features - 8), 0), 8));
+    *(u32x4*)(dst + 1024 * (WAVES * j + wave) + lane * 16) = v;
+  };
   auto load = [&](int8_t* dst, int stage, int j, int past) {
     const int group = WAVES * j + wave;
     if (F::GROUPS % WAVES == 0 || j < LOADS - 1 || all)
@@ -638,26 +651,46 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void linear_tile_kernel(Args
         acc[j][i] = multiply32<F16>(w[I & 1][i], x[I & 1][j], acc[j][i]);
         for (++done; asked * TF * CF < done * LOADS; ++asked) {
           __builtin_amdgcn_sched_barrier(0);
-          load(free, n + R - 1, asked, past);
+          if constexpr (AHEAD) {
+            hand_in(free, held[I % AHEAD][asked], n + R - 1, asked);
+            ask_rows(held[I % AHEAD][asked], n + R - 1 + AHEAD, asked);
+          } else {
+            load(free, n + R - 1, asked, past);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
     __builtin_amdgcn_sched_barrier(0);
+    if (AHEAD) wait_loads<63>();  // (what it has written is in LDS)
     fetch(ring(std::integral_constant<int, I + 1>()), ~I & 1);
-    arrivals();
+    if (!AHEAD) arrivals();
     barrier();
     return ++n == last;
   };
-  // (Zeros into the last stage, so that the compiler, which tracks what is on its way to which array, has met them
-  // all before the loop: otherwise it waits for everything each time around.)
-  load(ring(std::integral_constant<int, R - 1>()), 0, 0, (int)0x80000000);
-  auto begin_stage = [&](auto index) {
-    constexpr int I = decltype(index)::value;
+  if constexpr (AHEAD) {
+    u32x4 now[R - 1][LOADS];
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) load(ring(index), first + I, j, ends.past(first + I));
-  };
-  begin_all(begin_stage, std::make_integer_sequence<int, R - 1>());
-  arrivals();
+    for (int i = 0; i < R - 1 + AHEAD; ++i)
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) ask_rows(i < R - 1 ? now[i][j] : held[(i - (R - 1)) % AHEAD][j], first + i, j);
+    auto begin_stage = [&](auto index) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) hand_in(ring(index), now[decltype(index)::value][j], first + decltype(index)::value, j);
+    };
+    begin_all(begin_stage, std::make_integer_sequence<int, R - 1>());
+    wait_loads<63>();
+  } else {
+    // (Zeros into the last stage, so that the compiler, which tracks what is on its way to which array, has met them
+    // all before the loop: otherwise it waits for everything each time around.)
+    load(ring(std::integral_constant<int, R - 1>()), 0, 0, (int)0x80000000);
+    auto begin_stage = [&](auto index) {
+      constexpr int I = decltype(index)::value;
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) load(ring(index), first + I, j, ends.past(first + I));
+    };
+    begin_all(begin_stage, std::make_integer_sequence<int, R - 1>());
+    arrivals();
+  }
   barrier();
   fetch(lds0, 0);
   while (!step_all(step, std::make_integer_sequence<int, R % 2 ? 2 * R : R>())) {}
@@ -791,8 +824,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void linear_few_kernel(Args a) {
 
 // ------------------------------------------------------------------ rows that direct loads cannot take
 // Direct loads to LDS bring 16 bytes from a multiple of 16, and a row's last 16 must not reach into what follows.
-// Other rows (an odd length, an odd column of a wider buffer) are copied into rows of a multiple of 64 values, zeros
-// after their own.  Bound by its launch at small sizes: 999 and 777 rows of 1001 5.1 us from memory.
+// Other rows (an odd length, an odd column of a wider buffer) go by registers (ROWS64x64) or, where that would take
+// longer, are copied into rows of a multiple of 64 values, zeros after their own: 7000 rows of 5001 39 us, 3.6 TB/s, 999 and 777 rows of 1001 5.1.  Rows that they can take are not copied,
+// though 128 bytes of them straddle two lines: 16384 x 5000 -> 5000 729 us, copied 720; 4096 x 5000 -> 4096 151, 150; 2000 x
+// 1000 -> 2000 18, 26.
 struct PadArgs {
   struct Matrix {
     const uint16_t* from;
@@ -822,11 +857,12 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
 }
 
 // ------------------------------------------------------------------ launches
-enum Kernel { T64x32, T32x64, T64x64, T96x64, T96x128, T128x128, WIDE256, KERNELS };
+// (ROWS64x64: rows at any address)
+enum Kernel { T64x32, T32x64, T64x64, T96x64, T96x128, T128x128, WIDE256, ROWS64x64, KERNELS };
 
 // A kernel's tile and what its time is made of, in us: the launch, a round of 256 workgroups, a round's stage of 64
 // features, what a stage takes longer when all CUs are at it, each megabyte of rows and weight, and, in parts, the join and
-// each megabyte of their sums.  Fitted to 2523 times of 175 sizes whose operands come from memory, which they meet to 13%
+// each megabyte of their sums.  Fitted to 2950 times of 335 sizes whose operands come from memory, which they meet to 13%
 // (one sigma).
 struct Shape {
   int tc, tt;
@@ -836,9 +872,10 @@ constexpr Shape SHAPES[KERNELS] = {
     {64, 32, 3.25f, 1.7f, 0.158f, 0.000f, 0.173f, 3.7f, 0.35f},  {32, 64, 2.3f, 3.1f, 0.153f, 0.043f, 0.143f, 3.5f, 0.53f},
     {64, 64, 2.35f, 3.3f, 0.200f, 0.066f, 0.155f, 3.0f, 0.58f},  {96, 64, 2.6f, 5.1f, 0.261f, 0.055f, 0.143f, 1.3f, 0.77f},
     {96, 128, 2.2f, 7.8f, 0.393f, 0.053f, 0.132f, 0.1f, 0.68f},  {128, 128, 4.3f, 6.75f, 0.435f, 0.142f, 0.124f, 0.0f, 0.51f},
-    {256, 256, 8.45f, 2.9f, 1.122f, 0.224f, 0.071f, 0.0f, 0.37f},
+    {256, 256, 8.45f, 2.9f, 1.122f, 0.224f, 0.071f, 0.0f, 0.37f}, {64, 64, 4.4f, 2.35f, 0.275f, 0.033f, 0.207f, 3.0f, 0.40f},
 };
-constexpr float WIDE_ANY_ROUND = 36.f;  // (tiles that are not whole)
+constexpr float WIDE_ANY_ROUND = 36.f;              // (tiles that are not whole)
+constexpr float COPY = 4.7f, COPY_MEGABYTE = 0.11f;  // (of rows that are copied first, read and written)
 
 // Tiles of TC x TT of both sets.
 int64_t tiles_of(const Args& a, int count, int tc, int tt) {
@@ -851,6 +888,7 @@ int64_t tiles_of(const Args& a, int count, int tc, int tt) {
 struct Choice {
   Kernel kernel;
   int splits;
+  float us;
 };
 
 int64_t sums_bytes(const Args& a, int splits) {
@@ -890,19 +928,20 @@ float estimate(const Args& a, int count, Kernel k, int splits) {
 // idle over many features; they are tried while all their workgroups fit the card at once, with four stages each or more.
 // Measured, the best of one part / the parts: 99 x 8472 -> 64 30.4 / 9.9 us, 512 x 12288 -> 3072 72.8 / 60 (eight of the
 // wide kernel), 1280 x 13824 -> 5120 251 / 171 (two of it).  Over the 175 sizes the choice takes 1.9% more time than the
-// best of all, and the best of one part 13.9%.
-Choice choose(const Args& a, int count) {
-  Choice best = {WIDE256, 1};
-  float least = estimate(a, count, WIDE256, 1);
+// best of all, and the best of one part 13.9%.  Rows that direct loads cannot take are copied, or not, by the same measure.
+// Copied / as they are: 999 x 1001 -> 777 14.0 / 11.7 us, 2405 x 13 -> 20 11.0 / 7.2, 64 x 12001 -> 17000 262 / 219, 2000 x
+// 5001 -> 5000 144 / 345; over 160 such sizes the choice takes 0.8% more than the better one, copies alone 27%.
+Choice choose(const Args& a, int count, int first, int last) {
+  Choice best = {(Kernel)last, 1, estimate(a, count, (Kernel)last, 1)};
   const int stages = (a.features + 63) / 64;
-  for (int i = 0; i < KERNELS; ++i) {
+  for (int i = first; i <= last; ++i) {
     const Kernel k = (Kernel)i;
     const int64_t tiles = tiles_of(a, count, SHAPES[k].tc, SHAPES[k].tt);
     if (tiles >= (1 << 21)) continue;  // (a grid holds fewer than 2^32 threads)
     for (int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (splits > 1 && (tiles * splits > 256 || stages < 4 * splits)) break;
       const float us = estimate(a, count, k, splits);
-      if (us < least) best = {k, splits}, least = us;
+      if (us < best.us) best = {k, splits, us};
     }
   }
   return best;
@@ -928,6 +967,7 @@ int launch_kernel(Args& a, int count, const Choice& choice, hipStream_t st) {
     case T96x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 96, 64, 7, 8>), each, eight, 0, st, a); break;
     case T96x128: hipLaunchKernelGGL((linear_tile_kernel<F16, 96, 128, 5, 8>), each, eight, 0, st, a); break;
     case T128x128: hipLaunchKernelGGL((linear_tile_kernel<F16, 128, 128, 4, 8>), each, eight, 0, st, a); break;
+    case ROWS64x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 64, 64, 4, 8, 4>), each, eight, 0, st, a); break;
     default: {
       const uint32_t per_xcd = std::max(1, device_cu_count() / 8);
       const dim3 grid(8 * std::min(a.tiles_xcd, per_xcd)), block(64 * WIDE_WAVES);
@@ -995,6 +1035,8 @@ int plan(Plan& p, int32_t count, int32_t batch, const int32_t* rows, int32_t col
     HB_REQUIRE(batch > 0 && rows[i] > 0 && (int64_t)batch * rows[i] < (1ll << 31), "batch and rows must be positive, with fewer than 2^31 rows in all");
     p.few &= (int64_t)batch * rows[i] <= FEW_ROWS;
   }
+  bool copied[2][2] = {};
+  float megabytes = 0.f;
   p.pad.features = features;
   p.pad.padded = (features + 63) / 64 * 64;
   for (int i = 0; i < count; ++i) {
@@ -1008,7 +1050,17 @@ int plan(Plan& p, int32_t count, int32_t batch, const int32_t* rows, int32_t col
     s = {(const uint16_t*)q[0], (const uint16_t*)q[1], (const uint16_t*)q[2], (const uint16_t*)q[3], (const uint16_t*)q[4],
          (uint16_t*)q[5], st[0], st[1], st[2], st[3], st[4], st[5], st[6], st[7], (uint32_t)rows[i], (uint32_t)(batch * rows[i])};
     a.vectors &= aligned16(s.out) && s.out_b % 8 == 0 && s.out_n % 8 == 0;
-    if (p.few) continue;
+    copied[i][0] = !p.few && !direct(s.x, batch, rows[i], s.x_b, s.x_n, features);
+    copied[i][1] = !p.few && !direct(s.w, 1, columns, 0, s.w_n, features);
+    megabytes += 2e-6f * (float)(features + p.pad.padded) * ((copied[i][0] ? (float)s.tokens : 0.f) + (copied[i][1] ? (float)columns : 0.f));
+  }
+  if (p.few) return HB_OK;
+  p.choice = choose(a, count, T64x32, WIDE256);
+  if (megabytes > 0.f && features >= 8 && tiles_of(a, count, 64, 64) < (1 << 21)) {
+    const Choice as_they_are = choose(a, count, ROWS64x64, ROWS64x64);
+    if (as_they_are.us < p.choice.us + COPY + COPY_MEGABYTE * megabytes) p.choice = as_they_are;
+  }
+  if (p.choice.kernel != ROWS64x64) {
     auto copy = [&](const uint16_t*& from, int64_t& b, int64_t& n, uint32_t rows_of_one, uint32_t all) {
       uint16_t* const to = (uint16_t*)((char*)workspace + p.bytes);
       p.bytes += padded_bytes(all, features);
@@ -1019,17 +1071,17 @@ int plan(Plan& p, int32_t count, int32_t batch, const int32_t* rows, int32_t col
       n = p.pad.padded;
       b = n * rows_of_one;
     };
-    if (!direct(s.x, batch, rows[i], s.x_b, s.x_n, features)) copy(s.x, s.x_b, s.x_n, s.rows, s.tokens);
     int64_t none = 0;
-    if (!direct(s.w, 1, columns, 0, s.w_n, features)) copy(s.w, none, s.w_n, (uint32_t)columns, (uint32_t)columns);
+    for (int i = 0; i < count; ++i) {
+      Set& s = a.set[i];
+      if (copied[i][0]) copy(s.x, s.x_b, s.x_n, s.rows, s.tokens);
+      if (copied[i][1]) copy(s.w, none, s.w_n, (uint32_t)columns, (uint32_t)columns);
+    }
+    for (int i = p.copies; i < 4; ++i) p.pad.first[i + 1] = p.pad.first[p.copies];
+    if (p.copies && features % 8) a.features = p.pad.padded;  // (then every matrix is a copy)
   }
-  for (int i = p.copies; i < 4; ++i) p.pad.first[i + 1] = p.pad.first[p.copies];
-  if (p.copies && features % 8) a.features = p.pad.padded;  // (then every matrix is a copy)
-  if (!p.few) {
-    p.choice = choose(a, count);
-    a.sums = (float*)((char*)workspace + p.bytes);
-    p.bytes += sums_bytes(a, p.choice.splits);
-  }
+  a.sums = (float*)((char*)workspace + p.bytes);
+  p.bytes += sums_bytes(a, p.choice.splits);
   return HB_OK;
 }
 

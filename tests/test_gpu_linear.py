@@ -53,8 +53,20 @@ def test_sizes(rows, K, N, dtype):
 EPILOGUES = [(act, bias, more) for act in (None, "gelu", "silu") for bias in (True, False) for more in ("", "residual", "gate")]
 
 
+# rows that are no multiple of 16 bytes: copied first, where that pays, or not
+@pytest.mark.parametrize("dtype", [BF16, HALF])
+@pytest.mark.parametrize("rows, K, N", [(17, 3, 40), (17, 9, 16), (20, 13, 2405), (65, 63, 65), (64, 57, 64), (130, 58, 129), (300, 71, 1000), (999, 1001, 777),
+                                        (77, 4097, 3072), (40, 5003, 500), (18, 7001, 33), (2000, 5001, 5000), (600, 2999, 4001)])
+def test_rows_of_odd_lengths(rows, K, N, dtype):
+    x, layer = _normal(rows, K, dtype=dtype), _layer(K, N, dtype)
+    _check(linear(x, **layer), x=x, **layer)
+    pair = linear_pair(dict(x=x[None], **layer), dict(x=x[None, 5:17], **layer))
+    for got, rows_of in zip(pair, (x, x[5:17])):
+        _check(got[0], x=rows_of, **layer)
+
+
 @pytest.mark.parametrize("act, bias, more", EPILOGUES)
-@pytest.mark.parametrize("batch, rows, K, N", [(1, 1, 64, 100), (3, 5, 200, 72), (2, 33, 96, 200), (3, 170, 136, 1000), (2, 2048, 128, 4096),
+@pytest.mark.parametrize("batch, rows, K, N", [(3, 61, 99, 201), (1, 1, 64, 100), (3, 5, 200, 72), (2, 33, 96, 200), (3, 170, 136, 1000), (2, 2048, 128, 4096),
                                                (3, 1365, 128, 4096)])
 def test_epilogues(batch, rows, K, N, act, bias, more):
     x, layer = _normal(batch, rows, K), _layer(K, N, bias=bias)

@@ -146,20 +146,23 @@ def test_workspaces():
         parts = _workspace(rows, columns, features)[0] / (rows * columns * 4)
         assert parts in (2, 3, 4, 6, 8, 12, 16)
     assert _workspace(126, 27, 13952)[0] % (126 * 32 * 4) == 0
-    # rows and weights that are no multiple of 16 bytes
-    assert _workspace(300, 1000, 60)[0] == 1300 * 64 * 2
-    assert _workspace(300, 1000, 64, x=HELD + 2)[0] == 300 * 64 * 2
-    assert _workspace(300, 1000, 64, row=67)[0] == 300 * 64 * 2
-    assert _workspace(300, 1000, 60, count=2)[0] == 2 * 1300 * 64 * 2
-    # rows too far apart for one load's offset
-    assert _workspace(300, 1000, 64, row=1 << 23)[0] == 300 * 64 * 2
+    # rows and weights that direct loads cannot take (their strides, their address, too far apart), where copies pay
+    both, rows = 7000 * 5056 * 2, 2000 * 5056 * 2
+    assert _workspace(2000, 5000, 5001)[0] == both and _workspace(2000, 5000, 5001, count=2)[0] == 2 * both
+    assert _workspace(2000, 5000, 5056, x=HELD + 2)[0] == rows
+    assert _workspace(2000, 5000, 5056, row=5057)[0] == rows
+    assert _workspace(2000, 5000, 5056, row=1 << 23)[0] == rows
+    assert _workspace(2000, 5000, 3)[0] == 7000 * 64 * 2  # (rows of fewer than eight)
+    # and where they do not
+    for size in ((300, 1000, 60), (999, 777, 1001), (2405, 20, 13)):
+        assert _workspace(*size)[0] == 0
     for bad in (dict(rows=0), dict(columns=0), dict(features=0), dict(features=(1 << 20) + 1), dict(columns=(1 << 25) + 1), dict(count=0), dict(count=3), dict(batch=0),
                 dict(x=None), dict(x=HELD + 1), dict(row=-8)):
         assert _workspace(**(dict(rows=300, columns=1000, features=64) | bad))[0] == -1
 
 
 def test_a_workspace_too_small_is_refused():
-    for sizes in ((126, 32, 13952), (300, 1000, 60)):
+    for sizes in ((126, 32, 13952), (2000, 5000, 5001)):
         bytes, call, pointers, strides = _workspace(*sizes)
         assert bytes > 0
         for workspace, held in ((None, bytes), (HELD, bytes - 1), (HELD + 8, bytes)):
