@@ -857,25 +857,30 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
 }
 
 // ------------------------------------------------------------------ launches
-// (ROWS64x64: rows at any address)
-enum Kernel { T64x32, T32x64, T64x64, T96x64, T96x128, T128x128, WIDE256, ROWS64x64, KERNELS };
+// (TWO64x64: with half the stages in LDS, so that a CU has two workgroups; ROWS64x64: the same of rows at any address)
+enum Kernel { T64x32, T32x64, T64x64, TWO64x64, T96x64, T96x128, T128x128, WIDE256, ROWS64x64, KERNELS };
 
-// A kernel's tile and what its time is made of, in us: the launch, a round of 256 workgroups, a round's stage of 64
-// features, what a stage takes longer when all CUs are at it, each megabyte of rows and weight, and, in parts, the join and
-// each megabyte of their sums.  Fitted to 2950 times of 335 sizes whose operands come from memory, which they meet to 13%
-// (one sigma).
+// A kernel's tile, how many workgroups the card holds at once, and what its time is made of, in us: the launch, a round of so
+// many workgroups, a round's stage of 64 features, what a stage takes longer when all CUs are at it, each megabyte of rows
+// and weight, each million outputs, and, in parts, the join and each megabyte of their sums.  Fitted to 4418 times of 424 sizes
+// whose operands come from memory, which they meet to 12% (one sigma).
 struct Shape {
   int tc, tt;
-  float launch, round, stage, full, megabyte, join, sums;
+  float at_once, launch, round, stage, full, megabyte, outputs, join, sums;
 };
 constexpr Shape SHAPES[KERNELS] = {
-    {64, 32, 3.25f, 1.7f, 0.158f, 0.000f, 0.173f, 3.7f, 0.35f},  {32, 64, 2.3f, 3.1f, 0.153f, 0.043f, 0.143f, 3.5f, 0.53f},
-    {64, 64, 2.35f, 3.3f, 0.200f, 0.066f, 0.155f, 3.0f, 0.58f},  {96, 64, 2.6f, 5.1f, 0.261f, 0.055f, 0.143f, 1.3f, 0.77f},
-    {96, 128, 2.2f, 7.8f, 0.393f, 0.053f, 0.132f, 0.1f, 0.68f},  {128, 128, 4.3f, 6.75f, 0.435f, 0.142f, 0.124f, 0.0f, 0.51f},
-    {256, 256, 8.45f, 2.9f, 1.122f, 0.224f, 0.071f, 0.0f, 0.37f}, {64, 64, 4.4f, 2.35f, 0.275f, 0.033f, 0.207f, 3.0f, 0.40f},
+    {64, 32, 256.f, 4.4f, 1.0f, 0.148f, 0.002f, 0.172f, 1.39f, 3.7f, 0.00f},
+    {32, 64, 256.f, 3.0f, 2.4f, 0.147f, 0.043f, 0.145f, 1.36f, 3.7f, 0.00f},
+    {64, 64, 256.f, 3.4f, 2.3f, 0.196f, 0.063f, 0.153f, 1.09f, 3.3f, 0.28f},
+    {64, 64, 512.f, 3.7f, 1.9f, 0.231f, 0.231f, 0.169f, 0.95f, 3.0f, 0.40f},
+    {96, 64, 256.f, 3.8f, 3.5f, 0.261f, 0.050f, 0.150f, 1.12f, 2.0f, 0.43f},
+    {96, 128, 256.f, 5.9f, 3.6f, 0.400f, 0.033f, 0.130f, 1.40f, 0.9f, 0.51f},
+    {128, 128, 256.f, 8.0f, 2.7f, 0.454f, 0.058f, 0.128f, 1.57f, 0.0f, 0.48f},
+    {256, 256, 256.f, 5.6f, 1.5f, 1.133f, 0.081f, 0.085f, 0.82f, 3.9f, 0.36f},
+    {64, 64, 512.f, 2.4f, 4.3f, 0.270f, 0.345f, 0.236f, 0.60f, 2.9f, 0.81f},
 };
-constexpr float WIDE_ANY_ROUND = 36.f;              // (tiles that are not whole)
-constexpr float COPY = 4.7f, COPY_MEGABYTE = 0.11f;  // (of rows that are copied first, read and written)
+constexpr float WIDE_ANY_ROUND = 28.6f;              // (tiles that are not whole)
+constexpr float COPY = 4.3f, COPY_MEGABYTE = 0.116f;  // (of rows that are copied first, read and written)
 
 // Tiles of TC x TT of both sets.
 int64_t tiles_of(const Args& a, int count, int tc, int tt) {
@@ -914,12 +919,13 @@ Mode mode_of(const Args& a, int count) {
 // What a kernel takes for the sets, in us (whatever the activation, so that the workspace is known without it).
 float estimate(const Args& a, int count, Kernel k, int splits) {
   const Shape& s = SHAPES[k];
-  const float rounds = (float)(tiles_of(a, count, s.tc, s.tt) * splits) / 256.f, whole = std::floor(rounds), rest = rounds - whole;
+  const float rounds = (float)(tiles_of(a, count, s.tc, s.tt) * splits) / s.at_once, whole = std::floor(rounds), rest = rounds - whole;
   const float stages = (float)(((a.features + 63) / 64 + splits - 1) / splits);
   const float round = k == WIDE256 && splits == 1 && !whole_tiles(a, count) ? WIDE_ANY_ROUND : s.round;
-  const float rows = (float)a.set[0].tokens + (float)a.set[1].tokens + (float)count * (float)a.columns;
+  const float tokens = (float)a.set[0].tokens + (float)a.set[1].tokens, rows = tokens + (float)count * (float)a.columns;
   float us = s.launch + whole * (round + stages * (s.stage + s.full)) +
-             (rest > 0.f ? round + stages * (s.stage + s.full * rest * rest) : 0.f) + s.megabyte * 2e-6f * rows * (float)a.features;
+             (rest > 0.f ? round + stages * (s.stage + s.full * rest * rest) : 0.f) + s.megabyte * 2e-6f * rows * (float)a.features +
+             s.outputs * 1e-6f * tokens * (float)a.columns;
   if (splits > 1) us += s.join + s.sums * 1e-6f * (float)sums_bytes(a, splits);
   return us;
 }
@@ -927,10 +933,12 @@ float estimate(const Args& a, int count, Kernel k, int splits) {
 // The kernel, and the parts that it takes the features in, of the least estimate.  Parts pay where few tiles leave CUs
 // idle over many features; they are tried while all their workgroups fit the card at once, with four stages each or more.
 // Measured, the best of one part / the parts: 99 x 8472 -> 64 30.4 / 9.9 us, 512 x 12288 -> 3072 72.8 / 60 (eight of the
-// wide kernel), 1280 x 13824 -> 5120 251 / 171 (two of it).  Over the 175 sizes the choice takes 1.9% more time than the
-// best of all, and the best of one part 13.9%.  Rows that direct loads cannot take are copied, or not, by the same measure.
+// wide kernel), 1280 x 13824 -> 5120 251 / 171 (two of it).  Over 264 sizes the choice takes 1.6% more time than the best of
+// all; the best of one part takes 13.9% more over 175 of them.  TWO64x64 pays where many tiles are short: the best of the
+// others / with it 5993 x 128 -> 2752 47.5 / 39.5, 4576 x 64 -> 960 16.6 / 12.8, 657 x 1216 -> 2624 16.2 / 13.7; alone on
+// its CU it is slower (77 x 4096 -> 3072 27.6, T64x64 21.9); without it the choice takes 5.8% more than the best.  Rows that direct loads cannot take are copied, or not, by the same measure.
 // Copied / as they are: 999 x 1001 -> 777 14.0 / 11.7 us, 2405 x 13 -> 20 11.0 / 7.2, 64 x 12001 -> 17000 262 / 219, 2000 x
-// 5001 -> 5000 144 / 345; over 160 such sizes the choice takes 0.8% more than the better one, copies alone 27%.
+// 5001 -> 5000 144 / 345; over 160 such sizes the choice takes 1.0% more than the better one, copies alone 27%.
 Choice choose(const Args& a, int count, int first, int last) {
   Choice best = {(Kernel)last, 1, estimate(a, count, (Kernel)last, 1)};
   const int stages = (a.features + 63) / 64;
@@ -964,6 +972,7 @@ int launch_kernel(Args& a, int count, const Choice& choice, hipStream_t st) {
     case T64x32: hipLaunchKernelGGL((linear_tile_kernel<F16, 64, 32, 6, 4>), each, four, 0, st, a); break;
     case T32x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 32, 64, 8, 4>), each, four, 0, st, a); break;
     case T64x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 64, 64, 8, 8>), each, eight, 0, st, a); break;
+    case TWO64x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 64, 64, 4, 8>), each, eight, 0, st, a); break;
     case T96x64: hipLaunchKernelGGL((linear_tile_kernel<F16, 96, 64, 7, 8>), each, eight, 0, st, a); break;
     case T96x128: hipLaunchKernelGGL((linear_tile_kernel<F16, 96, 128, 5, 8>), each, eight, 0, st, a); break;
     case T128x128: hipLaunchKernelGGL((linear_tile_kernel<F16, 128, 128, 4, 8>), each, eight, 0, st, a); break;
