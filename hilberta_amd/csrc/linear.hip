@@ -858,7 +858,7 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
 
 // ------------------------------------------------------------------ launches
 // (TWO64x64: with half the stages in LDS, so that a CU has two workgroups; ROWS64x64: the same of rows at any address)
-enum Kernel { T64x32, T32x64, T64x64, TWO64x64, T96x64, T96x128, T128x128, WIDE256, ROWS64x64, KERNELS };
+enum Kernel { T64x32, T32x64, T64x64, TWO64x64, T96x64, T96x128, T128x128, WIDE256, ROWS64x64, KERNELS, FEW16 = KERNELS };
 
 // A kernel's tile, how many workgroups the card holds at once, and what its time is made of, in us: the launch, a round of so
 // many workgroups, a round's stage of 64 features, what a stage takes longer when all CUs are at it, each megabyte of rows
@@ -928,6 +928,17 @@ float estimate(const Args& a, int count, Kernel k, int splits) {
              s.outputs * 1e-6f * tokens * (float)a.columns;
   if (splits > 1) us += s.join + s.sums * 1e-6f * (float)sums_bytes(a, splits);
   return us;
+}
+
+// The same of linear_few_kernel: a wave's way through the features, or the read of the weights; both are slower for rows that
+// begin between 16 bytes.  What bounds a few rows, it / the others, us: 1 x 3072 -> 4096 8.2 / 11.6, 16 rows of it 9.7 / 12.4;
+// many features, 8 x 12288 -> 512 25.1 / 11.4 (in parts), or the weights of more rows, 16 x 3072 -> 9216 22.9 / 17.4, 8 x 14633
+// -> 9216 176 / 132.
+float estimate_few(const Args& a, int count, bool aligned) {
+  const float tokens = (float)std::max(a.set[0].tokens, a.set[1].tokens), slower = aligned ? 1.f : 1.6f + 0.05f * tokens;
+  const float megabytes = 2e-6f * (float)count * (float)a.columns * (float)a.features;
+  return std::max(2.3f + (float)a.features / 1024.f * (1.65f + 0.027f * tokens) * slower,
+                  3.f + megabytes * (0.25f + 0.007f * tokens) * slower);
 }
 
 // The kernel, and the parts that it takes the features in, of the least estimate.  Parts pay where few tiles leave CUs
@@ -1022,7 +1033,6 @@ struct Plan {
   Args a;
   PadArgs pad;
   Choice choice;
-  bool few;
   int copies;
   int64_t bytes;  // of copied rows, and of all
 };
@@ -1039,10 +1049,10 @@ int plan(Plan& p, int32_t count, int32_t batch, const int32_t* rows, int32_t col
   a.features = features;
   a.act = act;
   a.vectors = 1;
-  p.few = true;
+  bool few = true;
   for (int i = 0; i < count; ++i) {
     HB_REQUIRE(batch > 0 && rows[i] > 0 && (int64_t)batch * rows[i] < (1ll << 31), "batch and rows must be positive, with fewer than 2^31 rows in all");
-    p.few &= (int64_t)batch * rows[i] <= FEW_ROWS;
+    few &= (int64_t)batch * rows[i] <= FEW_ROWS;
   }
   bool copied[2][2] = {};
   float megabytes = 0.f;
@@ -1059,17 +1069,20 @@ int plan(Plan& p, int32_t count, int32_t batch, const int32_t* rows, int32_t col
     s = {(const uint16_t*)q[0], (const uint16_t*)q[1], (const uint16_t*)q[2], (const uint16_t*)q[3], (const uint16_t*)q[4],
          (uint16_t*)q[5], st[0], st[1], st[2], st[3], st[4], st[5], st[6], st[7], (uint32_t)rows[i], (uint32_t)(batch * rows[i])};
     a.vectors &= aligned16(s.out) && s.out_b % 8 == 0 && s.out_n % 8 == 0;
-    copied[i][0] = !p.few && !direct(s.x, batch, rows[i], s.x_b, s.x_n, features);
-    copied[i][1] = !p.few && !direct(s.w, 1, columns, 0, s.w_n, features);
+    copied[i][0] = !direct(s.x, batch, rows[i], s.x_b, s.x_n, features);
+    copied[i][1] = !direct(s.w, 1, columns, 0, s.w_n, features);
     megabytes += 2e-6f * (float)(features + p.pad.padded) * ((copied[i][0] ? (float)s.tokens : 0.f) + (copied[i][1] ? (float)columns : 0.f));
   }
-  if (p.few) return HB_OK;
   p.choice = choose(a, count, T64x32, WIDE256);
-  if (megabytes > 0.f && features >= 8 && tiles_of(a, count, 64, 64) < (1 << 21)) {
-    const Choice as_they_are = choose(a, count, ROWS64x64, ROWS64x64);
-    if (as_they_are.us < p.choice.us + COPY + COPY_MEGABYTE * megabytes) p.choice = as_they_are;
+  if (megabytes > 0.f) {
+    p.choice.us += COPY + COPY_MEGABYTE * megabytes;
+    if (features >= 8 && tiles_of(a, count, 64, 64) < (1 << 21)) {
+      const Choice as_they_are = choose(a, count, ROWS64x64, ROWS64x64);
+      if (as_they_are.us < p.choice.us) p.choice = as_they_are;
+    }
   }
-  if (p.choice.kernel != ROWS64x64) {
+  if (few && estimate_few(a, count, megabytes == 0.f) < p.choice.us) p.choice = {FEW16, 1};
+  if (p.choice.kernel < ROWS64x64) {
     auto copy = [&](const uint16_t*& from, int64_t& b, int64_t& n, uint32_t rows_of_one, uint32_t all) {
       uint16_t* const to = (uint16_t*)((char*)workspace + p.bytes);
       p.bytes += padded_bytes(all, features);
@@ -1100,7 +1113,7 @@ int launch(Plan& p, int count, hipStream_t st) {
     hipLaunchKernelGGL(pad_rows_kernel, dim3(std::min(p.pad.first[p.copies], PAD_GROUPS)), dim3(256), 0, st, p.pad);
     HB_HIP(hipGetLastError());
   }
-  if (!p.few) return launch_kernel<F16>(p.a, count, p.choice, st);
+  if (p.choice.kernel != FEW16) return launch_kernel<F16>(p.a, count, p.choice, st);
   p.a.tiles0 = (uint32_t)((p.a.columns + 15) / 16);
   hipLaunchKernelGGL((linear_few_kernel<F16>), dim3(p.a.tiles0 * count), dim3(64 * FEW_WAVES), 0, st, p.a);
   HB_HIP(hipGetLastError());

@@ -11,7 +11,7 @@ sets with weights of their own (a block's text and image rows) in one launch.
 
 Inference only: inputs that need a gradient are refused.  Launches are asynchronous on the current stream and can
 be captured into a graph.  Rows, weights and outputs may be row ranges or column blocks of larger buffers; rows
-that are no multiple of 16 bytes are copied into aligned ones first, and a long sum for few outputs is made in
+that are no multiple of 16 bytes may be copied into aligned ones first, and a long sum for few outputs is made in
 parts, joined in their order; both take a workspace for the call.  The reference has library calls here (in the
 transformer that hilberta/flux_adapter.py wraps).
 """

@@ -243,8 +243,8 @@ int hb_group_norm(int32_t batch, int64_t pixels, int32_t channels, int32_t group
  * elements, last dimensions contiguous.  out may be the residual itself; it may lie over nothing else that is read.
  * features up to 2^20, columns up to 2^25.  Rows may begin at any element.  `workspace` (hb_linear_workspace_bytes, 0
  * where none is needed and -1 where the sizes are rejected; 16-byte aligned, contents irrelevant before and after) holds x
- * and weights whose rows are no multiples of 16 bytes or lie too far apart, copied first unless both sets have at most 16
- * rows, and the sums of the parts that the features of few rows and columns are taken in. */
+ * and weights whose rows are no multiples of 16 bytes or lie too far apart, where copying them first pays, and the sums
+ * of the parts that the features of few rows and columns are taken in. */
 int64_t hb_linear_workspace_bytes(int32_t count, int32_t batch, const int32_t* rows, int32_t columns,
                                   int32_t features, void* const* pointers, const int64_t* strides);
 int hb_linear(int32_t count, int32_t batch, const int32_t* rows, int32_t columns, int32_t features,

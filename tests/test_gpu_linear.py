@@ -98,7 +98,8 @@ def test_long_sums():
 
 # few tiles over many features, which several workgroups share
 PARTS = [(126, 13952, 27), (383, 5200, 5024), (127, 8104, 5270), (17, 1543, 16), (20, 3001, 100), (100, 12345, 300), (1000, 8192, 520),
-         (512, 12288, 3072), (700, 9001, 1500), (1100, 8200, 1001), (513, 6000, 2048)]
+         (512, 12288, 3072), (700, 9001, 1500), (1100, 8200, 1001), (513, 6000, 2048),
+         (1, 12288, 10), (8, 12288, 512), (16, 14633, 129), (5, 7000, 1024)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, HALF])

@@ -139,10 +139,10 @@ def _workspace(rows, columns, features, *, x=HELD, row=None, count=1, batch=1):
 
 def test_workspaces():
     # whole tiles, or enough of them: nothing
-    for rows, columns, features in ((4096, 9216, 3072), (1, 18432, 3072), (16, 5, 12345), (77, 64, 64)):
+    for rows, columns, features in ((4096, 9216, 3072), (1, 18432, 3072), (16, 5, 1001), (77, 64, 64)):
         assert _workspace(rows, columns, features)[0] == 0
     # few tiles over many features: the sums of parts of them
-    for rows, columns, features in ((126, 32, 13952), (100, 304, 12288), (512, 3072, 12288)):
+    for rows, columns, features in ((126, 32, 13952), (100, 304, 12288), (512, 3072, 12288), (8, 512, 12288)):
         parts = _workspace(rows, columns, features)[0] / (rows * columns * 4)
         assert parts in (2, 3, 4, 6, 8, 12, 16)
     assert _workspace(126, 27, 13952)[0] % (126 * 32 * 4) == 0
