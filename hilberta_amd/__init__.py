@@ -10,12 +10,13 @@ rebuilt on hand-written HIP kernels behind a C ABI (include/hilberta_hip.h):
                     block-sparse flash-attention forward (bf16/fp16 MFMA, persistent)
   flux_inputs / flux_norm
                     FLUX attention inputs (RMSNorm + rotary + [text; image] layout) and the
-                    gated-residual AdaLN pass, one HIP kernel each
+                    gated-residual AdaLN pass, one HIP kernel each; the image decoder's group norm
   flux_model / sampling_layout
                     a FLUX-shaped denoiser step on these kernels and the sampling-scope layout
   flux_cond         conditioning layers of a few rows (embedders, modulations), streamed by HIP
   flux_int8         the blocks' linear layers in 8-bit integers: rows, AdaLN rows, products, and the Q/K/V
                     projection with the heads' RMSNorm and rotation in the same pass
+  flux_linear       linear layers in 16 bits with bias, activation, gate and residual in the same pass
   ops               the entry points as native torch operators (torch.ops.hilberta_hip.*), with
                     fake implementations for tracing
 
