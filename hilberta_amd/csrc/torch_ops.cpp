@@ -803,12 +803,17 @@ void linear_out(const Tensor& x, const Tensor& weight, const Maybe& bias, const 
   linear_sets({{x, weight, bias, residual, gate, out}}, act);
 }
 
-Tensor linear(const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& residual, const Maybe& gate, int64_t act) {
+// An output of the rows x by the layer of `weight`.
+Tensor linear_output(const Tensor& x, const Tensor& weight) {
   TORCH_CHECK_VALUE((x.dim() == 2 || x.dim() == 3) && weight.dim() == 2,
                     "x must be [rows, features] or [B, rows, features] and weight [out_features, features]");
   c10::SmallVector<int64_t, 3> sizes(x.sizes().begin(), x.sizes().end());
   sizes.back() = weight.size(0);
-  Tensor out = new_tensor(x, sizes, x.scalar_type());
+  return new_tensor(x, sizes, x.scalar_type());
+}
+
+Tensor linear(const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& residual, const Maybe& gate, int64_t act) {
+  Tensor out = linear_output(x, weight);
   linear_out(x, weight, bias, residual, gate, out, act);
   return out;
 }
@@ -817,6 +822,14 @@ void linear_pair_out(const Tensor& x, const Tensor& weight, const Maybe& bias, c
                      Tensor out, const Tensor& x2, const Tensor& weight2, const Maybe& bias2, const Maybe& residual2,
                      const Maybe& gate2, Tensor out2, int64_t act) {
   linear_sets({{x, weight, bias, residual, gate, out}, {x2, weight2, bias2, residual2, gate2, out2}}, act);
+}
+
+std::tuple<Tensor, Tensor> linear_pair(const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& residual,
+                                       const Maybe& gate, const Tensor& x2, const Tensor& weight2, const Maybe& bias2,
+                                       const Maybe& residual2, const Maybe& gate2, int64_t act) {
+  Tensor out = linear_output(x, weight), out2 = linear_output(x2, weight2);
+  linear_pair_out(x, weight, bias, residual, gate, out, x2, weight2, bias2, residual2, gate2, out2, act);
+  return {out, out2};
 }
 
 // ------------------------------------------------------------------ group norm
@@ -897,7 +910,7 @@ Tensor group_norm(const Tensor& x, int64_t groups, const Maybe& weight, const Ma
 // (the layers' operators that return their results write nothing)
 constexpr const char* WRITING[] = {"paired_fwd", "sparse_fwd", "int8_adaln", "int8_adaln_pair", "int8_linear_out",
                                    "int8_linear_pair_out", "int8_qkv_out", "linear_out", "linear_pair_out", "group_norm_out"};
-constexpr const char* RETURNING[] = {"int8_rows", "int8_linear", "int8_linear_rows", "int8_qkv", "linear", "group_norm"};
+constexpr const char* RETURNING[] = {"int8_rows", "int8_linear", "int8_linear_rows", "int8_qkv", "linear", "linear_pair", "group_norm"};
 
 // No derivative is recorded (the entry points refuse inputs that need one); a transform that takes one
 // is refused, as torch refuses an autograd.Function in one, for it would get zeros.
@@ -975,6 +988,7 @@ TORCH_LIBRARY(hilberta_hip, m) {
   m.def(("int8_qkv_out(" + qkv + "Tensor(a16!) out, float eps) -> ()").c_str(), tags);
   const std::string dense = "Tensor x$, Tensor weight$, Tensor? bias$, Tensor? residual$, Tensor? gate$, ";
   m.def(("linear(" + set(dense, "") + "SymInt act) -> Tensor").c_str(), tags);
+  m.def(("linear_pair(" + set(dense, "") + set(dense, "2") + "SymInt act) -> (Tensor, Tensor)").c_str(), tags);
   const std::string into = dense + "Tensor(o$!) out$, ";
   m.def(("linear_out(" + set(into, "") + "SymInt act) -> ()").c_str(), tags);
   m.def(("linear_pair_out(" + set(into, "") + set(into, "2") + "SymInt act) -> ()").c_str(), tags);
@@ -999,6 +1013,7 @@ void layer_operators(torch::Library& m) {
   m.impl("group_norm_out", group_norm_out);
   m.impl("linear", linear);
   m.impl("linear_out", linear_out);
+  m.impl("linear_pair", linear_pair);
   m.impl("linear_pair_out", linear_pair_out);
   m.impl("int8_rows", int8_rows);
   m.impl("int8_adaln", int8_adaln);

@@ -44,16 +44,18 @@ def linear(x, weight, bias=None, *, act=None, residual=None, gate=None, out=None
 
 
 def _set(x, weight, bias=None, residual=None, gate=None, out=None):
-    """Arguments of one row set, its output made if it has none."""
-    if out is None:
-        out = torch.empty(*x.shape[:-1], weight.shape[0], dtype=x.dtype, device=x.device)
-    return (x, weight, bias, residual, gate, out), out
+    return (x, weight, bias, residual, gate), out
 
 
 def linear_pair(first, second, *, act=None):
     """linear of two row sets in one launch: ``first`` and ``second`` are dicts of x, weight, bias, residual,
     gate and out, of one batch, layer shape, dtype and device; either may have no rows.  Returns both outputs."""
-    a, out_a = _set(**first)
-    b, out_b = _set(**second)
-    ops.linear_pair_out(*a, *b, _act(act))
+    (a, out_a), (b, out_b) = _set(**first), _set(**second)
+    if out_a is None and out_b is None:
+        return ops.linear_pair(*a, *b, _act(act))
+    if out_a is None or out_b is None:
+        x, weight = (a if out_a is None else b)[:2]
+        made = torch.empty(*x.shape[:-1], weight.shape[0], dtype=x.dtype, device=x.device)
+        out_a, out_b = (made, out_b) if out_a is None else (out_a, made)
+    ops.linear_pair_out(*a, out_a, *b, out_b, _act(act))
     return out_a, out_b

@@ -25,7 +25,7 @@ implementation for tracing and, for pair_rows alone, a CPU one:
   hilberta_hip::int8_adaln_pair, int8_linear_pair_out: two row sets' arguments (the second's names end in 2)
   hilberta_hip::linear(x, weight, bias?, residual?, gate?, act) -> Tensor
   hilberta_hip::linear_out(.. as linear up to gate?, out!, act) -> ()
-  hilberta_hip::linear_pair_out: two row sets' arguments (the second's names end in 2)
+  hilberta_hip::linear_pair, linear_pair_out: two row sets' arguments (the second's names end in 2)
   hilberta_hip::group_norm(x, groups, weight?, bias?, silu, eps) -> Tensor
   hilberta_hip::group_norm_out(x, groups, weight?, bias?, out!, silu, eps) -> ()
 
@@ -94,6 +94,10 @@ def _fake_linear(x, weight, bias, residual, gate, act):
     return x.new_empty((*x.shape[:-1], weight.shape[0]))
 
 
+def _fake_linear_pair(x, weight, bias, residual, gate, x2, weight2, *args):
+    return _fake_linear(x, weight, None, None, None, 0), _fake_linear(x2, weight2, None, None, None, 0)
+
+
 def _fake_group_norm(x, groups, weight, bias, silu, eps):
     if x.ndim == 3:
         return x.new_empty(x.shape)
@@ -140,7 +144,7 @@ def _load():
                  int8_adaln_pair=_fake_int8_adaln_pair, int8_linear=_fake_int8_linear,
                  int8_linear_rows=_fake_int8_linear_rows, int8_linear_out=_fake_none,
                  int8_linear_pair_out=_fake_none, int8_qkv=_fake_int8_qkv, int8_qkv_out=_fake_none,
-                 linear=_fake_linear, linear_out=_fake_none, linear_pair_out=_fake_none,
+                 linear=_fake_linear, linear_out=_fake_none, linear_pair=_fake_linear_pair, linear_pair_out=_fake_none,
                  group_norm=_fake_group_norm, group_norm_out=_fake_none)
     for name, fake in fakes.items():
         torch.library.register_fake(f"{_NS}::{name}", fake)
@@ -151,11 +155,11 @@ def _load():
 _NAMES = ("paired_fwd", "sparse_fwd", "pair_rows", "gather_rows", "_attention_workspace",
           "_workspace_keys", "_clear_workspaces", "int8_rows", "int8_adaln", "int8_adaln_pair", "int8_linear",
           "int8_linear_rows", "int8_linear_out", "int8_linear_pair_out", "int8_qkv", "int8_qkv_out",
-          "linear", "linear_out", "linear_pair_out", "group_norm", "group_norm_out")
+          "linear", "linear_out", "linear_pair", "linear_pair_out", "group_norm", "group_norm_out")
 try:
     _bound = _load()
 except (RuntimeError, OSError) as e:  # the package still imports, so that it can be (re)built
     _bound = [_Missing(name, str(e)) for name in _NAMES]
 (paired_fwd, sparse_fwd, pair_rows, gather_rows, attention_workspace, workspace_keys, clear_workspaces,
  int8_rows, int8_adaln, int8_adaln_pair, int8_linear, int8_linear_rows, int8_linear_out, int8_linear_pair_out,
- int8_qkv, int8_qkv_out, linear, linear_out, linear_pair_out, group_norm, group_norm_out) = _bound
+ int8_qkv, int8_qkv_out, linear, linear_out, linear_pair, linear_pair_out, group_norm, group_norm_out) = _bound

@@ -235,6 +235,14 @@ def test_pairs_into_one_buffer():
     linear_pair(dict(x=x[:, :77], **layer[0], out=both[:, :77]), dict(x=x[:, 77:], **layer[1], out=both[:, 77:]))
     _check(both[:, :77], x=x[:, :77], **layer[0])
     _check(both[:, 77:], x=x[:, 77:], **layer[1])
+    both.zero_()  # (one output given, one made)
+    made, given = linear_pair(dict(x=x[:, :77], **layer[0]), dict(x=x[:, 77:], **layer[1], out=both[:, 77:]))
+    _check(made, x=x[:, :77], **layer[0])
+    _check(given, x=x[:, 77:], **layer[1])
+    assert given.data_ptr() == both[:, 77:].data_ptr() and not both[:, :77].any()
+    given, made = linear_pair(dict(x=x[:, :77], **layer[0], out=both[:, :77]), dict(x=x[:, 77:], **layer[1]))
+    _check(given, x=x[:, :77], **layer[0])
+    _check(made, x=x[:, 77:], **layer[1])
 
 
 @pytest.mark.parametrize("rows", [3, 100, 4096])
@@ -329,6 +337,7 @@ def test_operators():
     args = (x, layer["weight"], layer["bias"], res, gate)
     torch.library.opcheck(hip.linear.default, (*args, 1), test_utils=checks)
     torch.library.opcheck(hip.linear_out.default, (*args, torch.empty_like(res), 0), test_utils=checks)
+    torch.library.opcheck(hip.linear_pair.default, (*args, *args, 2), test_utils=checks)
     torch.library.opcheck(hip.linear_pair_out.default, (*args, torch.empty_like(res), *args, torch.empty_like(res), 2), test_utils=checks)
 
 
