@@ -234,9 +234,10 @@ constexpr int WIDE = 256, WIDE_BAND = 4, WIDE_WAVES = 4;
 constexpr int WIDE_STAGE = 2 * WIDE * 128;                  // 64 KB
 constexpr int WIDE_LOADS = WIDE_STAGE / 1024 / WIDE_WAVES;  // 1 KB loads of a wave and stage
 
-// What the epilogue does.  All up to GATED are for whole tiles, each of one batch element, with aligned outputs, and work
-// on the sums in registers; ANY takes them through LDS, and PARTS, for a part of the features of any tile, stores the sums
-// themselves.  (One kernel for several kinds of tile keeps too much in registers.)
+// What the epilogue does.  All up to GATED are for tiles of one batch element each and work on the sums in registers, with
+// EDGE also where tiles are not whole; their columns are a multiple of eight and outputs aligned.  ANY takes any tile through
+// LDS (4173 x 3072 -> 9216 238 us, with EDGE 200; 9000 x 1024 -> 9000 with residual and gate 320, 227), and PARTS, for a part of the features of any tile, stores the sums themselves.  (One kernel for several kinds of tile keeps
+// too much in registers.)
 enum Mode { PLAIN, ACT_GELU, ACT_SILU, RESIDUAL, GATED, ANY, PARTS };
 
 // A wave's 128 x 128 sums: acc[i][j] are channels 16 i + 4 (lane / 16) .. + 3 of token 16 j + lane % 16.
@@ -268,21 +269,27 @@ __device__ __forceinline__ void halves(u32x4& a, u32x4& b) {
 // The epilogue of a whole tile of one batch element, a wave's part: tokens from t0 and channels from c0 on; `bias` and
 // `gate` are theirs, in LDS.  A store moves 128 bytes, whole lines, of 8 rows (64 of 16 rows: 16384 x 3072 x 12288 892
 // us, so 867).
-template <bool F16, int MODE>
-__device__ __forceinline__ void finish_wide(const Set& s, const Sums& acc, const float* bias, const float* gate, int c0,
+template <bool F16, int MODE, bool EDGE>
+__device__ __forceinline__ void finish_wide(const Args& a, const Set& s, const Sums& acc, const float* bias, const float* gate, int c0,
                                             uint32_t t0) {
   constexpr bool ADD = MODE == RESIDUAL || MODE == GATED;
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));  // (or addresses stay in registers from tile to tile)
   const int q = lane >> 4, c = c0 + (lane >> 3 & 1) * 32 + (q & 1) * 16 + (q >> 1) * 8;
-  const Place p = place_of(s, t0 + (lane & 7));
-  uint16_t* const out = s.out + p.b * s.out_b + (int64_t)p.n * s.out_n + c;
-  const uint16_t* const from = s.residual + p.b * s.r_b + (int64_t)p.n * s.r_n + c;
+  const Place p = place_of(s, EDGE ? t0 : t0 + (lane & 7));
+  const int64_t n = EDGE ? p.n + (lane & 7) : p.n;
+  uint16_t* const out = s.out + p.b * s.out_b + n * s.out_n + c;
+  const uint16_t* const from = s.residual + p.b * s.r_b + n * s.r_n + c;
+  const int rows = EDGE ? (int)(s.tokens - min(t0, s.tokens)) - (lane & 7) : 0;  // (from this lane's first on)
   constexpr int AHEAD = 2;
-  u32x4 res[AHEAD + 1][4];
+  u32x4 res[AHEAD + 1][4] = {};
   auto ask = [&](int j) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) res[j % (AHEAD + 1)][i] = *(const any_u32x4*)(from + (j * 16 + (i & 1) * 8) * s.r_n + (i >> 1) * 64);
+    for (int i = 0; i < 4; ++i) {
+      u32x4& to = res[j % (AHEAD + 1)][i];
+      const int row = j * 16 + (i & 1) * 8, across = (i >> 1) * 64;
+      if (!EDGE || (row < rows && c + across < a.columns)) to = *(const any_u32x4*)(from + row * s.r_n + across);
+    }
   };
   if (ADD) {
 #pragma unroll
@@ -319,7 +326,11 @@ __device__ __forceinline__ void finish_wide(const Set& s, const Sums& acc, const
       }
       halves(packed[0], packed[1]);
 #pragma unroll
-      for (int m = 0; m < 2; ++m) __builtin_nontemporal_store(packed[m], (u32x4*)(out + (j * 16 + m * 8) * s.out_n + h * 64));
+      for (int m = 0; m < 2; ++m) {
+        const int row = j * 16 + m * 8;
+        if (!EDGE || (row < rows && c + h * 64 < a.columns))
+          __builtin_nontemporal_store(packed[m], (u32x4*)(out + row * s.out_n + h * 64));
+      }
     }
     __builtin_amdgcn_sched_barrier(0);  // (all at once take more registers than there are)
   }
@@ -385,14 +396,14 @@ __device__ __forceinline__ void keep_sums(const Args& a, uint32_t part, int set,
   }
 }
 
-template <bool F16, int MODE>
+template <bool F16, int MODE, bool EDGE = false>
 __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) int8_t lds0[WIDE_STAGE];
   __shared__ __attribute__((aligned(1024))) int8_t lds1[WIDE_STAGE];
   __shared__ __attribute__((aligned(16))) float bias[2][WIDE], gate[2][WIDE];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), row = lane & 15, quarter = lane >> 4;
   const int wc = wave & 1, wt = wave >> 1;
-  constexpr bool WHOLE = MODE < ANY;
+  constexpr bool WHOLE = MODE < ANY && !EDGE;
   const Share mine = MODE == PARTS ? share_of(a) : Share{};
   const int start = mine.part * a.stages_each;
   const int stop = MODE == PARTS ? min(start + a.stages_each, (a.features + 63) / 64) : (a.features + 63) / 64;
@@ -519,8 +530,8 @@ __global__ __launch_bounds__(64 * WIDE_WAVES, 1) void linear_wide_kernel(Args a)
     const uint32_t t0 = done.t0 + wt * 128;
     if constexpr (MODE == PARTS) {
       keep_sums(a, mine.part, done.set, acc, c0, t0);
-    } else if constexpr (WHOLE) {
-      finish_wide<F16, MODE>(s, acc, &bias[parity][wc * 128], &gate[parity][wc * 128], c0, t0);
+    } else if constexpr (MODE < ANY) {
+      finish_wide<F16, MODE, EDGE>(a, s, acc, &bias[parity][wc * 128], &gate[parity][wc * 128], c0, t0);
     } else {
       int8_t* const box = lds1 + 1024 * wave;
 #pragma unroll 1
@@ -879,7 +890,7 @@ constexpr Shape SHAPES[KERNELS] = {
     {256, 256, 256.f, 5.6f, 1.5f, 1.133f, 0.081f, 0.085f, 0.82f, 3.9f, 0.36f},
     {64, 64, 512.f, 2.4f, 4.3f, 0.270f, 0.345f, 0.236f, 0.60f, 2.9f, 0.81f},
 };
-constexpr float WIDE_ANY_ROUND = 28.6f;              // (tiles that are not whole)
+constexpr float WIDE_ANY_ROUND = 28.6f;              // (through LDS)
 constexpr float COPY = 4.3f, COPY_MEGABYTE = 0.116f;  // (of rows that are copied first, read and written)
 
 // Tiles of TC x TT of both sets.
@@ -907,12 +918,19 @@ bool whole_tiles(const Args& a, int count) {
   return whole;
 }
 
+// Whether each of its tiles lies in one batch element, and all outputs are stored in 16 bytes.
+bool one_element(const Args& a, int count) {
+  bool one = a.vectors && a.columns % 8 == 0;
+  for (int i = 0; i < count; ++i) one &= a.set[i].tokens == a.set[i].rows || a.set[i].rows % WIDE == 0;
+  return one;
+}
+
 // The wide kernel's epilogue for these sets.
 Mode mode_of(const Args& a, int count) {
   const bool residual = a.set[0].residual, gate = a.set[0].gate;
-  bool whole = whole_tiles(a, count);
-  for (int i = 0; i < count; ++i) whole &= residual == !!a.set[i].residual && gate == !!a.set[i].gate;
-  if (!whole || (a.act != NONE && residual)) return ANY;
+  bool same = one_element(a, count);
+  for (int i = 0; i < count; ++i) same &= residual == !!a.set[i].residual && gate == !!a.set[i].gate;
+  if (!same || (a.act != NONE && residual)) return ANY;
   return a.act == GELU ? ACT_GELU : a.act == SILU ? ACT_SILU : gate ? GATED : residual ? RESIDUAL : PLAIN;
 }
 
@@ -921,7 +939,7 @@ float estimate(const Args& a, int count, Kernel k, int splits) {
   const Shape& s = SHAPES[k];
   const float rounds = (float)(tiles_of(a, count, s.tc, s.tt) * splits) / s.at_once, whole = std::floor(rounds), rest = rounds - whole;
   const float stages = (float)(((a.features + 63) / 64 + splits - 1) / splits);
-  const float round = k == WIDE256 && splits == 1 && !whole_tiles(a, count) ? WIDE_ANY_ROUND : s.round;
+  const float round = k == WIDE256 && splits == 1 && !one_element(a, count) ? WIDE_ANY_ROUND : s.round;
   const float tokens = (float)a.set[0].tokens + (float)a.set[1].tokens, rows = tokens + (float)count * (float)a.columns;
   float us = s.launch + whole * (round + stages * (s.stage + s.full)) +
              (rest > 0.f ? round + stages * (s.stage + s.full * rest * rest) : 0.f) + s.megabyte * 2e-6f * rows * (float)a.features +
@@ -966,6 +984,19 @@ Choice choose(const Args& a, int count, int first, int last) {
   return best;
 }
 
+template <bool F16, bool EDGE>
+void launch_wide(const Args& a, Mode mode, const dim3& grid, hipStream_t st) {
+  const dim3 block(64 * WIDE_WAVES);
+  switch (mode) {
+    case PLAIN: hipLaunchKernelGGL((linear_wide_kernel<F16, PLAIN, EDGE>), grid, block, 0, st, a); break;
+    case ACT_GELU: hipLaunchKernelGGL((linear_wide_kernel<F16, ACT_GELU, EDGE>), grid, block, 0, st, a); break;
+    case ACT_SILU: hipLaunchKernelGGL((linear_wide_kernel<F16, ACT_SILU, EDGE>), grid, block, 0, st, a); break;
+    case RESIDUAL: hipLaunchKernelGGL((linear_wide_kernel<F16, RESIDUAL, EDGE>), grid, block, 0, st, a); break;
+    case GATED: hipLaunchKernelGGL((linear_wide_kernel<F16, GATED, EDGE>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((linear_wide_kernel<F16, ANY>), grid, block, 0, st, a);
+  }
+}
+
 template <bool F16>
 int launch_kernel(Args& a, int count, const Choice& choice, hipStream_t st) {
   const int tc = SHAPES[choice.kernel].tc, tt = SHAPES[choice.kernel].tt, stages = (a.features + 63) / 64;
@@ -992,14 +1023,8 @@ int launch_kernel(Args& a, int count, const Choice& choice, hipStream_t st) {
       const uint32_t per_xcd = std::max(1, device_cu_count() / 8);
       const dim3 grid(8 * std::min(a.tiles_xcd, per_xcd)), block(64 * WIDE_WAVES);
       if (a.splits > 1) hipLaunchKernelGGL((linear_wide_kernel<F16, PARTS>), each, block, 0, st, a);
-      else switch (mode_of(a, count)) {
-        case PLAIN: hipLaunchKernelGGL((linear_wide_kernel<F16, PLAIN>), grid, block, 0, st, a); break;
-        case ACT_GELU: hipLaunchKernelGGL((linear_wide_kernel<F16, ACT_GELU>), grid, block, 0, st, a); break;
-        case ACT_SILU: hipLaunchKernelGGL((linear_wide_kernel<F16, ACT_SILU>), grid, block, 0, st, a); break;
-        case RESIDUAL: hipLaunchKernelGGL((linear_wide_kernel<F16, RESIDUAL>), grid, block, 0, st, a); break;
-        case GATED: hipLaunchKernelGGL((linear_wide_kernel<F16, GATED>), grid, block, 0, st, a); break;
-        default: hipLaunchKernelGGL((linear_wide_kernel<F16, ANY>), grid, block, 0, st, a);
-      }
+      else if (whole_tiles(a, count)) launch_wide<F16, false>(a, mode_of(a, count), grid, st);
+      else launch_wide<F16, true>(a, mode_of(a, count), grid, st);
     }
   }
   HB_HIP(hipGetLastError());

@@ -67,7 +67,7 @@ def test_rows_of_odd_lengths(rows, K, N, dtype):
 
 @pytest.mark.parametrize("act, bias, more", EPILOGUES)
 @pytest.mark.parametrize("batch, rows, K, N", [(3, 61, 99, 201), (1, 1, 64, 100), (3, 5, 200, 72), (2, 33, 96, 200), (3, 170, 136, 1000), (2, 2048, 128, 4096),
-                                               (3, 1365, 128, 4096)])
+                                               (3, 1365, 128, 4096), (1, 4173, 128, 4104), (2, 2048, 72, 4008)])
 def test_epilogues(batch, rows, K, N, act, bias, more):
     x, layer = _normal(batch, rows, K), _layer(K, N, bias=bias)
     if more:
@@ -200,6 +200,25 @@ def test_rows_anywhere(rows):
     x = _normal(batch, 1, K).expand(batch, rows, K)
     _check(linear(x, **layer), x=x, **layer)
     _check(linear(x[0], **layer), x=x[0], **layer)
+
+
+@pytest.mark.parametrize("more", ["", "residual", "gate"])
+@pytest.mark.parametrize("rows, N", [(4173, 4104), (4096, 4008), (4351, 4096), (4097, 4096)])
+def test_what_lies_beside_tiles_that_are_not_whole_stays(rows, N, more):
+    x, layer = _normal(1, rows, 128), _layer(128, N)
+    held = _normal(1, rows + 256, N + 264, seed=9)
+    before = held.clone()
+    out = held[:, 8:8 + rows, 8:8 + N]
+    if more:
+        layer["residual"] = out
+    if more == "gate":
+        layer["gate"] = _normal(1, N, std=0.5, seed=6)
+    linear(x, **layer, out=out)
+    if more:
+        layer["residual"] = before[:, 8:8 + rows, 8:8 + N]
+    _check(out, x=x, **layer)
+    out.copy_(before[:, 8:8 + rows, 8:8 + N])
+    assert torch.equal(held, before)
 
 
 @pytest.mark.parametrize("rows", [1, 60, 700, 4096])
