@@ -248,6 +248,19 @@ def test_pairs(text, image, K, N, more):
             assert out.shape == (2, 0, N)
 
 
+@pytest.mark.parametrize("text, image, K, N", [(77, 4096, 128, 4104), (4173, 300, 72, 4096), (512, 8192, 64, 3000)])
+@pytest.mark.parametrize("more", ["", "gate"])
+def test_pairs_of_one_element(text, image, K, N, more):
+    sets = []
+    for i, rows in enumerate((text, image)):
+        s = dict(x=_normal(1, rows, K, seed=i), **_layer(K, N, seed=10 * i))
+        if more:
+            s |= dict(residual=_normal(1, rows, N, seed=30 + i), gate=_normal(1, N, seed=40 + i))
+        sets.append(s)
+    for out, s in zip(linear_pair(*sets), sets):
+        _check(out, **s)
+
+
 def test_pairs_into_one_buffer():
     both, layer = _normal(1, 1100, 512), [_layer(128, 512, seed=i) for i in (0, 7)]
     x = _normal(1, 1100, 128, seed=3)
