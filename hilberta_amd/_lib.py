@@ -74,6 +74,7 @@ SIGNATURES = {
         [_c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_f32, _p, _c_i64, _c_i64, _p, _p, _p, _c_i64, _c_i64, _p, _c_i64, _p],
     ),
     "hb_linear_workspace_bytes": (_c_i64, [_c_int, _c_int, _p, _c_int, _c_int, _p, _p]),
+    "hb_linear_choice": (_c_int, [_c_int, _c_int, _p, _c_int, _c_int, _c_int, _p, _p, _p]),
     "hb_linear": (_c_int, [_c_int, _c_int, _p, _c_int, _c_int, _c_int, _c_int, _p, _p, _p, _c_i64, _p]),
     "hb_int8_rows": (_c_int, [_p, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _p, _p, _p]),
     "hb_int8_adaln": (_c_int, [_c_int, _c_int, _p, _c_int, _c_int, _c_int, _c_f32, _p, _p, _p]),

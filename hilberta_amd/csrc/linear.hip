@@ -890,7 +890,7 @@ constexpr Shape SHAPES[KERNELS] = {
     {256, 256, 256.f, 5.6f, 1.5f, 1.133f, 0.081f, 0.085f, 0.82f, 3.9f, 0.36f},
     {64, 64, 512.f, 2.4f, 4.3f, 0.270f, 0.345f, 0.236f, 0.60f, 2.9f, 0.81f},
 };
-constexpr float WIDE_ANY_ROUND = 28.6f;              // (through LDS)
+constexpr float WIDE_ANY_ROUND = 22.f;               // (through LDS; fitted to 180 sizes of that epilogue)
 constexpr float COPY = 4.3f, COPY_MEGABYTE = 0.116f;  // (of rows that are copied first, read and written)
 
 // Tiles of TC x TT of both sets.
@@ -934,12 +934,12 @@ Mode mode_of(const Args& a, int count) {
   return a.act == GELU ? ACT_GELU : a.act == SILU ? ACT_SILU : gate ? GATED : residual ? RESIDUAL : PLAIN;
 }
 
-// What a kernel takes for the sets, in us (whatever the activation, so that the workspace is known without it).
+// What a kernel takes for the sets, in us.
 float estimate(const Args& a, int count, Kernel k, int splits) {
   const Shape& s = SHAPES[k];
   const float rounds = (float)(tiles_of(a, count, s.tc, s.tt) * splits) / s.at_once, whole = std::floor(rounds), rest = rounds - whole;
   const float stages = (float)(((a.features + 63) / 64 + splits - 1) / splits);
-  const float round = k == WIDE256 && splits == 1 && !one_element(a, count) ? WIDE_ANY_ROUND : s.round;
+  const float round = k == WIDE256 && splits == 1 && mode_of(a, count) == ANY ? WIDE_ANY_ROUND : s.round;
   const float tokens = (float)a.set[0].tokens + (float)a.set[1].tokens, rows = tokens + (float)count * (float)a.columns;
   float us = s.launch + whole * (round + stages * (s.stage + s.full)) +
              (rest > 0.f ? round + stages * (s.stage + s.full * rest * rest) : 0.f) + s.megabyte * 2e-6f * rows * (float)a.features +
@@ -963,7 +963,9 @@ float estimate_few(const Args& a, int count, bool aligned) {
 // idle over many features; they are tried while all their workgroups fit the card at once, with four stages each or more.
 // Measured, the best of one part / the parts: 99 x 8472 -> 64 30.4 / 9.9 us, 512 x 12288 -> 3072 72.8 / 60 (eight of the
 // wide kernel), 1280 x 13824 -> 5120 251 / 171 (two of it).  Over 264 sizes the choice takes 1.6% more time than the best of
-// all; the best of one part takes 13.9% more over 175 of them.  TWO64x64 pays where many tiles are short: the best of the
+// all; the best of one part takes 13.9% more over 175 of them.  What the wide kernel's epilogue is counts: over 100 sizes with
+// an activation and a residual the choice takes 2.5% more than the best, and 29% as if it were in registers (1330 x 64 -> 1664
+// 8.9 / 34.9 us, 10240 x 128 -> 256 9.7 / 36.2); over 80 of several batch elements or odd columns 0.8%.  TWO64x64 pays where many tiles are short: the best of the
 // others / with it 5993 x 128 -> 2752 47.5 / 39.5, 4576 x 64 -> 960 16.6 / 12.8, 657 x 1216 -> 2624 16.2 / 13.7; alone on
 // its CU it is slower (77 x 4096 -> 3072 27.6, T64x64 21.9); without it the choice takes 5.8% more than the best.  Rows that direct loads cannot take are copied, or not, by the same measure.
 // Copied / as they are: 999 x 1001 -> 777 14.0 / 11.7 us, 2405 x 13 -> 20 11.0 / 7.2, 64 x 12001 -> 17000 262 / 219, 2000 x
@@ -1153,7 +1155,27 @@ using namespace hb;
 extern "C" int64_t hb_linear_workspace_bytes(int32_t count, int32_t batch, const int32_t* rows, int32_t columns,
                                              int32_t features, void* const* pointers, const int64_t* strides) {
   Plan p;
-  return plan(p, count, batch, rows, columns, features, NONE, pointers, strides, nullptr) ? -1 : p.bytes;
+  if (plan(p, count, batch, rows, columns, features, NONE, pointers, strides, nullptr)) return -1;
+  const int64_t bytes = p.bytes;
+  // (an activation before a residual only makes the wide kernel's whole sums slower, in favour of another kernel)
+  if (p.choice.kernel != WIDE256 || p.choice.splits > 1 || !p.a.set[0].residual) return bytes;
+  plan(p, count, batch, rows, columns, features, GELU, pointers, strides, nullptr);
+  return std::max(bytes, p.bytes);
+}
+
+extern "C" int hb_linear_choice(int32_t count, int32_t batch, const int32_t* rows, int32_t columns, int32_t features,
+                                int32_t act, void* const* pointers, const int64_t* strides, int32_t* choice) {
+  HB_REQUIRE(choice, "null pointer argument");
+  HB_REQUIRE(act >= 0 && act <= 2, "act must be 0 (none), 1 (GELU) or 2 (SiLU)");
+  Plan p;
+  const int rc = plan(p, count, batch, rows, columns, features, act, pointers, strides, nullptr);
+  if (rc) return rc;
+  const bool few = p.choice.kernel == FEW16, wide = p.choice.kernel == WIDE256 && p.choice.splits == 1;
+  choice[0] = few ? 16 : SHAPES[p.choice.kernel].tc;
+  choice[1] = few ? FEW_ROWS : SHAPES[p.choice.kernel].tt;
+  choice[2] = p.choice.splits;
+  choice[3] = wide && mode_of(p.a, count) == ANY;
+  return HB_OK;
 }
 
 extern "C" int hb_linear(int32_t count, int32_t batch, const int32_t* rows, int32_t columns, int32_t features,

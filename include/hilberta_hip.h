@@ -244,9 +244,13 @@ int hb_group_norm(int32_t batch, int64_t pixels, int32_t channels, int32_t group
  * features up to 2^20, columns up to 2^25.  Rows may begin at any element.  `workspace` (hb_linear_workspace_bytes, 0
  * where none is needed and -1 where the sizes are rejected; 16-byte aligned, contents irrelevant before and after) holds x
  * and weights whose rows are no multiples of 16 bytes or lie too far apart, where copying them first pays, and the sums
- * of the parts that the features of few rows and columns are taken in. */
+ * of the parts that the features of few rows and columns are taken in: enough for every activation.  hb_linear_choice
+ * says what such a call runs, from the host alone: choice [4] {channels of a tile, tokens of a tile, parts of the
+ * features, at most, 1 where tiles of 256 x 256 are finished through LDS}. */
 int64_t hb_linear_workspace_bytes(int32_t count, int32_t batch, const int32_t* rows, int32_t columns,
                                   int32_t features, void* const* pointers, const int64_t* strides);
+int hb_linear_choice(int32_t count, int32_t batch, const int32_t* rows, int32_t columns, int32_t features,
+                     int32_t act, void* const* pointers, const int64_t* strides, int32_t* choice);
 int hb_linear(int32_t count, int32_t batch, const int32_t* rows, int32_t columns, int32_t features,
               int32_t dtype, int32_t act, void* const* pointers, const int64_t* strides,
               void* workspace, int64_t workspace_bytes, hb_stream_t stream);
