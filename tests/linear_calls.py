@@ -23,3 +23,10 @@ def call(batch, rows, K, N, *, act=None, more="", out_row=None, shift=0, sets=No
     choice, lib = (ctypes.c_int32 * 4)(), _lib.load()
     assert lib.hb_linear_choice(*args, ACTS[act], p, s, choice) == 0, _lib.last_error()
     return tuple(choice), lib.hb_linear_workspace_bytes(*args, p, s)
+
+
+# (batch, rows of one set or two, features, columns) that the wide kernel takes in one part and finishes through LDS: tiles
+# of several batch elements, columns that are no multiple of eight
+GENERAL = [(3, 1365, 512, 4096), (3, 1365, 776, 4089), (32, 128, 776, 4096), (315, 13, 776, 4089), (1, 4096, 1032, 4094)]
+GENERAL_PAIRS = [(3, (700, 1365), 520, 4096), (3, (700, 1365), 520, 4091), (16, (112, 144), 520, 4092)]
+SHIFTS = [(0, 0), (1, 13), (2, 12)]  # outputs that many elements past 16 bytes, with rows so much longer

@@ -5,7 +5,7 @@ import random
 
 import pytest
 
-from tests.linear_calls import call
+from tests.linear_calls import GENERAL, GENERAL_PAIRS, SHIFTS, call
 
 
 @pytest.mark.parametrize("act", ["gelu", "silu"])
@@ -45,3 +45,12 @@ def test_refusals():
         call(1, 0, 64, 64)
     with pytest.raises(AssertionError, match="features must be"):
         call(1, 9, 0, 64)
+
+
+@pytest.mark.parametrize("size", GENERAL + GENERAL_PAIRS)
+def test_sizes_of_the_general_epilogue(size):
+    """What tests/test_gpu_linear_general.py runs takes the route that it is about."""
+    for act in (None, "gelu", "silu"):
+        for more in ("", "residual", "gate"):
+            for shift, longer in SHIFTS:
+                assert call(*size, act=act, more=more, out_row=size[3] + longer, shift=shift)[0] == (256, 256, 1, 1)
