@@ -386,15 +386,27 @@ int64_t size_of(int dtype) { return dtype == HB_DTYPE_F32 ? 4 : 2; }
 // Channels of a load of group_norm_few_kernel: the most that divide a group's.
 int few_width(int per) { return per % 8 == 0 ? 8 : per % 4 == 0 ? 4 : per % 2 == 0 ? 2 : 1; }
 
-// Whether a workgroup holds a group (and the launch all of them: a grid holds fewer than 2^32 threads).  One launch and
-// two, 512 channels in 32 groups, us: 256 pixels 7.4, 10.6; 1024 8.7, 10.6; with groups twice and four times as large
-// as a workgroup holds now 13.7, 10.9 and 30.4, 11.5.
-bool few(int64_t batch, int64_t pixels, int groups, int per) {
-  return pixels * (per / few_width(per)) <= (int64_t)UNITS * FEW_THREADS && batch * groups < (1ll << 32) / FEW_THREADS;
+// The kernels and chunks follow from an element's sizes alone, so that an image's result is the same in every batch: a
+// batch of more workgroups than a launch takes (a grid holds fewer than 2^32 threads) goes in slices.
+int32_t slice_of(int32_t batch, int64_t groups_of_one, int64_t threads) {
+  return (int32_t)std::min<int64_t>(batch, ((1ll << 32) - 1) / (groups_of_one * threads));
 }
 
-// Chunks of at least 16 KB, up to as many as there are CUs, and twice as many of twice the threads past 512 MB: by the
-// element alone, so that an image's result is the same in every batch.
+// The elements from `first` on.
+template <int DT>
+Args from_element(Args a, int32_t first) {
+  typedef typename Type<DT>::T T;
+  a.x = (const T*)a.x + first * a.x_b;
+  a.out = (T*)a.out + first * a.out_b;
+  a.sums += (int64_t)first * a.chunks * a.groups;
+  return a;
+}
+
+// Whether a workgroup holds a group.  One launch and two, 512 channels in 32 groups, us: 256 pixels 7.4, 10.6; 1024 8.7,
+// 10.6; with groups twice and four times as large as a workgroup holds now 13.7, 10.9 and 30.4, 11.5.
+bool few(int64_t pixels, int per) { return pixels * (per / few_width(per)) <= (int64_t)UNITS * FEW_THREADS; }
+
+// Chunks of at least 16 KB, up to as many as there are CUs, and twice as many of twice the threads past 512 MB.
 // us of 256, 512 chunks of 256 threads, and of 512 threads: 65536 pixels x 512 channels bf16 45.2, 47.3, 47.4, 47.0; 262144 x
 // 256 fp32 142, 146, 150, 159, bf16 85, 88, 81, 87; 2048 x 2048 x 128 bf16 578, 550, 543, 534.  Of 16384 x 512 18.2, 20.4,
 // 17.0, 23.8; 128 chunks 22.4: every workgroup of the second launch joins all chunks of its element.
@@ -402,12 +414,10 @@ struct Chunks {
   int64_t pixels, count;
   int threads;
 };
-Chunks chunks_of(int64_t batch, int64_t pixels, int channels, int dtype) {
+Chunks chunks_of(int64_t pixels, int channels, int dtype) {
   const int64_t row = channels * size_of(dtype);
   const int large = pixels * row > LARGE_BYTES ? 2 : 1;
-  // (a grid holds fewer than 2^32 threads, of up to 1024 a workgroup)
-  const int64_t most = std::min<int64_t>(256 * large, std::max<int64_t>(1, ((1ll << 32) - 1) / MAX_THREADS / batch));
-  const int64_t count = std::clamp<int64_t>(pixels * row / CHUNK_BYTES, 1, most);
+  const int64_t count = std::clamp<int64_t>(pixels * row / CHUNK_BYTES, 1, 256 * large);
   const int64_t each = (pixels + count - 1) / count;
   return {each, (pixels + each - 1) / each, THREADS * large};
 }
@@ -416,26 +426,34 @@ template <int DT, int W>
 int launch_few(const Args& a, int32_t batch, hipStream_t st) {
   const int64_t units = (int64_t)a.pixels * (a.per / W);
   const int threads = (int)std::clamp<int64_t>((units + 63) / 64 * 64, 64, FEW_THREADS);
-  hipLaunchKernelGGL((group_norm_few_kernel<DT, W>), dim3(a.groups, batch), dim3(threads), 0, st, a);
-  HB_HIP(hipGetLastError());
+  const int32_t slice = slice_of(batch, a.groups, threads);
+  for (int32_t b = 0; b < batch; b += slice) {
+    hipLaunchKernelGGL((group_norm_few_kernel<DT, W>), dim3(a.groups, std::min(slice, batch - b)), dim3(threads), 0, st, from_element<DT>(a, b));
+    HB_HIP(hipGetLastError());
+  }
   return HB_OK;
 }
 
 template <int DT, int EDGE>
 int launch_chunks(const Args& a, int32_t batch, bool stream_values, hipStream_t st) {
-  const dim3 grid(a.chunks, batch), block(a.vectors * a.rows);
-  hipLaunchKernelGGL((group_norm_sums_kernel<DT, EDGE>), grid, block, block.x * V * 2 * sizeof(float), st, a);
-  HB_HIP(hipGetLastError());
+  const dim3 block(a.vectors * a.rows);
   const size_t lds = 2 * a.groups * sizeof(float);
-  if (stream_values) hipLaunchKernelGGL((group_norm_kernel<DT, EDGE, true>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((group_norm_kernel<DT, EDGE, false>), grid, block, lds, st, a);
-  HB_HIP(hipGetLastError());
+  const int32_t slice = slice_of(batch, a.chunks, block.x);
+  for (int32_t b = 0; b < batch; b += slice) {
+    const dim3 grid(a.chunks, std::min(slice, batch - b));
+    const Args part = from_element<DT>(a, b);
+    hipLaunchKernelGGL((group_norm_sums_kernel<DT, EDGE>), grid, block, block.x * V * 2 * sizeof(float), st, part);
+    HB_HIP(hipGetLastError());
+    if (stream_values) hipLaunchKernelGGL((group_norm_kernel<DT, EDGE, true>), grid, block, lds, st, part);
+    else hipLaunchKernelGGL((group_norm_kernel<DT, EDGE, false>), grid, block, lds, st, part);
+    HB_HIP(hipGetLastError());
+  }
   return HB_OK;
 }
 
 template <int DT>
 int launch(Args& a, int32_t batch, hipStream_t st) {
-  if (few(batch, a.pixels, a.groups, a.per)) {
+  if (few(a.pixels, a.per)) {
     switch (few_width(a.per)) {
       case 8: return launch_few<DT, 8>(a, batch, st);
       case 4: return launch_few<DT, 4>(a, batch, st);
@@ -465,8 +483,8 @@ int check_sizes(int32_t batch, int64_t pixels, int32_t channels, int32_t groups,
 
 extern "C" int64_t hb_group_norm_workspace_bytes(int32_t batch, int64_t pixels, int32_t channels, int32_t groups, int32_t dtype) {
   if (check_sizes(batch, pixels, channels, groups, dtype) != HB_OK) return -1;
-  if (few(batch, pixels, groups, channels / groups)) return 0;
-  return batch * chunks_of(batch, pixels, channels, dtype).count * groups * (int64_t)sizeof(float2);
+  if (few(pixels, channels / groups)) return 0;
+  return batch * chunks_of(pixels, channels, dtype).count * groups * (int64_t)sizeof(float2);
 }
 
 extern "C" int hb_group_norm(int32_t batch, int64_t pixels, int32_t channels, int32_t groups, int32_t dtype, int32_t silu,
@@ -500,7 +518,7 @@ extern "C" int hb_group_norm(int32_t batch, int64_t pixels, int32_t channels, in
   const int64_t need = hb_group_norm_workspace_bytes(batch, pixels, channels, groups, dtype);
   if (need) {
     HB_REQUIRE(workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= need, "the workspace must hold %lld bytes, 8-byte aligned", (long long)need);
-    const Chunks c = chunks_of(batch, pixels, channels, dtype);
+    const Chunks c = chunks_of(pixels, channels, dtype);
     a.sums = (float2*)workspace;
     a.chunk = (uint32_t)c.pixels;
     a.chunks = (uint32_t)c.count;
