@@ -314,7 +314,7 @@ constexpr int UNITS = 2, FEW_THREADS = 1024;
 template <int DT, int W>
 __global__ __launch_bounds__(FEW_THREADS) void group_norm_few_kernel(Args a) {
   typedef typename Type<DT>::T T;
-  __shared__ float parts[2][FEW_THREADS / 64];
+  __shared__ float parts[3][FEW_THREADS / 64];
   const int g = blockIdx.x, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const uint32_t across = a.per / W, all = a.pixels * across;  // loads of a pixel, and of the group
   const T* const x = (const T*)a.x + blockIdx.y * a.x_b + g * a.per;
@@ -341,28 +341,41 @@ __global__ __launch_bounds__(FEW_THREADS) void group_norm_few_kernel(Args a) {
     if (a.weight) weight[i] = *(const Unit*)((const T*)a.weight + g * a.per + channel[i]);
     if (a.bias) bias[i] = *(const Unit*)((const T*)a.bias + g * a.per + channel[i]);
   }
-  auto total = [&](float s, float (&part)[FEW_THREADS / 64]) {
+  auto wave_total = [&](float s, float (&part)[FEW_THREADS / 64]) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) s += __shfl_xor(s, m, 64);
     if ((threadIdx.x & 63) == 0) part[wave] = s;
-    __syncthreads();
-    s = 0.f;
+  };
+  auto total = [&](const float (&part)[FEW_THREADS / 64]) {
+    float s = 0.f;
     for (int w = 0; w < waves; ++w) s += part[w];
     return s;
   };
-  float v[UNITS][W], sum = 0.f, squares = 0.f;
+  float v[UNITS][W], sum = 0.f, rest = 0.f, squares = 0.f;
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
     widen(raw[i], v[i]);
 #pragma unroll
     for (int k = 0; k < W; ++k) sum += v[i][k];  // (zeros past the group's values)
   }
-  const float n = (float)all * W, mean = total(sum, parts[0]) / n;
+  wave_total(sum, parts[0]);
+  __syncthreads();
+  const float n = (float)all * W, mean = total(parts[0]) / n;
+  // (the values' differences from the mean tell by how much its rounding missed theirs: a few values close together far
+  // from zero would be off by the mean's last bit in their deviations)
 #pragma unroll
   for (int i = 0; i < UNITS; ++i)
 #pragma unroll
-    for (int k = 0; k < W; ++k) squares += there[i] ? (v[i][k] - mean) * (v[i][k] - mean) : 0.f;
-  const float scale = __builtin_amdgcn_rsqf(total(squares, parts[1]) / n + a.eps);
+    for (int k = 0; k < W; ++k) {
+      v[i][k] = there[i] ? v[i][k] - mean : 0.f;
+      rest += v[i][k];
+      squares += v[i][k] * v[i][k];
+    }
+  wave_total(rest, parts[1]);
+  wave_total(squares, parts[2]);
+  __syncthreads();
+  const float missed = total(parts[1]) / n, var = fmaxf(total(parts[2]) / n - missed * missed, 0.f);
+  const float scale = __builtin_amdgcn_rsqf(var + a.eps);
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
     if (!there[i]) continue;
@@ -372,7 +385,7 @@ __global__ __launch_bounds__(FEW_THREADS) void group_norm_few_kernel(Args a) {
     Unit u;
 #pragma unroll
     for (int k = 0; k < W; ++k) {
-      const float y = activate((v[i][k] - mean) * (a.weight ? scale * w[k] : scale) + (a.bias ? b[k] : 0.f), a.silu);
+      const float y = activate((v[i][k] - missed) * (a.weight ? scale * w[k] : scale) + (a.bias ? b[k] : 0.f), a.silu);
       if constexpr (DT == HB_DTYPE_F32) u[k] = y;
       else u[k] = from_f<DT == HB_DTYPE_F16>(y);
     }
