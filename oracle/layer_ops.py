@@ -52,20 +52,20 @@ def relative(got, exact):
     return ((got.double() - exact).norm() / exact.norm().clamp_min(1e-30)).item()
 
 
-def group_norm(x, groups, weight=None, bias=None, act=None, eps=1e-6):
+def group_norm(x, groups, weight=None, bias=None, act=None, eps=1e-6, steps=99):
     """(out, bound) of act(GroupNorm(x) * weight + bias), x [B, pixels, C].
 
-    A kernel's mean comes of at most 16 joins of a thread's pixels, 67 additions over the workgroup's threads and 16
-    joins of chunks (in the sizes tested), each off by U of at most the mean's size plus the deviation; its variance's
-    relative error is twice that count of U and the square of the mean's error in deviations, halved by the root.  Then
-    come the difference, the two products, the sum, and SiLU as in ``linear``."""
+    A kernel's mean comes of ``steps`` additions and joins, each off by U of at most the mean's size plus the deviation:
+    16 joins of a thread's pixels, 67 additions over the workgroup's threads and 16 joins of chunks where nothing else is
+    said.  Its variance's relative error is twice that count of U and the square of the mean's error in deviations, halved
+    by the root.  Then come the difference, the two products, the sum, and SiLU as in ``linear``."""
     B, P, C = x.shape
     v = x.double().reshape(B, P, groups, C // groups)
     mean, var = v.mean((1, 3), keepdim=True), v.var((1, 3), keepdim=True, unbiased=False)
     std = (var + eps).sqrt()
-    dmean = 99 * U * (mean.abs() + var.sqrt())
+    dmean = steps * U * (mean.abs() + var.sqrt())
     n = (v - mean) / std
-    dn = (dmean + U * (v - mean).abs()) / std + n.abs() * (99 * U + (dmean / std) ** 2 + 4 * U)
+    dn = (dmean + U * (v - mean).abs()) / std + n.abs() * (steps * U + (dmean / std) ** 2 + 4 * U)
     n, dn = n.reshape(B, P, C), dn.reshape(B, P, C)
     w = 1.0 if weight is None else weight.double()
     b = 0.0 if bias is None else bias.double()
