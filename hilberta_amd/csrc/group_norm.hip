@@ -508,7 +508,8 @@ extern "C" int hb_group_norm(int32_t batch, int64_t pixels, int32_t channels, in
   const int rc = check_sizes(batch, pixels, channels, groups, dtype);
   if (rc) return rc;
   HB_REQUIRE(silu == 0 || silu == 1, "silu must be 0 or 1");
-  HB_REQUIRE(eps > 0.f, "eps must be positive");
+  // (the root takes a smaller number for zero: a group without deviation would be NaN)
+  HB_REQUIRE(eps >= 0x1p-126f, "eps must be at least 2^-126");
   const uintptr_t size = (uintptr_t)size_of(dtype);
   HB_REQUIRE((((uintptr_t)x | (uintptr_t)weight | (uintptr_t)bias | (uintptr_t)out) & (size - 1)) == 0, "every pointer must be aligned to its elements");
   HB_REQUIRE(x_batch_stride >= 0 && x_pixel_stride >= 0 && out_batch_stride >= 0 && out_pixel_stride >= 0, "strides must be non-negative");

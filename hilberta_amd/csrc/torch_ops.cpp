@@ -862,7 +862,7 @@ void group_norm_out(const Tensor& x, int64_t groups, const Maybe& weight, const 
   const Image m = image_of(x, "x");
   TORCH_CHECK_VALUE(m.channels > 0 && m.channels <= 8192, "x must have 1 to 8192 channels");
   TORCH_CHECK_VALUE(groups > 0 && m.channels % groups == 0, "groups must divide the channels");
-  TORCH_CHECK_VALUE(eps > 0, "eps must be positive");
+  TORCH_CHECK_VALUE(static_cast<float>(eps) >= std::numeric_limits<float>::min(), "eps must be at least 2^-126");
   for (const Tensor* t : {&w, &b})
     TORCH_CHECK_VALUE(!t->defined() || (t->dim() == 1 && t->size(0) == m.channels && t->is_contiguous() && t->scalar_type() == type),
                       "weight and bias must be contiguous [C] tensors of x's dtype");

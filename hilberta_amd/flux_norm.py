@@ -110,7 +110,8 @@ def group_norm(x, groups, weight=None, bias=None, *, act=None, eps=1e-6, out=Non
 
     x [B, pixels, C], [B, C, H, W] or [B, C, T, H, W], its channels last in memory (torch.channels_last,
     channels_last_3d) and its pixels evenly apart; bf16, fp16 or fp32, up to 8192 channels and 65535 batch
-    elements; weight and bias [C] of x's dtype; act None or "silu".  Statistics and values are fp32, rounded once.  ``out`` is like x and may be x itself.
+    elements; weight and bias [C] of x's dtype; act None or "silu"; eps 2^-126 or more.  Statistics and values are fp32, rounded once.
+    ``out`` is like x and may be x itself.
     Inference only; asynchronous on the current stream, and can be captured into a graph."""
     if act not in (None, "silu"):
         raise ValueError('act must be None or "silu"')

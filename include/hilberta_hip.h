@@ -222,7 +222,7 @@ int hb_adaln_modulate_pair(int32_t batch, const int32_t* rows, int32_t hidden, i
  * mean and var (of n, not n - 1) over the element's pixels and the group's channels; silu = 1: act is SiLU, else none;
  * statistics and values in fp32, one rounding.  x and out are [batch, pixels, channels] by element strides, channels
  * contiguous; groups divide the channels, which are up to 8192; batch up to 65535, pixels below 2^31; dtype may be HB_DTYPE_F32; weight and bias [channels] of
- * that type, or NULL.  out may be x itself.  `workspace`: hb_group_norm_workspace_bytes (0 for small groups, -1 where the
+ * that type, or NULL; eps is 2^-126 or more.  out may be x itself.  `workspace`: hb_group_norm_workspace_bytes (0 for small groups, -1 where the
  * sizes are rejected), 8-byte aligned, contents irrelevant before and after. */
 int64_t hb_group_norm_workspace_bytes(int32_t batch, int64_t pixels, int32_t channels,
                                       int32_t groups, int32_t dtype);

@@ -27,3 +27,9 @@ def test_close_values(P, C, G, roundings, mean):
     got, (exact, bound) = group_norm(x, G), L.group_norm(x, G)
     assert L.held(got, exact, bound).all()
     assert L.relative(got, exact) <= roundings * L.U
+
+
+@pytest.mark.parametrize("P", [50, 9000])
+def test_the_smallest_eps(P):
+    x, b = torch.full((1, P, 32), 3.25, device="cuda"), torch.randn(32, device="cuda")
+    assert torch.equal(group_norm(x, 4, None, b, eps=2.0**-126), b.expand(1, P, 32))
