@@ -52,16 +52,17 @@ def relative(got, exact):
     return ((got.double() - exact).norm() / exact.norm().clamp_min(1e-30)).item()
 
 
-def group_norm(x, groups, weight=None, bias=None, act=None, eps=1e-6, steps=99):
+def group_norm(x, groups, weight=None, bias=None, act=None, eps=1e-6, steps=99, statistics=None):
     """(out, bound) of act(GroupNorm(x) * weight + bias), x [B, pixels, C].
 
     A kernel's mean comes of ``steps`` additions and joins, each off by U of at most the mean's size plus the deviation:
     16 joins of a thread's pixels, 67 additions over the workgroup's threads and 16 joins of chunks where nothing else is
     said.  Its variance's relative error is twice that count of U and the square of the mean's error in deviations, halved
-    by the root.  Then come the difference, the two products, the sum, and SiLU as in ``linear``."""
+    by the root.  Then come the difference, the two products, the sum, and SiLU as in ``linear``.  ``statistics``: mean
+    and variance [B, 1, groups, 1], where x is a part of the image."""
     B, P, C = x.shape
     v = x.double().reshape(B, P, groups, C // groups)
-    mean, var = v.mean((1, 3), keepdim=True), v.var((1, 3), keepdim=True, unbiased=False)
+    mean, var = statistics or (v.mean((1, 3), keepdim=True), v.var((1, 3), keepdim=True, unbiased=False))
     std = (var + eps).sqrt()
     dmean = steps * U * (mean.abs() + var.sqrt())
     n = (v - mean) / std
