@@ -25,7 +25,8 @@ constexpr int V = 8;                  // channels of a thread
 constexpr int THREADS = 256, MAX_THREADS = 1024;
 constexpr int MAX_CHANNELS = 8192;
 constexpr int64_t CHUNK_BYTES = 16 << 10;
-constexpr int64_t LARGE_BYTES = 512ll << 20;
+constexpr int64_t LARGE_BYTES = 512ll << 20, LARGE_FLOAT_BYTES = 640ll << 20;
+constexpr int64_t LINE = 128;         // bytes of a cache line
 
 struct Args {
   const void* x;
@@ -419,20 +420,31 @@ Args from_element(Args a, int32_t first) {
 // 10.6; with groups twice and four times as large as a workgroup holds now 13.7, 10.9 and 30.4, 11.5.
 bool few(int64_t pixels, int per) { return pixels * (per / few_width(per)) <= (int64_t)UNITS * FEW_THREADS; }
 
-// Chunks of at least 16 KB, up to as many as there are CUs, and twice as many of twice the threads past 512 MB.
+// Chunks of at least 16 KB, up to as many as there are CUs.
 // us of 256, 512 chunks of 256 threads, and of 512 threads: 65536 pixels x 512 channels bf16 45.2, 47.3, 47.4, 47.0; 262144 x
 // 256 fp32 142, 146, 150, 159, bf16 85, 88, 81, 87; 2048 x 2048 x 128 bf16 578, 550, 543, 534.  Of 16384 x 512 18.2, 20.4,
 // 17.0, 23.8; 128 chunks 22.4: every workgroup of the second launch joins all chunks of its element.
+//
+// Twice as many of twice the threads where an element is large.  Once / twice, us, 128 channels: bf16 256 MB 131 / 135, 512
+// 269 / 258, 640 367 / 344, 1024 576 / 533, 2048 1200 / 1137; fp32 576 MB 351 / 361, 640 398 / 393, 1024 684 / 633, 1536 1030 /
+// 1028.  Rows that are neither whole lines nor some of one lose by it while they are short, 1024 MB: 20 channels bf16 912 /
+// 928, 60 933 / 1040, 96 609 / 637, 330 709 / 739, fp32 60 868 / 947, 100 795 / 846; but 320 channels bf16 588 / 557, 500 697 / 672,
+// 1002 751 / 720, fp32 250 734 / 726.  Fewer than eight channels are latency: 6 bf16 3400 / 1735.
+bool large(int64_t bytes, int64_t row, int channels, int dtype) {
+  return bytes > (dtype == HB_DTYPE_F32 ? LARGE_FLOAT_BYTES : LARGE_BYTES) &&
+         (row % LINE == 0 || LINE % row == 0 || row >= 1000 || channels < V);
+}
+
 struct Chunks {
   int64_t pixels, count;
   int threads;
 };
 Chunks chunks_of(int64_t pixels, int channels, int dtype) {
   const int64_t row = channels * size_of(dtype);
-  const int large = pixels * row > LARGE_BYTES ? 2 : 1;
-  const int64_t count = std::clamp<int64_t>(pixels * row / CHUNK_BYTES, 1, 256 * large);
+  const int times = large(pixels * row, row, channels, dtype) ? 2 : 1;
+  const int64_t count = std::clamp<int64_t>(pixels * row / CHUNK_BYTES, 1, 256 * times);
   const int64_t each = (pixels + count - 1) / count;
-  return {each, (pixels + each - 1) / each, THREADS * large};
+  return {each, (pixels + each - 1) / each, THREADS * times};
 }
 
 template <int DT, int W>
