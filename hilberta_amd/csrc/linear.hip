@@ -228,8 +228,9 @@ struct RowEnd {
 //  * An XCD takes a run of the tiles, four token tiles by all channel tiles at a time, so that its L2 serves both
 //    operands.
 // Bound by power: the clock falls with what the matrix pipes do, and products of 16 x 16 x 32 take less of it than those of
-// 32 x 32 x 16 (16384 x 12288 -> 3072 897 and 942 us).  That size with residual and gate 857 us, 1.44 PFLOP/s, where the
-// library's product alone takes 806 to 839; 8192 x 3072 -> 12288 with GELU 449 (442); 512 and 4096 rows, 3072 -> 9216, 210.
+// 32 x 32 x 16 (16384 x 12288 -> 3072 897 and 942 us).  By machine, that size with residual and gate takes 837 to 905 us,
+// 1.37 to 1.48 PFLOP/s, where the library's product alone takes 806 to 839; 8192 x 3072 -> 12288 with GELU 441 to 473 (442);
+// 512 and 4096 rows, 3072 -> 9216, 205 to 220.
 constexpr int WIDE = 256, WIDE_BAND = 4, WIDE_WAVES = 4;
 constexpr int WIDE_STAGE = 2 * WIDE * 128;                  // 64 KB
 constexpr int WIDE_LOADS = WIDE_STAGE / 1024 / WIDE_WAVES;  // 1 KB loads of a wave and stage
@@ -785,7 +786,8 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
 // ------------------------------------------------------------------ a few rows
 // 16 channels by up to 16 tokens a workgroup; its eight waves take turns at 128 features, straight from memory into the
 // matrix instruction's registers, and their sums meet in LDS.  Rows may lie at any address.  Bound by the weight's
-// read: 1 x 3072 -> 18432 25.8 us, 4.4 TB/s (a large copy reaches 4.9).
+// read: 1 x 3072 -> 18432 25.8 us, 4.4 TB/s (linear_rows_kernel takes 21.2 for one such layer and 16.2 for each of
+// seven).
 constexpr int FEW_ROWS = 16, FEW_WAVES = 8;
 
 template <bool F16>
@@ -871,10 +873,11 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
 // (TWO64x64: with half the stages in LDS, so that a CU has two workgroups; ROWS64x64: the same of rows at any address)
 enum Kernel { T64x32, T32x64, T64x64, TWO64x64, T96x64, T96x128, T128x128, WIDE256, ROWS64x64, KERNELS, FEW16 = KERNELS };
 
-// A kernel's tile, how many workgroups the card holds at once, and what its time is made of, in us: the launch, a round of so
+// A kernel's tile, how many workgroups the card's 256 CUs hold at once, and what its time is made of, in us: the launch, a round of so
 // many workgroups, a round's stage of 64 features, what a stage takes longer when all CUs are at it, each megabyte of rows
 // and weight, each million outputs, and, in parts, the join and each megabyte of their sums.  Fitted to 4418 times of 424 sizes
-// whose operands come from memory, which they meet to 12% (one sigma).
+// whose operands come from memory, which they meet to 12% (one sigma); some by more, 16384 x 5032 -> 5000 580 for 740 us, where
+// the choice is the same.
 struct Shape {
   int tc, tt;
   float at_once, launch, round, stage, full, megabyte, outputs, join, sums;

@@ -1,18 +1,20 @@
-"""The denoiser's and decoder's linear layers in 16 bits, with what follows them in the same pass (csrc/linear.hip).
+"""Linear layers in 16 bits with what follows them in the same pass (csrc/linear.hip).
 
 ``linear(x, weight, bias, act=act, residual=residual, gate=gate)`` computes, per row,
 
     out = residual + gate * act(x @ weight^T + bias)
 
-which a transformer block runs as a library product and one to three passes over its output
+for a caller's own layers (FluxTransformer has library products or 8-bit ones), which a transformer block runs as a library product and one to three passes over its output
 (``F.linear``, an activation, ``torch.addcmul``), and an image decoder as a convolution of one pixel and an
 addition.  Sums and epilogue are fp32, rounded once to the 16-bit output.  ``linear_pair`` does so for two row
 sets with weights of their own (a block's text and image rows) in one launch.
 
 Inference only: inputs that need a gradient are refused.  Launches are asynchronous on the current stream and can
 be captured into a graph.  Rows, weights and outputs may be row ranges or column blocks of larger buffers; rows
-that are no multiple of 16 bytes may be copied into aligned ones first, and a long sum for few outputs is made in
-parts, joined in their order; both take a workspace for the call.  The reference has library calls here (in the
+that are no multiple of 16 bytes may be copied into aligned ones first, weights in every call (a caller that keeps one
+pads its features and the rows' to a multiple of eight, with zeros), and a long sum for few outputs is made in
+parts, joined in their order; both take a workspace for the call.  A layer of one or two rows is read faster by
+flux_cond.linear_layers, which takes many layers at once.  The reference has library calls here (in the
 transformer that hilberta/flux_adapter.py wraps).
 """
 

@@ -108,7 +108,7 @@ def group_norm(x, groups, weight=None, bias=None, *, act=None, eps=1e-6, out=Non
     """act((x - mean) / sqrt(var + eps) * weight + bias), mean and variance of each batch element's ``groups`` groups of
     neighbouring channels over all pixels.
 
-    x [B, pixels, C], [B, C, H, W] or [B, C, T, H, W], its channels last in memory (torch.channels_last,
+    x [B, pixels, C] (torch.nn.GroupNorm takes three dimensions as [B, C, pixels]: such a map's x.transpose(1, 2)), [B, C, H, W] or [B, C, T, H, W], its channels last in memory (torch.channels_last,
     channels_last_3d) and its pixels evenly apart; bf16, fp16 or fp32, up to 8192 channels and 65535 batch
     elements; weight and bias [C] of x's dtype; act None or "silu"; eps 2^-126 or more.  Statistics and values are fp32, rounded once.
     ``out`` is like x and may be x itself.
