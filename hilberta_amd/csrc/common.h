@@ -34,7 +34,7 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // still hold (100 MB 18.6 -> 21.3 us; one tensor again and again, 246 MB 39.3 -> 44.9), and a little above
 // it they can: an input just written may still be there (one set of tensors again and again, 302 MB 53.2
 // -> 54.3; after the product that writes y 227 -> 225).  Inputs that repeat, by a stride of zero or more
-// gathered rows than there are, are read through the caches at every size.
+// gathered rows than there are, are read through the caches at every size (but for a group norm's image).
 constexpr int64_t CACHE_BYTES = 256ll << 20;
 
 template <bool STREAM, typename T>

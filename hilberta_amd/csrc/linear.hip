@@ -236,9 +236,10 @@ constexpr int WIDE_STAGE = 2 * WIDE * 128;                  // 64 KB
 constexpr int WIDE_LOADS = WIDE_STAGE / 1024 / WIDE_WAVES;  // 1 KB loads of a wave and stage
 
 // What the epilogue does.  All up to GATED are for tiles of one batch element each and work on the sums in registers, with
-// EDGE also where tiles are not whole; their columns are a multiple of eight and outputs aligned.  ANY takes any tile through
-// LDS (4173 x 3072 -> 9216 238 us, with EDGE 200; 9000 x 1024 -> 9000 with residual and gate 320, 227), and PARTS, for a part of the features of any tile, stores the sums themselves.  (One kernel for several kinds of tile keeps
-// too much in registers.)
+// EDGE also where tiles are not whole; their columns are a multiple of eight and outputs aligned.  ANY takes any tile
+// through LDS (4173 x 3072 -> 9216 238 us, with EDGE 200; 9000 x 1024 -> 9000 with residual and gate 320, 227), and PARTS,
+// for a part of the features of any tile, stores the sums themselves.  (One kernel for several kinds of tile keeps too much
+// in registers.)
 enum Mode { PLAIN, ACT_GELU, ACT_SILU, RESIDUAL, GATED, ANY, PARTS };
 
 // A wave's 128 x 128 sums: acc[i][j] are channels 16 i + 4 (lane / 16) .. + 3 of token 16 j + lane % 16.
@@ -962,17 +963,18 @@ float estimate_few(const Args& a, int count, bool aligned) {
                   3.f + megabytes * (0.25f + 0.007f * tokens) * slower);
 }
 
-// The kernel, and the parts that it takes the features in, of the least estimate.  Parts pay where few tiles leave CUs
-// idle over many features; they are tried while all their workgroups fit the card at once, with four stages each or more.
+// The kernel, and the parts that it takes the features in, of the least estimate.  Parts pay where few tiles leave CUs idle
+// over many features; they are tried while all their workgroups fit the card at once, with four stages each or more.
 // Measured, the best of one part / the parts: 99 x 8472 -> 64 30.4 / 9.9 us, 512 x 12288 -> 3072 72.8 / 60 (eight of the
 // wide kernel), 1280 x 13824 -> 5120 251 / 171 (two of it).  Over 264 sizes the choice takes 1.6% more time than the best of
-// all; the best of one part takes 13.9% more over 175 of them.  What the wide kernel's epilogue is counts: over 100 sizes with
-// an activation and a residual the choice takes 2.5% more than the best, and 29% as if it were in registers (1330 x 64 -> 1664
-// 8.9 / 34.9 us, 10240 x 128 -> 256 9.7 / 36.2); over 80 of several batch elements or odd columns 0.8%.  TWO64x64 pays where many tiles are short: the best of the
-// others / with it 5993 x 128 -> 2752 47.5 / 39.5, 4576 x 64 -> 960 16.6 / 12.8, 657 x 1216 -> 2624 16.2 / 13.7; alone on
-// its CU it is slower (77 x 4096 -> 3072 27.6, T64x64 21.9); without it the choice takes 5.8% more than the best.  Rows that direct loads cannot take are copied, or not, by the same measure.
-// Copied / as they are: 999 x 1001 -> 777 14.0 / 11.7 us, 2405 x 13 -> 20 11.0 / 7.2, 64 x 12001 -> 17000 262 / 219, 2000 x
-// 5001 -> 5000 144 / 345; over 160 such sizes the choice takes 1.0% more than the better one, copies alone 27%.
+// all; the best of one part takes 13.9% more over 175 of them.  What the wide kernel's epilogue is counts: over 100 sizes
+// with an activation and a residual the choice takes 2.5% more than the best, and 29% as if it were in registers (1330 x 64
+// -> 1664 8.9 / 34.9 us, 10240 x 128 -> 256 9.7 / 36.2); over 80 of several batch elements or odd columns 0.8%.  TWO64x64
+// pays where many tiles are short: the best of the others / with it 5993 x 128 -> 2752 47.5 / 39.5, 4576 x 64 -> 960 16.6 /
+// 12.8, 657 x 1216 -> 2624 16.2 / 13.7; alone on its CU it is slower (77 x 4096 -> 3072 27.6, T64x64 21.9); without it the
+// choice takes 5.8% more than the best.  Rows that direct loads cannot take are copied, or not, by the same measure. Copied
+// / as they are: 999 x 1001 -> 777 14.0 / 11.7 us, 2405 x 13 -> 20 11.0 / 7.2, 64 x 12001 -> 17000 262 / 219, 2000 x 5001
+// -> 5000 144 / 345; over 160 such sizes the choice takes 1.0% more than the better one, copies alone 27%.
 Choice choose(const Args& a, int count, int first, int last) {
   Choice best = {(Kernel)last, 1, estimate(a, count, (Kernel)last, 1)};
   const int stages = (a.features + 63) / 64;
